@@ -1,9 +1,10 @@
-"""Build the HIP library libf16acc_amd.so for gfx950 with hipcc, in-tree.
+"""Build the HIP libraries for gfx950 with hipcc, in-tree.
 
     python f16acc_amd/build.py
 
-The library is the whole native part of the package: kernels, per-shape tile
-table and the C ABI declared in include/f16acc.h.
+libf16acc_amd.so is the chunked GEMM: kernels, per-shape tile table and the C
+ABI declared in include/f16acc.h.  libf16acc_ops.so holds the 8-bit products and
+the mixture-of-experts operators (include/f16acc_ops.h).
 """
 
 import os
@@ -17,6 +18,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SRC = os.path.join(PKG, "csrc", "f16acc_gemm.hip")
 CHUNKRATE_SRC = os.path.join(PKG, "csrc", "chunkrate.hip")
+OPS_SRC = os.path.join(PKG, "csrc", "ops", "ops.hip")
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(OUT_DIR, "libf16acc_amd.so")
@@ -30,6 +32,8 @@ LIB_SPLITREDO = os.path.join(OUT_DIR, "libf16acc_amd_splitredo.so")
 # of the persistent kernel (-DF16ACC_NO_PERSISTENT=1): only bench.py's
 # persistent A/B loads it.
 LIB_NOPERSIST = os.path.join(OUT_DIR, "libf16acc_amd_nopersist.so")
+# The 8-bit products and the mixture-of-experts operators (include/f16acc_ops.h).
+LIB_OPS = os.path.join(OUT_DIR, "libf16acc_ops.so")
 # The native call path (csrc/host.cpp): a CPython module on torch's C++ headers.
 HOST_SRC = os.path.join(PKG, "csrc", "host.cpp")
 HOST = os.path.join(OUT_DIR, "f16acc_host.so")
@@ -104,13 +108,13 @@ def _finish(job, verbose):
 
 def build(verbose=False):
     """Compile the library, its no-redo, split-redo and no-persistent twins,
-    the chunkrate microbenchmark and the native call path (six compilers at
-    once)."""
+    the operators' library, the chunkrate microbenchmark and the native call
+    path (seven compilers at once)."""
     flags, libs = host_flags()
     jobs = [_start(HIP_FLAGS, SRC, LIB), _start(HIP_FLAGS + ["-DF16ACC_NO_REDO=1"], SRC, LIB_NOREDO),
             _start(HIP_FLAGS + ["-DF16ACC_SPLIT_REDO=1"], SRC, LIB_SPLITREDO),
             _start(HIP_FLAGS + ["-DF16ACC_NO_PERSISTENT=1"], SRC, LIB_NOPERSIST),
-            _start(COMMON_FLAGS, CHUNKRATE_SRC, CHUNKRATE), _start(flags, HOST_SRC, HOST, cxx(), libs)]
+            _start(HIP_FLAGS, OPS_SRC, LIB_OPS), _start(COMMON_FLAGS, CHUNKRATE_SRC, CHUNKRATE), _start(flags, HOST_SRC, HOST, cxx(), libs)]
     errors = []
     for job in jobs:
         try:

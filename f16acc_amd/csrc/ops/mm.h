@@ -1,0 +1,410 @@
+// The block-scaled product of e4m3 operands, as one product and as the products
+// of a set of experts:
+//
+//   c[m][n] = sum_kb sx[m][kb] * sw[n][kb] * sum_{k in kb} x[m][k] * w[n][k]
+//
+// x holds tokens (rows), w weight rows; kb are the blocks of 128 along K.  The
+// inner sum is one v_mfma_f32_16x16x128_f8f6f4 (K = 128, one block) into zero,
+// the outer one an FP32 multiply-add per element: 32 matrix cycles against 16
+// of the vector unit per 16 x 16 block step, which run side by side.  The
+// weights are the MFMA's rows and the tokens its columns, so a lane holds four
+// consecutive n of ONE token: its scale is one register per 16 tokens, already
+// multiplied by the weight block's scale.
+//
+// A workgroup stages BM tokens and BN weight rows by 128 K in LDS with
+// 16-byte global -> LDS copies, in a ring of NS stages; unit u of a row lies at
+// u ^ swz(row), which spreads the 16 rows of a fragment read over the banks.
+// Units past K, rows past M or N and tokens of other experts read zeros.
+#pragma once
+
+#include "common.h"
+
+namespace f16ops {
+
+struct MmArgs {
+  const uint8_t* x;  // [M][ldx] bytes, 16-byte aligned rows
+  int64_t ldx;
+  const float* sx;  // element (m, kb) at m * sxm + kb * sxk
+  int64_t sxm, sxk;
+  const uint8_t* w;  // [N][ldw]
+  int64_t ldw;
+  const float* sw;  // element (n or n / 128, kb) at i * swn + kb * swk
+  int64_t swn, swk;
+  const void* bias;  // [N] in the output's type, or NULL
+  void* c;
+  int64_t scm, scn;
+  int64_t M, N, K;
+  int ctype;
+  // Experts: the tile list (expert, first slot, end slot, -) and its length, the
+  // token row of each slot (NULL: the slot itself), the strides between experts.
+  const int4* tiles;
+  const int* ntiles;
+  const int* rows;
+  int64_t xrows;  // rows of x
+  int64_t we, swe;
+  // Gate and up: w holds the gate's N rows, then (at up bytes, its scales at
+  // sup elements) the up's; the result goes to q and its scales, quantised.
+  int64_t up, sup;
+  uint8_t* q;
+  int64_t ldq;
+  float* sq;
+  int64_t ldsq;
+};
+
+enum Epilogue { kStore = 0, kGatedQuant = 1 };
+
+template <int BM_, int BN_, int WM_, int WN_, int NS_, int OCC_>
+struct MmCfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, OCC = OCC_;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  static constexpr int LX = BM * 8 / THREADS, LW = BN * 8 / THREADS;  // 16-byte copies per lane and stage
+  static constexpr int X_BYTES = BM * kBlock, W_BYTES = BN * kBlock, S_BYTES = THREADS * 4;
+  static_assert(LX * THREADS == BM * 8 && LW * THREADS == BN * 8, "whole copies");
+  static_assert(BM <= THREADS, "one scale copy per stage covers the tokens");
+  static_assert(THREADS / 8 % 16 == 0, "a lane's units keep the swizzle phase");
+  static constexpr int stage_bytes(bool row_scales) {
+    return X_BYTES + W_BYTES + S_BYTES * (row_scales ? 1 + (BN + THREADS - 1) / THREADS : 1);
+  }
+};
+
+// Spreads the 16 rows that a fragment read touches over the LDS banks.
+__device__ __forceinline__ int swz(int row) { return ((row >> 1) ^ ((row & 1) << 2)) & 7; }
+
+// Rows row .. row + 15 (row = lane % 16) of a staged operand: lane group g holds
+// units g and g + 4 of the row's eight.  (The order of k inside a block is the
+// same for both operands, so any will do.)
+__device__ __forceinline__ i32x8 read_frag(const char LDS_AS* base, int row, int g) {
+  const char LDS_AS* r = base + row * kBlock;
+  const i32x4 lo = *(const i32x4 LDS_AS*)(r + ((g ^ swz(row)) << 4));
+  const i32x4 hi = *(const i32x4 LDS_AS*)(r + (((g + 4) ^ swz(row)) << 4));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ f32x4 mfma(const i32x8& w, const i32x8& x) {
+  const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// Four consecutive outputs of one token from FP32, rounded once.
+template <class T>
+__device__ __forceinline__ void store4(T* p, int64_t scn, int left, const f32x4& v, bool wide) {
+  if (wide && left >= 4) {
+    struct alignas(4 * sizeof(T)) Pack {
+      T t[4];
+    } k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k.t[i] = (T)v[i];
+    *(Pack*)p = k;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i * scn] = (T)v[i];
+  }
+}
+
+template <class C, bool ROW_SCALES, bool EXPERTS, int EPI>
+struct MmKernel {
+  static constexpr int STAGE = C::stage_bytes(ROW_SCALES);
+  static constexpr int LSW = ROW_SCALES ? (C::BN + C::THREADS - 1) / C::THREADS : 0;
+  static constexpr int LOADS = C::LX + C::LW + 1 + LSW;
+  static constexpr bool GATED = EPI == kGatedQuant;
+  static constexpr int BN_OUT = GATED ? C::BN / 2 : C::BN;  // columns of the result
+  static_assert((C::NS - 2) * LOADS <= 63, "outstanding copies must fit vmcnt");
+
+  // Where a lane's copies read.
+  struct Loader {
+    int x_off[EXPERTS ? C::LX : 1], x_step;
+    int w_off, w_step, u;  // u: the first k of the lane's units
+    int s_off;             // token scale
+    int sw_off[ROW_SCALES ? LSW : 1];
+    i32x4 xr, wr, ur, sr, swr;
+    int64_t sxk, swk;
+    int nk, krest;
+  };
+
+  __device__ static __forceinline__ void init(Loader& l, const MmArgs& p, int64_t m0, int m_left, int64_t n0,
+                                              const uint8_t* w, const float* sw, int tid) {
+    const int row = tid >> 3, u = (tid & 7) ^ swz(row);
+    l.u = u * 16;
+    l.nk = (int)cdiv(p.K, kBlock);
+    l.krest = (int)(p.K - (int64_t)(l.nk - 1) * kBlock);
+    l.x_step = (int)(C::THREADS / 8 * p.ldx);
+    l.w_step = (int)(C::THREADS / 8 * p.ldw);
+    l.w_off = (int)(row * p.ldw) + l.u;
+    if (EXPERTS) {
+#pragma unroll
+      for (int j = 0; j < C::LX; ++j) {
+        const int r = row + j * (C::THREADS / 8);
+        l.x_off[j] = kOob;
+        if (r < m_left) l.x_off[j] = (int)((p.rows ? p.rows[m0 + r] : (int)m0 + r) * p.ldx) + l.u;
+      }
+      l.xr = make_srd(p.x, p.xrows * p.ldx);
+      l.s_off = kOob;
+      if (tid < m_left) l.s_off = (int)((p.rows ? p.rows[m0 + tid] : (int)m0 + tid) * p.sxm * 4);
+      l.sr = make_srd(p.sx, kOob);
+    } else {
+      l.x_off[0] = (int)(row * p.ldx) + l.u;
+      l.xr = make_srd(p.x + m0 * p.ldx, m_left * p.ldx);
+      l.s_off = tid < m_left ? (int)(tid * p.sxm * 4) : kOob;
+      l.sr = make_srd(p.sx + m0 * p.sxm, kOob);
+    }
+    if (C::BM < C::THREADS && tid >= C::BM) l.s_off = kOob;
+    const int64_t n_left = p.N - n0;
+    l.wr = make_srd(w + n0 * p.ldw, n_left * p.ldw);
+    if (GATED) l.ur = make_srd(w + p.up + n0 * p.ldw, n_left * p.ldw);
+    if (ROW_SCALES) {
+      l.swr = make_srd(sw + n0 * p.swn, kOob);
+#pragma unroll
+      for (int j = 0; j < LSW; ++j) {
+        const int n = tid + j * C::THREADS;
+        l.sw_off[j] = n < C::BN && n < n_left ? (int)(n * p.swn * 4) : kOob;
+      }
+    }
+    l.sxk = p.sxk * 4;
+    l.swk = p.swk * 4;
+  }
+
+  __device__ static __forceinline__ i32x4 advanced(const i32x4& r, int64_t bytes) {
+    i32x4 q = r;
+    const uint64_t base = (((uint64_t)(uint32_t)r[1] << 32) | (uint32_t)r[0]) + (uint64_t)bytes;
+    q[0] = (int)(uint32_t)base;
+    q[1] = (int)(uint32_t)(base >> 32);
+    return q;
+  }
+
+  // Issues the copies of K block kb into the stage at `slot`.  Past the last
+  // block every unit reads zeros.
+  __device__ static __forceinline__ void issue(const Loader& l, int kb, int slot, int wave) {
+    const int left = kb < l.nk - 1 ? kBlock : kb == l.nk - 1 ? l.krest : 0;
+    const bool in = l.u < left;
+    const int base = slot + wave * 1024;
+    const i32x4 xr = advanced(l.xr, (int64_t)kb * kBlock), wr = advanced(l.wr, (int64_t)kb * kBlock);
+    if (EXPERTS) {
+#pragma unroll
+      for (int j = 0; j < C::LX; ++j) lds_dma16(xr, base + j * C::THREADS * 16, in ? l.x_off[j] : kOob);
+    } else {
+      const int off = in ? l.x_off[0] : kOob;
+#pragma unroll
+      for (int j = 0; j < C::LX; ++j) lds_dma16(srd_at(xr, j * l.x_step), base + j * C::THREADS * 16, off);
+    }
+    const int off = in ? l.w_off : kOob;
+    if (GATED) {
+      const i32x4 ur = advanced(l.ur, (int64_t)kb * kBlock);
+#pragma unroll
+      for (int j = 0; j < C::LW / 2; ++j)
+        lds_dma16(srd_at(wr, j * l.w_step), base + C::X_BYTES + j * C::THREADS * 16, off);
+#pragma unroll
+      for (int j = 0; j < C::LW / 2; ++j)
+        lds_dma16(srd_at(ur, j * l.w_step), base + C::X_BYTES + (C::LW / 2 + j) * C::THREADS * 16, off);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::LW; ++j)
+        lds_dma16(srd_at(wr, j * l.w_step), base + C::X_BYTES + j * C::THREADS * 16, off);
+    }
+    const int sbase = slot + C::X_BYTES + C::W_BYTES + wave * 256;
+    lds_dma4(advanced(l.sr, kb * l.sxk), sbase, left ? l.s_off : kOob);
+    if (ROW_SCALES) {
+      const i32x4 swr = advanced(l.swr, kb * l.swk);
+#pragma unroll
+      for (int j = 0; j < LSW; ++j)
+        lds_dma4(swr, sbase + C::S_BYTES * (1 + j), left ? l.sw_off[j] : kOob);
+    }
+  }
+
+  // Row of fragment j of the wave's weights in the staged tile.  Gated: the
+  // first half of the fragments are gate rows, the second the same up rows.
+  __device__ static __forceinline__ int w_row(int wn, int j) {
+    if (!GATED) return wn * C::TN + 16 * j;
+    return j < C::FN / 2 ? wn * (C::TN / 2) + 16 * j : C::BN / 2 + wn * (C::TN / 2) + 16 * (j - C::FN / 2);
+  }
+
+  __device__ static void run(const MmArgs& p, char LDS_AS* lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / C::WN, wn = wave % C::WN, t16 = lane & 15, g = lane >> 4;
+    int64_t m0, n0;
+    int m_left;
+    const uint8_t* w = p.w;
+    const float* sw = p.sw;
+    const uint32_t tiles_n = (uint32_t)cdiv(p.N, BN_OUT);
+    if (EXPERTS) {
+      const uint32_t total = (uint32_t)*p.ntiles * tiles_n;
+      if (blockIdx.x >= total) return;
+      const uint32_t id = xcd_order(blockIdx.x, total), t = id / tiles_n;
+      const int4 tile = p.tiles[t];
+      m0 = tile.y;
+      m_left = tile.z - tile.y;
+      n0 = (int64_t)(id - t * tiles_n) * BN_OUT;
+      w += tile.x * p.we;
+      sw += tile.x * p.swe;
+    } else {
+      const uint32_t tiles_m = (uint32_t)cdiv(p.M, C::BM);
+      uint32_t id = xcd_order(blockIdx.x, tiles_m * tiles_n);
+      // 8 tile rows at a time, column by column, so an XCD's tiles share operands
+      const uint32_t width = 8 * tiles_n, first = tiles_m > 8 ? id / width * 8 : 0;
+      const uint32_t gsz = tiles_m - first < 8 ? tiles_m - first : 8;
+      id -= first * tiles_n;
+      const uint32_t col = id / gsz;
+      m0 = (int64_t)(first + (id - col * gsz)) * C::BM;
+      n0 = (int64_t)col * C::BN;
+      m_left = (int)(p.M - m0 < C::BM ? p.M - m0 : C::BM);
+    }
+    Loader l;
+    init(l, p, m0, m_left, n0, w, sw, tid);
+    const int lds0 = __builtin_amdgcn_readfirstlane((int)(uint32_t)(size_t)lds);
+
+    f32x4 acc[C::FM][C::FN];
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+#pragma unroll
+    for (int s = 0; s < C::NS - 1; ++s) issue(l, s, lds0 + s * STAGE, wave);
+
+    // the weight block's scale: one value per wave (two where it is gated)
+    const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
+    const int64_t nb_last = cdiv(p.N, kBlock) - 1;
+    const float* swp = sw + (nb < nb_last ? nb : nb_last) * p.swn;
+
+    int slot = 0, next = C::NS - 1;
+    for (int kb = 0; kb < l.nk; ++kb) {
+      float sb = 0.0f, sb2 = 0.0f;
+      if (!ROW_SCALES) {
+        sb = swp[kb * p.swk];
+        if (GATED) sb2 = swp[p.sup + kb * p.swk];
+      }
+      wait_vm<(C::NS - 2) * LOADS>();
+      barrier();
+      issue(l, kb + C::NS - 1, lds0 + next * STAGE, wave);
+      const char LDS_AS* xs = lds + slot * STAGE;
+      const char LDS_AS* ws = xs + C::X_BYTES;
+      const float LDS_AS* ss = (const float LDS_AS*)(ws + C::W_BYTES);
+      i32x8 xf[C::FM];
+      float s[C::FM];
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        xf[i] = read_frag(xs, wm * C::TM + 16 * i + t16, g);
+        s[i] = ss[wm * C::TM + 16 * i + t16];
+      }
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        const int row = w_row(wn, j);
+        const i32x8 wf = read_frag(ws, row + t16, g);
+        if (ROW_SCALES) {
+          const f32x4 sr = *(const f32x4 LDS_AS*)(ss + C::THREADS + row + 4 * g);
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i) {
+            const f32x4 part = mfma(wf, xf[i]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], s[i] * sr[r], acc[i][j][r]);
+          }
+        } else {
+          const float b = GATED && j >= C::FN / 2 ? sb2 : sb;
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i) {
+            const f32x4 part = mfma(wf, xf[i]);
+            const float sc = s[i] * b;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc, acc[i][j][r]);
+          }
+        }
+      }
+      slot = slot + 1 == C::NS ? 0 : slot + 1;
+      next = next + 1 == C::NS ? 0 : next + 1;
+    }
+    wait_vm<0>();
+    if (GATED)
+      store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
+    else if (p.ctype == F16ACC_TYPE_F16)
+      store<f16>(p, acc, m0, m_left, n0, wm, wn, t16, g);
+    else if (p.ctype == F16ACC_TYPE_BF16)
+      store<bf16>(p, acc, m0, m_left, n0, wm, wn, t16, g);
+    else
+      store<float>(p, acc, m0, m_left, n0, wm, wn, t16, g);
+  }
+
+  template <class T>
+  __device__ static __forceinline__ void store(const MmArgs& p, f32x4 (&acc)[C::FM][C::FN], int64_t m0, int m_left,
+                                               int64_t n0, int wm, int wn, int t16, int g) {
+    const bool wide = p.scn == 1 && p.scm % 4 == 0 && (uintptr_t)p.c % (4 * sizeof(T)) == 0;
+#pragma unroll
+    for (int j = 0; j < C::FN; ++j) {
+      const int64_t n = n0 + wn * C::TN + 16 * j + 4 * g;
+      const int left = (int)(p.N - n < 4 ? p.N - n : 4);
+      if (left <= 0) continue;
+      f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r < left) b[r] = (float)((const T*)p.bias)[n + r];
+      }
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        const int m = wm * C::TM + 16 * i + t16;
+        if (m < m_left) store4<T>((T*)p.c + (m0 + m) * p.scm + n * p.scn, p.scn, left, acc[i][j] + b, wide);
+      }
+    }
+  }
+
+  // h = silu(gate) * up of the tile's 128 columns, quantised: they are one block
+  // of each token, whose maximum is over the lane groups and the waves beside
+  // each other.
+  __device__ static __forceinline__ void store_gated(const MmArgs& p, char LDS_AS* lds, f32x4 (&acc)[C::FM][C::FN],
+                                                     int64_t m0, int m_left, int64_t n0, int wm, int wn, int t16,
+                                                     int g) {
+    static_assert(!GATED || C::BN == 2 * kBlock, "a tile is one block of h");
+    barrier();  // the stages are free
+    uint32_t LDS_AS* most = (uint32_t LDS_AS*)lds;  // [WN][BM]
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < C::FN / 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float h = silu(acc[i][j][r]) * acc[i][j + C::FN / 2][r];
+          acc[i][j][r] = h;
+          m = umax(m, abs_bits(h));
+        }
+      m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+      m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+      if (g == 0) most[wn * C::BM + wm * C::TM + 16 * i + t16] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+      const int m = wm * C::TM + 16 * i + t16;
+      uint32_t bits = most[m];
+#pragma unroll
+      for (int k = 1; k < C::WN; ++k) bits = umax(bits, most[k * C::BM + m]);
+      const BlockScale bs = block_scale(bits);
+      if (m < m_left) {
+#pragma unroll
+        for (int j = 0; j < C::FN / 2; ++j)
+          *(int*)(p.q + (m0 + m) * p.ldq + n0 + wn * (C::TN / 2) + 16 * j + 4 * g) =
+              pack_e4m3(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], bs.inv);
+        if (wn == 0 && g == 0) p.sq[n0 / kBlock * p.ldsq + m0 + m] = bs.s;
+      }
+    }
+  }
+};
+
+template <class C, bool ROW_SCALES, bool EXPERTS, int EPI>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void mm_kernel(MmArgs p) {
+  using K = MmKernel<C, ROW_SCALES, EXPERTS, EPI>;
+  static_assert(K::STAGE * C::NS <= 160 * 1024, "LDS of a CU");
+  __shared__ __align__(1024) char smem[K::STAGE * C::NS];
+  K::run(p, (char LDS_AS*)smem);
+}
+
+template <class C, bool ROW_SCALES, bool EXPERTS, int EPI>
+int launch_mm(const MmArgs& p, int64_t max_tiles_m, hipStream_t stream) {
+  using K = MmKernel<C, ROW_SCALES, EXPERTS, EPI>;
+  const int64_t tiles = max_tiles_m * cdiv(p.N, K::BN_OUT);
+  if (tiles > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
+  hipLaunchKernelGGL((mm_kernel<C, ROW_SCALES, EXPERTS, EPI>), dim3((uint32_t)tiles), dim3(C::THREADS), 0, stream, p);
+  return hip_status();
+}
+
+}  // namespace f16ops

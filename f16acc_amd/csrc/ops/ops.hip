@@ -1,0 +1,412 @@
+// C ABI of the 8-bit block-scaled products and the mixture-of-experts
+// operators (include/f16acc_ops.h): argument checks, the choice of a kernel,
+// workspaces.
+#include "common.h"
+#include "mm.h"
+#include "moe.h"
+#include "quant.h"
+#include "small.h"
+
+using namespace f16ops;
+
+namespace {
+
+// Bytes from an element of a row to the last one's end stay below the copies'
+// 31-bit offsets.
+constexpr int64_t kMaxRow = 1 << 22;  // bytes between rows of a staged operand: 256 rows stay below 2^31
+constexpr int64_t kMaxExtent = (int64_t)1 << 40;
+
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+int64_t up128(int64_t v) { return cdiv(v, kBlock) * kBlock; }
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+bool wide_loads(const void* x, int type, int64_t sr, int64_t sc) {
+  return sc == 1 && aligned16(x) && sr * type_size(type) % 16 == 0;
+}
+
+template <class F>
+int by_type(int type, F f) {
+  switch (type) {
+    case F16ACC_TYPE_F16: return f((f16*)nullptr);
+    case F16ACC_TYPE_BF16: return f((bf16*)nullptr);
+    case F16ACC_TYPE_F32: return f((float*)nullptr);
+  }
+  return F16ACC_OPS_E_ARG;
+}
+
+int quant_check(const void* x, int type, int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0 || type < 0 || type > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
+  if (rows > kMaxExtent || cols > kMaxExtent) return F16ACC_OPS_E_UNSUPPORTED;
+  if (rows && cols && !x) return F16ACC_OPS_E_ARG;
+  return 0;
+}
+
+int out_check(const uint8_t* q, int64_t ldq, int64_t cols, const float* s) {
+  if (!q || !s) return F16ACC_OPS_E_ARG;
+  if (ldq < cols || ldq % kBlock || !aligned16(q)) return F16ACC_OPS_E_UNSUPPORTED;
+  return 0;
+}
+
+int quant_rows(const QuantArgs& p, int type, hipStream_t stream) {
+  const int64_t groups = cdiv(p.rows * (p.ldq / kBlock), 16);
+  if (groups == 0) return 0;
+  const uint32_t grid = (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus);
+  const bool wide = wide_loads(p.x, type, p.sr, p.sc);
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (wide)
+      hipLaunchKernelGGL((quant_rows_kernel<T, true>), dim3(grid), dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((quant_rows_kernel<T, false>), dim3(grid), dim3(256), 0, stream, p);
+    return hip_status();
+  });
+}
+
+template <bool ROWS, bool COLS, bool SQUARE>
+int quant_tile(const QuantArgs& p, int type, hipStream_t stream) {
+  const int64_t gx = cdiv(p.cols, kBlock), gy = cdiv(p.rows, kBlock);
+  if (gx == 0 || gy == 0) return 0;
+  if (gx > 0x7fffffff || gy > 65535) return F16ACC_OPS_E_UNSUPPORTED;
+  const bool wide = wide_loads(p.x, type, p.sr, p.sc);
+  const dim3 grid((uint32_t)gx, (uint32_t)gy);
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (wide)
+      hipLaunchKernelGGL((quant_tile_kernel<T, true, ROWS, COLS, SQUARE>), grid, dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((quant_tile_kernel<T, false, ROWS, COLS, SQUARE>), grid, dim3(256), 0, stream, p);
+    return hip_status();
+  });
+}
+
+int mm_check(const MmArgs& p) {
+  if (p.M < 0 || p.N < 0 || p.K < 0 || p.ctype < 0 || p.ctype > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
+  if (p.M == 0 || p.N == 0) return 0;
+  if (!p.c || (p.K && (!p.x || !p.w || !p.sx || !p.sw))) return F16ACC_OPS_E_ARG;
+  if (p.sxm < 0 || p.sxk < 0 || p.swn < 0 || p.swk < 0) return F16ACC_OPS_E_ARG;
+  if (p.ldx % 16 || p.ldw % 16 || p.ldx < p.K || p.ldw < p.K || p.ldx > kMaxRow || p.ldw > kMaxRow ||
+      !aligned16(p.x) || !aligned16(p.w))
+    return F16ACC_OPS_E_UNSUPPORTED;
+  if (p.sxm > kMaxRow / 4 || p.swn > kMaxRow / 4 || p.M > 0x7fffffff || p.N > 0x7fffffff)
+    return F16ACC_OPS_E_UNSUPPORTED;
+  return 0;
+}
+
+using Cfg256 = MmCfg<256, 256, 2, 2, 2, 1>;
+using Cfg128 = MmCfg<128, 128, 2, 2, 2, 2>;
+using Cfg64 = MmCfg<64, 64, 2, 2, 3, 2>;
+using Cfg32 = MmCfg<32, 64, 2, 2, 4, 2>;
+
+template <bool ROW_SCALES>
+int mm_pick(const MmArgs& p, hipStream_t stream) {
+  auto run = [&](auto* c) {
+    using C = std::remove_pointer_t<decltype(c)>;
+    return launch_mm<C, ROW_SCALES, false, kStore>(p, cdiv(p.M, C::BM), stream);
+  };
+  if (p.M <= 32) return run((Cfg32*)nullptr);
+  if (cdiv(p.M, 256) * cdiv(p.N, 256) >= kCus / 2) return run((Cfg256*)nullptr);
+  if (cdiv(p.M, 128) * cdiv(p.N, 128) >= kCus / 2) return run((Cfg128*)nullptr);
+  return run((Cfg64*)nullptr);
+}
+
+// The experts' tiles: gate and up, 128 columns of each; down.
+template <int BM>
+struct ExpertCfg;
+template <>
+struct ExpertCfg<32> {
+  using GateUp = MmCfg<32, 256, 1, 4, 2, 1>;
+  using Down = MmCfg<32, 128, 1, 4, 3, 2>;
+};
+template <>
+struct ExpertCfg<64> {
+  using GateUp = MmCfg<64, 256, 1, 4, 2, 1>;
+  using Down = MmCfg<64, 128, 1, 4, 3, 2>;
+};
+template <>
+struct ExpertCfg<128> {
+  using GateUp = MmCfg<128, 256, 2, 2, 2, 1>;
+  using Down = MmCfg<128, 128, 2, 2, 2, 2>;
+};
+
+int expert_tile(int64_t slots, int E) {
+  const int64_t mean = slots / E;
+  return mean >= 96 ? 128 : mean >= 32 ? 64 : 32;
+}
+
+struct ExpertsPlan {
+  int64_t slots, blocks, max_tiles, Dp, Ip;
+  int bm;
+  size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
+  ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
+    slots = T * k;
+    Dp = up128(D);
+    Ip = up128(I);
+    bm = expert_tile(slots, E);
+    blocks = cdiv(slots, kSortChunk);
+    max_tiles = slots / bm + (slots < E ? slots : E);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += up256(bytes);
+      return here;
+    };
+    xq = take(T * Dp);
+    xs = take(T * (Dp / kBlock) * 4);
+    hq = take(slots * Ip);
+    hs = take(slots * (Ip / kBlock) * 4);
+    ys = take(slots * D * 4);
+    counts = take(blocks * E * 4);
+    rows = take(slots * 4);
+    pos = take(slots * 4);
+    tiles = take(max_tiles * 16);
+    ntiles = take(4);
+    total = at;
+  }
+};
+
+template <int BM>
+int expert_products(const MmArgs& gu, const MmArgs& down, int64_t max_tiles, hipStream_t stream) {
+  const int rc = launch_mm<typename ExpertCfg<BM>::GateUp, false, true, kGatedQuant>(gu, max_tiles, stream);
+  if (rc) return rc;
+  return launch_mm<typename ExpertCfg<BM>::Down, false, true, kStore>(down, max_tiles, stream);
+}
+
+template <template <class, int> class Launch, class... A>
+int by_experts(int E, int type, A&&... args) {
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (E <= 64) return Launch<T, 1>::go(args...);
+    if (E <= 128) return Launch<T, 2>::go(args...);
+    if (E <= 256) return Launch<T, 4>::go(args...);
+    if (E <= 512) return Launch<T, 8>::go(args...);
+    return Launch<T, 16>::go(args...);
+  });
+}
+template <class T, int V>
+struct LaunchRoute {
+  static int go(const RouteArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((route_kernel<T, V>), dim3((uint32_t)cdiv(a.T, 4)), dim3(256), 0, s, a);
+    return hip_status();
+  }
+};
+template <class T, int V>
+struct LaunchRouteGrad {
+  static int go(const RouteArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((route_grad_kernel<T, V>), dim3((uint32_t)cdiv(a.T, 4)), dim3(256), 0, s, a);
+    return hip_status();
+  }
+};
+
+int route_check(const RouteArgs& a, int type) {
+  if (a.T < 0 || type < 0 || type > F16ACC_TYPE_F32 || a.E < 1 || a.k < 1 || a.k > a.E) return F16ACC_OPS_E_ARG;
+  if (a.E > kMaxExperts || a.k > 64 || a.T > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
+  if (a.T && (!a.x || !a.ids)) return F16ACC_OPS_E_ARG;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int f16acc_quant_rows(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
+                      int64_t ldq, float* s, int64_t lds, void* stream) {
+  int rc = quant_check(x, type, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  rc = out_check(q, ldq, cols, s);
+  if (rc) return rc;
+  QuantArgs p{x, rows, cols, sr, sc, q, ldq, s, lds, nullptr, 0, nullptr, 0};
+  return quant_rows(p, type, (hipStream_t)stream);
+}
+
+int f16acc_quant_both(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
+                      int64_t ldq, float* s, int64_t lds, uint8_t* qt, int64_t ldqt, float* st, int64_t ldst,
+                      void* stream) {
+  int rc = quant_check(x, type, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  if (!q && !qt) return F16ACC_OPS_E_ARG;
+  if (q && (rc = out_check(q, ldq, cols, s))) return rc;
+  if (qt && (rc = out_check(qt, ldqt, rows, st))) return rc;
+  if (q && ldq != up128(cols)) return F16ACC_OPS_E_UNSUPPORTED;
+  if (qt && ldqt != up128(rows)) return F16ACC_OPS_E_UNSUPPORTED;
+  QuantArgs p{x, rows, cols, sr, sc, q, ldq, s, lds, qt, ldqt, st, ldst};
+  if (q && qt) return quant_tile<true, true, false>(p, type, (hipStream_t)stream);
+  if (qt) return quant_tile<false, true, false>(p, type, (hipStream_t)stream);
+  return quant_rows(p, type, (hipStream_t)stream);
+}
+
+int f16acc_quant_weight(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
+                        int64_t ldq, float* s, int64_t lds, uint8_t* qt, int64_t ldqt, void* stream) {
+  int rc = quant_check(x, type, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  rc = out_check(q, ldq, cols, s);
+  if (!rc && qt) rc = out_check(qt, ldqt, rows, s);
+  if (rc) return rc;
+  if (ldq != up128(cols) || (qt && ldqt != up128(rows))) return F16ACC_OPS_E_UNSUPPORTED;
+  QuantArgs p{x, rows, cols, sr, sc, q, ldq, s, lds, qt, ldqt, nullptr, 0};
+  return qt ? quant_tile<true, true, true>(p, type, (hipStream_t)stream)
+            : quant_tile<true, false, true>(p, type, (hipStream_t)stream);
+}
+
+int f16acc_pack8(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t cols, int64_t s_r, int64_t s_c, int64_t ld,
+                 void* stream) {
+  if (rows < 0 || cols < 0 || ld < cols) return F16ACC_OPS_E_ARG;
+  if (rows == 0 || ld == 0) return 0;
+  if (!dst || (cols && !src)) return F16ACC_OPS_E_ARG;
+  if (ld % 16 || !aligned16(dst) || rows > kMaxExtent || ld > kMaxExtent) return F16ACC_OPS_E_UNSUPPORTED;
+  Pack8Args p{src, dst, rows, cols, s_r, s_c, ld};
+  const int64_t groups = cdiv(rows * (ld / 16), 256);
+  hipLaunchKernelGGL(pack8_kernel, dim3((uint32_t)(groups < 16 * kCus ? groups : 16 * kCus)), dim3(256), 0,
+                     (hipStream_t)stream, p);
+  return hip_status();
+}
+
+int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, int64_t sxk, const uint8_t* w,
+                  int64_t ldw, const float* sw, int64_t swn, int64_t swk, int row_scales, const void* bias, void* c,
+                  int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype, void* stream) {
+  if (row_scales != 0 && row_scales != 1) return F16ACC_OPS_E_ARG;
+  MmArgs p{};
+  p.x = x, p.ldx = ldx, p.sx = sx, p.sxm = sxm, p.sxk = sxk;
+  p.w = w, p.ldw = ldw, p.sw = sw, p.swn = swn, p.swk = swk;
+  p.bias = bias, p.c = c, p.scm = scm, p.scn = scn, p.M = M, p.N = N, p.K = K, p.ctype = ctype;
+  const int rc = mm_check(p);
+  if (rc || M == 0 || N == 0) return rc;
+  return row_scales ? mm_pick<true>(p, (hipStream_t)stream) : mm_pick<false>(p, (hipStream_t)stream);
+}
+
+size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4);
+}
+
+int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw, const float* sw,
+                      int64_t swn, int64_t swk, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
+                      void* workspace, size_t ws_bytes, void* stream) {
+  int rc = quant_check(x, type, M, K);
+  if (rc) return rc;
+  MmArgs p{};
+  p.x = (const uint8_t*)workspace, p.ldx = up128(K);
+  p.sx = (const float*)((const char*)workspace + up256(M * up128(K))), p.sxm = 1, p.sxk = M;
+  p.w = w, p.ldw = ldw, p.sw = sw, p.swn = swn, p.swk = swk;
+  p.bias = bias, p.c = y, p.scm = N, p.scn = 1, p.M = M, p.N = N, p.K = K, p.ctype = type;
+  if (M > 0 && N > 0 && K > 0 &&
+      (!workspace || (uintptr_t)workspace % 256 || ws_bytes < f16acc_linear_fp8_workspace(M, N, K)))
+    return F16ACC_OPS_E_WORKSPACE;
+  rc = mm_check(p);
+  if (rc || M == 0 || N == 0) return rc;
+  if (M <= 16 && wide_loads(x, type, sr, sc) && K > 0) {
+    SmallArgs a{x, sr, w, ldw, sw, swn, swk, bias, y, N, 1, M, N, K};
+    return by_type(type, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      hipLaunchKernelGGL((linear_small_kernel<T, 8>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0, (hipStream_t)stream, a);
+      return hip_status();
+    });
+  }
+  if (K > 0) {
+    QuantArgs q{x, M, K, sr, sc, (uint8_t*)workspace, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
+    rc = quant_rows(q, type, (hipStream_t)stream);
+    if (rc) return rc;
+  }
+  return mm_pick<false>(p, (hipStream_t)stream);
+}
+
+int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
+                 const float* bias, int groups, int top, int renorm, float scale, float* weights, int* ids,
+                 void* stream) {
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, bias, groups, top, renorm, scale, weights, ids, nullptr, 0, 0, nullptr};
+  const int rc = route_check(a, type);
+  if (rc) return rc;
+  if (groups < 1 || E % groups || top < 1 || top > groups || k > E / groups * top || (T && !weights))
+    return F16ACC_OPS_E_ARG;
+  if (groups > 64) return F16ACC_OPS_E_UNSUPPORTED;
+  if (T == 0) return 0;
+  return by_experts<LaunchRoute>(E, type, a, (hipStream_t)stream);
+}
+
+int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
+                      int renorm, float scale, const int* ids, const float* dw, int64_t dwt, int64_t dwk,
+                      void* dlogits, void* stream) {
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, nullptr, 1, 1, renorm, scale, nullptr, (int*)ids, dw, dwt, dwk, dlogits};
+  const int rc = route_check(a, type);
+  if (rc) return rc;
+  if (T && (!dw || !dlogits)) return F16ACC_OPS_E_ARG;
+  if (T == 0) return 0;
+  return by_experts<LaunchRouteGrad>(E, type, a, (hipStream_t)stream);
+}
+
+size_t f16acc_experts_workspace(int64_t T, int k, int E, int64_t D, int64_t I) {
+  if (T <= 0 || k <= 0 || E <= 0 || D <= 0 || I <= 0) return 0;
+  return ExpertsPlan(T, k, E, D, I).total;
+}
+
+int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const float* weights, int64_t wt,
+                   int64_t wk, const int* ids, int k, int E, int64_t D, int64_t I, const uint8_t* w1, int64_t w1e,
+                   int64_t w1u, int64_t ld1, const float* s1, int64_t s1e, int64_t s1u, int64_t s1n, int64_t s1k,
+                   const uint8_t* w2, int64_t w2e, int64_t ld2, const float* s2, int64_t s2e, int64_t s2n,
+                   int64_t s2k, void* y, void* workspace, size_t ws_bytes, void* stream_) {
+  int rc = quant_check(x, type, T, D);
+  if (rc) return rc;
+  if (k < 1 || E < 1 || D < 1 || I < 1) return F16ACC_OPS_E_ARG;
+  if (T == 0) return 0;
+  if (!weights || !ids || !w1 || !s1 || !w2 || !s2 || !y) return F16ACC_OPS_E_ARG;
+  if (w1e < 0 || w1u < 0 || s1e < 0 || s1u < 0 || s1n < 0 || s1k < 0 || w2e < 0 || s2e < 0 || s2n < 0 || s2k < 0)
+    return F16ACC_OPS_E_ARG;
+  if (E > kMaxExperts || ld1 % 16 || ld2 % 16 || w1e % 16 || w1u % 16 || w2e % 16 || ld1 < D ||
+      ld2 < I || ld1 > kMaxRow || ld2 > kMaxRow || up128(D) > kMaxRow || up128(I) > kMaxRow || !aligned16(w1) ||
+      !aligned16(w2))
+    return F16ACC_OPS_E_UNSUPPORTED;
+  // the copies address a token's (a slot's) row by a 31-bit offset
+  if (T > kOob / up128(D) || T > kOob / ((int64_t)k * up128(I))) return F16ACC_OPS_E_UNSUPPORTED;
+  const ExpertsPlan plan(T, k, E, D, I);
+  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
+  hipStream_t stream = (hipStream_t)stream_;
+  char* ws = (char*)workspace;
+  QuantArgs q{x, T, D, sr, sc, (uint8_t*)(ws + plan.xq), plan.Dp, (float*)(ws + plan.xs), T, nullptr, 0, nullptr, 0};
+  rc = quant_rows(q, type, stream);
+  if (rc) return rc;
+  SortArgs so{ids, plan.slots, E, k, plan.bm, (int*)(ws + plan.counts), (int*)(ws + plan.rows), (int*)(ws + plan.pos),
+              (int4*)(ws + plan.tiles), (int*)(ws + plan.ntiles), (int)plan.blocks};
+  hipLaunchKernelGGL(sort_count_kernel, dim3(so.blocks), dim3(256), 0, stream, so);
+  hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, stream, so);
+  hipLaunchKernelGGL(sort_place_kernel, dim3(so.blocks), dim3(256), 0, stream, so);
+  rc = hip_status();
+  if (rc) return rc;
+
+  MmArgs gu{};
+  gu.x = q.q, gu.ldx = plan.Dp, gu.sx = q.s, gu.sxm = 1, gu.sxk = T;
+  gu.w = w1, gu.ldw = ld1, gu.sw = s1, gu.swn = s1n, gu.swk = s1k, gu.we = w1e, gu.swe = s1e, gu.up = w1u, gu.sup = s1u;
+  gu.M = plan.slots, gu.N = I, gu.K = D;
+  gu.tiles = so.tiles, gu.ntiles = so.ntiles, gu.rows = so.rows, gu.xrows = T;
+  gu.q = (uint8_t*)(ws + plan.hq), gu.ldq = plan.Ip, gu.sq = (float*)(ws + plan.hs), gu.ldsq = plan.slots;
+  MmArgs down{};
+  down.x = gu.q, down.ldx = plan.Ip, down.sx = gu.sq, down.sxm = 1, down.sxk = plan.slots;
+  down.w = w2, down.ldw = ld2, down.sw = s2, down.swn = s2n, down.swk = s2k, down.we = w2e, down.swe = s2e;
+  down.c = ws + plan.ys, down.scm = D, down.scn = 1, down.ctype = F16ACC_TYPE_F32;
+  down.M = plan.slots, down.N = D, down.K = I;
+  down.tiles = so.tiles, down.ntiles = so.ntiles, down.rows = nullptr, down.xrows = plan.slots;
+  rc = plan.bm == 128  ? expert_products<128>(gu, down, plan.max_tiles, stream)
+       : plan.bm == 64 ? expert_products<64>(gu, down, plan.max_tiles, stream)
+                       : expert_products<32>(gu, down, plan.max_tiles, stream);
+  if (rc) return rc;
+
+  CombineArgs co{(const float*)(ws + plan.ys), weights, wt, wk, so.pos, T, D, k, y};
+  const dim3 grid((uint32_t)T, (uint32_t)cdiv(cdiv(D, 4), 256));
+  return by_type(type, [&](auto* t) {
+    using U = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL((combine_kernel<U>), grid, dim3(256), 0, stream, co);
+    return hip_status();
+  });
+}
+
+const char* f16acc_ops_strerror(int code) {
+  switch (code) {
+    case 0: return "f16acc: success";
+    case F16ACC_OPS_E_ARG: return "f16acc: invalid argument";
+    case F16ACC_OPS_E_UNSUPPORTED: return "f16acc: extent, stride or alignment not supported";
+    case F16ACC_OPS_E_WORKSPACE: return "f16acc: workspace missing, misaligned or too small";
+  }
+  return code > 0 ? hipGetErrorString((hipError_t)code) : "f16acc: unknown error";
+}
+
+int f16acc_ops_abi_version(void) { return 1; }
+
+}  // extern "C"

@@ -1,0 +1,189 @@
+// Quantisation to e4m3 in blocks of 128: rows (1 x 128), columns (128 x 1, the
+// result transposed), and squares (128 x 128), and the copy that gives stored
+// 8-bit rows the alignment the products read.
+#pragma once
+
+#include "common.h"
+
+namespace f16ops {
+
+struct QuantArgs {
+  const void* x;
+  int64_t rows, cols, sr, sc;  // element strides
+  uint8_t* q;                  // [rows][ldq], zero from cols to ldq
+  int64_t ldq;
+  float* s;  // scale of (row, block) at s[block * lds + row]; squares: s[rowblock * lds + block]
+  int64_t lds;
+  uint8_t* qt;  // [cols][ldqt], zero from rows to ldqt
+  int64_t ldqt;
+  float* st;  // scale of (column, rowblock) at st[rowblock * ldst + column]
+  int64_t ldst;
+};
+
+// One row of a matrix in blocks of 1 x 128.  16 lanes take a block, 8 elements
+// each: a wave reads four blocks with one 16-byte load a lane (16-bit types),
+// finds each block's maximum with four row rotations and writes 8 bytes a
+// lane.  Bound by memory: 2 bytes read and 1 written an element.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
+  const int64_t blocks = p.ldq / kBlock;
+  const int64_t total = p.rows * blocks;
+  const int lane = threadIdx.x & 15;
+  for (int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)gridDim.x * 16) {
+    const int64_t row = b / blocks, kb = b - row * blocks, c0 = kb * kBlock + lane * 8;
+    const T* x = (const T*)p.x + row * p.sr;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (WIDE && c0 + 8 <= p.cols) {
+      load_vec(x + c0, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < p.cols) v[i] = (float)x[(c0 + i) * p.sc];
+    }
+    uint32_t m = abs_bits(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
+    const BlockScale bs = block_scale(row_umax(m));
+    i32x2 o;
+    o[0] = pack_e4m3(v[0], v[1], v[2], v[3], bs.inv);
+    o[1] = pack_e4m3(v[4], v[5], v[6], v[7], bs.inv);
+    *(i32x2*)(p.q + row * p.ldq + c0) = o;
+    if (lane == 0) p.s[kb * p.lds + row] = bs.s;
+  }
+}
+
+// A 128 x 128 tile a workgroup: read once, quantised along its rows (ROWS), its
+// columns (COLS, written transposed through LDS) or both, or as one square
+// block (SQUARE, whose transpose has the same values and scales).
+// Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's
+// maximum is over the 16 lanes of a DPP row, a column's over the four DPP rows
+// of a wave and then the four waves.
+template <class T, bool WIDE, bool ROWS, bool COLS, bool SQUARE>
+__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs p) {
+  __shared__ __align__(16) uint8_t tile[COLS ? kBlock * (kBlock + 16) : 16];
+  __shared__ uint32_t part[4 * kBlock];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 4, c = tid & 15;
+  const int64_t kb = blockIdx.x, rb = blockIdx.y;
+  const int64_t r0 = rb * kBlock + r * 8, c0 = kb * kBlock + c * 8;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const T* x = (const T*)p.x + (r0 + i) * p.sr;
+    if (WIDE && r0 + i < p.rows && c0 + 8 <= p.cols) {
+      load_vec(x + c0, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = r0 + i < p.rows && c0 + j < p.cols ? (float)x[(c0 + j) * p.sc] : 0.0f;
+    }
+  }
+  if (SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
+    m = row_umax(m);
+    if ((lane & 15) == 0) part[wave * 4 + (lane >> 4)] = m;
+    __syncthreads();
+    m = part[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = umax(m, part[i]);
+    const BlockScale bs = block_scale(m);
+    if (tid == 0) p.s[rb * p.lds + kb] = bs.s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      i32x2 o;
+      o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], bs.inv);
+      o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], bs.inv);
+      if (r0 + i < p.rows) *(i32x2*)(p.q + (r0 + i) * p.ldq + c0) = o;
+    }
+    if (COLS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        i32x2 o;
+        o[0] = pack_e4m3(v[0][j], v[1][j], v[2][j], v[3][j], bs.inv);
+        o[1] = pack_e4m3(v[4][j], v[5][j], v[6][j], v[7][j], bs.inv);
+        *(i32x2*)(tile + (c * 8 + j) * (kBlock + 16) + r * 8) = o;
+      }
+    }
+  } else {
+    if (ROWS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t m = abs_bits(v[i][0]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
+        const BlockScale bs = block_scale(row_umax(m));
+        i32x2 o;
+        o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], bs.inv);
+        o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], bs.inv);
+        if (r0 + i < p.rows) {
+          *(i32x2*)(p.q + (r0 + i) * p.ldq + c0) = o;
+          if (c == 0) p.s[kb * p.lds + r0 + i] = bs.s;
+        }
+      }
+    }
+    if (COLS) {
+      uint32_t m[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m[j] = abs_bits(v[0][j]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m[j] = umax(m[j], abs_bits(v[i][j]));
+        m[j] = umax(m[j], (uint32_t)__shfl_xor((int)m[j], 16));
+        m[j] = umax(m[j], (uint32_t)__shfl_xor((int)m[j], 32));
+        if (lane < 16) part[wave * kBlock + c * 8 + j] = m[j];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int col = c * 8 + j;
+        const BlockScale bs =
+            block_scale(umax(umax(part[col], part[kBlock + col]), umax(part[2 * kBlock + col], part[3 * kBlock + col])));
+        i32x2 o;
+        o[0] = pack_e4m3(v[0][j], v[1][j], v[2][j], v[3][j], bs.inv);
+        o[1] = pack_e4m3(v[4][j], v[5][j], v[6][j], v[7][j], bs.inv);
+        *(i32x2*)(tile + col * (kBlock + 16) + r * 8) = o;
+        if (r == 0 && c0 + j < p.cols) p.st[rb * p.ldst + c0 + j] = bs.s;
+      }
+    }
+  }
+  if (COLS) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int col = k * 32 + (tid >> 3), u = tid & 7;
+      if (kb * kBlock + col < p.cols)
+        *(i32x4*)(p.qt + (kb * kBlock + col) * p.ldqt + rb * kBlock + u * 16) =
+            *(const i32x4*)(tile + col * (kBlock + 16) + u * 16);
+    }
+  }
+}
+
+// dst[r][c] = src[r * s_r + c * s_c] for c < cols, zero up to ld (a multiple of
+// 16): 8-bit rows of any strides laid out as the products read them.
+struct Pack8Args {
+  const uint8_t* src;
+  uint8_t* dst;
+  int64_t rows, cols, s_r, s_c, ld;
+};
+__global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) {
+  const int64_t units = p.ld / 16, total = p.rows * units;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / units, c = (i - r * units) * 16;
+    const uint8_t* s = p.src + r * p.s_r;
+    union {
+      uint8_t b[16];
+      i32x4 v;
+    } o;
+    if (p.s_c == 1 && c + 16 <= p.cols) {
+      __builtin_memcpy(o.b, s + c, 16);  // one 16-byte load: any alignment goes
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o.b[k] = c + k < p.cols ? s[(c + k) * p.s_c] : 0;
+    }
+    *(i32x4*)(p.dst + r * p.ld + c) = o.v;
+  }
+}
+
+}  // namespace f16ops
