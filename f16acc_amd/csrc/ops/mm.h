@@ -110,7 +110,7 @@ struct MmKernel {
   static constexpr int LOADS = C::LX + C::LW + 1 + LSW;
   static constexpr bool GATED = EPI == kGatedQuant;
   static constexpr int BN_OUT = GATED ? C::BN / 2 : C::BN;  // columns of the result
-  static_assert((C::NS - 2) * LOADS <= 63, "outstanding copies must fit vmcnt");
+  static_assert((C::NS - 1) * LOADS <= 63, "outstanding copies must fit vmcnt");
 
   // Where a lane's copies read.
   struct Loader {
@@ -219,7 +219,7 @@ struct MmKernel {
     return j < C::FN / 2 ? wn * (C::TN / 2) + 16 * j : C::BN / 2 + wn * (C::TN / 2) + 16 * (j - C::FN / 2);
   }
 
-  __device__ static void run(const MmArgs& p, char LDS_AS* lds) {
+  __device__ static __forceinline__ void run(const MmArgs& p, char LDS_AS* lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN, t16 = lane & 15, g = lane >> 4;
     int64_t m0, n0;
@@ -260,58 +260,104 @@ struct MmKernel {
       for (int j = 0; j < C::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-    for (int s = 0; s < C::NS - 1; ++s) issue(l, s, lds0 + s * STAGE, wave);
+    for (int s = 0; s < C::NS; ++s) issue(l, s, lds0 + s * STAGE, wave);
 
     // the weight block's scale: one value per wave (two where it is gated)
     const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
     const int64_t nb_last = cdiv(p.N, kBlock) - 1;
     const float* swp = sw + (nb < nb_last ? nb : nb_last) * p.swn;
 
-    int slot = 0, next = C::NS - 1;
+    // A wave's addresses in a stage; the fragments of an operand lie 16 rows apart.
+    const int frag = t16 * kBlock, lo = (g ^ swz(t16)) << 4, hi = ((g + 4) ^ swz(t16)) << 4;
+    const int xa = wm * C::TM * kBlock + frag, wa = C::X_BYTES + frag;
+    const int sa = C::X_BYTES + C::W_BYTES + (wm * C::TM + t16) * 4;
+
+    auto read = [&](int at) {
+      const i32x4 a = *(const i32x4 LDS_AS*)(lds + at + lo), b = *(const i32x4 LDS_AS*)(lds + at + hi);
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    i32x8 xf[C::FM], wf[2];
+    float s[C::FM], sb = 0.0f, sb2 = 0.0f;
+    f32x4 sr[4];
+
+    wait_vm<(C::NS - 1) * LOADS>();
+    barrier();
+    int slot = 0;
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+      xf[i] = read(xa + 16 * i * kBlock);
+      s[i] = *(const float LDS_AS*)(lds + sa + 64 * i);
+    }
+    wf[0] = read(wa + w_row(wn, 0) * kBlock);
+    if (ROW_SCALES) sr[0] = *(const f32x4 LDS_AS*)(lds + C::X_BYTES + C::W_BYTES + C::S_BYTES + (w_row(wn, 0) + 4 * g) * 4);
+    if (!ROW_SCALES) {
+      sb = swp[0];
+      if (GATED) sb2 = swp[p.sup];
+    }
+
     for (int kb = 0; kb < l.nk; ++kb) {
-      float sb = 0.0f, sb2 = 0.0f;
-      if (!ROW_SCALES) {
-        sb = swp[kb * p.swk];
-        if (GATED) sb2 = swp[p.sup + kb * p.swk];
-      }
-      wait_vm<(C::NS - 2) * LOADS>();
-      barrier();
-      issue(l, kb + C::NS - 1, lds0 + next * STAGE, wave);
-      const char LDS_AS* xs = lds + slot * STAGE;
-      const char LDS_AS* ws = xs + C::X_BYTES;
-      const float LDS_AS* ss = (const float LDS_AS*)(ws + C::W_BYTES);
-      i32x8 xf[C::FM];
-      float s[C::FM];
+      const int at = slot * STAGE, nslot = slot + 1 == C::NS ? 0 : slot + 1, nat = nslot * STAGE;
+      // products of the two scales
+      float sc[C::FM], sc2[GATED ? C::FM : 1];
 #pragma unroll
       for (int i = 0; i < C::FM; ++i) {
-        xf[i] = read_frag(xs, wm * C::TM + 16 * i + t16, g);
-        s[i] = ss[wm * C::TM + 16 * i + t16];
+        sc[i] = ROW_SCALES ? s[i] : s[i] * sb;
+        if (GATED) sc2[i] = s[i] * sb2;
       }
+      if (!ROW_SCALES && kb + 1 < l.nk) {
+        sb = swp[(kb + 1) * p.swk];
+        if (GATED) sb2 = swp[p.sup + (kb + 1) * p.swk];
+      }
+      f32x4 part[4];
+      auto finish = [&](int t) {
+        const int i = t % C::FM, j = t / C::FM;
+        const f32x4& v = part[t % 4];
+        if (ROW_SCALES) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], sc[i] * sr[j % 4][r], acc[i][j][r]);
+        } else {
+          const float f = GATED && j >= C::FN / 2 ? sc2[i] : sc[i];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], f, acc[i][j][r]);
+        }
+      };
 #pragma unroll
       for (int j = 0; j < C::FN; ++j) {
-        const int row = w_row(wn, j);
-        const i32x8 wf = read_frag(ws, row + t16, g);
-        if (ROW_SCALES) {
-          const f32x4 sr = *(const f32x4 LDS_AS*)(ss + C::THREADS + row + 4 * g);
+        if (j == C::FN - 1) {
+          // This wave has read all of this stage: once every wave has, and the next
+          // stage has landed, the copies of the stage after them may begin.
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          wait_vm<(C::NS - 2) * LOADS>();
+          barrier();
+          issue(l, kb + C::NS, lds0 + at, wave);
+        }
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i) {
-            const f32x4 part = mfma(wf, xf[i]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], s[i] * sr[r], acc[i][j][r]);
+        for (int i = 0; i < C::FM; ++i) {
+          const int t = j * C::FM + i;
+          part[t % 4] = mfma(wf[j & 1], xf[i]);
+          if (j < C::FN - 1) {
+            if (i == 0) {
+              wf[(j + 1) & 1] = read(at + wa + w_row(wn, j + 1) * kBlock);
+              if (ROW_SCALES)
+                sr[(j + 1) % 4] = *(const f32x4 LDS_AS*)(lds + at + C::X_BYTES + C::W_BYTES + C::S_BYTES +
+                                                         (w_row(wn, j + 1) + 4 * g) * 4);
+            }
+          } else {
+            // the next stage's operands, each as soon as its register is free
+            xf[i] = read(nat + xa + 16 * i * kBlock);
+            s[i] = *(const float LDS_AS*)(lds + nat + sa + 64 * i);
           }
-        } else {
-          const float b = GATED && j >= C::FN / 2 ? sb2 : sb;
-#pragma unroll
-          for (int i = 0; i < C::FM; ++i) {
-            const f32x4 part = mfma(wf, xf[i]);
-            const float sc = s[i] * b;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[r], sc, acc[i][j][r]);
-          }
+          if (t >= 2) finish(t - 2);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      slot = slot + 1 == C::NS ? 0 : slot + 1;
-      next = next + 1 == C::NS ? 0 : next + 1;
+      constexpr int T = C::FM * C::FN;
+      if (T >= 2) finish(T - 2);
+      finish(T - 1);
+      wf[0] = read(nat + wa + w_row(wn, 0) * kBlock);
+      if (ROW_SCALES)
+        sr[0] = *(const f32x4 LDS_AS*)(lds + nat + C::X_BYTES + C::W_BYTES + C::S_BYTES + (w_row(wn, 0) + 4 * g) * 4);
+      slot = nslot;
     }
     wait_vm<0>();
     if (GATED)

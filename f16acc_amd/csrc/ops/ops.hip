@@ -92,7 +92,7 @@ int mm_check(const MmArgs& p) {
   return 0;
 }
 
-using Cfg256 = MmCfg<256, 256, 2, 2, 2, 1>;
+using Cfg256 = MmCfg<256, 256, 4, 2, 2, 2>;
 using Cfg128 = MmCfg<128, 128, 2, 2, 2, 2>;
 using Cfg64 = MmCfg<64, 64, 2, 2, 3, 2>;
 using Cfg32 = MmCfg<32, 64, 2, 2, 4, 2>;
