@@ -173,43 +173,56 @@ struct MmKernel {
     return q;
   }
 
-  // Issues the copies of K block kb into the stage at `slot`.  Past the last
-  // block every unit reads zeros.
-  __device__ static __forceinline__ void issue(const Loader& l, int kb, int slot, int wave) {
+  // The copies of K block kb into the stage at `slot`, one by one: unit(0) .. unit(LOADS - 1).
+  // Past the last block every unit reads zeros.
+  struct Stage {
+    i32x4 xr, wr, ur, sr, swr;
+    int x_off, w_off, s_off;  // this lane's offsets, kOob past K
+    bool in, any;
+    int base, sbase;
+    const Loader* l;
+    __device__ __forceinline__ void unit(int j) const {
+      constexpr int STEP = C::THREADS * 16;
+      if (j < C::LX) {
+        if (EXPERTS)
+          lds_dma16(xr, base + j * STEP, in ? l->x_off[j] : kOob);
+        else
+          lds_dma16(srd_at(xr, j * l->x_step), base + j * STEP, x_off);
+      } else if (j < C::LX + C::LW) {
+        const int k = j - C::LX;
+        if (GATED && k >= C::LW / 2)
+          lds_dma16(srd_at(ur, (k - C::LW / 2) * l->w_step), base + C::X_BYTES + k * STEP, w_off);
+        else
+          lds_dma16(srd_at(wr, k * l->w_step), base + C::X_BYTES + k * STEP, w_off);
+      } else if (j == C::LX + C::LW) {
+        lds_dma4(sr, sbase, s_off);
+      } else if (ROW_SCALES) {
+        const int k = j - C::LX - C::LW - 1;
+        lds_dma4(swr, sbase + C::S_BYTES * (1 + k), any ? l->sw_off[k] : kOob);
+      }
+    }
+    __device__ __forceinline__ void all() const {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) unit(j);
+    }
+  };
+  __device__ static __forceinline__ Stage stage(const Loader& l, int kb, int slot, int wave) {
     const int left = kb < l.nk - 1 ? kBlock : kb == l.nk - 1 ? l.krest : 0;
-    const bool in = l.u < left;
-    const int base = slot + wave * 1024;
-    const i32x4 xr = advanced(l.xr, (int64_t)kb * kBlock), wr = advanced(l.wr, (int64_t)kb * kBlock);
-    if (EXPERTS) {
-#pragma unroll
-      for (int j = 0; j < C::LX; ++j) lds_dma16(xr, base + j * C::THREADS * 16, in ? l.x_off[j] : kOob);
-    } else {
-      const int off = in ? l.x_off[0] : kOob;
-#pragma unroll
-      for (int j = 0; j < C::LX; ++j) lds_dma16(srd_at(xr, j * l.x_step), base + j * C::THREADS * 16, off);
-    }
-    const int off = in ? l.w_off : kOob;
-    if (GATED) {
-      const i32x4 ur = advanced(l.ur, (int64_t)kb * kBlock);
-#pragma unroll
-      for (int j = 0; j < C::LW / 2; ++j)
-        lds_dma16(srd_at(wr, j * l.w_step), base + C::X_BYTES + j * C::THREADS * 16, off);
-#pragma unroll
-      for (int j = 0; j < C::LW / 2; ++j)
-        lds_dma16(srd_at(ur, j * l.w_step), base + C::X_BYTES + (C::LW / 2 + j) * C::THREADS * 16, off);
-    } else {
-#pragma unroll
-      for (int j = 0; j < C::LW; ++j)
-        lds_dma16(srd_at(wr, j * l.w_step), base + C::X_BYTES + j * C::THREADS * 16, off);
-    }
-    const int sbase = slot + C::X_BYTES + C::W_BYTES + wave * 256;
-    lds_dma4(advanced(l.sr, kb * l.sxk), sbase, left ? l.s_off : kOob);
-    if (ROW_SCALES) {
-      const i32x4 swr = advanced(l.swr, kb * l.swk);
-#pragma unroll
-      for (int j = 0; j < LSW; ++j)
-        lds_dma4(swr, sbase + C::S_BYTES * (1 + j), left ? l.sw_off[j] : kOob);
-    }
+    Stage st;
+    st.in = l.u < left;
+    st.any = left != 0;
+    st.xr = advanced(l.xr, (int64_t)kb * kBlock);
+    st.wr = advanced(l.wr, (int64_t)kb * kBlock);
+    if (GATED) st.ur = advanced(l.ur, (int64_t)kb * kBlock);
+    st.sr = advanced(l.sr, kb * l.sxk);
+    if (ROW_SCALES) st.swr = advanced(l.swr, kb * l.swk);
+    st.x_off = st.in ? l.x_off[0] : kOob;
+    st.w_off = st.in ? l.w_off : kOob;
+    st.s_off = st.any ? l.s_off : kOob;
+    st.base = slot + wave * 1024;
+    st.sbase = slot + C::X_BYTES + C::W_BYTES + wave * 256;
+    st.l = &l;
+    return st;
   }
 
   // Row of fragment j of the wave's weights in the staged tile.  Gated: the
@@ -260,7 +273,7 @@ struct MmKernel {
       for (int j = 0; j < C::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-    for (int s = 0; s < C::NS; ++s) issue(l, s, lds0 + s * STAGE, wave);
+    for (int s = 0; s < C::NS; ++s) stage(l, s, lds0 + s * STAGE, wave).all();
 
     // the weight block's scale: one value per wave (two where it is gated)
     const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
@@ -276,7 +289,10 @@ struct MmKernel {
       const i32x4 a = *(const i32x4 LDS_AS*)(lds + at + lo), b = *(const i32x4 LDS_AS*)(lds + at + hi);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    i32x8 xf[C::FM], wf[2];
+    constexpr int AHEAD = C::FN >= 4 ? 2 : 1, RING = AHEAD == 2 ? 4 : 2;  // fragments of w read ahead
+    static_assert(C::FN % RING == 0, "a stage starts with the ring's first slot");
+    static_assert(!ROW_SCALES || (RING == 4 && C::FM >= 2), "row scales are read AHEAD of their last use");
+    i32x8 xf[C::FM], wf[RING];
     float s[C::FM], sb = 0.0f, sb2 = 0.0f;
     f32x4 sr[4];
 
@@ -288,8 +304,14 @@ struct MmKernel {
       xf[i] = read(xa + 16 * i * kBlock);
       s[i] = *(const float LDS_AS*)(lds + sa + 64 * i);
     }
-    wf[0] = read(wa + w_row(wn, 0) * kBlock);
-    if (ROW_SCALES) sr[0] = *(const f32x4 LDS_AS*)(lds + C::X_BYTES + C::W_BYTES + C::S_BYTES + (w_row(wn, 0) + 4 * g) * 4);
+    auto read_w = [&](int base, int j) {
+      wf[j % RING] = read(base + wa + w_row(wn, j) * kBlock);
+      if (ROW_SCALES)
+        sr[j % 4] =
+            *(const f32x4 LDS_AS*)(lds + base + C::X_BYTES + C::W_BYTES + C::S_BYTES + (w_row(wn, j) + 4 * g) * 4);
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) read_w(0, j);
     if (!ROW_SCALES) {
       sb = swp[0];
       if (GATED) sb2 = swp[p.sup];
@@ -308,6 +330,7 @@ struct MmKernel {
         sb = swp[(kb + 1) * p.swk];
         if (GATED) sb2 = swp[p.sup + (kb + 1) * p.swk];
       }
+      const Stage next = stage(l, kb + C::NS, lds0 + at, wave);
       f32x4 part[4];
       auto finish = [&](int t) {
         const int i = t % C::FM, j = t / C::FM;
@@ -323,29 +346,27 @@ struct MmKernel {
       };
 #pragma unroll
       for (int j = 0; j < C::FN; ++j) {
-        if (j == C::FN - 1) {
+        if (j == C::FN - AHEAD) {
           // This wave has read all of this stage: once every wave has, and the next
           // stage has landed, the copies of the stage after them may begin.
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           wait_vm<(C::NS - 2) * LOADS>();
           barrier();
-          issue(l, kb + C::NS, lds0 + at, wave);
         }
 #pragma unroll
         for (int i = 0; i < C::FM; ++i) {
           const int t = j * C::FM + i;
-          part[t % 4] = mfma(wf[j & 1], xf[i]);
-          if (j < C::FN - 1) {
-            if (i == 0) {
-              wf[(j + 1) & 1] = read(at + wa + w_row(wn, j + 1) * kBlock);
-              if (ROW_SCALES)
-                sr[(j + 1) % 4] = *(const f32x4 LDS_AS*)(lds + at + C::X_BYTES + C::W_BYTES + C::S_BYTES +
-                                                         (w_row(wn, j + 1) + 4 * g) * 4);
-            }
-          } else {
-            // the next stage's operands, each as soon as its register is free
+          part[t % 4] = mfma(wf[j % RING], xf[i]);
+          if (i == 0) read_w(j < C::FN - AHEAD ? at : nat, (j + AHEAD) % C::FN);
+          if (j == C::FN - 1) {  // the next stage's tokens, each as soon as its register is free
             xf[i] = read(nat + xa + 16 * i * kBlock);
             s[i] = *(const float LDS_AS*)(lds + nat + sa + 64 * i);
+          }
+          if (j >= C::FN - AHEAD) {  // the copies, spread over the steps after the barrier
+            constexpr int STEPS = AHEAD * C::FM;
+            const int u = t - (C::FN - AHEAD) * C::FM;
+#pragma unroll
+            for (int k = u * LOADS / STEPS; k < (u + 1) * LOADS / STEPS; ++k) next.unit(k);
           }
           if (t >= 2) finish(t - 2);
           __builtin_amdgcn_sched_barrier(0);
@@ -354,9 +375,6 @@ struct MmKernel {
       constexpr int T = C::FM * C::FN;
       if (T >= 2) finish(T - 2);
       finish(T - 1);
-      wf[0] = read(nat + wa + w_row(wn, 0) * kBlock);
-      if (ROW_SCALES)
-        sr[0] = *(const f32x4 LDS_AS*)(lds + nat + C::X_BYTES + C::W_BYTES + C::S_BYTES + (w_row(wn, 0) + 4 * g) * 4);
       slot = nslot;
     }
     wait_vm<0>();

@@ -94,7 +94,7 @@ int mm_check(const MmArgs& p) {
 
 using Cfg256 = MmCfg<256, 256, 4, 2, 2, 2>;
 using Cfg128 = MmCfg<128, 128, 2, 2, 2, 2>;
-using Cfg64 = MmCfg<64, 64, 2, 2, 3, 2>;
+using Cfg64 = MmCfg<64, 64, 2, 1, 3, 2>;
 using Cfg32 = MmCfg<32, 64, 2, 2, 4, 2>;
 
 template <bool ROW_SCALES>
@@ -103,7 +103,9 @@ int mm_pick(const MmArgs& p, hipStream_t stream) {
     using C = std::remove_pointer_t<decltype(c)>;
     return launch_mm<C, ROW_SCALES, false, kStore>(p, cdiv(p.M, C::BM), stream);
   };
-  if (p.M <= 32) return run((Cfg32*)nullptr);
+  if constexpr (!ROW_SCALES) {
+    if (p.M <= 32) return run((Cfg32*)nullptr);
+  }
   if (cdiv(p.M, 256) * cdiv(p.N, 256) >= kCus / 2) return run((Cfg256*)nullptr);
   if (cdiv(p.M, 128) * cdiv(p.N, 128) >= kCus / 2) return run((Cfg128*)nullptr);
   return run((Cfg64*)nullptr);
