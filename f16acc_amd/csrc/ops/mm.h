@@ -35,6 +35,10 @@ struct MmArgs {
   int64_t scm, scn;
   int64_t M, N, K;
   int ctype;
+  // A split of K: workgroups (blockIdx.y) take ksplit blocks each and write FP32
+  // sums to parts[split][M][N]; 0: not split.
+  int ksplit;
+  float* parts;
   // Experts: the tile list (expert, first slot, end slot, -) and its length, the
   // token row of each slot (NULL: the slot itself), the strides between experts.
   const int4* tiles;
@@ -58,9 +62,13 @@ struct MmCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, OCC = OCC_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  static constexpr int LX = BM * 8 / THREADS, LW = BN * 8 / THREADS;  // 16-byte copies per lane and stage
+  // 16-byte copies per lane and stage; where BN is not whole copies, the first
+  // LW_LAST waves make one more
+  static constexpr int LX = BM * 8 / THREADS, LW = (BN * 8 + THREADS - 1) / THREADS;
+  static constexpr int LW_LAST = BN * 8 % THREADS / 64;
   static constexpr int X_BYTES = BM * kBlock, W_BYTES = BN * kBlock, S_BYTES = THREADS * 4;
-  static_assert(LX * THREADS == BM * 8 && LW * THREADS == BN * 8, "whole copies");
+  static_assert(LX * THREADS == BM * 8 && BN * 8 % 64 == 0, "whole copies");
+  static_assert(LW_LAST == 0 || NS == 2, "waves with unequal copies wait for all of them");
   static_assert(BM <= THREADS, "one scale copy per stage covers the tokens");
   static_assert(THREADS / 8 % 16 == 0, "a lane's units keep the swizzle phase");
   static constexpr int stage_bytes(bool row_scales) {
@@ -109,6 +117,8 @@ struct MmKernel {
   static constexpr int LSW = ROW_SCALES ? (C::BN + C::THREADS - 1) / C::THREADS : 0;
   static constexpr int LOADS = C::LX + C::LW + 1 + LSW;
   static constexpr bool GATED = EPI == kGatedQuant;
+  static constexpr bool TWO = GATED || (!ROW_SCALES && kBlock % C::TN != 0);  // two weight scales per wave
+  static_assert(GATED || C::TN <= kBlock + 16, "at most two blocks a wave");
   static constexpr int BN_OUT = GATED ? C::BN / 2 : C::BN;  // columns of the result
   static_assert((C::NS - 1) * LOADS <= 63, "outstanding copies must fit vmcnt");
 
@@ -120,15 +130,21 @@ struct MmKernel {
     int sw_off[ROW_SCALES ? LSW : 1];
     i32x4 xr, wr, ur, sr, swr;
     int64_t sxk, swk;
-    int nk, krest;
+    int k0, nk, last, krest;  // blocks k0 .. nk - 1 of K; the last block and its length
   };
 
   __device__ static __forceinline__ void init(Loader& l, const MmArgs& p, int64_t m0, int m_left, int64_t n0,
                                               const uint8_t* w, const float* sw, int tid) {
     const int row = tid >> 3, u = (tid & 7) ^ swz(row);
     l.u = u * 16;
-    l.nk = (int)cdiv(p.K, kBlock);
-    l.krest = (int)(p.K - (int64_t)(l.nk - 1) * kBlock);
+    l.last = (int)cdiv(p.K, kBlock) - 1;
+    l.krest = (int)(p.K - (int64_t)l.last * kBlock);
+    l.k0 = 0;
+    l.nk = l.last + 1;
+    if (!EXPERTS && p.ksplit) {
+      l.k0 = (int)blockIdx.y * p.ksplit;
+      l.nk = l.k0 + p.ksplit < l.nk ? l.k0 + p.ksplit : l.nk;
+    }
     l.x_step = (int)(C::THREADS / 8 * p.ldx);
     l.w_step = (int)(C::THREADS / 8 * p.ldw);
     l.w_off = (int)(row * p.ldw) + l.u;
@@ -179,7 +195,7 @@ struct MmKernel {
     i32x4 xr, wr, ur, sr, swr;
     int x_off, w_off, s_off;  // this lane's offsets, kOob past K
     bool in, any;
-    int base, sbase;
+    int base, sbase, wave;
     const Loader* l;
     __device__ __forceinline__ void unit(int j) const {
       constexpr int STEP = C::THREADS * 16;
@@ -192,7 +208,7 @@ struct MmKernel {
         const int k = j - C::LX;
         if (GATED && k >= C::LW / 2)
           lds_dma16(srd_at(ur, (k - C::LW / 2) * l->w_step), base + C::X_BYTES + k * STEP, w_off);
-        else
+        else if (C::LW_LAST == 0 || k < C::LW - 1 || wave < C::LW_LAST)
           lds_dma16(srd_at(wr, k * l->w_step), base + C::X_BYTES + k * STEP, w_off);
       } else if (j == C::LX + C::LW) {
         lds_dma4(sr, sbase, s_off);
@@ -207,7 +223,7 @@ struct MmKernel {
     }
   };
   __device__ static __forceinline__ Stage stage(const Loader& l, int kb, int slot, int wave) {
-    const int left = kb < l.nk - 1 ? kBlock : kb == l.nk - 1 ? l.krest : 0;
+    const int left = kb >= l.nk ? 0 : kb == l.last ? l.krest : kBlock;
     Stage st;
     st.in = l.u < left;
     st.any = left != 0;
@@ -221,6 +237,7 @@ struct MmKernel {
     st.s_off = st.any ? l.s_off : kOob;
     st.base = slot + wave * 1024;
     st.sbase = slot + C::X_BYTES + C::W_BYTES + wave * 256;
+    st.wave = wave;
     st.l = &l;
     return st;
   }
@@ -273,12 +290,15 @@ struct MmKernel {
       for (int j = 0; j < C::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
-    for (int s = 0; s < C::NS; ++s) stage(l, s, lds0 + s * STAGE, wave).all();
+    for (int s = 0; s < C::NS; ++s) stage(l, l.k0 + s, lds0 + s * STAGE, wave).all();
 
-    // the weight block's scale: one value per wave (two where it is gated)
+    // The weight blocks' scales: a wave's rows lie in one block or two, fragments
+    // from `jb` on in the second.  Gated: the gate's and the up's.
     const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
     const int64_t nb_last = cdiv(p.N, kBlock) - 1;
     const float* swp = sw + (nb < nb_last ? nb : nb_last) * p.swn;
+    const int64_t second = GATED ? p.sup : nb < nb_last ? p.swn : 0;
+    const int jb = GATED ? C::FN / 2 : (int)(kBlock - (n0 + wn * C::TN) % kBlock) / 16;
 
     // A wave's addresses in a stage; the fragments of an operand lie 16 rows apart.
     const int frag = t16 * kBlock, lo = (g ^ swz(t16)) << 4, hi = ((g + 4) ^ swz(t16)) << 4;
@@ -289,7 +309,7 @@ struct MmKernel {
       const i32x4 a = *(const i32x4 LDS_AS*)(lds + at + lo), b = *(const i32x4 LDS_AS*)(lds + at + hi);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    constexpr int AHEAD = C::FN >= 4 ? 2 : 1, RING = AHEAD == 2 ? 4 : 2;  // fragments of w read ahead
+    constexpr int AHEAD = C::FN > 2 ? 2 : 1, RING = AHEAD == 1 ? 2 : C::FN % 4 ? 3 : 4;  // fragments of w read ahead
     static_assert(C::FN % RING == 0, "a stage starts with the ring's first slot");
     static_assert(!ROW_SCALES || (RING == 4 && C::FM >= 2), "row scales are read AHEAD of their last use");
     i32x8 xf[C::FM], wf[RING];
@@ -313,33 +333,34 @@ struct MmKernel {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) read_w(0, j);
     if (!ROW_SCALES) {
-      sb = swp[0];
-      if (GATED) sb2 = swp[p.sup];
+      sb = swp[l.k0 * p.swk];
+      if (TWO) sb2 = swp[second + l.k0 * p.swk];
     }
 
-    for (int kb = 0; kb < l.nk; ++kb) {
+    int kb = l.k0;
+    do {
       const int at = slot * STAGE, nslot = slot + 1 == C::NS ? 0 : slot + 1, nat = nslot * STAGE;
       // products of the two scales
-      float sc[C::FM], sc2[GATED ? C::FM : 1];
+      float sc[C::FM], sc2[TWO ? C::FM : 1];
 #pragma unroll
       for (int i = 0; i < C::FM; ++i) {
         sc[i] = ROW_SCALES ? s[i] : s[i] * sb;
-        if (GATED) sc2[i] = s[i] * sb2;
+        if (TWO) sc2[i] = s[i] * sb2;
       }
       if (!ROW_SCALES && kb + 1 < l.nk) {
         sb = swp[(kb + 1) * p.swk];
-        if (GATED) sb2 = swp[p.sup + (kb + 1) * p.swk];
+        if (TWO) sb2 = swp[second + (kb + 1) * p.swk];
       }
       const Stage next = stage(l, kb + C::NS, lds0 + at, wave);
-      f32x4 part[4];
+      f32x4 part[3];
       auto finish = [&](int t) {
         const int i = t % C::FM, j = t / C::FM;
-        const f32x4& v = part[t % 4];
+        const f32x4& v = part[t % 3];
         if (ROW_SCALES) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], sc[i] * sr[j % 4][r], acc[i][j][r]);
         } else {
-          const float f = GATED && j >= C::FN / 2 ? sc2[i] : sc[i];
+          const float f = TWO && j >= (GATED ? C::FN / 2 : jb) ? sc2[i] : sc[i];
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], f, acc[i][j][r]);
         }
@@ -356,7 +377,8 @@ struct MmKernel {
 #pragma unroll
         for (int i = 0; i < C::FM; ++i) {
           const int t = j * C::FM + i;
-          part[t % 4] = mfma(wf[j % RING], xf[i]);
+          part[t % 3] = mfma(wf[j % RING], xf[i]);
+          __builtin_amdgcn_sched_barrier(0);
           if (i == 0) read_w(j < C::FN - AHEAD ? at : nat, (j + AHEAD) % C::FN);
           if (j == C::FN - 1) {  // the next stage's tokens, each as soon as its register is free
             xf[i] = read(nat + xa + 16 * i * kBlock);
@@ -376,38 +398,111 @@ struct MmKernel {
       if (T >= 2) finish(T - 2);
       finish(T - 1);
       slot = nslot;
-    }
+    } while (++kb < l.nk);
     wait_vm<0>();
-    if (GATED)
-      store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
-    else if (p.ctype == F16ACC_TYPE_F16)
-      store<f16>(p, acc, m0, m_left, n0, wm, wn, t16, g);
-    else if (p.ctype == F16ACC_TYPE_BF16)
-      store<bf16>(p, acc, m0, m_left, n0, wm, wn, t16, g);
-    else
-      store<float>(p, acc, m0, m_left, n0, wm, wn, t16, g);
+    // opaque, or the compiler forms the stores' addresses before the loop and
+    // holds (256 x 256: spills) them through it
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    store_all(p, lds, acc, m0, m_left, n0, wave, wm, wn, ln & 15, ln >> 4);
   }
 
+  __device__ static __forceinline__ void store_all(const MmArgs& p, char LDS_AS* lds, f32x4 (&acc)[C::FM][C::FN],
+                                                   int64_t m0, int m_left, int64_t n0, int wave, int wm, int wn,
+                                                   int t16, int g) {
+    if (GATED) {
+      store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
+    } else if (!EXPERTS && p.ksplit) {
+      MmArgs q = p;
+      q.c = p.parts + (int64_t)blockIdx.y * p.M * p.N;
+      q.scm = p.N, q.scn = 1, q.bias = nullptr;
+      store<float>(q, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+    } else if (p.ctype == F16ACC_TYPE_F16)
+      store<f16>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+    else if (p.ctype == F16ACC_TYPE_BF16)
+      store<bf16>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+    else
+      store<float>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+  }
+
+  // The wave's sums plus the bias, rounded once.  A lane's four consecutive
+  // columns of one token would go out as 8 bytes in every row of 16: 4096 x 4096 x
+  // 128 in bfloat16 took 30 us that way.  So 16 tokens at a time pass through LDS and
+  // leave as 16-byte units of whole row pieces (TN columns), at any alignment.
   template <class T>
-  __device__ static __forceinline__ void store(const MmArgs& p, f32x4 (&acc)[C::FM][C::FN], int64_t m0, int m_left,
-                                               int64_t n0, int wm, int wn, int t16, int g) {
-    const bool wide = p.scn == 1 && p.scm % 4 == 0 && (uintptr_t)p.c % (4 * sizeof(T)) == 0;
+  __device__ static __forceinline__ void store(const MmArgs& p, char LDS_AS* lds, f32x4 (&acc)[C::FM][C::FN],
+                                               int64_t m0, int m_left, int64_t n0, int wave, int wm, int wn, int t16,
+                                               int g) {
+    const int64_t nw = n0 + wn * C::TN;
+    if (p.bias) {
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j) {
-      const int64_t n = n0 + wn * C::TN + 16 * j + 4 * g;
-      const int left = (int)(p.N - n < 4 ? p.N - n : 4);
-      if (left <= 0) continue;
-      f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.bias) {
+      for (int j = 0; j < C::FN; ++j) {
+        const int64_t n = nw + 16 * j + 4 * g;
+        f32x4 b = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (r < left) b[r] = (float)((const T*)p.bias)[n + r];
-      }
+          if (n + r < p.N) b[r] = (float)((const T*)p.bias)[n + r];
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i) {
-        const int m = wm * C::TM + 16 * i + t16;
-        if (m < m_left) store4<T>((T*)p.c + (m0 + m) * p.scm + n * p.scn, p.scn, left, acc[i][j] + b, wide);
+        for (int i = 0; i < C::FM; ++i) acc[i][j] += b;
       }
+    }
+    if (p.scn != 1) {
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        const int64_t n = nw + 16 * j + 4 * g;
+        const int left = (int)(p.N - n < 4 ? p.N - n : 4);
+#pragma unroll
+        for (int i = 0; i < C::FM; ++i) {
+          const int m = wm * C::TM + 16 * i + t16;
+          if (m < m_left) store4<T>((T*)p.c + (m0 + m) * p.scm + n * p.scn, p.scn, left, acc[i][j], false);
+        }
+      }
+      return;
+    }
+    constexpr int E = 16 / sizeof(T), UNITS = C::TN / E, ROW = C::TN * sizeof(T) + 16;
+    static_assert(C::WAVES * 16 * (C::TN * 4 + 16) <= STAGE * C::NS, "staging fits the ring");
+    struct __attribute__((packed, aligned(sizeof(T)))) Unit {
+      i32x4 v;
+    };
+    typedef int Four __attribute__((ext_vector_type(sizeof(T))));  // four values
+    char LDS_AS* area = lds + wave * 16 * ROW;
+    barrier();  // every wave has read its last stage
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        union {
+          T t[4];
+          Four v;
+        } f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f.t[r] = (T)acc[i][j][r];
+        *(Four LDS_AS*)(area + t16 * ROW + (16 * j + 4 * g) * (int)sizeof(T)) = f.v;
+      }
+      wave_sync();
+      const int lane = g * 16 + t16;
+#pragma unroll
+      for (int k = 0; k < 16 * UNITS / 64; ++k) {
+        const int row = (k * 64 + lane) / UNITS, u = (k * 64 + lane) % UNITS;
+        const int m = wm * C::TM + 16 * i + row;
+        const int64_t n = nw + u * E;
+        if (m >= m_left || n >= p.N) continue;
+        T* c = (T*)p.c + (m0 + m) * p.scm + n;
+        const i32x4 v = *(const i32x4 LDS_AS*)(area + row * ROW + u * 16);
+        if (n + E <= p.N) {
+          ((Unit*)c)->v = v;
+        } else {
+          union {
+            i32x4 v;
+            T t[E];
+          } e;
+          e.v = v;
+#pragma unroll
+          for (int r = 0; r < E; ++r)
+            if (n + r < p.N) c[r] = e.t[r];
+        }
+      }
+      wave_sync();
     }
   }
 
@@ -454,6 +549,40 @@ struct MmKernel {
   }
 };
 
+// The splits' sums, in split order, plus the bias, rounded once.
+struct FinishArgs {
+  const float* parts;
+  int64_t M, N, scm, scn;
+  int splits;
+  const void* bias;
+  void* c;
+};
+template <class T>
+__global__ __launch_bounds__(256) void mm_finish_kernel(FinishArgs p) {
+  const int64_t size = p.M * p.N;
+  if (p.N % 4 == 0) {
+    const bool wide = p.scn == 1 && p.scm % 4 == 0 && (uintptr_t)p.c % (4 * sizeof(T)) == 0;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
+      const int64_t m = i / p.N, n = i - m * p.N;
+      f32x4 v = *(const f32x4*)(p.parts + i);
+      for (int s = 1; s < p.splits; ++s) v += *(const f32x4*)(p.parts + s * size + i);
+      if (p.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += (float)((const T*)p.bias)[n + r];
+      }
+      store4<T>((T*)p.c + m * p.scm + n * p.scn, p.scn, 4, v, wide);
+    }
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+      const int64_t m = i / p.N, n = i - m * p.N;
+      float v = p.parts[i];
+      for (int s = 1; s < p.splits; ++s) v += p.parts[s * size + i];
+      if (p.bias) v += (float)((const T*)p.bias)[n];
+      ((T*)p.c)[m * p.scm + n * p.scn] = (T)v;
+    }
+  }
+}
+
 template <class C, bool ROW_SCALES, bool EXPERTS, int EPI>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void mm_kernel(MmArgs p) {
   using K = MmKernel<C, ROW_SCALES, EXPERTS, EPI>;
@@ -463,11 +592,12 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void mm_kernel(MmArgs p) {
 }
 
 template <class C, bool ROW_SCALES, bool EXPERTS, int EPI>
-int launch_mm(const MmArgs& p, int64_t max_tiles_m, hipStream_t stream) {
+int launch_mm(const MmArgs& p, int64_t max_tiles_m, hipStream_t stream, int splits = 1) {
   using K = MmKernel<C, ROW_SCALES, EXPERTS, EPI>;
   const int64_t tiles = max_tiles_m * cdiv(p.N, K::BN_OUT);
   if (tiles > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
-  hipLaunchKernelGGL((mm_kernel<C, ROW_SCALES, EXPERTS, EPI>), dim3((uint32_t)tiles), dim3(C::THREADS), 0, stream, p);
+  hipLaunchKernelGGL((mm_kernel<C, ROW_SCALES, EXPERTS, EPI>), dim3((uint32_t)tiles, (uint32_t)splits), dim3(C::THREADS),
+                     0, stream, p);
   return hip_status();
 }
 

@@ -82,7 +82,7 @@ int quant_tile(const QuantArgs& p, int type, hipStream_t stream) {
 int mm_check(const MmArgs& p) {
   if (p.M < 0 || p.N < 0 || p.K < 0 || p.ctype < 0 || p.ctype > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
   if (p.M == 0 || p.N == 0) return 0;
-  if (!p.c || (p.K && (!p.x || !p.w || !p.sx || !p.sw))) return F16ACC_OPS_E_ARG;
+  if (p.K == 0 || !p.c || !p.x || !p.w || !p.sx || !p.sw) return F16ACC_OPS_E_ARG;
   if (p.sxm < 0 || p.sxk < 0 || p.swn < 0 || p.swk < 0) return F16ACC_OPS_E_ARG;
   if (p.ldx % 16 || p.ldw % 16 || p.ldx < p.K || p.ldw < p.K || p.ldx > kMaxRow || p.ldw > kMaxRow ||
       !aligned16(p.x) || !aligned16(p.w))
@@ -92,23 +92,80 @@ int mm_check(const MmArgs& p) {
   return 0;
 }
 
-using Cfg256 = MmCfg<256, 256, 4, 2, 2, 2>;
-using Cfg128 = MmCfg<128, 128, 2, 2, 2, 2>;
-using Cfg64 = MmCfg<64, 64, 2, 1, 3, 2>;
-using Cfg32 = MmCfg<32, 64, 2, 2, 4, 2>;
+// The tiles of one product (F16ACC_FP8_TILE_*): tokens x weight rows.
+using Tile0 = MmCfg<256, 256, 4, 2, 2, 2>;
+using Tile1 = MmCfg<128, 256, 2, 4, 2, 2>;
+using Tile2 = MmCfg<128, 128, 2, 2, 2, 2>;
+using Tile3 = MmCfg<64, 128, 2, 2, 3, 2>;
+using Tile4 = MmCfg<64, 64, 2, 1, 3, 2>;
+using Tile5 = MmCfg<32, 64, 1, 2, 4, 2>;
+constexpr struct {
+  int bm, bn;
+} kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 128}, {64, 64}, {32, 64}};
+constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+
+struct MmPlan {
+  int tile, ksplit, splits;  // ksplit 0: not split
+};
+
+MmPlan mm_plan(int64_t M, int64_t N, int64_t K, bool row_scales, int tile, int splits) {
+  const int64_t nk = cdiv(K, kBlock);
+  MmPlan plan{tile, 0, 1};
+  if (tile < 0) {
+    plan.tile = M <= 32 && !row_scales ? 5
+                : cdiv(M, 256) * cdiv(N, 256) >= kCus / 2 ? 0
+                : cdiv(M, 128) * cdiv(N, 128) >= kCus / 2 ? 2 : 4;
+  }
+  const int64_t tiles = cdiv(M, kTiles[plan.tile].bm) * cdiv(N, kTiles[plan.tile].bn);
+  int64_t want = splits > 0 ? splits : tiles >= kCus ? 1 : kCus / tiles;
+  if (splits <= 0 && want > nk / 4) want = nk / 4;
+  if (want > nk) want = nk;
+  if (want > 1) {
+    plan.ksplit = (int)cdiv(nk, want);
+    plan.splits = (int)cdiv(nk, plan.ksplit);
+    if (plan.splits == 1) plan.ksplit = 0;
+  }
+  return plan;
+}
+
+size_t parts_bytes(const MmPlan& plan, int64_t M, int64_t N) {
+  return plan.splits > 1 ? (size_t)plan.splits * M * N * 4 : 0;
+}
 
 template <bool ROW_SCALES>
-int mm_pick(const MmArgs& p, hipStream_t stream) {
+int mm_run(MmArgs p, const MmPlan& plan, void* workspace, hipStream_t stream) {
+  p.ksplit = plan.ksplit;
+  p.parts = (float*)workspace;
   auto run = [&](auto* c) {
     using C = std::remove_pointer_t<decltype(c)>;
-    return launch_mm<C, ROW_SCALES, false, kStore>(p, cdiv(p.M, C::BM), stream);
+    return launch_mm<C, ROW_SCALES, false, kStore>(p, cdiv(p.M, C::BM), stream, plan.splits);
   };
-  if constexpr (!ROW_SCALES) {
-    if (p.M <= 32) return run((Cfg32*)nullptr);
+  int rc = F16ACC_OPS_E_ARG;
+  if constexpr (ROW_SCALES) {
+    switch (plan.tile) {
+      case 0: rc = run((Tile0*)nullptr); break;
+      case 2: rc = run((Tile2*)nullptr); break;
+      case 4: rc = run((Tile4*)nullptr); break;
+    }
+  } else {
+    switch (plan.tile) {
+      case 0: rc = run((Tile0*)nullptr); break;
+      case 1: rc = run((Tile1*)nullptr); break;
+      case 2: rc = run((Tile2*)nullptr); break;
+      case 3: rc = run((Tile3*)nullptr); break;
+      case 4: rc = run((Tile4*)nullptr); break;
+      case 5: rc = run((Tile5*)nullptr); break;
+    }
   }
-  if (cdiv(p.M, 256) * cdiv(p.N, 256) >= kCus / 2) return run((Cfg256*)nullptr);
-  if (cdiv(p.M, 128) * cdiv(p.N, 128) >= kCus / 2) return run((Cfg128*)nullptr);
-  return run((Cfg64*)nullptr);
+  if (rc || plan.splits == 1) return rc;
+  FinishArgs f{p.parts, p.M, p.N, p.scm, p.scn, plan.splits, p.bias, p.c};
+  const int64_t groups = cdiv(p.M * p.N, p.N % 4 ? 256 : 1024);
+  return by_type(p.ctype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL((mm_finish_kernel<T>), dim3((uint32_t)(groups < 8 * kCus ? groups : 8 * kCus)), dim3(256), 0,
+                       stream, f);
+    return hip_status();
+  });
 }
 
 // The experts' tiles: gate and up, 128 columns of each; down.
@@ -264,20 +321,31 @@ int f16acc_pack8(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t cols, i
 
 int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, int64_t sxk, const uint8_t* w,
                   int64_t ldw, const float* sw, int64_t swn, int64_t swk, int row_scales, const void* bias, void* c,
-                  int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype, void* stream) {
+                  int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype, int tile, int splits,
+                  void* workspace, size_t ws_bytes, void* stream) {
   if (row_scales != 0 && row_scales != 1) return F16ACC_OPS_E_ARG;
+  if (tile < -1 || tile >= kNumTiles || splits < 0) return F16ACC_OPS_E_ARG;
   MmArgs p{};
   p.x = x, p.ldx = ldx, p.sx = sx, p.sxm = sxm, p.sxk = sxk;
   p.w = w, p.ldw = ldw, p.sw = sw, p.swn = swn, p.swk = swk;
   p.bias = bias, p.c = c, p.scm = scm, p.scn = scn, p.M = M, p.N = N, p.K = K, p.ctype = ctype;
   const int rc = mm_check(p);
   if (rc || M == 0 || N == 0) return rc;
-  return row_scales ? mm_pick<true>(p, (hipStream_t)stream) : mm_pick<false>(p, (hipStream_t)stream);
+  const MmPlan plan = mm_plan(M, N, K, row_scales, tile, splits);
+  const size_t need = parts_bytes(plan, M, N);
+  if (need && (!workspace || (uintptr_t)workspace % 256 || ws_bytes < need)) return F16ACC_OPS_E_WORKSPACE;
+  return row_scales ? mm_run<true>(p, plan, workspace, (hipStream_t)stream)
+                    : mm_run<false>(p, plan, workspace, (hipStream_t)stream);
+}
+
+size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, int tile, int splits) {
+  if (M <= 0 || N <= 0 || K <= 0 || tile < -1 || tile >= kNumTiles || splits < 0) return 0;
+  return up256(parts_bytes(mm_plan(M, N, K, row_scales != 0, tile, splits), M, N));
 }
 
 size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4);
+  return up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4) + f16acc_mm_fp8_workspace(M, N, K, 0, -1, 0);
 }
 
 int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw, const float* sw,
@@ -295,7 +363,7 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
     return F16ACC_OPS_E_WORKSPACE;
   rc = mm_check(p);
   if (rc || M == 0 || N == 0) return rc;
-  if (M <= 16 && wide_loads(x, type, sr, sc) && K > 0) {
+  if (M <= 16 && wide_loads(x, type, sr, sc)) {
     SmallArgs a{x, sr, w, ldw, sw, swn, swk, bias, y, N, 1, M, N, K};
     return by_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -303,12 +371,11 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
       return hip_status();
     });
   }
-  if (K > 0) {
-    QuantArgs q{x, M, K, sr, sc, (uint8_t*)workspace, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
-    rc = quant_rows(q, type, (hipStream_t)stream);
-    if (rc) return rc;
-  }
-  return mm_pick<false>(p, (hipStream_t)stream);
+  QuantArgs q{x, M, K, sr, sc, (uint8_t*)workspace, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
+  rc = quant_rows(q, type, (hipStream_t)stream);
+  if (rc) return rc;
+  return mm_run<false>(p, mm_plan(M, N, K, false, -1, 0),
+                       (char*)workspace + up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4), (hipStream_t)stream);
 }
 
 int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,

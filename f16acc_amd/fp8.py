@@ -124,12 +124,14 @@ def _packed(q):
     return out, out.shape[-1]
 
 
-def _product(x, ldx, sx, w, ldw, sw, M, N, K, out, row_scales, bias=None):
+def _product(x, ldx, sx, w, ldw, sw, M, N, K, out, row_scales, bias=None, tile=-1, splits=0):
     """out [M, N] from x [M, K] and w [N, K]; sx and sw are ([m], [kb]) and
-    ([n or n / 128], [kb]) indexed."""
+    ([n or n / 128], [kb]) indexed.  tile, splits: force the library's choices (tuning, tests)."""
+    n = _ops.mm_fp8_workspace(M, N, K, int(row_scales), tile, splits)
+    ws = torch.empty(n, dtype=torch.uint8, device=out.device) if n else None
     call(_ops.mm_fp8, out.device, ptr(x), ldx, ptr(sx), sx.stride(0), sx.stride(1), ptr(w), ldw, ptr(sw),
          sw.stride(0), sw.stride(1), int(row_scales), ptr(bias), ptr(out), out.stride(0), out.stride(1), M, N, K,
-         TYPES[out.dtype])
+         TYPES[out.dtype], tile, splits, ptr(ws), n)
     return out
 
 

@@ -67,14 +67,21 @@ int f16acc_pack8(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t cols, i
  * c[m][n] = sum over k of (x[m][k] sx[m][k / 128]) (w[n][k] sw[n'][k / 128]) + bias[n],
  * n' = n / 128 (row_scales 0) or n (row_scales 1).  Each block's sum is an FP32
  * MFMA sum, the blocks are added in FP32 in K order, one rounding to ctype.
+ *   K at least 1 where M and N are
  *   x [M][ldx], w [N][ldw]: bytes, rows 16-byte aligned and zero from K to the
  *   next multiple of 16
  *   sx, sw: element strides (sxm, sxk), (swn, swk), non-negative
  *   bias: [N] of ctype, or NULL;  c: element strides scm, scn
+ *   tile, splits: -1 and 0 leave the choice to the library; a tile number (0 to 5) and a number of parts
+ *   of K force them, for tuning
+ *   workspace: f16acc_mm_fp8_workspace bytes (FP32 sums of the parts of K, 0 if
+ *   not split), 256-byte aligned
  */
 int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, int64_t sxk, const uint8_t* w,
                   int64_t ldw, const float* sw, int64_t swn, int64_t swk, int row_scales, const void* bias, void* c,
-                  int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype, void* stream);
+                  int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype, int tile, int splits,
+                  void* workspace, size_t ws_bytes, void* stream);
+size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, int tile, int splits);
 
 /*
  * y = x w^T + bias with x [M, K] of `type` (element strides sr, sc) quantised in row blocks on

@@ -128,6 +128,28 @@ def test_mm_large_tiles_in_every_k_order():
         assert torch.equal(fp8.mm(a, sa, b.t(), sr.t(), torch.float32).double(), want)
 
 
+@pytest.mark.parametrize("tile,splits", [(t, s) for t in range(6) for s in (1, 3)])
+def test_mm_every_tile_and_split(tile, splits):
+    """The same product in every tile, whole and in parts of K: exact sums, ragged edges, both kinds of scales."""
+    g = torch.Generator().manual_seed(7)
+    for M, N, K in ((1, 1, 300), (300, 333, 1000), (513, 580, 640)):
+        a = torch.randint(-3, 4, (M, K), generator=g).float().to(F8).to(DEV)
+        b = torch.randint(-3, 4, (N, K), generator=g).float().to(F8).to(DEV)
+        sa = torch.exp2(torch.randint(-2, 3, (M, -(-K // 128)), generator=g).float()).to(DEV)
+        bias = torch.randint(-9, 9, (N,), generator=g).float().to(DEV)
+        x, ldx = fp8._packed(a)
+        w, ldw = fp8._packed(b)
+        for rows in (False, True):
+            if rows and tile not in (0, 2, 4):
+                continue
+            sb = torch.exp2(torch.randint(-2, 3, (N if rows else -(-N // 128), -(-K // 128)), generator=g).float()).to(DEV)
+            want = ref.values(a, sa) @ ref.values(b, sb, 1 if rows else 128).t() + bias.cpu().double()
+            for out in (torch.empty(M, N, device=DEV), torch.empty(N, M, device=DEV).t(),
+                        torch.zeros(M, N + 5, device=DEV)[:, 3:N + 3]):
+                fp8._product(x, ldx, sa, w, ldw, sb, M, N, K, out, rows, bias, tile, splits)
+                assert torch.equal(out.cpu().double(), want)
+
+
 def test_mm_layouts():
     M, N, K = 90, 150, 272
     a, sa = fp8.quantize(normal(M, K))
@@ -166,8 +188,9 @@ def test_mm_offsets_past_32_bits():
     q[-300:] = normal(300, K).to(F8).view(torch.uint8)
     s = torch.ones(M, K // 128, device=DEV)
     w, ws = weight(N, K)
-    c = fp8.mm(q.view(F8), s, w.t(), ws.t(), torch.float32)
-    assert torch.equal(c[-300:], fp8.mm(q.view(F8)[-300:].clone(), s[-300:], w.t(), ws.t(), torch.float32))
+    f32 = lambda q, s: fp8._product(q, K, s, w, K, ws, len(q), N, K, torch.empty(len(q), N, device=DEV), False, None, 4, 1)
+    c = f32(q.view(F8), s)  # (one tile and no split for both: the same sums in the same order)
+    assert torch.equal(c[-300:], f32(q.view(F8)[-300:].clone(), s[-300:]))
     ref.check_product(c[-20:], q.view(F8)[-20:].cpu().double(), ref.values(w, ws, 128))
     assert bool((c[:M - 300] == 0).all())
 

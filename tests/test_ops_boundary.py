@@ -23,14 +23,26 @@ def test_library_exports_every_declared_symbol():
     assert _ops.abi_version() == _ops.ABI_VERSION
 
 
+def test_every_argument_is_bound_with_its_c_type():
+    src = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "f16acc_ops.h")).read(), flags=re.S)
+    kinds = {"int": ctypes.c_int, "int64_t": ctypes.c_int64, "float": ctypes.c_float, "size_t": ctypes.c_size_t}
+    for name, args in re.findall(r"\b(f16acc_\w+)\s*\(([^)]*)\)", src):
+        want = [] if args.strip() == "void" else [
+            ctypes.c_void_p if "*" in a else kinds[a.split()[0]] for a in args.replace("const ", "").split(",")]
+        assert _ops._SIGNATURES[name] == want, name
+
+
 def test_mm_checks():
-    def call(x=256, ldx=256, sx=256, sxm=1, sxk=1, w=256, ldw=256, sw=256, swn=1, swk=1, rows=0, c=256, M=4, N=4, K=256, t=0):
-        return _ops.mm_fp8(x, ldx, sx, sxm, sxk, w, ldw, sw, swn, swk, rows, None, c, N, 1, M, N, K, t, None)
+    def call(x=256, ldx=256, sx=256, sxm=1, sxk=1, w=256, ldw=256, sw=256, swn=1, swk=1, rows=0, c=256, M=4, N=4, K=256, t=0, tile=-1,
+             splits=0):
+        return _ops.mm_fp8(x, ldx, sx, sxm, sxk, w, ldw, sw, swn, swk, rows, None, c, N, 1, M, N, K, t, tile, splits, None, 0, None)
 
     assert call(M=-1) == call(K=-1) == call(t=3) == call(rows=2) == call(c=None) == call(x=None) == _ops.E_ARG
     assert call(sx=None) == call(swn=-1) == call(sxk=-1) == _ops.E_ARG
     assert call(ldx=250) == call(ldw=128) == call(x=8) == call(w=264) == _ops.E_UNSUPPORTED
     assert call(K=1 << 23, ldx=1 << 23, ldw=1 << 23) == _ops.E_UNSUPPORTED
+    assert call(tile=6) == call(tile=-2) == call(splits=-1) == _ops.E_ARG
+    assert call(splits=2) == _ops.E_WORKSPACE and _ops.mm_fp8_workspace(4, 4, 256, 0, -1, 2) >= 2 * 4 * 4 * 4
     assert call(M=0) == call(N=0) == 0
 
 
