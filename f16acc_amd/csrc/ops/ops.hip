@@ -99,33 +99,73 @@ using Tile2 = MmCfg<128, 128, 2, 2, 2, 2>;
 using Tile3 = MmCfg<64, 128, 2, 2, 3, 2>;
 using Tile4 = MmCfg<64, 64, 2, 1, 3, 2>;
 using Tile5 = MmCfg<32, 64, 1, 2, 4, 2>;
-constexpr struct {
-  int bm, bn;
-} kTiles[] = {{256, 256}, {128, 256}, {128, 128}, {64, 128}, {64, 64}, {32, 64}};
+// What a tile costs, in microseconds, fitted to 5010 timed (shape, tile, split)
+// triples (M 32 .. 8192, N 256 .. 8960, K 512 .. 9000, weights out of the cache; 438
+// with row scales): a workgroup alone on its CU takes
+// start + kb * block, each further one beside it adds `share` of the blocks'
+// time; `per_cu` fit.  The picks made with it take 1.4 % (row scales 0.6 %) longer than the best
+// triple on geometric mean, 15 % at worst.
+struct TileCost {
+  double start, block, share;
+};
+struct TileInfo {
+  int bm, bn, per_cu;
+  TileCost square, row;  // row.block 0: not built with row scales
+};
+constexpr TileInfo kTiles[] = {
+    {256, 256, 1, {5.5, 1.36, 0.6}, {7.05, 1.79, 0.6}},   {128, 256, 1, {3.1, 0.85, 0.6}, {}},
+    {128, 128, 2, {2.9, 0.61, 0.6}, {3.2, 0.68, 0.61}},   {64, 128, 2, {1.8, 0.69, 0.35}, {}},
+    {64, 64, 3, {1.7, 0.61, 0.27}, {2.2, 0.42, 0.33}},    {32, 64, 3, {1.2, 0.52, 0.27}, {}},
+};
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
 struct MmPlan {
   int tile, ksplit, splits;  // ksplit 0: not split
 };
 
+MmPlan split_of(int tile, int64_t nk, int64_t splits) {
+  if (splits > nk) splits = nk;
+  const int64_t ks = cdiv(nk, splits), n = cdiv(nk, ks);
+  return MmPlan{tile, n > 1 ? (int)ks : 0, (int)n};
+}
+
+double cost_of(const MmPlan& plan, int64_t M, int64_t N, int64_t K, bool row_scales) {
+  const TileInfo& t = kTiles[plan.tile];
+  const TileCost& c = row_scales ? t.row : t.square;
+  const int64_t nk = cdiv(K, kBlock), kb = plan.ksplit ? plan.ksplit : nk;
+  const int64_t deep = cdiv(cdiv(M, t.bm) * cdiv(N, t.bn) * plan.splits, kCus);  // workgroups on a CU
+  const int64_t full = deep / t.per_cu, rest = deep % t.per_cu;
+  double us = full * (c.start + c.block * kb * (1 + (t.per_cu - 1) * c.share));
+  if (rest) us += c.start + c.block * kb * (1 + (rest - 1) * c.share);
+  const double floor = ((double)N * K + (double)M * K) * 0.19e-6;  // the operands from HBM
+  if (us < floor) us = floor;
+  const double outputs = (double)M * N * 1e-6;
+  if (t.per_cu == 1) us += 0.2 * outputs;  // no other workgroup runs while one stores
+  if (plan.splits > 1) us += 2.3 + 0.28 * plan.splits + 1.28 * plan.splits * outputs;
+  return us;
+}
+
 MmPlan mm_plan(int64_t M, int64_t N, int64_t K, bool row_scales, int tile, int splits) {
   const int64_t nk = cdiv(K, kBlock);
-  MmPlan plan{tile, 0, 1};
-  if (tile < 0) {
-    plan.tile = M <= 32 && !row_scales ? 5
-                : cdiv(M, 256) * cdiv(N, 256) >= kCus / 2 ? 0
-                : cdiv(M, 128) * cdiv(N, 128) >= kCus / 2 ? 2 : 4;
+  MmPlan best{};
+  double least = 0;
+  for (int t = 0; t < kNumTiles; ++t) {
+    if ((tile >= 0 && t != tile) || (row_scales && kTiles[t].row.block == 0)) continue;
+    const int64_t tiles = cdiv(M, kTiles[t].bm) * cdiv(N, kTiles[t].bn);
+    for (const int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      // (a part of at least two blocks; workgroups beyond a few rounds are not split)
+      const int64_t want = splits > 0 ? splits : s;
+      if (splits <= 0 && s > 1 && (s > nk / 2 || tiles * s > 4 * kCus)) break;
+      const MmPlan plan = split_of(t, nk, want);
+      const double us = cost_of(plan, M, N, K, row_scales);
+      if (least == 0 || us < least) {
+        best = plan;
+        least = us;
+      }
+      if (splits > 0) break;
+    }
   }
-  const int64_t tiles = cdiv(M, kTiles[plan.tile].bm) * cdiv(N, kTiles[plan.tile].bn);
-  int64_t want = splits > 0 ? splits : tiles >= kCus ? 1 : kCus / tiles;
-  if (splits <= 0 && want > nk / 4) want = nk / 4;
-  if (want > nk) want = nk;
-  if (want > 1) {
-    plan.ksplit = (int)cdiv(nk, want);
-    plan.splits = (int)cdiv(nk, plan.ksplit);
-    if (plan.splits == 1) plan.ksplit = 0;
-  }
-  return plan;
+  return best;
 }
 
 size_t parts_bytes(const MmPlan& plan, int64_t M, int64_t N) {
@@ -325,6 +365,7 @@ int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, i
                   void* workspace, size_t ws_bytes, void* stream) {
   if (row_scales != 0 && row_scales != 1) return F16ACC_OPS_E_ARG;
   if (tile < -1 || tile >= kNumTiles || splits < 0) return F16ACC_OPS_E_ARG;
+  if (tile >= 0 && row_scales && kTiles[tile].row.block == 0) return F16ACC_OPS_E_ARG;
   MmArgs p{};
   p.x = x, p.ldx = ldx, p.sx = sx, p.sxm = sxm, p.sxk = sxk;
   p.w = w, p.ldw = ldw, p.sw = sw, p.swn = swn, p.swk = swk;
@@ -340,6 +381,7 @@ int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, i
 
 size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, int tile, int splits) {
   if (M <= 0 || N <= 0 || K <= 0 || tile < -1 || tile >= kNumTiles || splits < 0) return 0;
+  if (tile >= 0 && row_scales && kTiles[tile].row.block == 0) return 0;
   return up256(parts_bytes(mm_plan(M, N, K, row_scales != 0, tile, splits), M, N));
 }
 
