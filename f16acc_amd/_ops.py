@@ -1,23 +1,27 @@
-"""ctypes binding of libf16acc_ops.so (the C ABI in include/f16acc_ops.h).
+"""Binding of libf16acc_ops.so: its C ABI (include/f16acc_ops.h) through ctypes,
+and `host`, the torch side of the operators (csrc/ops/torch_ops.cpp), which
+fp8.py and moe.py call.
 
-There is no fallback: if the library is missing, importing this module raises.
+There is no fallback: if a library is missing, importing this module raises.
 """
 
 import ctypes
+import importlib.util
 import os
 
 import torch
 
-from .build import LIB_OPS
+from .build import LIB_OPS, OPS_TORCH
 
-if not os.path.exists(LIB_OPS):
-    raise ImportError(f"{LIB_OPS} is not built; run `python f16acc_amd/build.py` (needs hipcc for gfx950)")
+for _f in (LIB_OPS, OPS_TORCH):
+    if not os.path.exists(_f):
+        raise ImportError(f"{_f} is not built; run `python f16acc_amd/build.py` (needs hipcc for gfx950)")
 
 _dll = ctypes.CDLL(LIB_OPS)
 
 _i64, _vp, _int, _f32, _size = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
-# name -> argument types; every function but the last three returns an error code
+# name -> argument types
 _SIGNATURES = {
     "f16acc_quant_rows": [_vp, _int] + [_i64] * 4 + [_vp, _i64, _vp, _i64, _vp],
     "f16acc_quant_both": [_vp, _int] + [_i64] * 4 + [_vp, _i64, _vp, _i64] * 2 + [_vp],
@@ -38,6 +42,7 @@ _SIGNATURES = {
 }
 EXPORTS = tuple(_SIGNATURES)  # the symbols include/f16acc_ops.h declares
 ABI_VERSION = 1
+E_ARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3
 
 
 def _bind(name):
@@ -50,44 +55,20 @@ def _bind(name):
 (quant_rows, quant_both, quant_weight, pack8, mm_fp8, linear_fp8, route, route_grad, experts, mm_fp8_workspace,
  linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
 
-E_ARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3
-TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
-FP8 = torch.float8_e4m3fn
-BLOCK = 128
-
 if abi_version() != ABI_VERSION:
     raise ImportError(f"{LIB_OPS} has ABI version {abi_version()}, this package needs {ABI_VERSION}: rebuild it")
 
 
-def call(f, dev, *args):
-    """f(*args, stream) on `dev`'s current torch stream; raises RuntimeError for a failure."""
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return call(f, dev, *args)
-    rc = f(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    if rc != 0:
-        raise RuntimeError(strerror(rc).decode())
+def _load_host(path=OPS_TORCH):
+    spec = importlib.util.spec_from_file_location("f16acc_ops_torch", path)
+    try:
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+    except ImportError as e:
+        raise ImportError(f"{path} does not load with torch {torch.__version__} (built for another?): rebuild it") from e
+    if mod.torch_version != torch.__version__.split("+")[0] or mod.abi_version != ABI_VERSION:
+        raise ImportError(f"{path} was built for torch {mod.torch_version}, ABI {mod.abi_version}: rebuild it")
+    return mod
 
 
-def ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def up(v, m):
-    return -(-v // m) * m
-
-
-def blocks(v):
-    return -(-v // BLOCK)
-
-
-def on_gpu(name, *tensors):
-    """The one GPU the given tensors (None: skipped) are on; ValueError otherwise."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or (dev is not None and t.device != dev):
-            raise ValueError(f"{name} needs tensors on one GPU")
-        dev = t.device
-    return dev
+host = _load_host()

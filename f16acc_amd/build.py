@@ -34,6 +34,9 @@ LIB_SPLITREDO = os.path.join(OUT_DIR, "libf16acc_amd_splitredo.so")
 LIB_NOPERSIST = os.path.join(OUT_DIR, "libf16acc_amd_nopersist.so")
 # The 8-bit products and the mixture-of-experts operators (include/f16acc_ops.h).
 LIB_OPS = os.path.join(OUT_DIR, "libf16acc_ops.so")
+# Their torch side (checks, allocation, autograd): a CPython module linked to it.
+OPS_TORCH_SRC = os.path.join(PKG, "csrc", "ops", "torch_ops.cpp")
+OPS_TORCH = os.path.join(OUT_DIR, "f16acc_ops_torch.so")
 # The native call path (csrc/host.cpp): a CPython module on torch's C++ headers.
 HOST_SRC = os.path.join(PKG, "csrc", "host.cpp")
 HOST = os.path.join(OUT_DIR, "f16acc_host.so")
@@ -80,6 +83,15 @@ def host_flags():
     return flags, [f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
 
 
+def ops_torch_flags():
+    """host_flags for the operators' torch side: torch's HIP streams, and the library beside it."""
+    flags, libs = host_flags()
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    flags = flags + ["-DTORCH_EXTENSION_NAME=f16acc_ops_torch", "-D__HIP_PLATFORM_AMD__=1", "-isystem",
+                     os.path.join(rocm, "include")]
+    return flags, libs + ["-lc10_hip", "-ltorch_hip", f"-L{OUT_DIR}", "-lf16acc_ops", "-Wl,-rpath,$ORIGIN"]
+
+
 def _start(flags, src, out, compiler=None, libs=()):
     """Start hipcc (or `compiler`) src -> a temporary file next to out."""
     os.makedirs(OUT_DIR, exist_ok=True)
@@ -108,14 +120,21 @@ def _finish(job, verbose):
 
 def build(verbose=False):
     """Compile the library, its no-redo, split-redo and no-persistent twins,
-    the operators' library, the chunkrate microbenchmark and the native call
-    path (seven compilers at once)."""
+    the operators' library and its torch side, the chunkrate microbenchmark and
+    the native call path (seven compilers at once)."""
     flags, libs = host_flags()
+    ops = _start(HIP_FLAGS, OPS_SRC, LIB_OPS)
     jobs = [_start(HIP_FLAGS, SRC, LIB), _start(HIP_FLAGS + ["-DF16ACC_NO_REDO=1"], SRC, LIB_NOREDO),
             _start(HIP_FLAGS + ["-DF16ACC_SPLIT_REDO=1"], SRC, LIB_SPLITREDO),
             _start(HIP_FLAGS + ["-DF16ACC_NO_PERSISTENT=1"], SRC, LIB_NOPERSIST),
-            _start(HIP_FLAGS, OPS_SRC, LIB_OPS), _start(COMMON_FLAGS, CHUNKRATE_SRC, CHUNKRATE), _start(flags, HOST_SRC, HOST, cxx(), libs)]
+            _start(COMMON_FLAGS, CHUNKRATE_SRC, CHUNKRATE), _start(flags, HOST_SRC, HOST, cxx(), libs)]
     errors = []
+    try:
+        _finish(ops, verbose)
+        flags, libs = ops_torch_flags()  # (links against the library)
+        jobs.append(_start(flags, OPS_TORCH_SRC, OPS_TORCH, cxx(), libs))
+    except RuntimeError as e:
+        errors.append(str(e))
     for job in jobs:
         try:
             _finish(job, verbose)

@@ -137,8 +137,6 @@ def test_mm_every_tile_and_split(tile, splits):
         b = torch.randint(-3, 4, (N, K), generator=g).float().to(F8).to(DEV)
         sa = torch.exp2(torch.randint(-2, 3, (M, -(-K // 128)), generator=g).float()).to(DEV)
         bias = torch.randint(-9, 9, (N,), generator=g).float().to(DEV)
-        x, ldx = fp8._packed(a)
-        w, ldw = fp8._packed(b)
         for rows in (False, True):
             if rows and tile not in (0, 2, 4):
                 continue
@@ -146,7 +144,7 @@ def test_mm_every_tile_and_split(tile, splits):
             want = ref.values(a, sa) @ ref.values(b, sb, 1 if rows else 128).t() + bias.cpu().double()
             for out in (torch.empty(M, N, device=DEV), torch.empty(N, M, device=DEV).t(),
                         torch.zeros(M, N + 5, device=DEV)[:, 3:N + 3]):
-                fp8._product(x, ldx, sa, w, ldw, sb, M, N, K, out, rows, bias, tile, splits)
+                fp8.mm_tile(a, sa, b.t(), sb.t(), out, tile, splits, bias)
                 assert torch.equal(out.cpu().double(), want)
 
 
@@ -188,7 +186,7 @@ def test_mm_offsets_past_32_bits():
     q[-300:] = normal(300, K).to(F8).view(torch.uint8)
     s = torch.ones(M, K // 128, device=DEV)
     w, ws = weight(N, K)
-    f32 = lambda q, s: fp8._product(q, K, s, w, K, ws, len(q), N, K, torch.empty(len(q), N, device=DEV), False, None, 4, 1)
+    f32 = lambda q, s: fp8.mm_tile(q, s, w.t(), ws.t(), torch.empty(len(q), N, device=DEV), 4, 1)
     c = f32(q.view(F8), s)  # (one tile and no split for both: the same sums in the same order)
     assert torch.equal(c[-300:], f32(q.view(F8)[-300:].clone(), s[-300:]))
     ref.check_product(c[-20:], q.view(F8)[-20:].cpu().double(), ref.values(w, ws, 128))
@@ -317,7 +315,7 @@ def test_refusals():
     x, (w, ws) = normal(4, 256), weight(64, 256)
     q, s = fp8.quantize(x)
     bad = [lambda: fp8.quantize(x.double()), lambda: fp8.quantize(x.cpu()), lambda: fp8.quantize(normal(2, 3, 4), True),
-           lambda: fp8.quantize_weight(x[0]), lambda: fp8.linear(x, w), lambda: fp8.linear(x, w, ws[:, :1]),
+           lambda: fp8.quantize_weight(x[0]), lambda: fp8.quantize(q), lambda: fp8.linear(x, w), lambda: fp8.linear(x, w, ws[:, :1]),
            lambda: fp8.linear(x, w, ws.double()), lambda: fp8.linear(x[:, :128], w, ws), lambda: fp8.linear(x, w.cpu(), ws),
            lambda: fp8.linear(x, w, ws, normal(63)), lambda: fp8.linear(x, w, ws, normal(64, dtype=torch.float32)),
            lambda: fp8.linear(x, x[:, :256], ws), lambda: fp8.linear(x.to(F8), w, ws), lambda: fp8.mm(q, s, w, ws),
