@@ -230,7 +230,6 @@ struct SortArgs {
   int blocks;
 };
 constexpr int kSortChunk = 2048;  // slots of one workgroup
-constexpr int kMaxExperts = 1024;
 
 __global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
   __shared__ int hist[kMaxExperts];

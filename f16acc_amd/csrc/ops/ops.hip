@@ -34,6 +34,16 @@ int by_type(int type, F f) {
   return F16ACC_OPS_E_ARG;
 }
 
+// ... and by the groups of four tokens (1, 2 or 4) that hold `tokens`.
+template <class F>
+int by_tokens(int tokens, int type, F f) {
+  return by_type(type, [&](auto* t) {
+    if (tokens <= 4) return f(t, std::integral_constant<int, 1>());
+    if (tokens <= 8) return f(t, std::integral_constant<int, 2>());
+    return f(t, std::integral_constant<int, 4>());
+  });
+}
+
 int quant_check(const void* x, int type, int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 0 || type < 0 || type > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
   if (rows > kMaxExtent || cols > kMaxExtent) return F16ACC_OPS_E_UNSUPPORTED;
@@ -72,9 +82,9 @@ int quant_tile(const QuantArgs& p, int type, hipStream_t stream) {
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (wide)
-      hipLaunchKernelGGL((quant_tile_kernel<T, true, ROWS, COLS, SQUARE>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((quant_tile_kernel<T, true, ROWS, COLS, SQUARE>), grid, dim3(512), 0, stream, p);
     else
-      hipLaunchKernelGGL((quant_tile_kernel<T, false, ROWS, COLS, SQUARE>), grid, dim3(256), 0, stream, p);
+      hipLaunchKernelGGL((quant_tile_kernel<T, false, ROWS, COLS, SQUARE>), grid, dim3(512), 0, stream, p);
     return hip_status();
   });
 }
@@ -232,14 +242,19 @@ int expert_tile(int64_t slots, int E) {
   return mean >= 96 ? 128 : mean >= 32 ? 64 : 32;
 }
 
+// Whether the two kernels for a few tokens run.
+bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots && k <= kFewK; }
+
 struct ExpertsPlan {
   int64_t slots, blocks, max_tiles, Dp, Ip;
   int bm;
+  size_t few;  // bytes of the hidden values of the kernels for a few tokens
   size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
   ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     slots = T * k;
     Dp = up128(D);
     Ip = up128(I);
+    few = few_tokens(T, k) ? (size_t)slots * Ip * 4 : 0;
     bm = expert_tile(slots, E);
     blocks = cdiv(slots, kSortChunk);
     max_tiles = slots / bm + (slots < E ? slots : E);
@@ -259,7 +274,7 @@ struct ExpertsPlan {
     pos = take(slots * 4);
     tiles = take(max_tiles * 16);
     ntiles = take(4);
-    total = at;
+    total = at > few ? at : few;
   }
 };
 
@@ -405,11 +420,21 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
     return F16ACC_OPS_E_WORKSPACE;
   rc = mm_check(p);
   if (rc || M == 0 || N == 0) return rc;
-  if (M <= 16 && wide_loads(x, type, sr, sc)) {
+  // Few tokens: one launch.  From 9 on its quantising, repeated by every workgroup, costs more
+  // than a pass of its own where there are many (16 tokens: 8960 x 1536 11.5 us against 12.4 on the
+  // tiles, 8192 x 8192 32 against 25).
+  if ((M <= 8 || (M <= 16 && N * K <= (1 << 25))) && wide_loads(x, type, sr, sc)) {
     SmallArgs a{x, sr, w, ldw, sw, swn, swk, bias, y, N, 1, M, N, K};
-    return by_type(type, [&](auto* t) {
+    return by_tokens((int)M, type, [&](auto* t, auto groups) {
       using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL((linear_small_kernel<T, 8>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0, (hipStream_t)stream, a);
+      constexpr int G = decltype(groups)::value;
+      // 16 waves deal K where the rows alone leave CUs idle
+      if (cdiv(N, 16) < kCus && cdiv(K, kBlock) >= 16)
+        hipLaunchKernelGGL((linear_small_kernel<T, 16, G>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), 0,
+                           (hipStream_t)stream, a);
+      else
+        hipLaunchKernelGGL((linear_small_kernel<T, 8, G>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0,
+                           (hipStream_t)stream, a);
       return hip_status();
     });
   }
@@ -471,6 +496,18 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_;
   char* ws = (char*)workspace;
+  if (plan.few && wide_loads(x, type, sr, sc)) {
+    FewArgs f{x,   sr,  (int)T, k,   E,   (int)plan.slots, ids, weights, wt,  wk,  D,   I, w1,          w1e,     w1u,
+              ld1, s1,  s1e,    s1u, s1n, s1k,             w2,  w2e,     ld2, s2,  s2e, s2n, s2k, (float*)ws, plan.Ip, y};
+    return by_type(type, [&](auto* t) {
+      using U = std::remove_pointer_t<decltype(t)>;
+      constexpr int G = 2;
+      hipLaunchKernelGGL((few_gate_up_kernel<U, 8, G>), dim3((uint32_t)cdiv(I, 32), (uint32_t)plan.slots), dim3(512), 0,
+                         stream, f);
+      hipLaunchKernelGGL((few_down_kernel<U, 16, G>), dim3((uint32_t)cdiv(D, 16)), dim3(1024), 0, stream, f);
+      return hip_status();
+    });
+  }
   QuantArgs q{x, T, D, sr, sc, (uint8_t*)(ws + plan.xq), plan.Dp, (float*)(ws + plan.xs), T, nullptr, 0, nullptr, 0};
   rc = quant_rows(q, type, stream);
   if (rc) return rc;

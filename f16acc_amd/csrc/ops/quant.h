@@ -30,7 +30,9 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
   const int64_t total = p.rows * blocks;
   const int lane = threadIdx.x & 15;
   for (int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)gridDim.x * 16) {
-    const int64_t row = b / blocks, kb = b - row * blocks, c0 = kb * kBlock + lane * 8;
+    // (64-bit division is a hundred instructions)
+    const int64_t row = total >> 32 ? b / blocks : (int64_t)((uint32_t)b / (uint32_t)blocks), kb = b - row * blocks;
+    const int64_t c0 = kb * kBlock + lane * 8;
     const T* x = (const T*)p.x + row * p.sr;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (WIDE && c0 + 8 <= p.cols) {
@@ -55,19 +57,20 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
 // A 128 x 128 tile a workgroup: read once, quantised along its rows (ROWS), its
 // columns (COLS, written transposed through LDS) or both, or as one square
 // block (SQUARE, whose transpose has the same values and scales).
-// Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's
+// Thread (r, c) holds rows 4 r .. 4 r + 3, columns 8 c .. 8 c + 7: a row's
 // maximum is over the 16 lanes of a DPP row, a column's over the four DPP rows
-// of a wave and then the four waves.
+// of a wave and then the eight waves.
 template <class T, bool WIDE, bool ROWS, bool COLS, bool SQUARE>
-__global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs p) {
-  __shared__ __align__(16) uint8_t tile[COLS ? kBlock * (kBlock + 16) : 16];
-  __shared__ uint32_t part[4 * kBlock];
+__global__ __launch_bounds__(512) void quant_tile_kernel(QuantArgs p) {
+  constexpr int LD = kBlock + 16;  // bytes of a transposed row in LDS
+  __shared__ __align__(16) uint8_t tile[COLS ? kBlock * LD : 16];
+  __shared__ __align__(16) uint32_t part[SQUARE ? 32 : 8 * kBlock];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 4, c = tid & 15;
   const int64_t kb = blockIdx.x, rb = blockIdx.y;
-  const int64_t r0 = rb * kBlock + r * 8, c0 = kb * kBlock + c * 8;
-  float v[8][8];
+  const int64_t r0 = rb * kBlock + r * 4, c0 = kb * kBlock + c * 8;
+  float v[4][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const T* x = (const T*)p.x + (r0 + i) * p.sr;
     if (WIDE && r0 + i < p.rows && c0 + 8 <= p.cols) {
       load_vec(x + c0, v[i]);
@@ -76,86 +79,77 @@ __global__ __launch_bounds__(256) void quant_tile_kernel(QuantArgs p) {
       for (int j = 0; j < 8; ++j) v[i][j] = r0 + i < p.rows && c0 + j < p.cols ? (float)x[(c0 + j) * p.sc] : 0.0f;
     }
   }
+  auto store_rows = [&](int i, float inv) {
+    i32x2 o;
+    o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], inv);
+    o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], inv);
+    if (r0 + i < p.rows) *(i32x2*)(p.q + (r0 + i) * p.ldq + c0) = o;
+  };
+  auto stage_column = [&](int j, float inv) {
+    *(int*)(tile + (c * 8 + j) * LD + r * 4) = pack_e4m3(v[0][j], v[1][j], v[2][j], v[3][j], inv);
+  };
   if (SQUARE) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
     m = row_umax(m);
-    if ((lane & 15) == 0) part[wave * 4 + (lane >> 4)] = m;
+    if (c == 0) part[r] = m;
     __syncthreads();
-    m = part[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) m = umax(m, part[i]);
-    const BlockScale bs = block_scale(m);
+    const BlockScale bs = block_scale(umax(row_umax(part[c]), row_umax(part[16 + c])));
     if (tid == 0) p.s[rb * p.lds + kb] = bs.s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      i32x2 o;
-      o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], bs.inv);
-      o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], bs.inv);
-      if (r0 + i < p.rows) *(i32x2*)(p.q + (r0 + i) * p.ldq + c0) = o;
+    for (int i = 0; i < 4; ++i) store_rows(i, bs.inv);
+    if (COLS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) stage_column(j, bs.inv);
     }
+  } else {
     if (COLS) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        i32x2 o;
-        o[0] = pack_e4m3(v[0][j], v[1][j], v[2][j], v[3][j], bs.inv);
-        o[1] = pack_e4m3(v[4][j], v[5][j], v[6][j], v[7][j], bs.inv);
-        *(i32x2*)(tile + (c * 8 + j) * (kBlock + 16) + r * 8) = o;
+        uint32_t m = umax(umax(abs_bits(v[0][j]), abs_bits(v[1][j])), umax(abs_bits(v[2][j]), abs_bits(v[3][j])));
+        m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+        m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+        if (lane < 16) part[wave * kBlock + c * 8 + j] = m;
       }
     }
-  } else {
     if (ROWS) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         uint32_t m = abs_bits(v[i][0]);
 #pragma unroll
         for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
         const BlockScale bs = block_scale(row_umax(m));
-        i32x2 o;
-        o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], bs.inv);
-        o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], bs.inv);
-        if (r0 + i < p.rows) {
-          *(i32x2*)(p.q + (r0 + i) * p.ldq + c0) = o;
-          if (c == 0) p.s[kb * p.lds + r0 + i] = bs.s;
-        }
+        store_rows(i, bs.inv);
+        if (c == 0 && r0 + i < p.rows) p.s[kb * p.lds + r0 + i] = bs.s;
       }
     }
     if (COLS) {
-      uint32_t m[8];
+      __syncthreads();
+      if (tid < kBlock) {  // a thread per column
+        uint32_t m = part[tid];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        m[j] = abs_bits(v[0][j]);
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m[j] = umax(m[j], abs_bits(v[i][j]));
-        m[j] = umax(m[j], (uint32_t)__shfl_xor((int)m[j], 16));
-        m[j] = umax(m[j], (uint32_t)__shfl_xor((int)m[j], 32));
-        if (lane < 16) part[wave * kBlock + c * 8 + j] = m[j];
+        for (int i = 1; i < 8; ++i) m = umax(m, part[i * kBlock + tid]);
+        const BlockScale bs = block_scale(m);
+        part[tid] = __float_as_uint(bs.inv);
+        if (kb * kBlock + tid < p.cols) p.st[rb * p.ldst + kb * kBlock + tid] = bs.s;
       }
       __syncthreads();
+      float inv[8];
+      load_vec((const float*)part + c * 8, inv);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = c * 8 + j;
-        const BlockScale bs =
-            block_scale(umax(umax(part[col], part[kBlock + col]), umax(part[2 * kBlock + col], part[3 * kBlock + col])));
-        i32x2 o;
-        o[0] = pack_e4m3(v[0][j], v[1][j], v[2][j], v[3][j], bs.inv);
-        o[1] = pack_e4m3(v[4][j], v[5][j], v[6][j], v[7][j], bs.inv);
-        *(i32x2*)(tile + col * (kBlock + 16) + r * 8) = o;
-        if (r == 0 && c0 + j < p.cols) p.st[rb * p.ldst + c0 + j] = bs.s;
-      }
+      for (int j = 0; j < 8; ++j) stage_column(j, inv[j]);
     }
   }
   if (COLS) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int col = k * 32 + (tid >> 3), u = tid & 7;
+    for (int k = 0; k < 2; ++k) {
+      const int col = k * 64 + (tid >> 3), u = tid & 7;
       if (kb * kBlock + col < p.cols)
-        *(i32x4*)(p.qt + (kb * kBlock + col) * p.ldqt + rb * kBlock + u * 16) =
-            *(const i32x4*)(tile + col * (kBlock + 16) + u * 16);
+        *(i32x4*)(p.qt + (kb * kBlock + col) * p.ldqt + rb * kBlock + u * 16) = *(const i32x4*)(tile + col * LD + u * 16);
     }
   }
 }

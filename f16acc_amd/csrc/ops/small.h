@@ -14,37 +14,55 @@
 
 namespace f16ops {
 
-// A lane's share of block kb of a token row: k of units g and g + 4.
-template <class T>
-__device__ __forceinline__ void load_token(const T* x, int64_t k0, int64_t K, int g, bool in, float (&v)[32]) {
+// A wave's block of 128 columns of up to 16 token rows, quantised on the way:
+// 16 lanes take a token, 8 values each, four tokens at a time (a lane that
+// quantised its own 32 operand values would spend as much on 15 absent tokens as
+// on one), and the values pass through LDS into the MFMA's layout.
+struct TokenBlock {
+  static constexpr int ROW = kBlock + 16;  // bytes: rows on different banks
+  uint8_t q[16 * ROW];
+  float s[16];
+};
+
+// Rows row(t) of x (NULL: zeros) from k0, for t < tokens <= 4 G; every group's loads are
+// in flight together.
+template <class T, int G, class Row>
+__device__ __forceinline__ i32x8 quant_tokens(TokenBlock& b, Row row, int tokens, int64_t k0, int64_t K, int lane,
+                                              float* s) {
+  const int c = lane & 15;
+  const int64_t k = k0 + 8 * c;
+  float v[G][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t k = k0 + 64 * h + 16 * g;
-    float t[16];
-    if (in && k + 16 <= K) {
-      load_vec(x + k, t);
+  for (int i = 0; i < G; ++i) {
+    const int t = 4 * i + (lane >> 4);
+    const T* x = t < tokens ? row(t) : nullptr;
+    if (x && k + 8 <= K) {
+      load_vec(x + k, v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) t[i] = in && k + i < K ? (float)x[k + i] : 0.0f;
+      for (int j = 0; j < 8; ++j) v[i][j] = x && k + j < K ? (float)x[k + j] : 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[16 * h + i] = t[i];
   }
-}
-
-// The lane's share quantised, and its block's scale.
-__device__ __forceinline__ i32x8 quant_token(const float (&v)[32], float* s) {
-  uint32_t m = abs_bits(v[0]);
 #pragma unroll
-  for (int i = 1; i < 32; ++i) m = umax(m, abs_bits(v[i]));
-  m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-  m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-  const BlockScale bs = block_scale(m);
-  *s = bs.s;
-  i32x8 q;
+  for (int i = 0; i < G; ++i) {
+    const int t = 4 * i + (lane >> 4);
+    uint32_t m = abs_bits(v[i][0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = pack_e4m3(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], bs.inv);
-  return q;
+    for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
+    const BlockScale bs = block_scale(row_umax(m));
+    i32x2 o;
+    o[0] = pack_e4m3(v[i][0], v[i][1], v[i][2], v[i][3], bs.inv);
+    o[1] = pack_e4m3(v[i][4], v[i][5], v[i][6], v[i][7], bs.inv);
+    *(i32x2*)(b.q + t * TokenBlock::ROW + 8 * c) = o;
+    if (c == 0) b.s[t] = bs.s;
+  }
+  wave_sync();
+  const int t16 = lane & 15, g = lane >> 4;
+  *s = b.s[t16];
+  const uint8_t* q = b.q + t16 * TokenBlock::ROW + 16 * g;
+  const i32x4 lo = *(const i32x4*)q, hi = *(const i32x4*)(q + 64);
+  wave_sync();
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // A lane's share of block kb of a weight row (zero from K to the next multiple
@@ -69,26 +87,30 @@ struct SmallArgs {
   int64_t M, N, K;
 };
 
-template <class T, int W>
+template <class T, int W, int G>
 __global__ __launch_bounds__(64 * W) void linear_small_kernel(SmallArgs p) {
   __shared__ f32x4 sums[W][64];
+  __shared__ __align__(16) TokenBlock tokens[W];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t16 = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + t16 < p.N ? n0 + t16 : p.N - 1;
   const uint8_t* w = p.w + n * p.ldw;
   const float* sw = p.sw + n0 / kBlock * p.swn;
-  const T* x = (const T*)p.x + (int64_t)t16 * p.ldx;
   const bool in = t16 < p.M;
   const int nk = (int)cdiv(p.K, kBlock);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  i32x8 next;
+  if (wave < nk) next = load_weight(w, (int64_t)wave * kBlock, p.K, g);
+#pragma unroll 1
   for (int kb = wave; kb < nk; kb += W) {
-    const i32x8 wf = load_weight(w, (int64_t)kb * kBlock, p.K, g);
-    float v[32], s;
-    load_token(x, (int64_t)kb * kBlock, p.K, g, in, v);
+    const i32x8 wf = next;
+    if (kb + W < nk) next = load_weight(w, (int64_t)(kb + W) * kBlock, p.K, g);
     const float sb = sw[kb * p.swk];
-    const f32x4 part = mfma(wf, quant_token(v, &s));
-    acc += part * (s * sb);
+    float s;
+    const i32x8 xf = quant_tokens<T, G>(tokens[wave], [&](int t) { return (const T*)p.x + t * p.ldx; }, (int)p.M,
+                                     (int64_t)kb * kBlock, p.K, lane, &s);
+    acc += mfma(wf, xf) * (s * sb);
   }
   sums[wave][lane] = acc;
   __syncthreads();
@@ -105,6 +127,241 @@ __global__ __launch_bounds__(64 * W) void linear_small_kernel(SmallArgs p) {
   }
   const bool wide = p.scn == 1 && p.scm % 4 == 0 && (uintptr_t)p.c % (4 * sizeof(T)) == 0;
   store4<T>((T*)p.c + (int64_t)t16 * p.scm + row * p.scn, p.scn, left, acc, wide);
+}
+
+// ---------------------------------------------------------------------------
+// The experts' feed-forward for at most 8 tokens: no sorting.  Token t is column
+// t of every expert's products, zero where the token does not go there, so the
+// down kernel adds all experts of a token in one register, and the routing weight
+// is a factor of the block's scale.
+//
+// The hidden values are quantised between the products, and a sum that the 8-bit
+// matrix instructions round at 1e-5 lands on the other side of an e4m3 tie once
+// in some hundred values: with one token that showed as 2e-3 of the result.
+// Weights are what the kernels wait for, so the first product converts both
+// operands to binary16 (exactly) and sums in FP32 on the 16-bit instructions.
+// ---------------------------------------------------------------------------
+
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 8 e4m3 values as binary16.
+__device__ __forceinline__ f16x8 halves(int lo, int hi) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+struct Halves {
+  f16x8 v[4];
+  __device__ __forceinline__ explicit Halves(const i32x8& q) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = halves(q[2 * i], q[2 * i + 1]);
+  }
+};
+__device__ __forceinline__ f32x4 exact_product(const i32x8& w, const Halves& x) {
+  const Halves h(w);
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.v[i], x.v[i], sum, 0, 0, 0);
+  return sum;
+}
+
+// (4 tokens of 64 experts, 8 each, 2048 x 1024: 55 us against 60 on the tiles; 16: 178 against 88)
+constexpr int kFewTokens = 8, kFewSlots = 128, kFewK = 16;
+
+struct FewArgs {
+  const void* x;
+  int64_t ldx;
+  int T, k, E, slots;
+  const int* ids;
+  const float* weights;
+  int64_t wt, wk;
+  int64_t D, I;
+  const uint8_t* w1;
+  int64_t w1e, w1u, ld1;
+  const float* s1;
+  int64_t s1e, s1u, s1n, s1k;
+  const uint8_t* w2;
+  int64_t w2e, ld2;
+  const float* s2;
+  int64_t s2e, s2n, s2k;
+  float* h;  // [slots][ldh], at each (token, expert)'s first slot
+  int64_t ldh;
+  void* y;
+};
+
+// h of 32 hidden columns of one expert, the one of slot blockIdx.y where that is its
+// first.  The waves deal the blocks of D, the next one's weights in flight while one
+// is multiplied.  All ids lie in the wave's registers: what the
+// expert's tokens are is a ballot and no further load.
+template <class T, int W, int G>
+__global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
+  constexpr int WORDS = kFewSlots / 64;
+  __shared__ f32x4 sums[W][4][64];
+  __shared__ __align__(16) TokenBlock tokens[W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t16 = lane & 15, g = lane >> 4, slot0 = blockIdx.y;
+  const int e = p.ids[slot0];
+  int id[WORDS];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) id[i] = 64 * i + lane < p.slots ? p.ids[64 * i + lane] : -1;
+  uint64_t same[WORDS + 1];
+  bool earlier = false;
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    same[i] = __builtin_amdgcn_ballot_w64(id[i] == e);
+    const int below = slot0 - 64 * i;
+    earlier |= below > 0 && (same[i] & (below >= 64 ? ~0ull : (1ull << below) - 1)) != 0;
+  }
+  same[WORDS] = 0;
+  if (e < 0 || e >= p.E || earlier) return;  // (the same in every wave)
+  int slot = -1;  // the token's first slot with this expert
+  if (t16 < p.T) {
+    const int at = t16 * p.k, sh = at & 63;
+    uint64_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i)
+      if (i == at >> 6) lo = same[i], hi = same[i + 1];
+    const uint64_t bits = ((lo >> sh) | (sh ? hi << (64 - sh) : 0)) & ((1ull << p.k) - 1);
+    if (bits) slot = at + __builtin_ctzll(bits);
+  }
+  const int64_t n0 = (int64_t)blockIdx.x * 32;
+  const int64_t na = n0 + t16 < p.I ? n0 + t16 : p.I - 1, nb = n0 + 16 + t16 < p.I ? n0 + 16 + t16 : p.I - 1;
+  const uint8_t* w = p.w1 + e * p.w1e;
+  const uint8_t *wa = w + na * p.ld1, *wb = w + nb * p.ld1;
+  const float* sw = p.s1 + e * p.s1e + n0 / kBlock * p.s1n;
+  const int nk = (int)cdiv(p.D, kBlock);
+  f32x4 acc[4] = {};  // gate, gate, up, up
+  const uint32_t here = (uint32_t)__builtin_amdgcn_ballot_w64(slot >= 0);  // bit t: token t goes there
+  i32x8 next[4];
+  auto load = [&](int kb) {
+    const int64_t k0 = (int64_t)kb * kBlock;
+    next[0] = load_weight(wa, k0, p.D, g);
+    next[1] = load_weight(wb, k0, p.D, g);
+    next[2] = load_weight(wa + p.w1u, k0, p.D, g);
+    next[3] = load_weight(wb + p.w1u, k0, p.D, g);
+  };
+  if (wave < nk) load(wave);
+#pragma unroll 1
+  for (int kb = wave; kb < nk; kb += W) {
+    const float sg = sw[kb * p.s1k], su = sw[p.s1u + kb * p.s1k];
+    const i32x8 wf[4] = {next[0], next[1], next[2], next[3]};
+    if (kb + W < nk) load(kb + W);
+    float s;
+    const Halves xh(quant_tokens<T, G>(
+        tokens[wave], [&](int t) { return (here >> t) & 1 ? (const T*)p.x + t * p.ldx : nullptr; }, p.T,
+        (int64_t)kb * kBlock, p.D, lane, &s));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += exact_product(wf[i], xh) * (s * (i < 2 ? sg : su));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave >= 2 || slot < 0) return;  // wave 0: columns 0 .. 15, wave 1: 16 .. 31
+  f32x4 gate = sums[0][wave][lane], up = sums[0][2 + wave][lane];
+#pragma unroll
+  for (int i = 1; i < W; ++i) {
+    gate += sums[i][wave][lane];
+    up += sums[i][2 + wave][lane];
+  }
+  const int64_t n = n0 + 16 * wave + 4 * g;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < p.I) p.h[slot * p.ldh + n + r] = silu(gate[r]) * up[r];
+}
+
+// y of 16 columns: the waves deal the (expert, block of I) pairs, the next one's
+// weights in flight while one is multiplied.
+template <class T, int W, int G>
+__global__ __launch_bounds__(64 * W) void few_down_kernel(FewArgs p) {
+  __shared__ int ids[kFewSlots], expert[kFewSlots], firsts[kFewSlots / 64], index[kMaxExperts];
+  __shared__ float weights[kFewSlots], weight[kFewSlots][16];
+  __shared__ short slot_of[kFewSlots][16];
+  __shared__ f32x4 sums[W][64];
+  __shared__ __align__(16) TokenBlock tokens[W];
+  static_assert(64 * W >= kFewSlots, "a thread per slot");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t16 = lane & 15, g = lane >> 4;
+  // the distinct experts, in order of their first slots; index[e]: the lowest slot
+  // with expert e, then the expert's place among them
+  for (int i = tid; i < p.E; i += 64 * W) index[i] = kFewSlots;
+  int e = -1;
+  if (tid < p.slots) {
+    e = p.ids[tid];
+    weights[tid] = p.weights[tid / p.k * p.wt + tid % p.k * p.wk];
+    if (e >= p.E) e = -1;
+    ids[tid] = e;
+  }
+  lds_barrier();
+  if (e >= 0) atomicMin(&index[e], tid);
+  lds_barrier();
+  const bool first = e >= 0 && index[e] == tid;
+  const uint64_t mask = __builtin_amdgcn_ballot_w64(first);
+  if (tid < kFewSlots && lane == 0) firsts[wave] = __popcll(mask);
+  lds_barrier();
+  int count = 0, at = 0;
+#pragma unroll
+  for (int i = 0; i < kFewSlots / 64; ++i) {
+    if (i == wave) at = count;
+    count += firsts[i];
+  }
+  at += __popcll(mask & ((1ull << lane) - 1));
+  if (first) {
+    expert[at] = e;
+    index[e] = at;
+  }
+  lds_barrier();
+  const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + t16 < p.D ? n0 + t16 : p.D - 1;
+  const int nk = (int)cdiv(p.I, kBlock), units = count * nk;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  i32x8 next;
+  float snext = 0.0f;
+  auto load = [&](int u) {
+    const int d = u / nk, kb = u - d * nk, ex = expert[d];
+    next = load_weight(p.w2 + ex * p.w2e + n * p.ld2, (int64_t)kb * kBlock, p.I, g);
+    snext = p.s2[ex * p.s2e + n0 / kBlock * p.s2n + kb * p.s2k];
+  };
+  if (wave < units) load(wave);
+  // while the first weights are on their way: each token's first slot with each
+  // expert, and its weights (a token may name an expert twice)
+  for (int i = tid; i < count * 16; i += 64 * W) slot_of[i >> 4][i & 15] = -1;
+  lds_barrier();
+  if (e >= 0) {
+    const int t = tid / p.k, end = t * p.k + p.k;
+    bool mine = true;
+    float sum = weights[tid];
+    for (int j = t * p.k; j < tid; ++j) mine &= ids[j] != e;
+    for (int j = tid + 1; j < end; ++j)
+      if (ids[j] == e) sum += weights[j];
+    if (mine) {
+      slot_of[index[e]][t] = (short)tid;
+      weight[index[e]][t] = sum;
+    }
+  }
+  lds_barrier();
+#pragma unroll 1
+  for (int u = wave; u < units; u += W) {
+    const int d = u / nk, kb = u - d * nk, slot = slot_of[d][t16];
+    const i32x8 wf = next;
+    const float sb = snext;
+    if (u + W < units) load(u + W);
+    float s;
+    const i32x8 xf = quant_tokens<float, G>(
+        tokens[wave], [&](int t) { return slot_of[d][t] >= 0 ? p.h + slot_of[d][t] * p.ldh : nullptr; }, p.T,
+        (int64_t)kb * kBlock, p.I, lane, &s);
+    const float f = slot >= 0 ? s * sb * weight[d][t16] : 0.0f;
+    acc += mfma(wf, xf) * f;
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || t16 >= p.T) return;
+#pragma unroll
+  for (int i = 1; i < W; ++i) acc += sums[i][lane];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n0 + 4 * g + r < p.D) ((T*)p.y)[t16 * p.D + n0 + 4 * g + r] = (T)acc[r];
 }
 
 }  // namespace f16ops
