@@ -114,8 +114,9 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = (float)k.t[i];
 }
 
-// SiLU.
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
+// SiLU, to a few units in the last place: the hardware's exponential and
+// reciprocal (a correctly rounded quotient was a fifth of the gated product's time).
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // Raw buffer resource over `bytes` bytes at `base` (stride 0; reads past the
 // end return 0).  Wave-uniform.

@@ -46,7 +46,10 @@ struct MmArgs {
   const int* rows;
   int64_t xrows;  // rows of x
   int64_t we, swe;
-  // Gate and up: w holds the gate's N rows, then (at up bytes, its scales at
+  int tile_rows;  // tokens per entry of the tile list, a multiple of the kernel's
+  // Down (kSlots): binary16 values c of a slot over a power of two for each of its
+  // wave tiles, sq[n / TN][slot].
+  // Gate and up (kGatedQuant): w holds the gate's N rows, then (at up bytes, its scales at
   // sup elements) the up's; the result goes to q and its scales, quantised.
   int64_t up, sup;
   uint8_t* q;
@@ -55,7 +58,7 @@ struct MmArgs {
   int64_t ldsq;
 };
 
-enum Epilogue { kStore = 0, kGatedQuant = 1 };
+enum Epilogue { kStore = 0, kGatedQuant = 1, kSlots = 2 };
 
 template <int BM_, int BN_, int WM_, int WN_, int NS_, int OCC_>
 struct MmCfg {
@@ -258,12 +261,14 @@ struct MmKernel {
     const float* sw = p.sw;
     const uint32_t tiles_n = (uint32_t)cdiv(p.N, BN_OUT);
     if (EXPERTS) {
-      const uint32_t total = (uint32_t)*p.ntiles * tiles_n;
+      const uint32_t parts = (uint32_t)p.tile_rows / C::BM, total = (uint32_t)*p.ntiles * parts * tiles_n;
       if (blockIdx.x >= total) return;
       const uint32_t id = xcd_order(blockIdx.x, total), t = id / tiles_n;
-      const int4 tile = p.tiles[t];
-      m0 = tile.y;
-      m_left = tile.z - tile.y;
+      const int4 tile = p.tiles[t / parts];
+      const int first = tile.y + (int)(t % parts) * C::BM;
+      if (first >= tile.z) return;
+      m0 = first;
+      m_left = tile.z - first < C::BM ? tile.z - first : C::BM;
       n0 = (int64_t)(id - t * tiles_n) * BN_OUT;
       w += tile.x * p.we;
       sw += tile.x * p.swe;
@@ -412,6 +417,8 @@ struct MmKernel {
                                                    int t16, int g) {
     if (GATED) {
       store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
+    } else if (EPI == kSlots) {
+      store_slots(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
     } else if (!EXPERTS && p.ksplit) {
       MmArgs q = p;
       q.c = p.parts + (int64_t)blockIdx.y * p.M * p.N;
@@ -504,6 +511,35 @@ struct MmKernel {
       }
       wave_sync();
     }
+  }
+
+  // A slot's results wait in memory for the sum over its token's experts, and at
+  // four bytes they were a quarter of the layer's time (4096 tokens, 8 experts each,
+  // width 2048: 268 MB written and read).  They are held as binary16 over a power of two
+  // that brings the largest of the wave tile's columns below 4: 11 bits, whatever
+  // the magnitude, 2^-12 of a value where the sum's own rounding is 2^-9 or 2^-12.
+  __device__ static __forceinline__ void store_slots(const MmArgs& p, char LDS_AS* lds, f32x4 (&acc)[C::FM][C::FN],
+                                                     int64_t m0, int m_left, int64_t n0, int wave, int wm, int wn,
+                                                     int t16, int g) {
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = umax(m, abs_bits(acc[i][j][r]));
+      m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+      m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+      uint32_t e = m >> 23;
+      e = e < 27 ? 27 : e > 253 ? 253 : e;
+      const float inv = __uint_as_float((254 - e) << 23);
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) acc[i][j] *= inv;
+      const int row = wm * C::TM + 16 * i + t16;
+      if (g == 0 && row < m_left && n0 + wn * C::TN < p.N)
+        p.sq[(n0 / C::TN + wn) * p.ldsq + m0 + row] = __uint_as_float(e << 23);
+    }
+    store<f16>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
   }
 
   // h = silu(gate) * up of the tile's 128 columns, quantised: they are one block

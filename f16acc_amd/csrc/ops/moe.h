@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.h"
+#include "quant.h"
 
 namespace f16ops {
 
@@ -218,98 +219,121 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a) {
 
 // Slots (token t's j-th expert is slot t k + j) sorted by expert, in slot order
 // within one, without atomics on the order: every position is a count.
+// Two launches: chunks of slots are counted by expert (beside the quantising of
+// the tokens, which needs no sorting); then every chunk adds up the counts before
+// its own and places its slots, and the first also writes the products' tiles.
 struct SortArgs {
   const int* ids;
   int64_t slots;
-  int E, k, bm;   // bm: tokens per tile of the products
-  int* counts;    // [blocks][E]: a block's slots of each expert, then where they begin
-  int* rows;      // [sorted position] -> token
-  int* pos;       // [slot] -> sorted position, -1: none
-  int4* tiles;    // (expert, first, end, 0)
+  int E, k, bm;  // bm: tokens per tile of the products
+  int* counts;   // [chunks][E]
+  int* rows;     // [sorted position] -> token
+  int* pos;      // [slot] -> sorted position, -1: none
+  int4* tiles;   // (expert, first, end, 0)
   int* ntiles;
-  int blocks;
+  int chunks;
 };
-constexpr int kSortChunk = 2048;  // slots of one workgroup
+constexpr int kSortChunk = 512;  // slots of one workgroup
 
-__global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a) {
-  __shared__ int hist[kMaxExperts];
+__device__ __forceinline__ void count_chunk(const SortArgs& a, int chunk, int* hist) {
   for (int e = threadIdx.x; e < a.E; e += 256) hist[e] = 0;
   __syncthreads();
-  const int64_t s0 = (int64_t)blockIdx.x * kSortChunk;
-  for (int i = threadIdx.x; i < kSortChunk && s0 + i < a.slots; i += 256) {
-    const int e = a.ids[s0 + i];
+  const int64_t s0 = (int64_t)chunk * kSortChunk;
+#pragma unroll
+  for (int i = 0; i < kSortChunk; i += 256) {
+    const int64_t s = s0 + i + threadIdx.x;
+    const int e = s < a.slots ? a.ids[s] : -1;
     if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += 256) a.counts[(int64_t)blockIdx.x * a.E + e] = hist[e];
+  for (int e = threadIdx.x; e < a.E; e += 256) a.counts[(int64_t)chunk * a.E + e] = hist[e];
 }
 
-// One workgroup: where each block's slots of each expert begin, and the tiles.
-__global__ __launch_bounds__(1024) void sort_scan_kernel(SortArgs a) {
-  __shared__ int begin[kMaxExperts], first[kMaxExperts];
-  const int e = threadIdx.x;
-  int total = 0;
-  if (e < a.E)
-    for (int b = 0; b < a.blocks; ++b) total += a.counts[(int64_t)b * a.E + e];
-  const int tiles = (total + a.bm - 1) / a.bm;
-  begin[e] = total;
-  first[e] = tiles;
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void quant_count_kernel(QuantArgs q, SortArgs a) {
+  __shared__ int hist[kMaxExperts];
+  if ((int)blockIdx.x < a.chunks)
+    count_chunk(a, blockIdx.x, hist);
+  else
+    quant_rows<T, WIDE>(q, blockIdx.x - a.chunks, gridDim.x - a.chunks);
+}
+
+// The waves of a chunk take turns in slot order; within one, a slot's rank is
+// the number of lower lanes with its expert.
+__global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a) {
+  __shared__ int next[kMaxExperts], sums[kMaxExperts], first[kMaxExperts];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // per expert: all its slots, and those of earlier chunks; `per` threads an expert
+  for (int e = tid; e < kMaxExperts; e += 1024) sums[e] = next[e] = 0;
   __syncthreads();
-  for (int d = 1; d < kMaxExperts; d <<= 1) {
-    const int u = e >= d ? begin[e - d] : 0, v = e >= d ? first[e - d] : 0;
-    __syncthreads();
-    begin[e] += u;
-    first[e] += v;
-    __syncthreads();
+  int p2 = 1;
+  while (p2 < a.E) p2 <<= 1;
+  const int per = kMaxExperts / p2, e0 = tid & (p2 - 1), part = tid / p2;
+  if (e0 < a.E) {
+    int all = 0, before = 0;
+#pragma unroll 4
+    for (int c = part; c < a.chunks; c += per) {
+      const int n = a.counts[(int64_t)c * a.E + e0];
+      all += n;
+      before += c < (int)blockIdx.x ? n : 0;
+    }
+    if (all) atomicAdd(&sums[e0], all);
+    if (before) atomicAdd(&next[e0], before);
   }
-  if (e == kMaxExperts - 1) *a.ntiles = first[e];
-  if (e >= a.E) return;
-  int at = begin[e] - total;
-  const int end = begin[e];
-  for (int i = 0, t = first[e] - tiles; i < tiles; ++i, ++t)
-    a.tiles[t] = int4{e, at + i * a.bm, at + (i + 1) * a.bm < end ? at + (i + 1) * a.bm : end, 0};
-  for (int b = 0; b < a.blocks; ++b) {
-    int* c = a.counts + (int64_t)b * a.E + e;
-    const int n = *c;
-    *c = at;
-    at += n;
-  }
-}
-
-// A chunk's slots to their positions.  The waves take turns in slot order; within one, a
-// slot's rank is the number of lower lanes with its expert.
-__global__ __launch_bounds__(256) void sort_place_kernel(SortArgs a) {
-  __shared__ int next[kMaxExperts];
-  for (int e = threadIdx.x; e < a.E; e += 256) next[e] = a.counts[(int64_t)blockIdx.x * a.E + e];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t s0 = (int64_t)blockIdx.x * kSortChunk;
-  for (int i = 0; i < kSortChunk / 256; ++i) {
-    const int64_t s = s0 + i * 256 + threadIdx.x;
-    const int e = s < a.slots ? a.ids[s] : -1;
-    const bool in = e >= 0 && e < a.E;
-    uint64_t same = __builtin_amdgcn_ballot_w64(in);
+  __syncthreads();
+  const int total = sums[tid], tiles = (total + a.bm - 1) / a.bm;
+  __syncthreads();
+  // inclusive sums over the experts, of slots and of tiles
+  int begin = total, tile = tiles;
 #pragma unroll
-    for (int b = 0; b < 10; ++b) {
-      const uint64_t m = __builtin_amdgcn_ballot_w64((e >> b) & 1);
-      same &= (e >> b) & 1 ? m : ~m;
-    }
-    const int rank = __popcll(same & ((1ull << lane) - 1)), n = __popcll(same);
-    int p = -1;
-    for (int w = 0; w < 4; ++w) {
-      __syncthreads();
-      if (w == wave && in) {
-        p = next[e] + rank;
-        if (rank == n - 1) next[e] = p + 1;
-      }
-    }
-    if (s < a.slots) a.pos[s] = in ? p : -1;
-    if (in) a.rows[p] = (int)(s / a.k);
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(begin, d), v = __shfl_up(tile, d);
+    if (lane >= d) begin += u, tile += v;
   }
+  if (lane == 63) sums[wave] = begin, first[wave] = tile;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) begin += sums[w], tile += first[w];
+  next[tid] += begin - total;
+  if (blockIdx.x == 0) {
+    if (tid == kMaxExperts - 1) *a.ntiles = tile;
+    int at = begin - total;
+    for (int t = tile - tiles; t < tile; ++t, at += a.bm)
+      a.tiles[t] = int4{tid, at, at + a.bm < begin ? at + a.bm : begin, 0};
+  }
+  __syncthreads();
+  const int64_t s = (int64_t)blockIdx.x * kSortChunk + tid;
+  const bool mine = tid < kSortChunk && s < a.slots;
+  const int e = mine ? a.ids[s] : -1;
+  const bool in = e >= 0 && e < a.E;
+  uint64_t same = __builtin_amdgcn_ballot_w64(in);
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64((e >> b) & 1);
+    same &= (e >> b) & 1 ? m : ~m;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1)), n = __popcll(same);
+  int p = -1;
+#pragma unroll
+  for (int w = 0; w < kSortChunk / 64; ++w) {
+    if (w == wave && in) {
+      p = next[e] + rank;
+      if (rank == n - 1) next[e] = p + 1;
+    }
+    lds_barrier();
+  }
+  if (mine) a.pos[s] = p;
+  if (in) a.rows[p] = (int)(s / a.k);
 }
 
 // y[t] = sum_j weights[t][j] * ys[pos[t][j]], j in order, FP32, rounded once.
+// ys are binary16 over a power of two for each `block` columns.  A thread takes
+// eight columns; bound by reading ys.
 struct CombineArgs {
-  const float* ys;  // [slots][D]
+  const f16* ys;  // [slots][ld]
+  int64_t ld;
+  const float* scale;  // [ld / block][slots]
+  int block;
+  int64_t slots;
   const float* weights;
   int64_t wt, wk;
   const int* pos;
@@ -319,25 +343,31 @@ struct CombineArgs {
 };
 template <class T>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
-  const int64_t quads = cdiv(a.D, 4);
-  const int64_t t = blockIdx.x;
-  const bool wide = a.D % 4 == 0;
-  for (int64_t d = (int64_t)blockIdx.y * 256 + threadIdx.x; d < quads; d += (int64_t)gridDim.y * 256) {
-    const int left = (int)(a.D - 4 * d < 4 ? a.D - 4 * d : 4);
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j = 0; j < a.k; ++j) {
-      const int p = a.pos[t * a.k + j];
-      if (p < 0) continue;
-      const float w = a.weights[t * a.wt + j * a.wk];
-      const float* y = a.ys + p * a.D + 4 * d;
-      if (wide) {
-        sum += w * *(const f32x4*)y;
-      } else {
-        for (int r = 0; r < left; ++r) sum[r] += w * y[r];
-      }
-    }
-    T* y = (T*)a.y + t * a.D + 4 * d;
-    for (int r = 0; r < left; ++r) y[r] = (T)sum[r];
+  const int64_t t = blockIdx.x, n = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
+  if (n >= a.D) return;
+  float sum[8] = {};
+#pragma unroll 4
+  for (int j = 0; j < a.k; ++j) {
+    const int p = a.pos[t * a.k + j];
+    if (p < 0) continue;
+    const float w = a.weights[t * a.wt + j * a.wk] * a.scale[n / a.block * a.slots + p];
+    float v[8];
+    load_vec(a.ys + p * a.ld + n, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+  }
+  T* y = (T*)a.y + t * a.D + n;
+  if (a.D % 8 == 0) {
+    struct alignas(16) Pack {
+      T t[8];
+    } o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.t[i] = (T)sum[i];
+    *(Pack*)y = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < a.D) y[i] = (T)sum[i];
   }
 }
 

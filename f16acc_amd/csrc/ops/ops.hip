@@ -57,7 +57,7 @@ int out_check(const uint8_t* q, int64_t ldq, int64_t cols, const float* s) {
   return 0;
 }
 
-int quant_rows(const QuantArgs& p, int type, hipStream_t stream) {
+int launch_quant_rows(const QuantArgs& p, int type, hipStream_t stream) {
   const int64_t groups = cdiv(p.rows * (p.ldq / kBlock), 16);
   if (groups == 0) return 0;
   const uint32_t grid = (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus);
@@ -218,45 +218,50 @@ int mm_run(MmArgs p, const MmPlan& plan, void* workspace, hipStream_t stream) {
   });
 }
 
-// The experts' tiles: gate and up, 128 columns of each; down.
-template <int BM>
+// The experts' tiles by the mean number of tokens an expert has: gate and up (128
+// columns of each), down.  4096 tokens, 8 of 64 experts each, 2048 x 1024, gate and up /
+// down: 232 / 202 us on 256, 256 / 167 on 128; with 25 tokens an expert
+// 110 us in all on 128, 124 on 32; with 10 106 and 105.
+template <int ROWS>
 struct ExpertCfg;
 template <>
 struct ExpertCfg<32> {
-  using GateUp = MmCfg<32, 256, 1, 4, 2, 1>;
-  using Down = MmCfg<32, 128, 1, 4, 3, 2>;
-};
-template <>
-struct ExpertCfg<64> {
-  using GateUp = MmCfg<64, 256, 1, 4, 2, 1>;
-  using Down = MmCfg<64, 128, 1, 4, 3, 2>;
+  using GateUp = MmCfg<32, 256, 1, 4, 4, 1>;
+  using Down = MmCfg<32, 64, 1, 2, 4, 2>;
 };
 template <>
 struct ExpertCfg<128> {
-  using GateUp = MmCfg<128, 256, 2, 2, 2, 1>;
+  using GateUp = MmCfg<128, 256, 2, 4, 2, 2>;
+  using Down = MmCfg<128, 128, 2, 2, 2, 2>;
+};
+template <>
+struct ExpertCfg<256> {
+  using GateUp = MmCfg<256, 256, 4, 2, 2, 2>;
   using Down = MmCfg<128, 128, 2, 2, 2, 2>;
 };
 
 int expert_tile(int64_t slots, int E) {
   const int64_t mean = slots / E;
-  return mean >= 96 ? 128 : mean >= 32 ? 64 : 32;
+  return mean >= 192 ? 256 : mean >= 24 ? 128 : 32;
 }
+int down_block(int tile) { return tile == 32 ? ExpertCfg<32>::Down::TN : ExpertCfg<128>::Down::TN; }
 
 // Whether the two kernels for a few tokens run.
 bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots && k <= kFewK; }
 
 struct ExpertsPlan {
-  int64_t slots, blocks, max_tiles, Dp, Ip;
+  int64_t slots, chunks, max_tiles, Dp, Ip;
   int bm;
   size_t few;  // bytes of the hidden values of the kernels for a few tokens
-  size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
+  int64_t ldy;
+  size_t xq, xs, hq, hs, ys, yscale, counts, rows, pos, tiles, ntiles, total;
   ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     slots = T * k;
     Dp = up128(D);
     Ip = up128(I);
     few = few_tokens(T, k) ? (size_t)slots * Ip * 4 : 0;
     bm = expert_tile(slots, E);
-    blocks = cdiv(slots, kSortChunk);
+    chunks = cdiv(slots, kSortChunk);
     max_tiles = slots / bm + (slots < E ? slots : E);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -268,8 +273,10 @@ struct ExpertsPlan {
     xs = take(T * (Dp / kBlock) * 4);
     hq = take(slots * Ip);
     hs = take(slots * (Ip / kBlock) * 4);
-    ys = take(slots * D * 4);
-    counts = take(blocks * E * 4);
+    ldy = cdiv(D, 8) * 8;
+    ys = take(slots * ldy * 2);
+    yscale = take(cdiv(D, down_block(bm)) * slots * 4);
+    counts = take(chunks * E * 4);
     rows = take(slots * 4);
     pos = take(slots * 4);
     tiles = take(max_tiles * 16);
@@ -282,7 +289,8 @@ template <int BM>
 int expert_products(const MmArgs& gu, const MmArgs& down, int64_t max_tiles, hipStream_t stream) {
   const int rc = launch_mm<typename ExpertCfg<BM>::GateUp, false, true, kGatedQuant>(gu, max_tiles, stream);
   if (rc) return rc;
-  return launch_mm<typename ExpertCfg<BM>::Down, false, true, kStore>(down, max_tiles, stream);
+  using Down = typename ExpertCfg<BM>::Down;
+  return launch_mm<Down, false, true, kSlots>(down, max_tiles * (BM / Down::BM), stream);
 }
 
 template <template <class, int> class Launch, class... A>
@@ -329,7 +337,7 @@ int f16acc_quant_rows(const void* x, int type, int64_t rows, int64_t cols, int64
   rc = out_check(q, ldq, cols, s);
   if (rc) return rc;
   QuantArgs p{x, rows, cols, sr, sc, q, ldq, s, lds, nullptr, 0, nullptr, 0};
-  return quant_rows(p, type, (hipStream_t)stream);
+  return launch_quant_rows(p, type, (hipStream_t)stream);
 }
 
 int f16acc_quant_both(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
@@ -345,7 +353,7 @@ int f16acc_quant_both(const void* x, int type, int64_t rows, int64_t cols, int64
   QuantArgs p{x, rows, cols, sr, sc, q, ldq, s, lds, qt, ldqt, st, ldst};
   if (q && qt) return quant_tile<true, true, false>(p, type, (hipStream_t)stream);
   if (qt) return quant_tile<false, true, false>(p, type, (hipStream_t)stream);
-  return quant_rows(p, type, (hipStream_t)stream);
+  return launch_quant_rows(p, type, (hipStream_t)stream);
 }
 
 int f16acc_quant_weight(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
@@ -439,7 +447,7 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
     });
   }
   QuantArgs q{x, M, K, sr, sc, (uint8_t*)workspace, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
-  rc = quant_rows(q, type, (hipStream_t)stream);
+  rc = launch_quant_rows(q, type, (hipStream_t)stream);
   if (rc) return rc;
   return mm_run<false>(p, mm_plan(M, N, K, false, -1, 0),
                        (char*)workspace + up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4), (hipStream_t)stream);
@@ -509,14 +517,20 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
     });
   }
   QuantArgs q{x, T, D, sr, sc, (uint8_t*)(ws + plan.xq), plan.Dp, (float*)(ws + plan.xs), T, nullptr, 0, nullptr, 0};
-  rc = quant_rows(q, type, stream);
-  if (rc) return rc;
   SortArgs so{ids, plan.slots, E, k, plan.bm, (int*)(ws + plan.counts), (int*)(ws + plan.rows), (int*)(ws + plan.pos),
-              (int4*)(ws + plan.tiles), (int*)(ws + plan.ntiles), (int)plan.blocks};
-  hipLaunchKernelGGL(sort_count_kernel, dim3(so.blocks), dim3(256), 0, stream, so);
-  hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, stream, so);
-  hipLaunchKernelGGL(sort_place_kernel, dim3(so.blocks), dim3(256), 0, stream, so);
-  rc = hip_status();
+              (int4*)(ws + plan.tiles), (int*)(ws + plan.ntiles), (int)plan.chunks};
+  const int64_t groups = cdiv(T * (plan.Dp / kBlock), 16);
+  const dim3 quant_grid((uint32_t)(so.chunks + (groups < 16 * kCus ? groups : 16 * kCus)));
+  const bool wide = wide_loads(x, type, sr, sc);
+  rc = by_type(type, [&](auto* t) {
+    using U = std::remove_pointer_t<decltype(t)>;
+    if (wide)
+      hipLaunchKernelGGL((quant_count_kernel<U, true>), quant_grid, dim3(256), 0, stream, q, so);
+    else
+      hipLaunchKernelGGL((quant_count_kernel<U, false>), quant_grid, dim3(256), 0, stream, q, so);
+    hipLaunchKernelGGL(sort_place_kernel, dim3(so.chunks), dim3(1024), 0, stream, so);
+    return hip_status();
+  });
   if (rc) return rc;
 
   MmArgs gu{};
@@ -528,16 +542,19 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   MmArgs down{};
   down.x = gu.q, down.ldx = plan.Ip, down.sx = gu.sq, down.sxm = 1, down.sxk = plan.slots;
   down.w = w2, down.ldw = ld2, down.sw = s2, down.swn = s2n, down.swk = s2k, down.we = w2e, down.swe = s2e;
-  down.c = ws + plan.ys, down.scm = D, down.scn = 1, down.ctype = F16ACC_TYPE_F32;
+  down.c = ws + plan.ys, down.scm = plan.ldy, down.scn = 1;
+  down.sq = (float*)(ws + plan.yscale), down.ldsq = plan.slots;
+  gu.tile_rows = down.tile_rows = plan.bm;
   down.M = plan.slots, down.N = D, down.K = I;
   down.tiles = so.tiles, down.ntiles = so.ntiles, down.rows = nullptr, down.xrows = plan.slots;
-  rc = plan.bm == 128  ? expert_products<128>(gu, down, plan.max_tiles, stream)
-       : plan.bm == 64 ? expert_products<64>(gu, down, plan.max_tiles, stream)
-                       : expert_products<32>(gu, down, plan.max_tiles, stream);
+  rc = plan.bm == 256   ? expert_products<256>(gu, down, plan.max_tiles, stream)
+       : plan.bm == 128 ? expert_products<128>(gu, down, plan.max_tiles, stream)
+                        : expert_products<32>(gu, down, plan.max_tiles, stream);
   if (rc) return rc;
 
-  CombineArgs co{(const float*)(ws + plan.ys), weights, wt, wk, so.pos, T, D, k, y};
-  const dim3 grid((uint32_t)T, (uint32_t)cdiv(cdiv(D, 4), 256));
+  CombineArgs co{(const f16*)(ws + plan.ys), plan.ldy, down.sq, down_block(plan.bm), plan.slots, weights, wt, wk,
+                 so.pos, T, D, k, y};
+  const dim3 grid((uint32_t)T, (uint32_t)cdiv(cdiv(D, 8), 256));
   return by_type(type, [&](auto* t) {
     using U = std::remove_pointer_t<decltype(t)>;
     hipLaunchKernelGGL((combine_kernel<U>), grid, dim3(256), 0, stream, co);

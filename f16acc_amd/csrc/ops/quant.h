@@ -25,11 +25,11 @@ struct QuantArgs {
 // finds each block's maximum with four row rotations and writes 8 bytes a
 // lane.  Bound by memory: 2 bytes read and 1 written an element.
 template <class T, bool WIDE>
-__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
+__device__ __forceinline__ void quant_rows(const QuantArgs& p, uint32_t group, uint32_t groups) {
   const int64_t blocks = p.ldq / kBlock;
   const int64_t total = p.rows * blocks;
   const int lane = threadIdx.x & 15;
-  for (int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)gridDim.x * 16) {
+  for (int64_t b = (int64_t)group * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)groups * 16) {
     // (64-bit division is a hundred instructions)
     const int64_t row = total >> 32 ? b / blocks : (int64_t)((uint32_t)b / (uint32_t)blocks), kb = b - row * blocks;
     const int64_t c0 = kb * kBlock + lane * 8;
@@ -52,6 +52,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
     *(i32x2*)(p.q + row * p.ldq + c0) = o;
     if (lane == 0) p.s[kb * p.lds + row] = bs.s;
   }
+}
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
+  quant_rows<T, WIDE>(p, blockIdx.x, gridDim.x);
 }
 
 // A 128 x 128 tile a workgroup: read once, quantised along its rows (ROWS), its
