@@ -35,7 +35,7 @@ _SIGNATURES = {
                       + [_vp] + [_i64] * 3 + [_vp] + [_i64] * 4 + [_vp] + [_i64] * 2 + [_vp] + [_i64] * 3
                       + [_vp, _vp, _size, _vp],
     "f16acc_mm_fp8_workspace": [_i64] * 3 + [_int] * 3,
-    "f16acc_linear_fp8_workspace": [_i64] * 3,
+    "f16acc_linear_fp8_workspace": [_i64] * 3 + [_vp, _i64],
     "f16acc_experts_workspace": [_i64, _int, _int, _i64, _i64],
     "f16acc_ops_strerror": [_int],
     "f16acc_ops_abi_version": [],

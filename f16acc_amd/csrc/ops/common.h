@@ -114,6 +114,9 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = (float)k.t[i];
 }
 
+// SiLU with FP32's accuracy, where few values are asked for and what is
+// quantised from them should fall on the right side of a tie.
+__device__ __forceinline__ float silu_exact(float g) { return g / (1.0f + expf(-g)); }
 // SiLU, to a few units in the last place: the hardware's exponential and
 // reciprocal (a correctly rounded quotient was a fifth of the gated product's time).
 __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }

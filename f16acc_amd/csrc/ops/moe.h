@@ -22,6 +22,8 @@ struct RouteArgs {
   const float* dw;  // [T][k], stride dwt between tokens, dwk between experts
   int64_t dwt, dwk;
   void* dx;  // [T][E] contiguous
+  bool wide;     // a lane's V logits are one load
+  int lanes;     // lanes of a group where that is a power of two, else 0
 };
 
 // Order-preserving map of a float to an unsigned integer, -inf lowest; 0 is
@@ -55,12 +57,16 @@ __device__ __forceinline__ void scores(const RouteArgs& a, int64_t t, int lane, 
                                        bool* nan) {
   const T* row = (const T*)a.x + t * a.st;
   bool bad = false;
+  if (a.wide) {  // V divides E and rows are aligned to V elements
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    x[i] = e < a.E ? (float)row[e * a.se] : -INFINITY;
-    bad |= x[i] != x[i];
+    for (int i = 0; i < V; ++i) x[i] = -INFINITY;
+    if (lane * V < a.E) load_vec(row + lane * V, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = lane * V + i < a.E ? (float)row[(lane * V + i) * a.se] : -INFINITY;
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) bad |= x[i] != x[i];
   *nan = __builtin_amdgcn_ballot_w64(bad) != 0;
   if (a.sigmoid) {
 #pragma unroll
@@ -97,6 +103,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   bool nan;
   scores<T, V>(a, t, lane, x, p, &nan);
   uint32_t key[V];
+  float keys[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = lane * V + i;
@@ -104,10 +111,37 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     if (a.sigmoid || a.bias) f = p[i] + (a.bias && e < a.E ? a.bias[e] : 0.0f);
     if (!(x[i] > -INFINITY) || !(f > -INFINITY) || e >= a.E) f = -INFINITY;
     key[i] = f > -INFINITY ? sortable(f + 0.0f) : 0u;  // (-0 and 0 are a tie)
-    if (a.groups > 1) lds[wave][e] = f;
+    keys[i] = f;
   }
-  if (a.groups > 1) {
-    // a lane per group: its best key, or for sigmoid scores its best two's sum
+  if (a.lanes) {
+    // groups of whole lanes: the best key, for sigmoid scores the best two's sum, by
+    // exchanges within the group's lanes
+    float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      b2 = fmaxf(b2, fminf(b1, keys[i]));
+      b1 = fmaxf(b1, keys[i]);
+    }
+    for (int d = 1; d < a.lanes; d <<= 1) {
+      const float o1 = __shfl_xor(b1, d), o2 = __shfl_xor(b2, d);
+      b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+      b1 = fmaxf(b1, o1);
+    }
+    const float score = a.sigmoid && b2 > -INFINITY ? b1 + b2 : b1;
+    const int mine = lane / a.lanes;
+    int rank = 0;
+    for (int j = 0; j < a.groups; ++j) {
+      const float o = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(score), j * a.lanes));
+      rank += o > score || (o == score && j < mine);
+    }
+    if (rank >= a.top) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = 0u;
+    }
+  } else if (a.groups > 1) {
+    // a lane per group
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = keys[i];
     wave_sync();
     const int size = a.E / a.groups;
     float b1 = -INFINITY, b2 = -INFINITY;
@@ -207,13 +241,21 @@ __global__ __launch_bounds__(256) void route_grad_kernel(RouteArgs a) {
     dot += dp[i] * p[i];
   }
   if (!a.sigmoid) dot = wave_sum(dot);
-  T* out = (T*)a.dx + t * a.E;
+  T* out = (T*)a.dx + t * a.E + lane * V;
+  struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Pack {
+    T t[V];
+  } o;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    float d = a.sigmoid ? dp[i] * p[i] * (1.0f - p[i]) : p[i] * (dp[i] - dot);
-    if (nan) d = __uint_as_float(0x7fc00000u);
-    if (e < a.E) out[e] = (T)d;
+    const float d = a.sigmoid ? dp[i] * p[i] * (1.0f - p[i]) : p[i] * (dp[i] - dot);
+    o.t[i] = (T)(nan ? __uint_as_float(0x7fc00000u) : d);
+  }
+  if (a.E % V == 0) {  // (the rows are aligned to V elements then: dx is contiguous)
+    if (lane * V < a.E) *(Pack*)out = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane * V + i < a.E) out[i] = o.t[i];
   }
 }
 

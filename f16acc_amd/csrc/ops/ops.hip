@@ -218,6 +218,22 @@ int mm_run(MmArgs p, const MmPlan& plan, void* workspace, hipStream_t stream) {
   });
 }
 
+// The workspace of linear: the quantised tokens and their scales, the weight where its rows
+// have to be copied, the parts of a split of K.
+struct LinearPlan {
+  bool packed;
+  int64_t ld;
+  size_t scales, weight, parts, total;
+  LinearPlan(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
+    packed = !aligned16(w) || ldw % 16 || K % 16 || ldw > kMaxRow;
+    ld = cdiv(K, 16) * 16;
+    scales = up256(M * up128(K));
+    weight = scales + up256(M * cdiv(K, kBlock) * 4);
+    parts = weight + (packed ? up256(N * ld) : 0);
+    total = parts + up256(parts_bytes(mm_plan(M, N, K, false, -1, 0), M, N));
+  }
+};
+
 // The experts' tiles by the mean number of tokens an expert has: gate and up (128
 // columns of each), down.  4096 tokens, 8 of 64 experts each, 2048 x 1024, gate and up /
 // down: 232 / 202 us on 256, 256 / 167 on 128; with 25 tokens an expert
@@ -304,16 +320,26 @@ int by_experts(int E, int type, A&&... args) {
     return Launch<T, 16>::go(args...);
   });
 }
+// What the scores' loads and the groups' exchanges rely on, for V experts a lane.
+template <class T, int V>
+RouteArgs route_args(RouteArgs a) {
+  a.wide = a.se == 1 && a.E % V == 0 && a.st % V == 0 && (uintptr_t)a.x % (V * sizeof(T) < 16 ? V * sizeof(T) : 16) == 0;
+  const int size = a.groups ? a.E / a.groups : 0, lanes = size / V;
+  a.lanes = a.groups > 1 && size % V == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  return a;
+}
 template <class T, int V>
 struct LaunchRoute {
-  static int go(const RouteArgs& a, hipStream_t s) {
+  static int go(RouteArgs a, hipStream_t s) {
+    a = route_args<T, V>(a);
     hipLaunchKernelGGL((route_kernel<T, V>), dim3((uint32_t)cdiv(a.T, 4)), dim3(256), 0, s, a);
     return hip_status();
   }
 };
 template <class T, int V>
 struct LaunchRouteGrad {
-  static int go(const RouteArgs& a, hipStream_t s) {
+  static int go(RouteArgs a, hipStream_t s) {
+    a = route_args<T, V>(a);
     hipLaunchKernelGGL((route_grad_kernel<T, V>), dim3((uint32_t)cdiv(a.T, 4)), dim3(256), 0, s, a);
     return hip_status();
   }
@@ -408,29 +434,26 @@ size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, 
   return up256(parts_bytes(mm_plan(M, N, K, row_scales != 0, tile, splits), M, N));
 }
 
-size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
+size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4) + f16acc_mm_fp8_workspace(M, N, K, 0, -1, 0);
+  return LinearPlan(M, N, K, w, ldw).total;
 }
 
 int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw, const float* sw,
                       int64_t swn, int64_t swk, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
-                      void* workspace, size_t ws_bytes, void* stream) {
+                      void* workspace, size_t ws_bytes, void* stream_) {
   int rc = quant_check(x, type, M, K);
   if (rc) return rc;
-  MmArgs p{};
-  p.x = (const uint8_t*)workspace, p.ldx = up128(K);
-  p.sx = (const float*)((const char*)workspace + up256(M * up128(K))), p.sxm = 1, p.sxk = M;
-  p.w = w, p.ldw = ldw, p.sw = sw, p.swn = swn, p.swk = swk;
-  p.bias = bias, p.c = y, p.scm = N, p.scn = 1, p.M = M, p.N = N, p.K = K, p.ctype = type;
-  if (M > 0 && N > 0 && K > 0 &&
-      (!workspace || (uintptr_t)workspace % 256 || ws_bytes < f16acc_linear_fp8_workspace(M, N, K)))
-    return F16ACC_OPS_E_WORKSPACE;
-  rc = mm_check(p);
-  if (rc || M == 0 || N == 0) return rc;
-  // Few tokens: one launch.  From 9 on its quantising, repeated by every workgroup, costs more
-  // than a pass of its own where there are many (16 tokens: 8960 x 1536 11.5 us against 12.4 on the
-  // tiles, 8192 x 8192 32 against 25).
+  if (N < 0) return F16ACC_OPS_E_ARG;
+  if (M == 0 || N == 0) return 0;
+  if (K == 0 || !w || !sw || !y || swn < 0 || swk < 0) return F16ACC_OPS_E_ARG;
+  if (ldw < K && N > 1) return F16ACC_OPS_E_UNSUPPORTED;
+  hipStream_t stream = (hipStream_t)stream_;
+  const LinearPlan plan(M, N, K, w, ldw);
+  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
+  // Few tokens: one launch, from the rows as they are.  From 9 tokens on its quantising,
+  // repeated by every workgroup, costs more than a pass of its own where there are many (16 tokens:
+  // 8960 x 1536 11.5 us against 12.4 on the tiles, 8192 x 8192 32 against 25).
   if ((M <= 8 || (M <= 16 && N * K <= (1 << 25))) && wide_loads(x, type, sr, sc)) {
     SmallArgs a{x, sr, w, ldw, sw, swn, swk, bias, y, N, 1, M, N, K};
     return by_tokens((int)M, type, [&](auto* t, auto groups) {
@@ -438,25 +461,47 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
       constexpr int G = decltype(groups)::value;
       // 16 waves deal K where the rows alone leave CUs idle
       if (cdiv(N, 16) < kCus && cdiv(K, kBlock) >= 16)
-        hipLaunchKernelGGL((linear_small_kernel<T, 16, G>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL((linear_small_kernel<T, 16, G>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), 0, stream, a);
       else
-        hipLaunchKernelGGL((linear_small_kernel<T, 8, G>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL((linear_small_kernel<T, 8, G>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0, stream, a);
       return hip_status();
     });
   }
-  QuantArgs q{x, M, K, sr, sc, (uint8_t*)workspace, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
-  rc = launch_quant_rows(q, type, (hipStream_t)stream);
+  char* ws = (char*)workspace;
+  MmArgs p{};
+  p.x = (const uint8_t*)ws, p.ldx = up128(K);
+  p.sx = (const float*)(ws + plan.scales), p.sxm = 1, p.sxk = M;
+  p.w = plan.packed ? (const uint8_t*)ws + plan.weight : w, p.ldw = plan.packed ? plan.ld : ldw;
+  p.sw = sw, p.swn = swn, p.swk = swk;
+  p.bias = bias, p.c = y, p.scm = N, p.scn = 1, p.M = M, p.N = N, p.K = K, p.ctype = type;
+  rc = mm_check(p);
   if (rc) return rc;
-  return mm_run<false>(p, mm_plan(M, N, K, false, -1, 0),
-                       (char*)workspace + up256(M * up128(K)) + up256(M * cdiv(K, kBlock) * 4), (hipStream_t)stream);
+  QuantArgs q{x, M, K, sr, sc, (uint8_t*)ws, p.ldx, (float*)p.sx, M, nullptr, 0, nullptr, 0};
+  if (plan.packed) {
+    Pack8Args pk{w, (uint8_t*)p.w, N, K, ldw, 1, plan.ld};
+    const int64_t packs = cdiv(N * (plan.ld / 16), 256), groups = cdiv(M * (p.ldx / kBlock), 16);
+    const uint32_t np = (uint32_t)(packs < 16 * kCus ? packs : 16 * kCus);
+    const dim3 grid(np + (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus));
+    const bool wide = wide_loads(x, type, sr, sc);
+    rc = by_type(type, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      if (wide)
+        hipLaunchKernelGGL((quant_pack_kernel<T, true>), grid, dim3(256), 0, stream, q, pk, np);
+      else
+        hipLaunchKernelGGL((quant_pack_kernel<T, false>), grid, dim3(256), 0, stream, q, pk, np);
+      return hip_status();
+    });
+  } else {
+    rc = launch_quant_rows(q, type, stream);
+  }
+  if (rc) return rc;
+  return mm_run<false>(p, mm_plan(M, N, K, false, -1, 0), ws + plan.parts, stream);
 }
 
 int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
                  const float* bias, int groups, int top, int renorm, float scale, float* weights, int* ids,
                  void* stream) {
-  RouteArgs a{logits, T, st, se, E, k, sigmoid, bias, groups, top, renorm, scale, weights, ids, nullptr, 0, 0, nullptr};
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, bias, groups, top, renorm, scale, weights, ids, nullptr, 0, 0, nullptr, false, 0};
   const int rc = route_check(a, type);
   if (rc) return rc;
   if (groups < 1 || E % groups || top < 1 || top > groups || k > E / groups * top || (T && !weights))
@@ -469,10 +514,11 @@ int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se
 int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
                       int renorm, float scale, const int* ids, const float* dw, int64_t dwt, int64_t dwk,
                       void* dlogits, void* stream) {
-  RouteArgs a{logits, T, st, se, E, k, sigmoid, nullptr, 1, 1, renorm, scale, nullptr, (int*)ids, dw, dwt, dwk, dlogits};
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, nullptr, 1, 1, renorm, scale, nullptr, (int*)ids, dw, dwt, dwk, dlogits, false, 0};
   const int rc = route_check(a, type);
   if (rc) return rc;
   if (T && (!dw || !dlogits)) return F16ACC_OPS_E_ARG;
+  if (!aligned16(dlogits)) return F16ACC_OPS_E_UNSUPPORTED;
   if (T == 0) return 0;
   return by_experts<LaunchRouteGrad>(E, type, a, (hipStream_t)stream);
 }

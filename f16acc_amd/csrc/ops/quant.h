@@ -165,10 +165,10 @@ struct Pack8Args {
   uint8_t* dst;
   int64_t rows, cols, s_r, s_c, ld;
 };
-__global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) {
+__device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32_t groups) {
   const int64_t units = p.ld / 16, total = p.rows * units;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / units, c = (i - r * units) * 16;
+  for (int64_t i = (int64_t)group * 256 + threadIdx.x; i < total; i += (int64_t)groups * 256) {
+    const int64_t r = total >> 32 ? i / units : (int64_t)((uint32_t)i / (uint32_t)units), c = (i - r * units) * 16;
     const uint8_t* s = p.src + r * p.s_r;
     union {
       uint8_t b[16];
@@ -182,6 +182,17 @@ __global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) {
     }
     *(i32x4*)(p.dst + r * p.ld + c) = o.v;
   }
+}
+__global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) { pack8(p, blockIdx.x, gridDim.x); }
+
+// Both at once, for a product of new tokens with a weight whose rows are not aligned: the
+// first `packs` workgroups copy.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void quant_pack_kernel(QuantArgs q, Pack8Args p, uint32_t packs) {
+  if (blockIdx.x < packs)
+    pack8(p, blockIdx.x, packs);
+  else
+    quant_rows<T, WIDE>(q, blockIdx.x - packs, gridDim.x - packs);
 }
 
 }  // namespace f16ops

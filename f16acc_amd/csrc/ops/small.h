@@ -65,12 +65,30 @@ __device__ __forceinline__ i32x8 quant_tokens(TokenBlock& b, Row row, int tokens
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A lane's share of block kb of a weight row (zero from K to the next multiple
-// of 16).
+// A lane's share of block kb of a weight row, at any address (a 16-byte load goes
+// from any, and costs the same from an aligned one).
+__device__ __forceinline__ i32x4 load_unit(const uint8_t* w, int64_t k, int64_t K) {
+  union {
+    uint8_t b[16];
+    i32x4 v;
+  } u;
+  u.v = i32x4{0, 0, 0, 0};
+  if (k + 16 <= K) {
+    __builtin_memcpy(u.b, w + k, 16);
+  } else {
+#pragma unroll 1
+    for (int i = 0; k + i < K; ++i) {
+      const int byte = w[k + i] << (8 * (i & 3));
+      u.v[0] |= i < 4 ? byte : 0;
+      u.v[1] |= i >= 4 && i < 8 ? byte : 0;
+      u.v[2] |= i >= 8 && i < 12 ? byte : 0;
+      u.v[3] |= i >= 12 ? byte : 0;
+    }
+  }
+  return u.v;
+}
 __device__ __forceinline__ i32x8 load_weight(const uint8_t* w, int64_t k0, int64_t K, int g) {
-  i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-  if (k0 + 16 * g < K) lo = *(const i32x4*)(w + k0 + 16 * g);
-  if (k0 + 64 + 16 * g < K) hi = *(const i32x4*)(w + k0 + 64 + 16 * g);
+  const i32x4 lo = load_unit(w, k0 + 16 * g, K), hi = load_unit(w, k0 + 64 + 16 * g, K);
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -269,7 +287,7 @@ __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
   const int64_t n = n0 + 16 * wave + 4 * g;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (n + r < p.I) p.h[slot * p.ldh + n + r] = silu(gate[r]) * up[r];
+    if (n + r < p.I) p.h[slot * p.ldh + n + r] = silu_exact(gate[r]) * up[r];
 }
 
 // y of 16 columns: the waves deal the (expert, block of I) pairs, the next one's

@@ -263,9 +263,11 @@ struct Train : torch::autograd::Function<Train> {
 Tensor stored(const Tensor& x, const Tensor& w_, const Tensor& w_scale, const Maybe& bias) {
   const Tensor x2 = rows_of(x);
   const int64_t M = x2.size(0), K = x2.size(1), N = w_.size(0);
-  const Operand w = packed(w_);
+  // rows of any alignment go as they are (the library copies them where it has to)
+  const bool rows = (K <= 1 || w_.stride(1) == 1) && (N <= 1 || w_.stride(0) >= K);
+  const Operand w = rows ? Operand{w_, N > 1 ? w_.stride(0) : up(K, 16)} : packed(w_);
   Tensor y = empty(with_last(x, N), x, x.scalar_type());
-  const size_t n = f16acc_linear_fp8_workspace(M, N, K);
+  const size_t n = f16acc_linear_fp8_workspace(M, N, K, bytes(w.q), w.ld);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);
   check_rc(f16acc_linear_fp8(x2.const_data_ptr(), type_of(x), x2.stride(0), x2.stride(1), bytes(w.q), w.ld,

@@ -85,10 +85,11 @@ size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, 
 
 /*
  * y = x w^T + bias with x [M, K] of `type` (element strides sr, sc) quantised in row blocks on
- * the way and w, sw a square-block weight as in f16acc_mm_fp8; y [M][N] contiguous and bias of the same
- * type.  Needs a workspace of f16acc_linear_fp8_workspace bytes, 256-byte aligned.
+ * the way; w [N][ldw] bytes of any alignment, ldw at least K, with square-block scales sw as in
+ * f16acc_mm_fp8; y [M][N] contiguous and bias of x's type; K at least 1.
+ * Workspace of f16acc_linear_fp8_workspace bytes, 256-byte aligned.
  */
-size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K);
+size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw);
 int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw, const float* sw,
                       int64_t swn, int64_t swk, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
                       void* workspace, size_t ws_bytes, void* stream);
@@ -109,8 +110,8 @@ int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se
                  const float* bias, int groups, int top, int renorm, float scale, float* weights, int* ids,
                  void* stream);
 
-/* Gradient of f16acc_route's weights: dw [T][k] (element strides dwt, dwk) to dlogits [T][E], contiguous, of the
- * logits' type. */
+/* Gradient of f16acc_route's weights: dw [T][k] (element strides dwt, dwk) to dlogits [T][E], contiguous, 16-byte
+ * aligned, of the logits' type. */
 int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
                       int renorm, float scale, const int* ids, const float* dw, int64_t dwt, int64_t dwk,
                       void* dlogits, void* stream);

@@ -214,6 +214,23 @@ def test_linear_stored_weight(M, N, K, bias, dtype):
     ref.check_product(y, ref.rounded(x), ref.values(w, ws, 128), b)
 
 
+@pytest.mark.parametrize("M", [1, 7, 12, 40, 200])
+def test_linear_weight_rows_at_any_address(M):
+    """Rows that start anywhere and end anywhere, NaN bytes around them; a row-major [K, N] weight."""
+    K, N = 403, 70
+    w, ws = weight(N, K)
+    x = normal(M, K)
+    want = fp8.linear(x, w, ws)
+    ref.check_product(want, ref.rounded(x), ref.values(w, ws, 128))
+    for pad, off in ((5, 3), (13, 0), (45, 16), (16, 8)):
+        hold = torch.full((N * (K + pad) + 64,), float("nan")).to(F8).to(DEV)
+        v = hold[off:off + N * (K + pad)].view(N, K + pad)[:, :K]
+        v.copy_(w)
+        assert torch.equal(fp8.linear(x, v, ws), want)
+    assert torch.equal(fp8.linear(x, w.t().contiguous().t(), ws), want)
+    assert torch.equal(fp8.linear(x, w[:1], ws[:1]), fp8.linear(x, w[:1].clone(), ws[:1]))
+
+
 def test_linear_views_and_leading_dimensions():
     w, ws = weight(96, 256)
     x = normal(4, 6, 512)

@@ -60,14 +60,18 @@ def test_quantisation_checks():
 
 
 def test_linear_and_workspace_checks():
-    need = _ops.linear_fp8_workspace(100, 64, 300)
-    assert need >= 100 * 384 + 100 * 3 * 4 and _ops.linear_fp8_workspace(0, 64, 300) == 0
+    need = _ops.linear_fp8_workspace(100, 64, 300, 256, 304)
+    assert need >= 100 * 384 + 100 * 3 * 4 and _ops.linear_fp8_workspace(0, 64, 300, 256, 304) == 0
+    # K is no multiple of 16, or the rows are not aligned: room for a copy of the weight
+    assert need >= _ops.linear_fp8_workspace(100, 64, 304, 256, 304) + 64 * 304
+    assert _ops.linear_fp8_workspace(100, 64, 304, 264, 304) >= _ops.linear_fp8_workspace(100, 64, 304, 256, 304) + 64 * 304
 
-    def call(ws=256, n=need, M=100, t=0):
-        return _ops.linear_fp8(256, t, 300, 1, 256, 304, 256, 3, 1, None, 256, M, 64, 300, ws, n, None)
+    def call(ws=256, n=need, M=100, t=0, ldw=304, K=300, w=256):
+        return _ops.linear_fp8(256, t, 300, 1, w, ldw, 256, 3, 1, None, 256, M, 64, K, ws, n, None)
 
     assert call(ws=None) == call(n=need - 1) == call(ws=128) == _ops.E_WORKSPACE
-    assert call(t=4) == call(M=-2) == _ops.E_ARG
+    assert call(t=4) == call(M=-2) == call(K=0) == call(w=None) == _ops.E_ARG
+    assert call(ldw=299) == _ops.E_UNSUPPORTED and call(M=0) == 0
 
 
 def test_route_checks():
@@ -79,6 +83,7 @@ def test_route_checks():
     assert call(E=1025) == call(E=130, groups=65, k=1) == call(E=200, k=65) == _ops.E_UNSUPPORTED
     assert call(T=0) == 0
     assert _ops.route_grad(256, 0, 4, 16, 1, 16, 2, 0, 1, 1.0, 256, None, 2, 1, 256, None) == _ops.E_ARG
+    assert _ops.route_grad(256, 0, 4, 16, 1, 16, 2, 0, 1, 1.0, 256, 256, 2, 1, 264, None) == _ops.E_UNSUPPORTED
 
 
 def test_experts_checks():
