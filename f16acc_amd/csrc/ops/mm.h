@@ -321,9 +321,23 @@ struct MmKernel {
     float s[C::FM], sb = 0.0f, sb2 = 0.0f;
     f32x4 sr[4];
 
+    int slot = 0, kb = l.k0;
     wait_vm<(C::NS - 1) * LOADS>();
     barrier();
-    int slot = 0;
+    // A wave without a token (the last tile of an expert or of M) copies its share
+    // and leaves the matrix unit to the others: a half-empty tile takes little over
+    // half the time.
+    if (wm * C::TM >= m_left) {
+      do {
+        wait_vm<(C::NS - 2) * LOADS>();
+        barrier();
+        stage(l, kb + C::NS, lds0 + slot * STAGE, wave).all();
+        slot = slot + 1 == C::NS ? 0 : slot + 1;
+      } while (++kb < l.nk);
+      wait_vm<0>();
+      store_all(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < C::FM; ++i) {
       xf[i] = read(xa + 16 * i * kBlock);
@@ -342,7 +356,6 @@ struct MmKernel {
       if (TWO) sb2 = swp[second + l.k0 * p.swk];
     }
 
-    int kb = l.k0;
     do {
       const int at = slot * STAGE, nslot = slot + 1 == C::NS ? 0 : slot + 1, nat = nslot * STAGE;
       // products of the two scales
