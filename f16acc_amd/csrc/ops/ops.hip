@@ -275,7 +275,7 @@ struct ExpertsPlan {
     slots = T * k;
     Dp = up128(D);
     Ip = up128(I);
-    few = few_tokens(T, k) ? (size_t)slots * Ip * 4 : 0;
+    few = few_tokens(T, k) ? up256(slots * Ip * 4) + up256(sizeof(FewMap)) : 0;
     bm = expert_tile(slots, E);
     chunks = cdiv(slots, kSortChunk);
     max_tiles = slots / bm + (slots < E ? slots : E);
@@ -552,11 +552,12 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   char* ws = (char*)workspace;
   if (plan.few && wide_loads(x, type, sr, sc)) {
     FewArgs f{x,   sr,  (int)T, k,   E,   (int)plan.slots, ids, weights, wt,  wk,  D,   I, w1,          w1e,     w1u,
-              ld1, s1,  s1e,    s1u, s1n, s1k,             w2,  w2e,     ld2, s2,  s2e, s2n, s2k, (float*)ws, plan.Ip, y};
+              ld1, s1,  s1e,    s1u, s1n, s1k,             w2,  w2e,     ld2, s2,  s2e, s2n, s2k, (float*)ws, plan.Ip,
+              (FewMap*)(ws + up256(plan.slots * plan.Ip * 4)), y};
     return by_type(type, [&](auto* t) {
       using U = std::remove_pointer_t<decltype(t)>;
       constexpr int G = 2;
-      hipLaunchKernelGGL((few_gate_up_kernel<U, 8, G>), dim3((uint32_t)cdiv(I, 32), (uint32_t)plan.slots), dim3(512), 0,
+      hipLaunchKernelGGL((few_gate_up_kernel<U, 8, G>), dim3((uint32_t)cdiv(I, 32), (uint32_t)plan.slots + 1), dim3(512), 0,
                          stream, f);
       hipLaunchKernelGGL((few_down_kernel<U, 16, G>), dim3((uint32_t)cdiv(D, 16)), dim3(1024), 0, stream, f);
       return hip_status();

@@ -24,8 +24,8 @@ struct TokenBlock {
   float s[16];
 };
 
-// Rows row(t) of x (NULL: zeros) from k0, for t < tokens <= 4 G; every group's loads are
-// in flight together.
+// Rows row(t) of x (NULL: zeros) from k0, for t < tokens <= 4 G (row is asked for every
+// t < 4 G); every group's loads are in flight together.
 template <class T, int G, class Row>
 __device__ __forceinline__ i32x8 quant_tokens(TokenBlock& b, Row row, int tokens, int64_t k0, int64_t K, int lane,
                                               float* s) {
@@ -35,7 +35,8 @@ __device__ __forceinline__ i32x8 quant_tokens(TokenBlock& b, Row row, int tokens
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     const int t = 4 * i + (lane >> 4);
-    const T* x = t < tokens ? row(t) : nullptr;
+    const T* x = row(t);  // (by every lane: it may exchange between lanes)
+    if (t >= tokens) x = nullptr;
     if (x && k + 8 <= K) {
       load_vec(x + k, v[i]);
     } else {
@@ -189,6 +190,14 @@ __device__ __forceinline__ f32x4 exact_product(const i32x8& w, const Halves& x) 
 // (4 tokens of 64 experts, 8 each, 2048 x 1024: 55 us against 60 on the tiles; 16: 178 against 88)
 constexpr int kFewTokens = 8, kFewSlots = 128, kFewK = 16;
 
+// What the down kernel reads of the routing: the distinct experts in order of their
+// first slots, and each token's first slot with each of them (-1: none) and its weight.
+struct FewMap {
+  int count, expert[kFewSlots];
+  int slot[kFewSlots][kFewTokens];
+  float weight[kFewSlots][kFewTokens];
+};
+
 struct FewArgs {
   const void* x;
   int64_t ldx;
@@ -207,13 +216,63 @@ struct FewArgs {
   int64_t s2e, s2n, s2k;
   float* h;  // [slots][ldh], at each (token, expert)'s first slot
   int64_t ldh;
+  FewMap* map;
   void* y;
 };
 
+// Fills p.map, by one workgroup while the others multiply.
+template <int THREADS>
+__device__ __forceinline__ void few_map(const FewArgs& p) {
+  __shared__ int ids[kFewSlots], index[kMaxExperts], firsts[kFewSlots / 64];
+  __shared__ float weights[kFewSlots];
+  static_assert(THREADS >= kFewSlots, "a thread per slot");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // index[e]: the lowest slot with expert e, then the expert's place
+  for (int i = tid; i < p.E; i += THREADS) index[i] = kFewSlots;
+  int e = -1;
+  if (tid < p.slots) {
+    e = p.ids[tid];
+    weights[tid] = p.weights[tid / p.k * p.wt + tid % p.k * p.wk];
+    if (e >= p.E) e = -1;
+    ids[tid] = e;
+  }
+  __syncthreads();
+  if (e >= 0) atomicMin(&index[e], tid);
+  __syncthreads();
+  const bool first = e >= 0 && index[e] == tid;
+  const uint64_t mask = __builtin_amdgcn_ballot_w64(first);
+  if (tid < kFewSlots && lane == 0) firsts[wave] = __popcll(mask);
+  __syncthreads();
+  int count = 0, at = 0;
+#pragma unroll
+  for (int i = 0; i < kFewSlots / 64; ++i) {
+    if (i == wave) at = count;
+    count += firsts[i];
+  }
+  at += __popcll(mask & ((1ull << lane) - 1));
+  if (first) {
+    p.map->expert[at] = e;
+    index[e] = at;
+  }
+  if (tid == 0) p.map->count = count;
+  for (int i = tid; i < count * kFewTokens; i += THREADS) p.map->slot[0][i] = -1;
+  __syncthreads();
+  if (e < 0) return;
+  // (a token may name an expert twice: its first slot has both weights)
+  const int t = tid / p.k;
+  float sum = weights[tid];
+  for (int j = t * p.k; j < tid; ++j)
+    if (ids[j] == e) return;
+  for (int j = tid + 1; j < (t + 1) * p.k; ++j)
+    if (ids[j] == e) sum += weights[j];
+  p.map->slot[index[e]][t] = tid;
+  p.map->weight[index[e]][t] = sum;
+}
+
 // h of 32 hidden columns of one expert, the one of slot blockIdx.y where that is its
 // first.  The waves deal the blocks of D, the next one's weights in flight while one
-// is multiplied.  All ids lie in the wave's registers: what the
-// expert's tokens are is a ballot and no further load.
+// is multiplied.  All ids lie in the wave's registers: what the expert's tokens are
+// is a ballot and no further load.
 template <class T, int W, int G>
 __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
   constexpr int WORDS = kFewSlots / 64;
@@ -221,6 +280,10 @@ __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
   __shared__ __align__(16) TokenBlock tokens[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t16 = lane & 15, g = lane >> 4, slot0 = blockIdx.y;
+  if (slot0 == p.slots) {  // (the last row of workgroups)
+    if (blockIdx.x == 0) few_map<64 * W>(p);
+    return;
+  }
   const int e = p.ids[slot0];
   int id[WORDS];
 #pragma unroll
@@ -294,83 +357,43 @@ __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
 // weights in flight while one is multiplied.
 template <class T, int W, int G>
 __global__ __launch_bounds__(64 * W) void few_down_kernel(FewArgs p) {
-  __shared__ int ids[kFewSlots], expert[kFewSlots], firsts[kFewSlots / 64], index[kMaxExperts];
-  __shared__ float weights[kFewSlots], weight[kFewSlots][16];
-  __shared__ short slot_of[kFewSlots][16];
   __shared__ f32x4 sums[W][64];
   __shared__ __align__(16) TokenBlock tokens[W];
-  static_assert(64 * W >= kFewSlots, "a thread per slot");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t16 = lane & 15, g = lane >> 4;
-  // the distinct experts, in order of their first slots; index[e]: the lowest slot
-  // with expert e, then the expert's place among them
-  for (int i = tid; i < p.E; i += 64 * W) index[i] = kFewSlots;
-  int e = -1;
-  if (tid < p.slots) {
-    e = p.ids[tid];
-    weights[tid] = p.weights[tid / p.k * p.wt + tid % p.k * p.wk];
-    if (e >= p.E) e = -1;
-    ids[tid] = e;
-  }
-  lds_barrier();
-  if (e >= 0) atomicMin(&index[e], tid);
-  lds_barrier();
-  const bool first = e >= 0 && index[e] == tid;
-  const uint64_t mask = __builtin_amdgcn_ballot_w64(first);
-  if (tid < kFewSlots && lane == 0) firsts[wave] = __popcll(mask);
-  lds_barrier();
-  int count = 0, at = 0;
-#pragma unroll
-  for (int i = 0; i < kFewSlots / 64; ++i) {
-    if (i == wave) at = count;
-    count += firsts[i];
-  }
-  at += __popcll(mask & ((1ull << lane) - 1));
-  if (first) {
-    expert[at] = e;
-    index[e] = at;
-  }
-  lds_barrier();
+  const int t16 = lane & 15, g = lane >> 4, t = t16 < kFewTokens ? t16 : kFewTokens - 1;
+  const FewMap* map = p.map;
   const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + t16 < p.D ? n0 + t16 : p.D - 1;
-  const int nk = (int)cdiv(p.I, kBlock), units = count * nk;
+  const int nk = (int)cdiv(p.I, kBlock), units = map->count * nk;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   i32x8 next;
-  float snext = 0.0f;
-  auto load = [&](int u) {
-    const int d = u / nk, kb = u - d * nk, ex = expert[d];
-    next = load_weight(p.w2 + ex * p.w2e + n * p.ld2, (int64_t)kb * kBlock, p.I, g);
-    snext = p.s2[ex * p.s2e + n0 / kBlock * p.s2n + kb * p.s2k];
+  float snext = 0.0f, wnext = 0.0f;
+  int slots = -1, d = wave / nk, kb = wave - d * nk;  // slots: lane l holds token l's slot with the expert
+  auto load = [&]() {
+    const int64_t e = map->expert[d];
+    next = load_weight(p.w2 + e * p.w2e + n * p.ld2, (int64_t)kb * kBlock, p.I, g);
+    snext = p.s2[e * p.s2e + n0 / kBlock * p.s2n + kb * p.s2k];
+    slots = map->slot[d][t];
+    wnext = map->weight[d][t];
   };
-  if (wave < units) load(wave);
-  // while the first weights are on their way: each token's first slot with each
-  // expert, and its weights (a token may name an expert twice)
-  for (int i = tid; i < count * 16; i += 64 * W) slot_of[i >> 4][i & 15] = -1;
-  lds_barrier();
-  if (e >= 0) {
-    const int t = tid / p.k, end = t * p.k + p.k;
-    bool mine = true;
-    float sum = weights[tid];
-    for (int j = t * p.k; j < tid; ++j) mine &= ids[j] != e;
-    for (int j = tid + 1; j < end; ++j)
-      if (ids[j] == e) sum += weights[j];
-    if (mine) {
-      slot_of[index[e]][t] = (short)tid;
-      weight[index[e]][t] = sum;
-    }
-  }
-  lds_barrier();
+  if (wave < units) load();
 #pragma unroll 1
   for (int u = wave; u < units; u += W) {
-    const int d = u / nk, kb = u - d * nk, slot = slot_of[d][t16];
     const i32x8 wf = next;
-    const float sb = snext;
-    if (u + W < units) load(u + W);
+    const int here = t16 < p.T ? slots : -1, at = kb;
+    const float f = here >= 0 ? snext * wnext : 0.0f;
+    kb += W;
+    while (kb >= nk) kb -= nk, ++d;
+    if (u + W < units) load();
     float s;
     const i32x8 xf = quant_tokens<float, G>(
-        tokens[wave], [&](int t) { return slot_of[d][t] >= 0 ? p.h + slot_of[d][t] * p.ldh : nullptr; }, p.T,
-        (int64_t)kb * kBlock, p.I, lane, &s);
-    const float f = slot >= 0 ? s * sb * weight[d][t16] : 0.0f;
-    acc += mfma(wf, xf) * f;
+        tokens[wave],
+        [&](int i) {
+          const int slot = __shfl(here, i);
+          return slot >= 0 ? p.h + slot * p.ldh : nullptr;
+        },
+        p.T, (int64_t)at * kBlock, p.I, lane, &s);
+    const f32x4 part = mfma(wf, xf);
+    if (here >= 0) acc += part * (s * f);
   }
   sums[wave][lane] = acc;
   __syncthreads();
