@@ -453,14 +453,23 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   if (i32.scalar_type() == at::kLong) i32 = i32.clamp(-1, E).to(at::kInt);  // (a cast alone would wrap)
   i32 = i32.contiguous();
   const Operand p1 = packed(w1), p2 = packed(w2);
-  const size_t n = f16acc_experts_workspace(T, (int)k, (int)E, D, I);
+  // The kernels address rows of the quantised tokens and hidden values by 31 bits:
+  // more tokens than that go in parts.
+  const int64_t most = 0x7fff0000 / std::max(up(D, kBlock), k * up(I, kBlock));
+  const int64_t part = std::min(T, std::max<int64_t>(most, 1));
+  const size_t n = f16acc_experts_workspace(part, (int)k, (int)E, D, I);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);
-  check_rc(f16acc_experts(x2.const_data_ptr(), type_of(x), T, x2.stride(0), x2.stride(1), floats(wt), wt.stride(0),
-                          wt.stride(1), (const int*)i32.const_data_ptr(), (int)k, (int)E, D, I, bytes(p1.q),
-                          p1.q.stride(0), p1.q.stride(1), p1.ld, floats(s1), s1.stride(0), s1.stride(1), s1.stride(2),
-                          s1.stride(3), bytes(p2.q), p2.q.stride(0), p2.ld, floats(s2), s2.stride(0), s2.stride(1),
-                          s2.stride(2), y.data_ptr(), bytes(ws), n, on.stream));
+  for (int64_t t = 0; t < T; t += part) {
+    const int64_t tokens = std::min(part, T - t);
+    check_rc(f16acc_experts((const char*)x2.const_data_ptr() + t * x2.stride(0) * x2.element_size(), type_of(x),
+                            tokens, x2.stride(0), x2.stride(1), floats(wt) + t * wt.stride(0), wt.stride(0),
+                            wt.stride(1), (const int*)i32.const_data_ptr() + t * k, (int)k, (int)E, D, I, bytes(p1.q),
+                            p1.q.stride(0), p1.q.stride(1), p1.ld, floats(s1), s1.stride(0), s1.stride(1),
+                            s1.stride(2), s1.stride(3), bytes(p2.q), p2.q.stride(0), p2.ld, floats(s2), s2.stride(0),
+                            s2.stride(1), s2.stride(2), (char*)y.data_ptr() + t * D * y.element_size(), bytes(ws), n,
+                            on.stream));
+  }
   return y;
 }
 

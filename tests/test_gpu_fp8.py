@@ -295,6 +295,21 @@ def test_linear_bias_and_stored_weight_gradients():
     assert torch.equal(db, dy.sum(0))
 
 
+def test_linear_gradients_from_expanded_and_strided_grads():
+    x, w = normal(30, 40, dtype=torch.float32).requires_grad_(), normal(20, 40, dtype=torch.float32, seed=2).requires_grad_()
+    for dy in (torch.ones((), device=DEV).expand(30, 20), normal(20, 30, dtype=torch.float32, seed=3).t()):
+        got = torch.autograd.grad(fp8.linear(x, w), (x, w), dy)
+        want = torch.autograd.grad(fp8.linear(x, w), (x, w), dy.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):  # there is no second derivative
+        dx, = torch.autograd.grad(fp8.linear(x, w).sum(), x, create_graph=True)
+        torch.autograd.grad(dx.sum(), w)
+    a = normal(6, 5, 40, dtype=torch.float32)
+    view = a.transpose(0, 1).requires_grad_()
+    dx, = torch.autograd.grad(fp8.linear(view, w).square().sum(), view)
+    assert dx.shape == view.shape
+
+
 def test_linear_empty_gradients():
     x, w = torch.zeros(0, 32, device=DEV, requires_grad=True), normal(8, 32, dtype=torch.float32).requires_grad_()
     dx, dw = torch.autograd.grad(fp8.linear(x, w).sum(), (x, w))

@@ -243,6 +243,19 @@ def test_experts_views_types_and_leading_dimensions():
     assert empty.shape == (0, 256)
 
 
+def test_experts_offsets_past_32_bits():
+    T, D = 1100000, 2048
+    _, _, _, *w = layer(1, 4, 1, D, 128)
+    x = torch.zeros(T, D, dtype=torch.float16, device=DEV)
+    tail = normal(600, D)
+    x[-600:] = tail
+    ids = (torch.arange(T, device=DEV) % 5 - 1).to(torch.int32).view(T, 1)  # -1 .. 3
+    weights = torch.ones(T, 1, device=DEV)
+    y = moe.experts(x, weights, ids, *w)
+    assert bool((y[:-600] == 0).all())
+    check_experts(y[-600:], (tail, weights[-600:], ids[-600:], *w))
+
+
 def test_experts_non_finite_tokens_stay_apart():
     for T in (6, 60, 500):
         args = list(layer(T, 4, 2, 256, 128))
