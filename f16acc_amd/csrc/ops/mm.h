@@ -301,7 +301,10 @@ struct MmKernel {
     // from `jb` on in the second.  Gated: the gate's and the up's.
     const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
     const int64_t nb_last = cdiv(p.N, kBlock) - 1;
-    const float* swp = sw + (nb < nb_last ? nb : nb_last) * p.swn;
+    // (read through the scalar cache: a vector load among the copies would make the
+    // compiler wait for all of them)
+    typedef const float __attribute__((address_space(4)))* Scalar;
+    const Scalar swp = (Scalar)(uintptr_t)(sw + (nb < nb_last ? nb : nb_last) * p.swn);
     const int64_t second = GATED ? p.sup : nb < nb_last ? p.swn : 0;
     const int jb = GATED ? C::FN / 2 : (int)(kBlock - (n0 + wn * C::TN) % kBlock) / 16;
 

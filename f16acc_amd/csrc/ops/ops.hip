@@ -104,7 +104,7 @@ int mm_check(const MmArgs& p) {
 
 // The tiles of one product (F16ACC_FP8_TILE_*): tokens x weight rows.
 using Tile0 = MmCfg<256, 256, 4, 2, 2, 2>;
-using Tile1 = MmCfg<128, 256, 2, 4, 2, 2>;
+using Tile1 = MmCfg<128, 256, 2, 4, 3, 2>;
 using Tile2 = MmCfg<128, 128, 2, 2, 2, 2>;
 using Tile3 = MmCfg<64, 128, 2, 2, 3, 2>;
 using Tile4 = MmCfg<64, 64, 2, 1, 3, 2>;
@@ -247,7 +247,7 @@ struct ExpertCfg<32> {
 };
 template <>
 struct ExpertCfg<128> {
-  using GateUp = MmCfg<128, 256, 2, 4, 2, 2>;
+  using GateUp = MmCfg<128, 256, 2, 4, 3, 2>;
   using Down = MmCfg<128, 128, 2, 2, 2, 2>;
 };
 template <>
