@@ -111,10 +111,10 @@ using Tile4 = MmCfg<64, 64, 2, 1, 3, 2>;
 using Tile5 = MmCfg<32, 64, 1, 2, 4, 2>;
 // What a tile costs, in microseconds, fitted to 5010 timed (shape, tile, split)
 // triples (M 32 .. 8192, N 256 .. 8960, K 512 .. 9000, weights out of the cache; 438
-// with row scales): a workgroup alone on its CU takes
-// start + kb * block, each further one beside it adds `share` of the blocks'
-// time; `per_cu` fit.  The picks made with it take 1.4 % (row scales 0.6 %) longer than the best
-// triple on geometric mean, 15 % at worst.
+// with row scales): a workgroup alone on its CU takes start + kb * block, each
+// further one beside it adds `share` of the blocks' time; `per_cu` fit.  The
+// picks made with it take 1.2 % (row scales 0.1 %) longer than the best triple on
+// geometric mean, 11 % at worst.
 struct TileCost {
   double start, block, share;
 };
@@ -123,9 +123,9 @@ struct TileInfo {
   TileCost square, row;  // row.block 0: not built with row scales
 };
 constexpr TileInfo kTiles[] = {
-    {256, 256, 1, {5.5, 1.36, 0.6}, {7.05, 1.79, 0.6}},   {128, 256, 1, {3.1, 0.85, 0.6}, {}},
-    {128, 128, 2, {2.9, 0.61, 0.6}, {3.2, 0.68, 0.61}},   {64, 128, 2, {1.8, 0.69, 0.35}, {}},
-    {64, 64, 3, {1.7, 0.61, 0.27}, {2.2, 0.42, 0.33}},    {32, 64, 3, {1.2, 0.52, 0.27}, {}},
+    {256, 256, 1, {3.8, 1.20, 0.6}, {7.1, 1.79, 0.6}},    {128, 256, 1, {2.3, 0.745, 0.6}, {}},
+    {128, 128, 2, {2.2, 0.60, 0.61}, {3.2, 0.67, 0.62}},  {64, 128, 2, {1.9, 0.45, 0.55}, {}},
+    {64, 64, 3, {1.7, 0.43, 0.33}, {2.1, 0.41, 0.34}},    {32, 64, 3, {1.3, 0.34, 0.32}, {}},
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -147,11 +147,11 @@ double cost_of(const MmPlan& plan, int64_t M, int64_t N, int64_t K, bool row_sca
   const int64_t full = deep / t.per_cu, rest = deep % t.per_cu;
   double us = full * (c.start + c.block * kb * (1 + (t.per_cu - 1) * c.share));
   if (rest) us += c.start + c.block * kb * (1 + (rest - 1) * c.share);
-  const double floor = ((double)N * K + (double)M * K) * 0.19e-6;  // the operands from HBM
+  const double floor = ((double)N * K + (double)M * K) * 0.17e-6;  // the operands from HBM
   if (us < floor) us = floor;
   const double outputs = (double)M * N * 1e-6;
-  if (t.per_cu == 1) us += 0.2 * outputs;  // no other workgroup runs while one stores
-  if (plan.splits > 1) us += 2.3 + 0.28 * plan.splits + 1.28 * plan.splits * outputs;
+  if (t.per_cu == 1) us += 0.3 * outputs;  // no other workgroup runs while one stores
+  if (plan.splits > 1) us += 2.1 + 0.25 * plan.splits + 1.36 * plan.splits * outputs;
   return us;
 }
 
