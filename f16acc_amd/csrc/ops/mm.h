@@ -65,13 +65,9 @@ struct MmCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, OCC = OCC_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  // 16-byte copies per lane and stage; where BN is not whole copies, the first
-  // LW_LAST waves make one more
-  static constexpr int LX = BM * 8 / THREADS, LW = (BN * 8 + THREADS - 1) / THREADS;
-  static constexpr int LW_LAST = BN * 8 % THREADS / 64;
+  static constexpr int LX = BM * 8 / THREADS, LW = BN * 8 / THREADS;  // 16-byte copies per lane and stage
   static constexpr int X_BYTES = BM * kBlock, W_BYTES = BN * kBlock, S_BYTES = THREADS * 4;
-  static_assert(LX * THREADS == BM * 8 && BN * 8 % 64 == 0, "whole copies");
-  static_assert(LW_LAST == 0 || NS == 2, "waves with unequal copies wait for all of them");
+  static_assert(LX * THREADS == BM * 8 && LW * THREADS == BN * 8, "whole copies");
   static_assert(BM <= THREADS, "one scale copy per stage covers the tokens");
   static_assert(THREADS / 8 % 16 == 0, "a lane's units keep the swizzle phase");
   static constexpr int stage_bytes(bool row_scales) {
@@ -120,8 +116,7 @@ struct MmKernel {
   static constexpr int LSW = ROW_SCALES ? (C::BN + C::THREADS - 1) / C::THREADS : 0;
   static constexpr int LOADS = C::LX + C::LW + 1 + LSW;
   static constexpr bool GATED = EPI == kGatedQuant;
-  static constexpr bool TWO = GATED || (!ROW_SCALES && kBlock % C::TN != 0);  // two weight scales per wave
-  static_assert(GATED || C::TN <= kBlock + 16, "at most two blocks a wave");
+  static_assert(GATED || kBlock % C::TN == 0, "a wave's weight rows lie in one block");
   static constexpr int BN_OUT = GATED ? C::BN / 2 : C::BN;  // columns of the result
   static_assert((C::NS - 1) * LOADS <= 63, "outstanding copies must fit vmcnt");
 
@@ -198,7 +193,7 @@ struct MmKernel {
     i32x4 xr, wr, ur, sr, swr;
     int x_off, w_off, s_off;  // this lane's offsets, kOob past K
     bool in, any;
-    int base, sbase, wave;
+    int base, sbase;
     const Loader* l;
     __device__ __forceinline__ void unit(int j) const {
       constexpr int STEP = C::THREADS * 16;
@@ -211,7 +206,7 @@ struct MmKernel {
         const int k = j - C::LX;
         if (GATED && k >= C::LW / 2)
           lds_dma16(srd_at(ur, (k - C::LW / 2) * l->w_step), base + C::X_BYTES + k * STEP, w_off);
-        else if (C::LW_LAST == 0 || k < C::LW - 1 || wave < C::LW_LAST)
+        else
           lds_dma16(srd_at(wr, k * l->w_step), base + C::X_BYTES + k * STEP, w_off);
       } else if (j == C::LX + C::LW) {
         lds_dma4(sr, sbase, s_off);
@@ -240,7 +235,6 @@ struct MmKernel {
     st.s_off = st.any ? l.s_off : kOob;
     st.base = slot + wave * 1024;
     st.sbase = slot + C::X_BYTES + C::W_BYTES + wave * 256;
-    st.wave = wave;
     st.l = &l;
     return st;
   }
@@ -297,16 +291,13 @@ struct MmKernel {
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) stage(l, l.k0 + s, lds0 + s * STAGE, wave).all();
 
-    // The weight blocks' scales: a wave's rows lie in one block or two, fragments
-    // from `jb` on in the second.  Gated: the gate's and the up's.
+    // The weight block's scale, one value a wave (gated: the gate's and the up's), read
+    // through the scalar cache: a vector load among the copies would make the
+    // compiler wait for all of them.
     const int64_t nb = GATED ? n0 / kBlock : (n0 + wn * C::TN) / kBlock;
     const int64_t nb_last = cdiv(p.N, kBlock) - 1;
-    // (read through the scalar cache: a vector load among the copies would make the
-    // compiler wait for all of them)
     typedef const float __attribute__((address_space(4)))* Scalar;
     const Scalar swp = (Scalar)(uintptr_t)(sw + (nb < nb_last ? nb : nb_last) * p.swn);
-    const int64_t second = GATED ? p.sup : nb < nb_last ? p.swn : 0;
-    const int jb = GATED ? C::FN / 2 : (int)(kBlock - (n0 + wn * C::TN) % kBlock) / 16;
 
     // A wave's addresses in a stage; the fragments of an operand lie 16 rows apart.
     const int frag = t16 * kBlock, lo = (g ^ swz(t16)) << 4, hi = ((g + 4) ^ swz(t16)) << 4;
@@ -317,7 +308,7 @@ struct MmKernel {
       const i32x4 a = *(const i32x4 LDS_AS*)(lds + at + lo), b = *(const i32x4 LDS_AS*)(lds + at + hi);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    constexpr int AHEAD = C::FN > 2 ? 2 : 1, RING = AHEAD == 1 ? 2 : C::FN % 4 ? 3 : 4;  // fragments of w read ahead
+    constexpr int AHEAD = C::FN > 2 ? 2 : 1, RING = AHEAD == 1 ? 2 : 4;  // fragments of w read ahead
     static_assert(C::FN % RING == 0, "a stage starts with the ring's first slot");
     static_assert(!ROW_SCALES || (RING == 4 && C::FM >= 2), "row scales are read AHEAD of their last use");
     i32x8 xf[C::FM], wf[RING];
@@ -356,21 +347,21 @@ struct MmKernel {
     for (int j = 0; j < AHEAD; ++j) read_w(0, j);
     if (!ROW_SCALES) {
       sb = swp[l.k0 * p.swk];
-      if (TWO) sb2 = swp[second + l.k0 * p.swk];
+      if (GATED) sb2 = swp[p.sup + l.k0 * p.swk];
     }
 
     do {
       const int at = slot * STAGE, nslot = slot + 1 == C::NS ? 0 : slot + 1, nat = nslot * STAGE;
       // products of the two scales
-      float sc[C::FM], sc2[TWO ? C::FM : 1];
+      float sc[C::FM], sc2[GATED ? C::FM : 1];
 #pragma unroll
       for (int i = 0; i < C::FM; ++i) {
         sc[i] = ROW_SCALES ? s[i] : s[i] * sb;
-        if (TWO) sc2[i] = s[i] * sb2;
+        if (GATED) sc2[i] = s[i] * sb2;
       }
       if (!ROW_SCALES && kb + 1 < l.nk) {
         sb = swp[(kb + 1) * p.swk];
-        if (TWO) sb2 = swp[second + (kb + 1) * p.swk];
+        if (GATED) sb2 = swp[p.sup + (kb + 1) * p.swk];
       }
       const Stage next = stage(l, kb + C::NS, lds0 + at, wave);
       f32x4 part[3];
@@ -381,7 +372,7 @@ struct MmKernel {
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], sc[i] * sr[j % 4][r], acc[i][j][r]);
         } else {
-          const float f = TWO && j >= (GATED ? C::FN / 2 : jb) ? sc2[i] : sc[i];
+          const float f = GATED && j >= C::FN / 2 ? sc2[i] : sc[i];
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], f, acc[i][j][r]);
         }

