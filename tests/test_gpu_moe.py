@@ -176,7 +176,8 @@ def check_experts(y, args):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T,E,k,D,I", [(1, 1, 1, 16, 16), (1, 8, 3, 256, 128), (2, 4, 4, 130, 70), (5, 3, 2, 200, 300),
                                        (16, 8, 4, 256, 384), (40, 5, 2, 272, 144), (200, 4, 2, 256, 260), (300, 3, 3, 384, 256),
-                                       (700, 4, 2, 128, 640)])
+                                       (700, 4, 2, 128, 640), (1, 1024, 64, 128, 128), (3, 20, 20, 128, 140), (8, 16, 16, 130, 128),
+                                       (9, 24, 16, 128, 128), (5, 1000, 3, 128, 16)])
 def test_experts(T, E, k, D, I, dtype):
     args = layer(T, E, k, D, I, dtype)
     y = moe.experts(*args)
@@ -239,6 +240,10 @@ def test_experts_views_types_and_leading_dimensions():
     assert torch.equal(moe.experts(*a), want)
     y = moe.experts(args[0].view(2, 12, 256), args[1].view(2, 12, 2), args[2].view(2, 12, 2), *args[3:])
     assert torch.equal(y.view(24, 256), want)
+    few = [args[0][:2].clone(), args[1][:2], args[2][:2], *args[3:]]
+    check_experts(moe.experts(*few), few)
+    few[0] = torch.cat([few[0][:, :1], few[0]], 1)[:, 1:]  # rows that no 16-byte load fits
+    check_experts(moe.experts(*few), few)
     empty = moe.experts(args[0][:0], args[1][:0], args[2][:0], *args[3:])
     assert empty.shape == (0, 256)
 
