@@ -114,11 +114,11 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = (float)k.t[i];
 }
 
-// SiLU with FP32's accuracy, where few values are asked for and what is
-// quantised from them should fall on the right side of a tie.
+// SiLU with FP32's accuracy, behind sums of that accuracy: what is quantised from
+// it should fall on the right side of a tie.
 __device__ __forceinline__ float silu_exact(float g) { return g / (1.0f + expf(-g)); }
-// SiLU, to a few units in the last place: the hardware's exponential and
-// reciprocal (a correctly rounded quotient was a fifth of the gated product's time).
+// SiLU, to a few units in the last place, behind 8-bit sums: the hardware's exponential
+// and reciprocal (a correctly rounded quotient was a fifth of the gated product's time).
 __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // Raw buffer resource over `bytes` bytes at `base` (stride 0; reads past the

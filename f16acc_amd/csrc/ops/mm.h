@@ -27,6 +27,15 @@
 // values over nine binades, at most 5e-5 of the sum of magnitudes.  Everything
 // past one block's sum is FP32.
 //
+// Gate and up may take the other way (kGatedExact): their result is quantised, and a sum
+// that is off by 1e-5 falls on the other side of an e4m3 tie once in some hundred
+// values.  Then both operands are converted to binary16, which is exact, and the
+// block is four v_mfma_f32_16x16x32_f16 in FP32: twice the matrix cycles and, on
+// 64 x 64 sums a wave, two conversions for each MFMA, which bound it (dealing them one by
+// one between the MFMAs gained 2 %).  4096 tokens, 8 of 64 experts, 2048 x 1024: 373 us
+// on 128 x 256 tiles against 193 in 8 bits on 256 x 256 (profiled; 256 x 256 spills
+// with the halves).
+//
 // Measured (bfloat16 result): 8192^3 450 us, 2440 TFLOPS, where a library's product with
 // one scale for everything reaches 2770; 4096^3 64 us, 2150; with a scale for each
 // weight row 531 us.  On 8192^3 the matrix unit is busy 61 % of the cycles, at
@@ -75,7 +84,7 @@ struct MmArgs {
   int64_t ldsq;
 };
 
-enum Epilogue { kStore = 0, kGatedQuant = 1, kSlots = 2 };
+enum Epilogue { kStore = 0, kGatedQuant = 1, kSlots = 2, kGatedExact = 3 };
 
 template <int BM_, int BN_, int WM_, int WN_, int NS_, int OCC_>
 struct MmCfg {
@@ -110,6 +119,30 @@ __device__ __forceinline__ f32x4 mfma(const i32x8& w, const i32x8& x) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
 }
 
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 8 e4m3 values as binary16.
+__device__ __forceinline__ f16x8 halves(int lo, int hi) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+struct Halves {
+  f16x8 v[4];
+  Halves() = default;
+  __device__ __forceinline__ explicit Halves(const i32x8& q) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = halves(q[2 * i], q[2 * i + 1]);
+  }
+};
+
+__device__ __forceinline__ f32x4 mfma_f16(const f16x8& w, const f16x8& x, const f32x4& sum) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(w, x, sum, 0, 0, 0);
+}
+
 // Four consecutive outputs of one token from FP32, rounded once.
 template <class T>
 __device__ __forceinline__ void store4(T* p, int64_t scn, int left, const f32x4& v, bool wide) {
@@ -132,7 +165,7 @@ struct MmKernel {
   static constexpr int STAGE = C::stage_bytes(ROW_SCALES);
   static constexpr int LSW = ROW_SCALES ? (C::BN + C::THREADS - 1) / C::THREADS : 0;
   static constexpr int LOADS = C::LX + C::LW + 1 + LSW;
-  static constexpr bool GATED = EPI == kGatedQuant;
+  static constexpr bool EXACT = EPI == kGatedExact, GATED = EPI == kGatedQuant || EXACT;
   static_assert(GATED || kBlock % C::TN == 0, "a wave's weight rows lie in one block");
   static constexpr int BN_OUT = GATED ? C::BN / 2 : C::BN;  // columns of the result
   static_assert((C::NS - 1) * LOADS <= 63, "outstanding copies must fit vmcnt");
@@ -381,51 +414,95 @@ struct MmKernel {
         if (GATED) sb2 = swp[p.sup + (kb + 1) * p.swk];
       }
       const Stage next = stage(l, kb + C::NS, lds0 + at, wave);
-      f32x4 part[3];
-      auto finish = [&](int t) {
-        const int i = t % C::FM, j = t / C::FM;
-        const f32x4& v = part[t % 3];
-        if (ROW_SCALES) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], sc[i] * sr[j % 4][r], acc[i][j][r]);
-        } else {
-          const float f = GATED && j >= C::FN / 2 ? sc2[i] : sc[i];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], f, acc[i][j][r]);
-        }
+      auto turn = [&](int j) {
+        if (j != C::FN - AHEAD) return;
+        // This wave has read all of this stage: once every wave has, and the next
+        // stage has landed, the copies of the stage after them may begin.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_vm<(C::NS - 2) * LOADS>();
+        barrier();
       };
+      if constexpr (EXACT) {  // the block's sums on the 16-bit instructions
+        f32x4 part[2][C::FM];  // a weight fragment's sums are added while the next one's form
+        auto finish = [&](int j) {
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j) {
-        if (j == C::FN - AHEAD) {
-          // This wave has read all of this stage: once every wave has, and the next
-          // stage has landed, the copies of the stage after them may begin.
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          wait_vm<(C::NS - 2) * LOADS>();
-          barrier();
-        }
+          for (int i = 0; i < C::FM; ++i) {
+            const float f = j >= C::FN / 2 ? sc2[i] : sc[i];
 #pragma unroll
-        for (int i = 0; i < C::FM; ++i) {
-          const int t = j * C::FM + i;
-          part[t % 3] = mfma(wf[j % RING], xf[i]);
-          __builtin_amdgcn_sched_barrier(0);
-          if (i == 0) read_w(j < C::FN - AHEAD ? at : nat, (j + AHEAD) % C::FN);
-          if (j == C::FN - 1) {  // the next stage's tokens, each as soon as its register is free
-            xf[i] = read(nat + xa + 16 * i * kBlock);
-            s[i] = *(const float LDS_AS*)(lds + nat + sa + 64 * i);
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(part[j % 2][i][r], f, acc[i][j][r]);
           }
-          if (j >= C::FN - AHEAD) {  // the copies, spread over the steps after the barrier
-            constexpr int STEPS = AHEAD * C::FM;
-            const int u = t - (C::FN - AHEAD) * C::FM;
+        };
+        Halves xh[C::FM];
 #pragma unroll
-            for (int k = u * LOADS / STEPS; k < (u + 1) * LOADS / STEPS; ++k) next.unit(k);
+        for (int i = 0; i < C::FM; ++i) xh[i] = Halves(xf[i]);
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j) {
+          turn(j);
+          const Halves wh(wf[j % RING]);
+          read_w(j < C::FN - AHEAD ? at : nat, (j + AHEAD) % C::FN);
+          f32x4(&sum)[C::FM] = part[j % 2];
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i) sum[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < C::FM; ++i) sum[i] = mfma_f16(wh.v[k], xh[i].v[k], sum[i]);
+          if (j == C::FN - 1) {
+#pragma unroll
+            for (int i = 0; i < C::FM; ++i) {
+              xf[i] = read(nat + xa + 16 * i * kBlock);
+              s[i] = *(const float LDS_AS*)(lds + nat + sa + 64 * i);
+            }
           }
-          if (t >= 2) finish(t - 2);
-          __builtin_amdgcn_sched_barrier(0);
+          if (j >= C::FN - AHEAD) {
+            const int u = j - (C::FN - AHEAD);
+#pragma unroll
+            for (int k = u * LOADS / AHEAD; k < (u + 1) * LOADS / AHEAD; ++k) next.unit(k);
+          }
+          if (j) finish(j - 1);
         }
+        finish(C::FN - 1);
+      } else {
+        f32x4 part[3];
+        auto finish = [&](int t) {
+          const int i = t % C::FM, j = t / C::FM;
+          const f32x4& v = part[t % 3];
+          if (ROW_SCALES) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], sc[i] * sr[j % 4][r], acc[i][j][r]);
+          } else {
+            const float f = GATED && j >= C::FN / 2 ? sc2[i] : sc[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[r], f, acc[i][j][r]);
+          }
+        };
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j) {
+          turn(j);
+#pragma unroll
+          for (int i = 0; i < C::FM; ++i) {
+            const int t = j * C::FM + i;
+            part[t % 3] = mfma(wf[j % RING], xf[i]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i == 0) read_w(j < C::FN - AHEAD ? at : nat, (j + AHEAD) % C::FN);
+            if (j == C::FN - 1) {  // the next stage's tokens, each as soon as its register is free
+              xf[i] = read(nat + xa + 16 * i * kBlock);
+              s[i] = *(const float LDS_AS*)(lds + nat + sa + 64 * i);
+            }
+            if (j >= C::FN - AHEAD) {  // the copies, spread over the steps after the barrier
+              constexpr int STEPS = AHEAD * C::FM;
+              const int u = t - (C::FN - AHEAD) * C::FM;
+#pragma unroll
+              for (int k = u * LOADS / STEPS; k < (u + 1) * LOADS / STEPS; ++k) next.unit(k);
+            }
+            if (t >= 2) finish(t - 2);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        constexpr int T = C::FM * C::FN;
+        if (T >= 2) finish(T - 2);
+        finish(T - 1);
       }
-      constexpr int T = C::FM * C::FN;
-      if (T >= 2) finish(T - 2);
-      finish(T - 1);
       slot = nslot;
     } while (++kb < l.nk);
     wait_vm<0>();
@@ -582,7 +659,7 @@ struct MmKernel {
       for (int j = 0; j < C::FN / 2; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float h = silu(acc[i][j][r]) * acc[i][j + C::FN / 2][r];
+          const float h = (EXACT ? silu_exact(acc[i][j][r]) : silu(acc[i][j][r])) * acc[i][j + C::FN / 2][r];
           acc[i][j][r] = h;
           m = umax(m, abs_bits(h));
         }

@@ -236,7 +236,7 @@ struct LinearPlan {
 
 // The experts' tiles by the mean number of tokens an expert has: gate and up (128
 // columns of each), down.  4096 tokens, 8 of 64 experts each, 2048 x 1024, gate and up /
-// down: 232 / 202 us on 256, 256 / 167 on 128; with 25 tokens an expert
+// down, 8-bit sums: 232 / 202 us on 256, 256 / 167 on 128; with 25 tokens an expert
 // 110 us in all on 128, 124 on 32; with 10 106 and 105.
 template <int ROWS>
 struct ExpertCfg;
@@ -301,9 +301,16 @@ struct ExpertsPlan {
   }
 };
 
-template <int BM>
+// EXACT: gate and up on the 16-bit matrix instructions.  Up to 191 tokens an expert, where
+// weights are most of the time, they always do (in all, 64 experts of 2048 x 1024, 8 a
+// token, exact / 8-bit: 77 tokens 102 / 98 us, 512 127 / 113, 1024 173 / 142).  Past that
+// matrix instructions are the time (4096: 500 / 352), and it goes by the type: results in
+// binary16 and FP32 show the difference (3.0e-4 of the 2-norm off, or 1.3e-3 to 1.8e-3),
+// beside bfloat16's own rounding of 1.7e-3 it makes 2.4e-3 and the 8-bit sums stay.
+template <int BM, bool EXACT>
 int expert_products(const MmArgs& gu, const MmArgs& down, int64_t max_tiles, hipStream_t stream) {
-  const int rc = launch_mm<typename ExpertCfg<BM>::GateUp, false, true, kGatedQuant>(gu, max_tiles, stream);
+  using GateUp = typename ExpertCfg<EXACT && BM == 256 ? 128 : BM>::GateUp;
+  const int rc = launch_mm<GateUp, false, true, EXACT ? kGatedExact : kGatedQuant>(gu, max_tiles * (BM / GateUp::BM), stream);
   if (rc) return rc;
   using Down = typename ExpertCfg<BM>::Down;
   return launch_mm<Down, false, true, kSlots>(down, max_tiles * (BM / Down::BM), stream);
@@ -595,9 +602,10 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   gu.tile_rows = down.tile_rows = plan.bm;
   down.M = plan.slots, down.N = D, down.K = I;
   down.tiles = so.tiles, down.ntiles = so.ntiles, down.rows = nullptr, down.xrows = plan.slots;
-  rc = plan.bm == 256   ? expert_products<256>(gu, down, plan.max_tiles, stream)
-       : plan.bm == 128 ? expert_products<128>(gu, down, plan.max_tiles, stream)
-                        : expert_products<32>(gu, down, plan.max_tiles, stream);
+  rc = plan.bm == 32    ? expert_products<32, true>(gu, down, plan.max_tiles, stream)
+       : plan.bm == 128 ? expert_products<128, true>(gu, down, plan.max_tiles, stream)
+       : type == F16ACC_TYPE_BF16 ? expert_products<256, false>(gu, down, plan.max_tiles, stream)
+                                  : expert_products<256, true>(gu, down, plan.max_tiles, stream);
   if (rc) return rc;
 
   CombineArgs co{(const f16*)(ws + plan.ys), plan.ldy, down.sq, down_block(plan.bm), plan.slots, weights, wt, wk,

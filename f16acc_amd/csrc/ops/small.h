@@ -156,40 +156,20 @@ __global__ __launch_bounds__(64 * W) void linear_small_kernel(SmallArgs p) {
 // down kernel adds all experts of a token in one register, and the routing weight
 // is a factor of the block's scale.
 //
-// The hidden values are quantised between the products, and a sum that the 8-bit
-// matrix instructions round at 1e-5 lands on the other side of an e4m3 tie once
-// in some hundred values: with one token that showed as 2e-3 of the result.
-// Weights are what the kernels wait for, so the first product converts both
-// operands to binary16 (exactly) and sums in FP32 on the 16-bit instructions.
+// The hidden values are quantised between the products, so the first product's sums
+// are exact (binary16 operands, FP32 sums): what the 8-bit matrix instructions drop
+// showed as 2e-3 of one token's result, and weights are what the kernels wait for.
 //
 // Measured: one token through 6 of 64 experts, 2048 x 1024, 38 MB of weights: 11.3 + 9.7
 // us against 7.6 at the copy rate.  What is left is latency: a launch, the ids, the
 // weights, one wait after another, on two launches.
 // ---------------------------------------------------------------------------
 
-typedef f16 f16x2 __attribute__((ext_vector_type(2)));
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-
-// 8 e4m3 values as binary16.
-__device__ __forceinline__ f16x8 halves(int lo, int hi) {
-  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
-  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
-  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-struct Halves {
-  f16x8 v[4];
-  __device__ __forceinline__ explicit Halves(const i32x8& q) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = halves(q[2 * i], q[2 * i + 1]);
-  }
-};
 __device__ __forceinline__ f32x4 exact_product(const i32x8& w, const Halves& x) {
   const Halves h(w);
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.v[i], x.v[i], sum, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) sum = mfma_f16(h.v[i], x.v[i], sum);
   return sum;
 }
 
