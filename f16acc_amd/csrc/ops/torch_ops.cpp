@@ -5,13 +5,19 @@
 //
 // Everything runs on the current stream of the operands' device and allocates
 // through torch's allocator; nothing synchronises and nothing is kept between
-// calls.  A failed check raises ValueError, a failed launch RuntimeError.
+// calls.  A failed check raises ValueError, a failed launch RuntimeError, and a call that
+// something records or differentiates forward NotImplementedError.
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <torch/version.h>
 
+#include <initializer_list>
 #include <tuple>
 #include <vector>
 
@@ -38,12 +44,56 @@ int type_of(const Tensor& t) {
          : t.scalar_type() == at::kBFloat16 ? F16ACC_TYPE_BF16 : F16ACC_TYPE_F32;
 }
 
-void check_float(const char* name, const Tensor& t) {
-  REQUIRE(t.is_cuda(), name, " needs tensors on one GPU");
-  REQUIRE(is_type(t.scalar_type()), name, " needs torch.float16, bfloat16 or float32, not ", t.scalar_type());
+// Whether torch records the calls (torch.jit.trace, make_fx and export) or runs them on
+// stand-ins (fake and functional tensors, torch.func's transforms).  The kernels write
+// through pointers, which none of these sees: what it replays would hold the allocation
+// alone and return uninitialised memory.
+bool recorded() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing()) return true;
+  const c10::DispatchKeySet in = c10::impl::tls_local_dispatch_key_set().included_;
+  if (in.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || in.has(c10::DispatchKey::PreDispatch)) return true;
+  return Modes::any_modes_set() &&
+         (Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FUNCTIONAL));
+}
+
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
+// Refuses a call whose result torch would take for something that it is not.
+void check_call(const char* name, std::initializer_list<const Tensor*> tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded(), name,
+                              " cannot be traced: its kernels write through pointers, which no trace records");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const Tensor* t : tensors)
+      TORCH_CHECK_NOT_IMPLEMENTED(!t || !has_tangent(*t), name, " has no forward-mode derivative");
+}
+
+// A tensor that is nothing but strided memory: no wrapper around another, no lazily negated view.
+void check_plain(const char* name, const Tensor& t) {
+  using Key = c10::DispatchKey;
+  static const uint64_t allowed = c10::DispatchKeySet({Key::CUDA, Key::HIP, Key::ADInplaceOrView, Key::AutogradCUDA,
+                                                       Key::AutogradHIP, Key::AutocastCUDA})
+                                      .raw_repr();
+  REQUIRE((t.key_set().raw_repr() & ~allowed) == 0 && t.layout() == at::kStrided, name,
+          " needs plain strided tensors, got one with ", t.key_set());
 }
 void check_device(const char* name, const Tensor& t, const Tensor& u) {
   REQUIRE(t.is_cuda() && u.device() == t.device(), name, " needs tensors on one GPU");
+  check_plain(name, u);
+}
+void check_float(const char* name, const Tensor& t) {
+  check_device(name, t, t);
+  REQUIRE(is_type(t.scalar_type()), name, " needs torch.float16, bfloat16 or float32, not ", t.scalar_type());
+}
+const Tensor* maybe(const Maybe& t) { return t ? &*t : nullptr; }
+
+// A gradient that autograd hands over, as plain memory.
+Tensor check_grad(const char* name, const Tensor& grad) {
+  check_call(name, {&grad});
+  const Tensor g = grad.resolve_neg();  // (torch may negate lazily what came through complex numbers)
+  check_plain(name, g);
+  return g;
 }
 
 // The device of a tensor made current, and its current stream.
@@ -115,6 +165,7 @@ Squares quant_weight(const Tensor& w, bool transposed) {
 }
 
 std::tuple<Tensor, Tensor> quantize(const Tensor& x, bool transposed) {
+  check_call("quantize", {&x});
   check_float("quantize", x);
   REQUIRE(x.dim() >= 1 && (!transposed || x.dim() == 2), "quantize needs ",
         transposed ? "a 2-d tensor to transpose" : "one dimension or more", ", got ", x.sizes());
@@ -129,6 +180,7 @@ std::tuple<Tensor, Tensor> quantize(const Tensor& x, bool transposed) {
 }
 
 std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w) {
+  check_call("quantize_weight", {&w});
   check_float("quantize_weight", w);
   REQUIRE(w.dim() >= 2, "quantize_weight needs [..., N, K], got ", w.sizes());
   at::NoGradGuard no_grad;
@@ -189,7 +241,8 @@ void product(const Tensor& x, int64_t ldx, const Tensor& sx, const Tensor& w, in
 
 Tensor mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType out_dtype,
           const Maybe& bias, const Maybe& out_, int tile, int splits) {
-  for (const Tensor* t : {&a_scale, &b, &b_scale}) check_device("fp8.mm", a, *t);
+  check_call("fp8.mm", {&a, &a_scale, &b, &b_scale});
+  for (const Tensor* t : {&a, &a_scale, &b, &b_scale}) check_device("fp8.mm", a, *t);
   REQUIRE(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0), "fp8.mm needs (M, K) @ (K, N), got ", a.sizes(), " @ ",
         b.sizes());
   const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
@@ -243,7 +296,7 @@ struct Train : torch::autograd::Function<Train> {
     const Tensor &qt = saved[0], &st = saved[1], &wqt = saved[2], &ws = saved[3];
     const auto shape = ctx->saved_data["shape"].toIntVector();
     const int64_t need = ctx->saved_data["need"].toInt(), K = shape.back();
-    const Tensor dy = rows_of(grads[0]);
+    const Tensor dy = rows_of(check_grad("fp8.linear", grads[0]));
     const int64_t M = dy.size(0), N = dy.size(1);
     const auto [r, c] = quant_both(dy, need & 1, need & 2);
     Tensor dx, dw;
@@ -291,7 +344,7 @@ struct Stored : torch::autograd::Function<Stored> {
     const Tensor &w = saved[0], &w_scale = saved[1];
     const auto shape = ctx->saved_data["shape"].toIntVector();
     const int64_t need = ctx->saved_data["need"].toInt(), N = w.size(0), K = w.size(1);
-    const Tensor dy = rows_of(grads[0]);
+    const Tensor dy = rows_of(check_grad("fp8.linear", grads[0]));
     Tensor dx, db;
     if (need & 1) {
       const Rows r = quant_rows(dy);
@@ -306,6 +359,7 @@ struct Stored : torch::autograd::Function<Stored> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w, const Maybe& w_scale, const Maybe& bias) {
+  check_call("fp8.linear", {&x, &w, maybe(w_scale), maybe(bias)});
   check_float("fp8.linear", x);
   check_device("fp8.linear", x, w);
   if (w_scale) check_device("fp8.linear", x, *w_scale);
@@ -383,7 +437,7 @@ struct Route : torch::autograd::Function<Route> {
     const int64_t o = ctx->saved_data["o"].toInt();
     Tensor dx = empty(logits.sizes(), logits, logits.scalar_type());
     if (!grads[0].defined()) return {dx.zero_(), {}, {}};
-    const Tensor x = rows_of(logits), dw = rows_of(grads[0]);
+    const Tensor x = rows_of(logits), dw = rows_of(check_grad("route", grads[0]));
     const On on(x);
     check_rc(f16acc_route_grad(x.const_data_ptr(), type_of(x), x.size(0), x.stride(0), x.stride(1), (int)x.size(1),
                                (int)(o >> 2), (o >> 1) & 1, o & 1, (float)ctx->saved_data["scale"].toDouble(),
@@ -395,6 +449,7 @@ struct Route : torch::autograd::Function<Route> {
 
 std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::string& scoring, const Maybe& bias,
                                  int64_t groups, int64_t top, bool renormalize, double scale) {
+  check_call("route", {&logits, maybe(bias)});
   check_float("route", logits);
   REQUIRE(logits.dim() >= 1, "route needs [..., E] logits");
   const int64_t E = logits.size(-1);
@@ -421,6 +476,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
 
 Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const Tensor& w1, const Tensor& s1,
                const Tensor& w2, const Tensor& s2) {
+  check_call("experts", {&x, &weights, &ids, &w1, &s1, &w2, &s2});
   check_float("experts", x);
   for (const Tensor* t : {&weights, &ids, &w1, &s1, &w2, &s2}) check_device("experts", x, *t);
   const bool dims = x.dim() >= 1 && w1.dim() == 4 && w1.size(1) == 2 && w2.dim() == 3;

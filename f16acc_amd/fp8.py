@@ -15,7 +15,9 @@ sum, times its two scales, in FP32, and rounds once to the result's type.  (The
 of the result's 2-norm, 5e-5 of the sum of magnitudes at most, measured.)
 
 Everything runs on the current torch stream of the operands' GPU, allocates
-through torch, and does not synchronise.  Wrong arguments raise ValueError.
+through torch, and does not synchronise.  Wrong arguments raise ValueError; a call
+that torch traces (torch.jit.trace, make_fx, export, torch.func) or differentiates
+forward raises NotImplementedError.
 """
 
 import torch

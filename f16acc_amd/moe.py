@@ -5,7 +5,8 @@
 
 Everything runs on the current torch stream of the operands' GPU, allocates
 through torch, and does not synchronise: the tokens are sorted by expert on the
-device.  Wrong arguments raise ValueError.
+device.  Wrong arguments raise ValueError; a call that torch traces (torch.jit.trace,
+make_fx, export, torch.func) or differentiates forward raises NotImplementedError.
 """
 
 from ._ops import host
