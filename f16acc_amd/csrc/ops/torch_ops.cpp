@@ -270,12 +270,15 @@ void first_derivative_only() {
 // y = x w^T; dx = dy w, dw = dy^T x, each from operands quantised along its own
 // contraction: x and dy in blocks of 128 channels and of 128 tokens, w in
 // squares, which serve both of its products.
-Tensor train_forward(const Tensor& x2, const Tensor& w, bool need_x, bool need_w, Rows* cols, Squares* sq) {
+// The result is no view: autograd forbids changing a view that a function returned in place.
+Tensor train_forward(const Tensor& x, const Tensor& w, bool need_x, bool need_w, Rows* cols, Squares* sq) {
+  const Tensor x2 = rows_of(x);
   auto [r, c] = quant_both(x2, true, need_w);
   *cols = c;
   *sq = quant_weight(w, need_x);
-  Tensor y = empty({x2.size(0), w.size(0)}, x2, x2.scalar_type());
-  product(r.q, r.q.size(1), r.s.t(), sq->q, sq->q.size(1), sq->s, false, x2.size(1), y);
+  const Tensor y = empty(with_last(x, w.size(0)), x, x.scalar_type());
+  product(r.q, r.q.size(1), r.s.t(), sq->q, sq->q.size(1), sq->s, false, x2.size(1),
+          y.view({x2.size(0), w.size(0)}));
   return y;
 }
 
@@ -283,12 +286,12 @@ struct Train : torch::autograd::Function<Train> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
     Rows cols;
     Squares sq;
-    const Tensor y = train_forward(rows_of(x), w, x.requires_grad(), w.requires_grad(), &cols, &sq);
+    const Tensor y = train_forward(x, w, x.requires_grad(), w.requires_grad(), &cols, &sq);
     ctx->save_for_backward({cols.q, cols.s, sq.qt, sq.s});
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["dtype"] = (int64_t)w.scalar_type();
     ctx->saved_data["need"] = (int64_t)x.requires_grad() + 2 * (int64_t)w.requires_grad();
-    return y.view(with_last(x, w.size(0)));
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_derivative_only();
@@ -389,7 +392,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const Maybe& w_scale, const Mayb
     } else {
       Rows cols;
       Squares sq;
-      y = train_forward(rows_of(x), w, false, false, &cols, &sq).view(with_last(x, N));
+      y = train_forward(x, w, false, false, &cols, &sq);
     }
     return bias ? y + *bias : y;
   }
