@@ -267,30 +267,32 @@ void first_derivative_only() {
   TORCH_CHECK(!c10::GradMode::is_enabled(), "f16acc: there is no second derivative (create_graph)");
 }
 
-// y = x w^T; dx = dy w, dw = dy^T x, each from operands quantised along its own
+// y = x w^T + bias; dx = dy w, dw = dy^T x, each from operands quantised along its own
 // contraction: x and dy in blocks of 128 channels and of 128 tokens, w in
 // squares, which serve both of its products.
 // The result is no view: autograd forbids changing a view that a function returned in place.
-Tensor train_forward(const Tensor& x, const Tensor& w, bool need_x, bool need_w, Rows* cols, Squares* sq) {
+Tensor train_forward(const Tensor& x, const Tensor& w, const Maybe& bias, bool need_x, bool need_w, Rows* cols,
+                     Squares* sq) {
   const Tensor x2 = rows_of(x);
   auto [r, c] = quant_both(x2, true, need_w);
   *cols = c;
   *sq = quant_weight(w, need_x);
   const Tensor y = empty(with_last(x, w.size(0)), x, x.scalar_type());
   product(r.q, r.q.size(1), r.s.t(), sq->q, sq->q.size(1), sq->s, false, x2.size(1),
-          y.view({x2.size(0), w.size(0)}));
+          y.view({x2.size(0), w.size(0)}), bias);
   return y;
 }
 
 struct Train : torch::autograd::Function<Train> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias) {
     Rows cols;
     Squares sq;
-    const Tensor y = train_forward(x, w, x.requires_grad(), w.requires_grad(), &cols, &sq);
+    const Tensor y = train_forward(x, w, bias, x.requires_grad(), w.requires_grad(), &cols, &sq);
     ctx->save_for_backward({cols.q, cols.s, sq.qt, sq.s});
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["dtype"] = (int64_t)w.scalar_type();
-    ctx->saved_data["need"] = (int64_t)x.requires_grad() + 2 * (int64_t)w.requires_grad();
+    ctx->saved_data["need"] = (int64_t)x.requires_grad() + 2 * (int64_t)w.requires_grad() +
+                              4 * (int64_t)(bias && bias->requires_grad());
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -301,8 +303,9 @@ struct Train : torch::autograd::Function<Train> {
     const int64_t need = ctx->saved_data["need"].toInt(), K = shape.back();
     const Tensor dy = rows_of(check_grad("fp8.linear", grads[0]));
     const int64_t M = dy.size(0), N = dy.size(1);
-    const auto [r, c] = quant_both(dy, need & 1, need & 2);
-    Tensor dx, dw;
+    Rows r, c;
+    if (need & 3) std::tie(r, c) = quant_both(dy, need & 1, need & 2);
+    Tensor dx, dw, db;
     if (need & 1) {
       dx = empty({M, K}, dy, dy.scalar_type());
       product(r.q, r.q.size(1), r.s.t(), wqt, wqt.size(1), ws.t(), false, N, dx);
@@ -312,7 +315,8 @@ struct Train : torch::autograd::Function<Train> {
       dw = empty({N, K}, dy, (at::ScalarType)ctx->saved_data["dtype"].toInt());
       product(c.q, c.q.size(1), c.s.t(), qt, qt.size(1), st.t(), true, M, dw);
     }
-    return {dx, dw};
+    if (need & 4) db = dy.sum(0);
+    return {dx, dw, db};
   }
 };
 
@@ -385,19 +389,14 @@ Tensor linear(const Tensor& x, const Tensor& w, const Maybe& w_scale, const Mayb
     return bias ? y + *bias : y;
   }
   const bool grad = c10::GradMode::is_enabled();
-  if (!w_scale) {
-    Tensor y;
-    if (grad && (x.requires_grad() || w.requires_grad())) {
-      y = Train::apply(x, w);
-    } else {
-      Rows cols;
-      Squares sq;
-      y = train_forward(x, w, false, false, &cols, &sq);
-    }
-    return bias ? y + *bias : y;
-  }
   Maybe b;
   if (bias) b = bias->contiguous();
+  if (!w_scale) {
+    if (grad && (x.requires_grad() || w.requires_grad() || (b && b->requires_grad()))) return Train::apply(x, w, b);
+    Rows cols;
+    Squares sq;
+    return train_forward(x, w, b, false, false, &cols, &sq);
+  }
   if (grad && (x.requires_grad() || (b && b->requires_grad()))) return Stored::apply(x, w, *w_scale, b);
   return stored(x, w, *w_scale, b);
 }
