@@ -27,6 +27,7 @@ _SIGNATURES = {
     "f16acc_quant_both": [_vp, _int] + [_i64] * 4 + [_vp, _i64, _vp, _i64] * 2 + [_vp],
     "f16acc_quant_weight": [_vp, _int] + [_i64] * 4 + [_vp, _i64, _vp, _i64, _vp, _i64, _vp],
     "f16acc_pack8": [_vp, _vp] + [_i64] * 5 + [_vp],
+    "f16acc_column_sums": [_vp, _int] + [_i64] * 4 + [_vp, _vp, _size, _vp],
     "f16acc_mm_fp8": [_vp, _i64, _vp, _i64, _i64] * 2 + [_int, _vp, _vp] + [_i64] * 5 + [_int] * 3 + [_vp, _size, _vp],
     "f16acc_linear_fp8": [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_vp, _size, _vp],
     "f16acc_route": [_vp, _int] + [_i64] * 3 + [_int] * 3 + [_vp] + [_int] * 3 + [_f32, _vp, _vp, _vp],
@@ -34,6 +35,7 @@ _SIGNATURES = {
     "f16acc_experts": [_vp, _int] + [_i64] * 3 + [_vp, _i64, _i64, _vp, _int, _int] + [_i64] * 2
                       + [_vp] + [_i64] * 3 + [_vp] + [_i64] * 4 + [_vp] + [_i64] * 2 + [_vp] + [_i64] * 3
                       + [_vp, _vp, _size, _vp],
+    "f16acc_column_sums_workspace": [_i64, _i64],
     "f16acc_mm_fp8_workspace": [_i64] * 3 + [_int] * 3,
     "f16acc_linear_fp8_workspace": [_i64] * 3 + [_vp, _i64],
     "f16acc_experts_workspace": [_i64, _int, _int, _i64, _i64],
@@ -52,8 +54,8 @@ def _bind(name):
     return f
 
 
-(quant_rows, quant_both, quant_weight, pack8, mm_fp8, linear_fp8, route, route_grad, experts, mm_fp8_workspace,
- linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
+(quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad, experts,
+ column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
 
 if abi_version() != ABI_VERSION:
     raise ImportError(f"{LIB_OPS} has ABI version {abi_version()}, this package needs {ABI_VERSION}: rebuild it")

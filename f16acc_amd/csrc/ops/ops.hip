@@ -6,6 +6,7 @@
 #include "moe.h"
 #include "quant.h"
 #include "small.h"
+#include "sums.h"
 
 using namespace f16ops;
 
@@ -87,6 +88,12 @@ int quant_tile(const QuantArgs& p, int type, hipStream_t stream) {
       hipLaunchKernelGGL((quant_tile_kernel<T, false, ROWS, COLS, SQUARE>), grid, dim3(512), 0, stream, p);
     return hip_status();
   });
+}
+
+// Parts of the rows of a column sum: four workgroups a CU, of 256 rows at least.
+int64_t sum_parts(int64_t rows, int64_t cols) {
+  const int64_t want = cdiv(4 * kCus, cdiv(cols, 64)), most = cdiv(rows, 256);
+  return want < most ? want : most > 1 ? most : 1;
 }
 
 int mm_check(const MmArgs& p) {
@@ -413,6 +420,36 @@ int f16acc_pack8(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t cols, i
   hipLaunchKernelGGL(pack8_kernel, dim3((uint32_t)(groups < 16 * kCus ? groups : 16 * kCus)), dim3(256), 0,
                      (hipStream_t)stream, p);
   return hip_status();
+}
+
+size_t f16acc_column_sums_workspace(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0 || rows > kMaxExtent || cols > kMaxExtent) return 0;
+  const int64_t parts = sum_parts(rows, cols);
+  return parts > 1 ? up256(parts * cols * 4) : 0;
+}
+
+int f16acc_column_sums(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, void* out,
+                       void* workspace, size_t ws_bytes, void* stream) {
+  const int rc = quant_check(x, type, rows, cols);
+  if (rc || cols == 0) return rc;
+  if (!out) return F16ACC_OPS_E_ARG;
+  if (cols > 0x3fffffff) return F16ACC_OPS_E_UNSUPPORTED;
+  const size_t need = f16acc_column_sums_workspace(rows, cols);
+  if (need && (!workspace || (uintptr_t)workspace % 256 || ws_bytes < need)) return F16ACC_OPS_E_WORKSPACE;
+  const int64_t parts = sum_parts(rows, cols);
+  const uint32_t gx = (uint32_t)cdiv(cols, 64);
+  const SumArgs p{x, rows, cols, sr, sc, cdiv(rows, parts), parts > 1 ? workspace : out};
+  const SumArgs join{workspace, parts, cols, cols, 1, parts, out};
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (parts == 1) {
+      hipLaunchKernelGGL((column_sums_kernel<T, T>), dim3(gx), dim3(256), 0, (hipStream_t)stream, p);
+    } else {
+      hipLaunchKernelGGL((column_sums_kernel<T, float>), dim3(gx, (uint32_t)parts), dim3(256), 0, (hipStream_t)stream, p);
+      hipLaunchKernelGGL((column_sums_kernel<float, T>), dim3(gx), dim3(256), 0, (hipStream_t)stream, join);
+    }
+    return hip_status();
+  });
 }
 
 int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, int64_t sxk, const uint8_t* w,

@@ -263,6 +263,19 @@ Tensor mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor&
   return out;
 }
 
+// The gradient of a bias.  (Not torch's sum: recorded in a graph, it clears its counters by a
+// node that replays do not run right, and was wrong from the second replay on.)
+Tensor column_sums(const Tensor& dy) {
+  const int64_t M = dy.size(0), N = dy.size(1);
+  const size_t n = f16acc_column_sums_workspace(M, N);
+  Tensor ws, out = empty({N}, dy, dy.scalar_type());
+  if (n) ws = empty({(int64_t)n}, dy, at::kByte);
+  const On on(dy);
+  check_rc(f16acc_column_sums(dy.const_data_ptr(), type_of(dy), M, N, dy.stride(0), dy.stride(1), out.data_ptr(),
+                              bytes(ws), n, on.stream));
+  return out;
+}
+
 void first_derivative_only() {
   TORCH_CHECK(!c10::GradMode::is_enabled(), "f16acc: there is no second derivative (create_graph)");
 }
@@ -315,7 +328,7 @@ struct Train : torch::autograd::Function<Train> {
       dw = empty({N, K}, dy, (at::ScalarType)ctx->saved_data["dtype"].toInt());
       product(c.q, c.q.size(1), c.s.t(), qt, qt.size(1), st.t(), true, M, dw);
     }
-    if (need & 4) db = dy.sum(0);
+    if (need & 4) db = column_sums(dy);
     return {dx, dw, db};
   }
 };
@@ -360,7 +373,7 @@ struct Stored : torch::autograd::Function<Stored> {
       product(r.q, r.q.size(1), r.s.t(), wt.q, wt.ld, w_scale.t(), false, N, dx);
       dx = dx.view(shape);
     }
-    if (need & 2) db = dy.sum(0);
+    if (need & 2) db = column_sums(dy);
     return {dx, {}, {}, db};
   }
 };

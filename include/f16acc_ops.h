@@ -64,6 +64,15 @@ int f16acc_pack8(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t cols, i
                  void* stream);
 
 /*
+ * out[c] = sum over r of x[r][c] in FP32, rounded once: a bias's gradient.  x [rows, cols] of `type` (element
+ * strides sr, sc; any), out [cols] of the same type.  Workspace of
+ * f16acc_column_sums_workspace bytes (0 where one pass does), 256-byte aligned.
+ */
+size_t f16acc_column_sums_workspace(int64_t rows, int64_t cols);
+int f16acc_column_sums(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, void* out,
+                       void* workspace, size_t ws_bytes, void* stream);
+
+/*
  * c[m][n] = sum over k of (x[m][k] sx[m][k / 128]) (w[n][k] sw[n'][k / 128]) + bias[n],
  * n' = n / 128 (row_scales 0) or n (row_scales 1).  Each block's sum is an FP32
  * MFMA sum, the blocks are added in FP32 in K order, one rounding to ctype.

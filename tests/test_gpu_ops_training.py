@@ -58,3 +58,55 @@ def test_a_bias_that_a_second_rounding_would_lose():
     b = torch.ones(2, device=DEV).half()
     for lead in (x.requires_grad_(), x.detach()):
         assert fp8.linear(lead, w, bias=b)[0, 0].item() == 2050.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N", [(1, 1), (2, 300), (700, 1), (3000, 65), (16384, 40), (257, 2048)])
+def test_bias_gradient(M, N, dtype):
+    """The sum of a column's gradients in FP32, one rounding; strided and expanded gradients."""
+    x, w = normal(M, 16, dtype=dtype), normal(N, 16, dtype=dtype, seed=2)
+    q, s = fp8.quantize_weight(w)
+    for dy in (normal(M, N, dtype=dtype, seed=3), normal(N, M, dtype=dtype, seed=4).t(),
+               normal(N, dtype=dtype, seed=5).expand(M, N), normal(M, 3 * N + 1, dtype=dtype, seed=6)[:, 1::3]):
+        exact = dy.double().sum(0)
+        bound = M * 2.0 ** -23 * dy.double().abs().sum(0) + ref.ROUND[dtype] * exact.abs() + 2.0 ** -25
+        for layer in ((w,), (q, s)):
+            b = normal(N, dtype=dtype, seed=7).requires_grad_()
+            db, = torch.autograd.grad(fp8.linear(x, *layer, bias=b), b, dy)
+            assert db.dtype == dtype and db.shape == b.shape
+            assert bool(((db.double() - exact).abs() <= bound).all())
+            again, = torch.autograd.grad(fp8.linear(x, *layer, bias=b), b, dy)
+            assert torch.equal(again, db)
+
+
+@pytest.mark.parametrize("M,N,K", [(100, 64, 128), (16384, 1536, 256), (40000, 200, 128)])
+def test_recorded_training_steps_replay(M, N, K):
+    """Forward and backward in one graph, replayed with other gradients and the program's own sums in between."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    fresh = lambda *shape: torch.randn(*shape, generator=g, device=DEV).half()
+    x, w, b = fresh(M, K).requires_grad_(), fresh(N, K).requires_grad_(), fresh(N).requires_grad_()
+    q, s = fp8.quantize_weight(w.detach())
+    dy = fresh(M, N)
+
+    def step():
+        return (*torch.autograd.grad(fp8.linear(x, w, bias=b), (x, w, b), dy),
+                *torch.autograd.grad(fp8.linear(x, q, s, b), (x, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        dy.copy_(fresh(M, N))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.randn(1000, 1000, device=DEV).sum()
+        torch.cuda.synchronize()
+        for name, a, c in zip(("dx", "dw", "db", "stored dx", "stored db"), out, want):
+            assert torch.equal(a, c), name
