@@ -73,8 +73,6 @@ struct MmArgs {
   int64_t xrows;  // rows of x
   int64_t we, swe;
   int tile_rows;  // tokens per entry of the tile list, a multiple of the kernel's
-  // Down (kSlots): binary16 values c of a slot over a power of two for each of its
-  // wave tiles, sq[n / TN][slot].
   // Gate and up (kGatedQuant): w holds the gate's N rows, then (at up bytes, its scales at
   // sup elements) the up's; the result goes to q and its scales, quantised.
   int64_t up, sup;
@@ -84,7 +82,7 @@ struct MmArgs {
   int64_t ldsq;
 };
 
-enum Epilogue { kStore = 0, kGatedQuant = 1, kSlots = 2, kGatedExact = 3 };
+enum Epilogue { kStore = 0, kGatedQuant = 1, kGatedExact = 2 };
 
 template <int BM_, int BN_, int WM_, int WN_, int NS_, int OCC_>
 struct MmCfg {
@@ -518,9 +516,13 @@ struct MmKernel {
                                                    int t16, int g) {
     if (GATED) {
       store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
-    } else if (EPI == kSlots) {
-      store_slots(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
-    } else if (!EXPERTS && p.ksplit) {
+    } else if (EXPERTS) {
+      // A slot's results wait in memory for the sum over its token's experts, in FP32: they are
+      // parts of that sum.  (As binary16 over a power of two for each wave tile's columns
+      // 4096 tokens of 8 experts each, width 2048, took 355 us against 390, and lost what lay 2^14
+      // below the largest column.)
+      store<float>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
+    } else if (p.ksplit) {
       MmArgs q = p;
       q.c = p.parts + (int64_t)blockIdx.y * p.M * p.N;
       q.scm = p.N, q.scn = 1, q.bias = nullptr;
@@ -612,35 +614,6 @@ struct MmKernel {
       }
       wave_sync();
     }
-  }
-
-  // A slot's results wait in memory for the sum over its token's experts, and at
-  // four bytes they were a quarter of the layer's time (4096 tokens, 8 experts each,
-  // width 2048: 268 MB written and read).  They are held as binary16 over a power of two
-  // that brings the largest of the wave tile's columns below 4: 11 bits, whatever
-  // the magnitude, 2^-12 of a value where the sum's own rounding is 2^-9 or 2^-12.
-  __device__ static __forceinline__ void store_slots(const MmArgs& p, char LDS_AS* lds, f32x4 (&acc)[C::FM][C::FN],
-                                                     int64_t m0, int m_left, int64_t n0, int wave, int wm, int wn,
-                                                     int t16, int g) {
-#pragma unroll
-    for (int i = 0; i < C::FM; ++i) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < C::FN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m = umax(m, abs_bits(acc[i][j][r]));
-      m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-      m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-      uint32_t e = m >> 23;
-      e = e < 27 ? 27 : e > 253 ? 253 : e;
-      const float inv = __uint_as_float((254 - e) << 23);
-#pragma unroll
-      for (int j = 0; j < C::FN; ++j) acc[i][j] *= inv;
-      const int row = wm * C::TM + 16 * i + t16;
-      if (g == 0 && row < m_left && n0 + wn * C::TN < p.N)
-        p.sq[(n0 / C::TN + wn) * p.ldsq + m0 + row] = __uint_as_float(e << 23);
-    }
-    store<f16>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
   }
 
   // h = silu(gate) * up of the tile's 128 columns, quantised: they are one block

@@ -371,14 +371,10 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a) {
 }
 
 // y[t] = sum_j weights[t][j] * ys[pos[t][j]], j in order, FP32, rounded once.
-// ys are binary16 over a power of two for each `block` columns.  A thread takes
-// eight columns; bound by reading ys.
+// A thread takes eight columns; bound by reading ys.
 struct CombineArgs {
-  const f16* ys;  // [slots][ld]
+  const float* ys;  // [slots][ld]
   int64_t ld;
-  const float* scale;  // [ld / block][slots]
-  int block;
-  int64_t slots;
   const float* weights;
   int64_t wt, wk;
   const int* pos;
@@ -395,7 +391,7 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
   for (int j = 0; j < a.k; ++j) {
     const int p = a.pos[t * a.k + j];
     if (p < 0) continue;
-    const float w = a.weights[t * a.wt + j * a.wk] * a.scale[n / a.block * a.slots + p];
+    const float w = a.weights[t * a.wt + j * a.wk];
     float v[8];
     load_vec(a.ys + p * a.ld + n, v);
 #pragma unroll

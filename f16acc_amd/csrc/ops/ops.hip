@@ -267,7 +267,6 @@ int expert_tile(int64_t slots, int E) {
   const int64_t mean = slots / E;
   return mean >= 192 ? 256 : mean >= 24 ? 128 : 32;
 }
-int down_block(int tile) { return tile == 32 ? ExpertCfg<32>::Down::TN : ExpertCfg<128>::Down::TN; }
 
 // Whether the two kernels for a few tokens run.
 bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots && k <= kFewK; }
@@ -277,7 +276,7 @@ struct ExpertsPlan {
   int bm;
   size_t few;  // bytes of the hidden values of the kernels for a few tokens
   int64_t ldy;
-  size_t xq, xs, hq, hs, ys, yscale, counts, rows, pos, tiles, ntiles, total;
+  size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
   ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     slots = T * k;
     Dp = up128(D);
@@ -297,8 +296,7 @@ struct ExpertsPlan {
     hq = take(slots * Ip);
     hs = take(slots * (Ip / kBlock) * 4);
     ldy = cdiv(D, 8) * 8;
-    ys = take(slots * ldy * 2);
-    yscale = take(cdiv(D, down_block(bm)) * slots * 4);
+    ys = take(slots * ldy * 4);
     counts = take(chunks * E * 4);
     rows = take(slots * 4);
     pos = take(slots * 4);
@@ -320,7 +318,7 @@ int expert_products(const MmArgs& gu, const MmArgs& down, int64_t max_tiles, hip
   const int rc = launch_mm<GateUp, false, true, EXACT ? kGatedExact : kGatedQuant>(gu, max_tiles * (BM / GateUp::BM), stream);
   if (rc) return rc;
   using Down = typename ExpertCfg<BM>::Down;
-  return launch_mm<Down, false, true, kSlots>(down, max_tiles * (BM / Down::BM), stream);
+  return launch_mm<Down, false, true, kStore>(down, max_tiles * (BM / Down::BM), stream);
 }
 
 template <template <class, int> class Launch, class... A>
@@ -635,7 +633,6 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   down.x = gu.q, down.ldx = plan.Ip, down.sx = gu.sq, down.sxm = 1, down.sxk = plan.slots;
   down.w = w2, down.ldw = ld2, down.sw = s2, down.swn = s2n, down.swk = s2k, down.we = w2e, down.swe = s2e;
   down.c = ws + plan.ys, down.scm = plan.ldy, down.scn = 1;
-  down.sq = (float*)(ws + plan.yscale), down.ldsq = plan.slots;
   gu.tile_rows = down.tile_rows = plan.bm;
   down.M = plan.slots, down.N = D, down.K = I;
   down.tiles = so.tiles, down.ntiles = so.ntiles, down.rows = nullptr, down.xrows = plan.slots;
@@ -645,8 +642,7 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
                                   : expert_products<256, true>(gu, down, plan.max_tiles, stream);
   if (rc) return rc;
 
-  CombineArgs co{(const f16*)(ws + plan.ys), plan.ldy, down.sq, down_block(plan.bm), plan.slots, weights, wt, wk,
-                 so.pos, T, D, k, y};
+  CombineArgs co{(const float*)(ws + plan.ys), plan.ldy, weights, wt, wk, so.pos, T, D, k, y};
   const dim3 grid((uint32_t)T, (uint32_t)cdiv(cdiv(D, 8), 256));
   return by_type(type, [&](auto* t) {
     using U = std::remove_pointer_t<decltype(t)>;

@@ -1,0 +1,54 @@
+"""The experts' results on their way to the weighted sum: no column's value depends on the columns beside it,
+and FP32 results keep FP32's accuracy."""
+
+import pytest
+import torch
+
+from f16acc_amd import fp8, moe
+from tests import ops_reference as ref
+from tests.test_gpu_moe import layer
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+TOKENS = [3, 20, 100, 500]  # over 2 experts, 1 a token: the kernels for few tokens, tiles of 32, 128 and 256
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", TOKENS)
+def test_a_column_does_not_see_its_neighbours(T, dtype):
+    """One row of w2 holds a NaN, or is 2^18 times as large as the others: every other column keeps its bits."""
+    x, weights, ids, w1, s1, w2, s2 = layer(T, 2, 1, 256, 128, dtype)
+    row = 37
+    w2 = w2.float().div(120.0 * 512.0).clamp(-2.0 ** -6, 2.0 ** -6).to(F8)  # (e4m3's smallest values)
+    w2[:, row] = torch.zeros((), device=w2.device).to(F8)
+    others = [n for n in range(256) if n != row]
+    want = moe.experts(x, weights, ids, w1, s1, w2, s2)
+    assert bool((want[:, others] != 0).any())
+    spoilt = w2.clone()
+    spoilt[:, row, 5] = torch.tensor(float("nan"), device=w2.device).to(F8)
+    y = moe.experts(x, weights, ids, w1, s1, spoilt, s2)
+    assert bool(torch.isnan(y[:, row]).all()) and torch.equal(y[:, others], want[:, others])
+    large = w2.clone()
+    large[:, row] = torch.tensor(448.0, device=w2.device).to(F8)
+    y = moe.experts(x, weights, ids, w1, s1, large, s2)
+    assert torch.equal(y[:, others], want[:, others])
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_fp32_results_are_summed_in_fp32(T):
+    """Each column of the result is one hidden value times a power of two, so what rounds is FP32 alone: the gate's
+    and the up's sums of 128 exact products (good to 1e-6 at worst: sums of up to 30 times the result), SiLU and the
+    scales.  Of the 8-bit hidden values 1e-5 may lie on the other side of a tie: of at most 128000 values 1.3 are expected,
+    and 12 are let pass."""
+    x, weights, ids, w1, s1, w2, s2 = layer(T, 2, 2, 128, 128, torch.float32, seed=21)
+    w2 = torch.eye(128, device=x.device).mul(2.0).to(F8).expand(2, 128, 128).contiguous()
+    s2 = torch.full_like(s2, 0.25)
+    y = moe.experts(x, weights, ids, w1, s1, w2, s2).cpu().double()
+    want, parts = torch.zeros(y.shape, dtype=torch.float64), torch.zeros(y.shape, dtype=torch.float64)
+    for j in range(2):
+        one = torch.full_like(ids, -1)
+        one[:, j] = ids[:, j]
+        part = ref.experts(x, weights, one, w1, s1, w2, s2)
+        want, parts = want + part, parts + part.abs()
+    off = (y - want).abs() > 2e-5 * parts
+    assert int(off.sum()) <= 12, (int(off.sum()), ((y - want).abs() / parts.clamp(min=1e-30)).median().item())
