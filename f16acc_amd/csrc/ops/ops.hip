@@ -271,20 +271,25 @@ int expert_tile(int64_t slots, int E) {
 // Whether the two kernels for a few tokens run.
 bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots && k <= kFewK; }
 
+int64_t tile_count(int64_t slots, int E, int bm) { return slots / bm + (slots < E ? slots : E); }
+
+// Where things lie in the workspace, and its size, which is enough for any smaller T as well: the
+// tile list has room for the smallest tiles, and the hidden values of the kernels for a few
+// tokens for as many tokens as they may take.
 struct ExpertsPlan {
   int64_t slots, chunks, max_tiles, Dp, Ip;
   int bm;
-  size_t few;  // bytes of the hidden values of the kernels for a few tokens
+  bool few;  // the kernels for a few tokens run (if x's rows allow their loads)
   int64_t ldy;
   size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
   ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     slots = T * k;
     Dp = up128(D);
     Ip = up128(I);
-    few = few_tokens(T, k) ? up256(slots * Ip * 4) + up256(sizeof(FewMap)) : 0;
+    few = few_tokens(T, k);
     bm = expert_tile(slots, E);
     chunks = cdiv(slots, kSortChunk);
-    max_tiles = slots / bm + (slots < E ? slots : E);
+    max_tiles = tile_count(slots, E, bm);
     size_t at = 0;
     auto take = [&](size_t bytes) {
       const size_t here = at;
@@ -300,9 +305,14 @@ struct ExpertsPlan {
     counts = take(chunks * E * 4);
     rows = take(slots * 4);
     pos = take(slots * 4);
-    tiles = take(max_tiles * 16);
+    tiles = take(tile_count(slots, E, 32) * 16);
     ntiles = take(4);
-    total = at > few ? at : few;
+    total = at;
+    if (few_tokens(1, k)) {
+      const int64_t t = kFewSlots / k < kFewTokens ? kFewSlots / k : kFewTokens;
+      const size_t hidden = up256((T < t ? T : t) * k * Ip * 4) + up256(sizeof(FewMap));
+      if (total < hidden) total = hidden;
+    }
   }
 };
 

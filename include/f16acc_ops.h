@@ -83,8 +83,8 @@ int f16acc_column_sums(const void* x, int type, int64_t rows, int64_t cols, int6
  *   bias: [N] of ctype, or NULL;  c: element strides scm, scn
  *   tile, splits: -1 and 0 leave the choice to the library; a tile number (0 to 5) and a number of parts
  *   of K force them, for tuning
- *   workspace: f16acc_mm_fp8_workspace bytes (FP32 sums of the parts of K, 0 if
- *   not split), 256-byte aligned
+ *   workspace: f16acc_mm_fp8_workspace bytes for exactly these sizes (FP32 sums of the parts of
+ *   K, 0 if not split; fewer rows may need more), 256-byte aligned
  */
 int f16acc_mm_fp8(const uint8_t* x, int64_t ldx, const float* sx, int64_t sxm, int64_t sxk, const uint8_t* w,
                   int64_t ldw, const float* sw, int64_t swn, int64_t swk, int row_scales, const void* bias, void* c,
@@ -96,7 +96,7 @@ size_t f16acc_mm_fp8_workspace(int64_t M, int64_t N, int64_t K, int row_scales, 
  * y = x w^T + bias with x [M, K] of `type` (element strides sr, sc) quantised in row blocks on
  * the way; w [N][ldw] bytes of any alignment, ldw at least K, with square-block scales sw as in
  * f16acc_mm_fp8; y [M][N] contiguous and bias of x's type; K at least 1.
- * Workspace of f16acc_linear_fp8_workspace bytes, 256-byte aligned.
+ * Workspace of f16acc_linear_fp8_workspace bytes for exactly these sizes, 256-byte aligned.
  */
 size_t f16acc_linear_fp8_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw);
 int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw, const float* sw,
@@ -134,7 +134,7 @@ int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64
  *   w1 [E][2][I][D] (gate, up), expert stride w1e bytes, up at w1u, rows ld1
  *   s1 of (e, gate or up, n / 128, k / 128): strides s1e, s1u, s1n, s1k
  *   w2 [E][D][I], strides w2e, ld2;  s2: s2e, s2n, s2k
- * Workspace of f16acc_experts_workspace bytes, 256-byte aligned.
+ * Workspace of f16acc_experts_workspace bytes, 256-byte aligned; it is enough for any smaller T too.
  */
 size_t f16acc_experts_workspace(int64_t T, int k, int E, int64_t D, int64_t I);
 int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const float* weights, int64_t wt,
