@@ -8,6 +8,7 @@
 // calls.  A failed check raises ValueError, a failed launch RuntimeError, and a call that
 // something records or differentiates forward NotImplementedError.
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -104,7 +105,10 @@ struct On {
       : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-void check_rc(int rc) { TORCH_CHECK(rc == 0, f16acc_ops_strerror(rc)); }
+void check_rc(int rc) {
+  REQUIRE(rc != F16ACC_OPS_E_ARG, f16acc_ops_strerror(rc));
+  TORCH_CHECK(rc == 0, f16acc_ops_strerror(rc));
+}
 
 Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType t) {
   return at::empty(sizes, like.options().dtype(t).requires_grad(false));
@@ -255,11 +259,23 @@ Tensor mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor&
   REQUIRE(row_scales || b_scale.sizes() == at::IntArrayRef({blocks(K), blocks(N)}), "b_scale must be ",
         at::IntArrayRef({blocks(K), blocks(N)}), " or ", at::IntArrayRef({blocks(K), N}), ", got ", b_scale.sizes());
   REQUIRE(is_type(out_dtype), "fp8.mm writes torch.float16, bfloat16 or float32, not ", out_dtype);
+  Maybe b_;
+  if (out_) {
+    check_device("fp8.mm_tile", a, *out_);
+    REQUIRE(out_->sizes() == at::IntArrayRef({M, N}), "out must be ", at::IntArrayRef({M, N}), ", got ", out_->sizes());
+    REQUIRE(at::has_internal_overlap(*out_) != at::MemOverlap::Yes, "out must not share memory between its elements");
+  }
+  if (bias) {
+    check_device("fp8.mm_tile", a, *bias);
+    REQUIRE(bias->sizes() == at::IntArrayRef({N}) && bias->scalar_type() == out_dtype, "bias must be ", out_dtype, " [", N,
+            "], got ", bias->scalar_type(), " ", bias->sizes());
+    b_ = bias->contiguous();
+  }
   const Tensor out = out_ ? *out_ : empty({M, N}, a, out_dtype);
   if (M == 0 || N == 0) return out;
   if (K == 0) return out.zero_();
   const Operand x = packed(a), w = packed(b.t());
-  product(x.q, x.ld, a_scale, w.q, w.ld, b_scale.t(), row_scales, K, out, bias, tile, splits);
+  product(x.q, x.ld, a_scale, w.q, w.ld, b_scale.t(), row_scales, K, out, b_, tile, splits);
   return out;
 }
 
