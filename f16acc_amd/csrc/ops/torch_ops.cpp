@@ -273,7 +273,7 @@ Tensor mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor&
   }
   const Tensor out = out_ ? *out_ : empty({M, N}, a, out_dtype);
   if (M == 0 || N == 0) return out;
-  if (K == 0) return out.zero_();
+  if (K == 0) return b_ ? out.copy_(b_->expand({M, N})) : out.zero_();
   const Operand x = packed(a), w = packed(b.t());
   product(x.q, x.ld, a_scale, w.q, w.ld, b_scale.t(), row_scales, K, out, b_, tile, splits);
   return out;

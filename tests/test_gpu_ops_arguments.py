@@ -28,3 +28,14 @@ def test_mm_tile_refuses_what_does_not_fit():
     bias = normal(3 * N, dtype=torch.float32)[::3]
     f(out, bias)
     ref.check_product(out, ref.values(a, sa), ref.values(w, ws, 128), bias)
+
+
+def test_mm_tile_without_a_product_is_the_bias():
+    M, N = 5, 7
+    z = lambda *s: torch.zeros(*s, device=DEV)
+    out, bias = torch.full((M, N), 3.0, device=DEV), normal(N, dtype=torch.float32)
+    a, b = z(M, 0).to(torch.float8_e4m3fn), z(0, N).to(torch.float8_e4m3fn)
+    fp8.mm_tile(a, z(M, 0), b, z(0, 1), out, -1, 0)
+    assert bool((out == 0).all())
+    fp8.mm_tile(a, z(M, 0), b, z(0, 1), out, -1, 0, bias)
+    assert torch.equal(out, bias.expand(M, N))
