@@ -205,6 +205,10 @@ std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w) {
   return {q.narrow(-1, 0, K), s};
 }
 
+// The products address a tile's rows by 31-bit offsets: rows of an operand, and of its scales, may be
+// this many bytes apart.  What lies further apart is copied.
+constexpr int64_t kMaxRow = 1 << 22;
+
 // An e4m3 operand [..., rows, K] with rows as the products read them: itself, or a copy
 // whose rows are 16-byte aligned and zero from K to the next multiple of 16.
 struct Operand {
@@ -213,7 +217,7 @@ struct Operand {
 };
 Operand packed(const Tensor& q) {
   const int64_t d = q.dim(), rows = q.size(-2), K = q.size(-1), ld = rows > 1 ? q.stride(-2) : up(K, 16);
-  bool as_it_is = K % 16 == 0 && (q.stride(-1) == 1 || K <= 1) && ld >= K && ld % 16 == 0 &&
+  bool as_it_is = K % 16 == 0 && (q.stride(-1) == 1 || K <= 1) && ld >= K && ld % 16 == 0 && ld <= kMaxRow &&
                   (uintptr_t)q.const_data_ptr() % 16 == 0;
   for (int64_t i = 0; i < d - 2; ++i) as_it_is = as_it_is && q.stride(i) % 16 == 0;
   if (as_it_is) return {q, ld};
@@ -224,6 +228,11 @@ Operand packed(const Tensor& q) {
   const On on(q);
   check_rc(f16acc_pack8(bytes(src), bytes(out), src.size(0), K, src.stride(0), src.stride(1), up(K, 16), on.stream));
   return {out, up(K, 16)};
+}
+
+// Scales ([rows], [blocks of K]) as the products read them.
+Tensor near(const Tensor& s) {
+  return s.stride(0) <= kMaxRow / 4 ? s : s.clone(at::MemoryFormat::Contiguous);
 }
 
 // ---------------------------------------------------------------------------
@@ -275,7 +284,7 @@ Tensor mm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor&
   if (M == 0 || N == 0) return out;
   if (K == 0) return b_ ? out.copy_(b_->expand({M, N})) : out.zero_();
   const Operand x = packed(a), w = packed(b.t());
-  product(x.q, x.ld, a_scale, w.q, w.ld, b_scale.t(), row_scales, K, out, b_, tile, splits);
+  product(x.q, x.ld, near(a_scale), w.q, w.ld, near(b_scale.t()), row_scales, K, out, b_, tile, splits);
   return out;
 }
 
@@ -349,8 +358,8 @@ struct Train : torch::autograd::Function<Train> {
   }
 };
 
-Tensor stored(const Tensor& x, const Tensor& w_, const Tensor& w_scale, const Maybe& bias) {
-  const Tensor x2 = rows_of(x);
+Tensor stored(const Tensor& x, const Tensor& w_, const Tensor& w_scale_, const Maybe& bias) {
+  const Tensor x2 = rows_of(x), w_scale = near(w_scale_);
   const int64_t M = x2.size(0), K = x2.size(1), N = w_.size(0);
   // rows of any alignment go as they are (the library copies them where it has to)
   const bool rows = (K <= 1 || w_.stride(1) == 1) && (N <= 1 || w_.stride(0) >= K);
@@ -386,7 +395,7 @@ struct Stored : torch::autograd::Function<Stored> {
       const Rows r = quant_rows(dy);
       const Operand wt = packed(w.t());
       dx = empty({dy.size(0), K}, dy, dy.scalar_type());
-      product(r.q, r.q.size(1), r.s.t(), wt.q, wt.ld, w_scale.t(), false, N, dx);
+      product(r.q, r.q.size(1), r.s.t(), wt.q, wt.ld, near(w_scale.t()), false, N, dx);
       dx = dx.view(shape);
     }
     if (need & 2) db = column_sums(dy);

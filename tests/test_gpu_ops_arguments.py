@@ -3,9 +3,9 @@
 import pytest
 import torch
 
-from f16acc_amd import fp8
+from f16acc_amd import fp8, moe
 from tests import ops_reference as ref
-from tests.test_gpu_fp8 import DEV, normal, weight
+from tests.test_gpu_fp8 import DEV, F8, normal, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,40 @@ def test_mm_tile_without_a_product_is_the_bias():
     assert bool((out == 0).all())
     fp8.mm_tile(a, z(M, 0), b, z(0, 1), out, -1, 0, bias)
     assert torch.equal(out, bias.expand(M, N))
+
+
+def test_rows_more_than_4_mib_apart():
+    M, N, K, far = 20, 24, 256, (1 << 22) + 64
+    a, sa = fp8.quantize(normal(M, K))
+    w, ws = weight(N, K)
+    want = fp8.mm(a, sa, w.t(), ws.t(), torch.float32)
+    pool = torch.zeros(N * far, dtype=torch.uint8, device=DEV).view(F8)
+    apart = lambda t: pool[:t.shape[0] * far].view(t.shape[0], far)[:, :K].copy_(t)
+    assert torch.equal(fp8.mm(apart(a), sa, w.t(), ws.t(), torch.float32), want)
+    assert torch.equal(fp8.mm(a, sa, apart(w).t(), ws.t(), torch.float32), want)
+    x = normal(M, K)
+    assert torch.equal(fp8.linear(x, apart(w), ws), fp8.linear(x, w, ws))
+    args = torch.ones(M, 1, device=DEV), torch.zeros(M, 1, dtype=torch.int32, device=DEV)
+    w2 = torch.zeros(2, 3, far, dtype=torch.uint8, device=DEV).view(F8)[:, :, :128]
+    small = fp8.quantize_weight(normal(2, 2, 128, 3)), fp8.quantize_weight(normal(2, 3, 128))
+    w2.copy_(small[1][0])
+    x3 = normal(M, 3)
+    assert torch.equal(moe.experts(x3, *args, *small[0], w2, small[1][1]), moe.experts(x3, *args, *small[0], *small[1]))
+
+
+def test_scales_more_than_4_mib_apart():
+    M, N, K, far = 20, 200, 256, (1 << 20) + 16
+    x = normal(M, K)
+    a, sa = fp8.quantize(x)
+    w, ws = weight(N, K)
+    b, sb = fp8.quantize(normal(N, K, seed=5))
+    pool = torch.zeros(N * far, device=DEV)
+    apart = lambda t: pool[:t.shape[0] * far].view(t.shape[0], far)[:, :t.shape[1]].copy_(t)
+    want = fp8.mm(a, sa, w.t(), ws.t())
+    assert torch.equal(fp8.mm(a, apart(sa), w.t(), ws.t()), want)
+    assert torch.equal(fp8.mm(a[:1], apart(sa[:1]), w.t(), ws.t()), fp8.mm(a[:1], sa[:1], w.t(), ws.t()))
+    assert torch.equal(fp8.mm(a, sa, w.t(), apart(ws).t()), want)
+    assert torch.equal(fp8.mm(a, sa, b.t(), apart(sb).t()), fp8.mm(a, sa, b.t(), sb.t()))
+    assert torch.equal(fp8.linear(x, w, apart(ws)), fp8.linear(x, w, ws))
+    grad = lambda s: torch.autograd.grad(fp8.linear(x.requires_grad_(), w, s), x, normal(M, N, seed=3))[0]
+    assert torch.equal(grad(apart(ws)), grad(ws))
