@@ -194,9 +194,10 @@ std::tuple<Tensor, Tensor> quantize_weight(const Tensor& w) {
   ss.back() = blocks(K);
   ss[ss.size() - 2] = blocks(N);
   const Tensor q = empty(qs, w, kF8), s = empty(ss, w, at::kFloat);
+  if (w.numel() == 0) return {q.narrow(-1, 0, K), s};
   const Tensor w3 = w.detach().reshape({-1, N, K});
   const On on(w);
-  for (int64_t i = 0; w.numel() && i < w3.size(0); ++i) {
+  for (int64_t i = 0; i < w3.size(0); ++i) {
     const Tensor wi = w3[i];
     check_rc(f16acc_quant_weight(wi.const_data_ptr(), type_of(w), N, K, wi.stride(0), wi.stride(1),
                                  bytes(q) + i * N * qs.back(), qs.back(), floats(s) + i * blocks(N) * blocks(K),

@@ -76,3 +76,11 @@ def test_scales_more_than_4_mib_apart():
     assert torch.equal(fp8.linear(x, w, apart(ws)), fp8.linear(x, w, ws))
     grad = lambda s: torch.autograd.grad(fp8.linear(x.requires_grad_(), w, s), x, normal(M, N, seed=3))[0]
     assert torch.equal(grad(apart(ws)), grad(ws))
+
+
+@pytest.mark.parametrize("shape", [(0, 0), (0, 5), (5, 0), (3, 0, 40), (3, 40, 0), (0, 4, 4), (2, 0, 130, 7), (2, 2, 0, 7)])
+def test_empty_weights(shape):
+    for dtype in (torch.float16, torch.float32):
+        q, s = fp8.quantize_weight(torch.zeros(shape, dtype=dtype, device=DEV))
+        assert q.shape == shape and q.dtype == F8 and s.dtype == torch.float32
+        assert s.shape == (*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128))
