@@ -51,7 +51,7 @@ __device__ __forceinline__ void quant_rows(const QuantArgs& p, uint32_t group, u
     o[0] = pack_e4m3(v[0], v[1], v[2], v[3], bs.inv);
     o[1] = pack_e4m3(v[4], v[5], v[6], v[7], bs.inv);
     *(i32x2*)(p.q + row * p.ldq + c0) = o;
-    if (lane == 0) p.s[kb * p.lds + row] = bs.s;
+    if (lane == 0 && c0 < p.cols) p.s[kb * p.lds + row] = bs.s;  // (what pads a row has no scale)
   }
 }
 template <class T, bool WIDE>

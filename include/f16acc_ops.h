@@ -36,15 +36,16 @@ extern "C" {
 /*
  * Row blocks of x [rows, cols] (element strides sr, sc; any): q [rows][ldq]
  * bytes, ldq a multiple of 128 and at least cols, zero from cols on, 16-byte
- * aligned; the scale of (row, block) at s[block * lds + row].
+ * aligned; the scale of (row, block) at s[block * lds + row], for the ceil(cols / 128) blocks that hold
+ * a column; lds at least rows.
  */
 int f16acc_quant_rows(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
                       int64_t ldq, float* s, int64_t lds, void* stream);
 
 /*
- * x read once and quantised in both directions: row blocks as above (q NULL:
- * not wanted), and blocks of 128 rows of each column, transposed: qt
- * [cols][ldqt], ldqt a multiple of 128 and at least rows, zero from rows on, the
+ * x read once and quantised in both directions: row blocks as above, ldq the next multiple of
+ * 128 from cols (q NULL: not wanted), and blocks of 128 rows of each column, transposed: qt
+ * [cols][ldqt], ldqt the next multiple of 128 from rows, zero from rows on, the
  * scale of (column, row block) at st[block * ldst + column] (qt NULL: not wanted).
  */
 int f16acc_quant_both(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
@@ -54,7 +55,7 @@ int f16acc_quant_both(const void* x, int type, int64_t rows, int64_t cols, int64
 /*
  * Square blocks: q [rows][ldq], the scale of a block at s[rowblock * lds +
  * block]; with qt the same values transposed, [cols][ldqt], whose scales are s read
- * the other way round.
+ * the other way round.  ldq and ldqt as in f16acc_quant_both.
  */
 int f16acc_quant_weight(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
                         int64_t ldq, float* s, int64_t lds, uint8_t* qt, int64_t ldqt, void* stream);

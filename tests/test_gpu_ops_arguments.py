@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from f16acc_amd import fp8, moe
+from f16acc_amd import _ops, fp8, moe
 from tests import ops_reference as ref
 from tests.test_gpu_fp8 import DEV, F8, normal, weight
 
@@ -84,3 +84,17 @@ def test_empty_weights(shape):
         q, s = fp8.quantize_weight(torch.zeros(shape, dtype=dtype, device=DEV))
         assert q.shape == shape and q.dtype == F8 and s.dtype == torch.float32
         assert s.shape == (*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128))
+
+
+@pytest.mark.parametrize("rows,cols,ldq", [(5, 200, 256), (5, 200, 640), (70, 1, 256), (3, 128, 1280)])
+def test_rows_wider_than_their_blocks(rows, cols, ldq):
+    """The C ABI's rows may be padded by whole blocks: zeros, and no scale past the last block with a column."""
+    x = normal(rows, cols)
+    q = torch.full((rows, ldq), 7, dtype=torch.uint8, device=DEV)
+    blocks = -(-cols // 128)
+    s = torch.full((ldq // 128 + 2, rows), 7.0, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _ops.quant_rows(x.data_ptr(), 0, rows, cols, cols, 1, q.data_ptr(), ldq, s.data_ptr(), rows, stream) == 0
+    want = fp8.quantize(x)
+    assert torch.equal(q[:, :cols], want[0].view(torch.uint8)) and bool((q[:, cols:] == 0).all())
+    assert torch.equal(s[:blocks].t(), want[1]) and bool((s[blocks:] == 7.0).all())
