@@ -575,14 +575,17 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("torch_version") = TORCH_VERSION;  // the module uses torch's C++ types, which change between versions
   m.attr("abi_version") = f16acc_ops_abi_version();
-  m.def("quantize", &quantize);
-  m.def("quantize_weight", &quantize_weight);
+  typedef py::call_guard<py::gil_scoped_release> Free;  // other threads run during checks, allocation and launch
+  m.def("quantize", &quantize, Free());
+  m.def("quantize_weight", &quantize_weight, Free());
   m.def("mm", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, py::object dtype,
                  const Maybe& bias, const Maybe& out, int tile, int splits) {
     REQUIRE(THPDtype_Check(dtype.ptr()), "fp8.mm writes torch.float16, bfloat16 or float32");
-    return mm(a, sa, b, sb, ((THPDtype*)dtype.ptr())->scalar_type, bias, out, tile, splits);
+    const at::ScalarType type = ((THPDtype*)dtype.ptr())->scalar_type;
+    py::gil_scoped_release free;
+    return mm(a, sa, b, sb, type, bias, out, tile, splits);
   });
-  m.def("linear", &linear);
-  m.def("route", &route);
-  m.def("experts", &experts);
+  m.def("linear", &linear, Free());
+  m.def("route", &route, Free());
+  m.def("experts", &experts, Free());
 }
