@@ -26,7 +26,8 @@ PACK_MIN_MACS = 1 << 24
 # kernels as they are and whose plan needs no workspace; it returns None for
 # every other call, which then takes the general path below.
 _host = _lib.host
-_compiling = torch.compiler.is_compiling  # a traced call takes the general path, as it did
+_compiling = torch.compiler.is_compiling  # a compiled call takes the general path, as it did
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 _host.setup(torch._C._cuda_getCurrentRawStream, PACK_MIN_MACS, *map(_lib.address, (
     _lib.gemm, _lib.gemm_bias, _lib.workspace_size, _lib.tile_config, _lib.strerror)))
 
@@ -51,9 +52,18 @@ _ws_sizes = {}  # problem key -> f16acc_workspace_size result
 _WS_MEMO_MAX = 4096
 
 
+def recorded():
+    """Whether torch.jit.trace or make_fx records the calls: the kernels write
+    through pointers, so it would record the output's allocation alone, and replay
+    uninitialised memory."""
+    return not _compiling() and (torch.jit.is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None)
+
+
 def _validate(a, b, out_dtype):
     """Real checks, not asserts (python -O keeps them): a wrong shape or dtype
     would let the kernel read past the end of b (kernel.py:85-90)."""
+    if recorded():
+        raise NotImplementedError("f16acc: mm cannot be traced: its kernels write through pointers, which no trace records")
     if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0]:
         raise ValueError(f"mm needs (M, K) @ (K, N), got {tuple(a.shape)} @ {tuple(b.shape)}")
     if a.dtype != torch.float16 or b.dtype != torch.float16 or not (a.is_cuda and b.is_cuda) or a.device != b.device:
@@ -69,7 +79,8 @@ def mm(a, b, out_dtype=torch.float16, chunked=True):
     chunked:   True  -> 32-long K chunks rounded to fp16 and added into an FP32
                         sum, tiles with an inf/NaN sum redone in FP32
                False -> plain FP32 accumulation
-    Raises ValueError for bad shapes, dtypes or devices (kernel.py:87-90).
+    Raises ValueError for bad shapes, dtypes or devices (kernel.py:87-90), and
+    NotImplementedError under torch.jit.trace and make_fx.
     """
     if (out_dtype is torch.float16 or out_dtype is torch.float32) and not _compiling():
         c = _host.mm(a, b, None, out_dtype is torch.float32, bool(chunked))

@@ -5,7 +5,8 @@
 Same behaviour as the reference's f16acc/patch.py:17-40: only
 torch.nn.functional.linear is replaced (nn.Linear.forward calls it through
 the module attribute).  Calls whose input is not fp16 on a GPU, whose weight
-is not fp16, that run with gradients enabled, or that have fewer than
+is not fp16, that run with gradients enabled, that torch.jit.trace or make_fx
+records, or that have fewer than
 MIN_ROWS rows (decode steps: memory-bound) go to the original F.linear and
 are counted under calls["original"]; the rest go through mm and are counted
 under calls["chunked"].  An fp16 bias is added in the GEMM's store with the
@@ -18,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .kernel import mm, mm_bias
+from .kernel import mm, mm_bias, recorded
 
 MIN_ROWS = 128
 _orig = F.linear
@@ -36,7 +37,7 @@ def linear(x, w, b=None):
             return y
     rows = x.shape[:-1].numel()
     eligible = (x.is_cuda and x.dtype == torch.float16 and w.dtype == torch.float16 and rows >= MIN_ROWS
-                and not torch.is_grad_enabled())
+                and not torch.is_grad_enabled() and not recorded())
     if not eligible:
         calls["original"] += 1
         return _orig(x, w, b)
