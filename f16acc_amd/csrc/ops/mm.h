@@ -102,16 +102,6 @@ struct MmCfg {
 // Spreads the 16 rows that a fragment read touches over the LDS banks.
 __device__ __forceinline__ int swz(int row) { return ((row >> 1) ^ ((row & 1) << 2)) & 7; }
 
-// Rows row .. row + 15 (row = lane % 16) of a staged operand: lane group g holds
-// units g and g + 4 of the row's eight.  (The order of k inside a block is the
-// same for both operands, so any will do.)
-__device__ __forceinline__ i32x8 read_frag(const char LDS_AS* base, int row, int g) {
-  const char LDS_AS* r = base + row * kBlock;
-  const i32x4 lo = *(const i32x4 LDS_AS*)(r + ((g ^ swz(row)) << 4));
-  const i32x4 hi = *(const i32x4 LDS_AS*)(r + (((g + 4) ^ swz(row)) << 4));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
 __device__ __forceinline__ f32x4 mfma(const i32x8& w, const i32x8& x) {
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
@@ -347,7 +337,9 @@ struct MmKernel {
     typedef const float __attribute__((address_space(4)))* Scalar;
     const Scalar swp = (Scalar)(uintptr_t)(sw + (nb < nb_last ? nb : nb_last) * p.swn);
 
-    // A wave's addresses in a stage; the fragments of an operand lie 16 rows apart.
+    // A wave's addresses in a stage; the fragments of an operand lie 16 rows apart.  Lane group g
+    // holds units g and g + 4 of a row's eight.  (The order of k inside a block is the same for both
+    // operands, so any will do.)
     const int frag = t16 * kBlock, lo = (g ^ swz(t16)) << 4, hi = ((g + 4) ^ swz(t16)) << 4;
     const int xa = wm * C::TM * kBlock + frag, wa = C::X_BYTES + frag;
     const int sa = C::X_BYTES + C::W_BYTES + (wm * C::TM + t16) * 4;
