@@ -6,7 +6,7 @@ import torch.nn.functional as F
 
 from f16acc_amd import fp8, moe
 from tests import ops_reference as ref
-from tests.test_gpu_fp8 import DEV, normal, weight
+from tests.test_gpu_fp8 import DEV, F8, normal, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,30 @@ def test_recorded_training_steps_replay(M, N, K):
         torch.cuda.synchronize()
         for name, a, c in zip(("dx", "dw", "db", "stored dx", "stored db"), out, want):
             assert torch.equal(a, c), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 130, 200), (3, 1, 70), (9, 128, 128), (17, 260, 129), (130, 96, 272),
+                                   (257, 300, 520), (500, 77, 1000)])
+def test_stored_weight_gradients(M, N, K, dtype):
+    x = normal(M, K, dtype=dtype).requires_grad_()
+    b = normal(N, dtype=dtype, seed=5).requires_grad_()
+    w, s = weight(N, K)
+    dy = normal(M, N, dtype=dtype, seed=3)
+    dx, db = torch.autograd.grad(fp8.linear(x, w, s, b), (x, b), dy)
+    ref.check_product(dx, ref.rounded(dy), ref.values(w, s, 128).t())
+    exact = dy.double().sum(0).cpu()
+    # FP32 sums of M terms, one rounding
+    bound = M * 2.0 ** -23 * dy.double().abs().sum(0).cpu() + ref.ROUND[dtype] * exact.abs() + 1e-30
+    assert db.dtype == dtype and bool(((db.double().cpu() - exact).abs() <= bound).all())
+    alone, = torch.autograd.grad(fp8.linear(x, w, s), x, dy)
+    assert torch.equal(alone, dx)
+    # the same weight in other layouts, the same gradient of another
+    wide = torch.full((N, K + 5), float("nan")).to(F8).to(DEV)
+    wide[:, 3:K + 3] = w
+    for v in (w.t().contiguous().t(), wide[:, 3:K + 3]):
+        other, = torch.autograd.grad(fp8.linear(x, v, s, b), x, dy.t().contiguous().t())
+        assert torch.equal(other, dx)
+    cube = x.detach().view(M, 1, K).requires_grad_()
+    other, = torch.autograd.grad(fp8.linear(cube, w, s), cube, dy.view(M, 1, N))
+    assert torch.equal(other.view(M, K), dx)
