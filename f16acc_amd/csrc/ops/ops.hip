@@ -269,7 +269,7 @@ int expert_tile(int64_t slots, int E) {
 }
 
 // Whether the two kernels for a few tokens run.
-bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots && k <= kFewK; }
+bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots; }
 
 int64_t tile_count(int64_t slots, int E, int bm) { return slots / bm + (slots < E ? slots : E); }
 
@@ -609,7 +609,7 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
               (FewMap*)(ws + up256(plan.slots * plan.Ip * 4)), y};
     return by_type(type, [&](auto* t) {
       using U = std::remove_pointer_t<decltype(t)>;
-      constexpr int G = 2;
+      constexpr int G = (kFewTokens + 3) / 4;
       hipLaunchKernelGGL((few_gate_up_kernel<U, 8, G>), dim3((uint32_t)cdiv(I, 32), (uint32_t)plan.slots + 1), dim3(512), 0,
                          stream, f);
       hipLaunchKernelGGL((few_down_kernel<U, 16, G>), dim3((uint32_t)cdiv(D, 16)), dim3(1024), 0, stream, f);

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * W) void linear_small_kernel(SmallArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// The experts' feed-forward for at most 8 tokens: no sorting.  Token t is column
+// The experts' feed-forward for at most 4 tokens: no sorting.  Token t is column
 // t of every expert's products, zero where the token does not go there, so the
 // down kernel adds all experts of a token in one register, and the routing weight
 // is a factor of the block's scale.
@@ -173,8 +173,12 @@ __device__ __forceinline__ f32x4 exact_product(const i32x8& w, const Halves& x) 
   return sum;
 }
 
-// (4 tokens of 64 experts, 8 each, 2048 x 1024: 55 us against 60 on the tiles; 16: 178 against 88)
-constexpr int kFewTokens = 8, kFewSlots = 128, kFewK = 16;
+// At most 4 tokens and 16 slots.  Here and on the tiles, in us (bfloat16, in a graph; 8 tokens
+// here with two groups of four):
+//   64 experts of 2048 x 1024, 8 a token: 1 token 20 / 38, 2 32 / 40, 4 55 / 48, 8 100 / 72
+//   16 of 4096 x 2048, 2 a token:         1 token 20 / 49, 4 39 / 55, 8 65 / 59
+//   128 of 1024 x 512, 4 a token:         1 token 10 / 26, 4 15 / 26, 8 30 / 30
+constexpr int kFewTokens = 4, kFewSlots = 16;
 
 // What the down kernel reads of the routing: the distinct experts in order of their
 // first slots, and each token's first slot with each of them (-1: none) and its weight.
@@ -209,10 +213,10 @@ struct FewArgs {
 // Fills p.map, by one workgroup while the others multiply.
 template <int THREADS>
 __device__ __forceinline__ void few_map(const FewArgs& p) {
-  __shared__ int ids[kFewSlots], index[kMaxExperts], firsts[kFewSlots / 64];
+  __shared__ int ids[kFewSlots], index[kMaxExperts];
   __shared__ float weights[kFewSlots];
-  static_assert(THREADS >= kFewSlots, "a thread per slot");
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  static_assert(kFewSlots <= 64, "the first wave has a lane per slot");  // (and reads index before it writes it)
+  const int tid = threadIdx.x, lane = tid & 63;
   // index[e]: the lowest slot with expert e, then the expert's place
   for (int i = tid; i < p.E; i += THREADS) index[i] = kFewSlots;
   int e = -1;
@@ -227,21 +231,14 @@ __device__ __forceinline__ void few_map(const FewArgs& p) {
   __syncthreads();
   const bool first = e >= 0 && index[e] == tid;
   const uint64_t mask = __builtin_amdgcn_ballot_w64(first);
-  if (tid < kFewSlots && lane == 0) firsts[wave] = __popcll(mask);
-  __syncthreads();
-  int count = 0, at = 0;
-#pragma unroll
-  for (int i = 0; i < kFewSlots / 64; ++i) {
-    if (i == wave) at = count;
-    count += firsts[i];
-  }
-  at += __popcll(mask & ((1ull << lane) - 1));
   if (first) {
+    const int at = __popcll(mask & ((1ull << lane) - 1));
     p.map->expert[at] = e;
     index[e] = at;
   }
-  if (tid == 0) p.map->count = count;
-  for (int i = tid; i < count * kFewTokens; i += THREADS) p.map->slot[0][i] = -1;
+  if (tid == 0) p.map->count = __popcll(mask);
+  if (tid < kFewSlots * kFewTokens) p.map->slot[0][tid] = -1;
+  static_assert(THREADS >= kFewSlots * kFewTokens, "a thread per entry");
   __syncthreads();
   if (e < 0) return;
   // (a token may name an expert twice: its first slot has both weights)
@@ -261,7 +258,6 @@ __device__ __forceinline__ void few_map(const FewArgs& p) {
 // is a ballot and no further load.
 template <class T, int W, int G>
 __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
-  constexpr int WORDS = kFewSlots / 64;
   __shared__ f32x4 sums[W][4][64];
   __shared__ __align__(16) TokenBlock tokens[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -271,27 +267,14 @@ __global__ __launch_bounds__(64 * W) void few_gate_up_kernel(FewArgs p) {
     return;
   }
   const int e = p.ids[slot0];
-  int id[WORDS];
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) id[i] = 64 * i + lane < p.slots ? p.ids[64 * i + lane] : -1;
-  uint64_t same[WORDS + 1];
-  bool earlier = false;
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) {
-    same[i] = __builtin_amdgcn_ballot_w64(id[i] == e);
-    const int below = slot0 - 64 * i;
-    earlier |= below > 0 && (same[i] & (below >= 64 ? ~0ull : (1ull << below) - 1)) != 0;
-  }
-  same[WORDS] = 0;
+  const int id = lane < p.slots ? p.ids[lane] : -1;
+  const uint64_t same = __builtin_amdgcn_ballot_w64(id == e);
+  const bool earlier = (same & ((1ull << slot0) - 1)) != 0;
   if (e < 0 || e >= p.E || earlier) return;  // (the same in every wave)
   int slot = -1;  // the token's first slot with this expert
   if (t16 < p.T) {
-    const int at = t16 * p.k, sh = at & 63;
-    uint64_t lo = 0, hi = 0;
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i)
-      if (i == at >> 6) lo = same[i], hi = same[i + 1];
-    const uint64_t bits = ((lo >> sh) | (sh ? hi << (64 - sh) : 0)) & ((1ull << p.k) - 1);
+    const int at = t16 * p.k;
+    const uint64_t bits = (same >> at) & ((1ull << p.k) - 1);
     if (bits) slot = at + __builtin_ctzll(bits);
   }
   const int64_t n0 = (int64_t)blockIdx.x * 32;

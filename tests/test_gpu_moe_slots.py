@@ -6,7 +6,7 @@ import torch
 
 from f16acc_amd import fp8, moe
 from tests import ops_reference as ref
-from tests.test_gpu_moe import layer
+from tests.test_gpu_moe import check_experts, layer
 
 pytestmark = pytest.mark.gpu
 F8 = torch.float8_e4m3fn
@@ -52,3 +52,15 @@ def test_fp32_results_are_summed_in_fp32(T):
         want, parts = want + part, parts + part.abs()
     off = (y - want).abs() > 2e-5 * parts
     assert int(off.sum()) <= 12, (int(off.sum()), ((y - want).abs() / parts.clamp(min=1e-30)).median().item())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,E,k", [(1, 20, 16), (4, 9, 4), (2, 8, 8), (3, 1000, 5), (4, 1, 1), (5, 6, 3), (1, 30, 17), (2, 9, 9)])
+def test_around_the_limits_of_the_kernels_for_few_tokens(T, E, k, dtype):
+    """4 tokens and 16 slots: distinct experts, the same one in several slots of a token, and none."""
+    args = list(layer(T, E, k, 144, 130, dtype, seed=T))
+    check_experts(moe.experts(*args), args)
+    args[2][:, ::2] = E - 1
+    check_experts(moe.experts(*args), args)
+    args[2][-1, :] = torch.arange(k) % 2 - 1  # -1, 0, -1, 0 ...
+    check_experts(moe.experts(*args), args)
