@@ -242,9 +242,13 @@ struct LinearPlan {
 };
 
 // The experts' tiles by the mean number of tokens an expert has: gate and up (128
-// columns of each), down.  4096 tokens, 8 of 64 experts each, 2048 x 1024, gate and up /
-// down, 8-bit sums: 232 / 202 us on 256, 256 / 167 on 128; with 25 tokens an expert
-// 110 us in all on 128, 124 on 32; with 10 106 and 105.
+// columns of each), down.  In all, in us, bfloat16, in a graph, for 64 experts of 2048 x 1024 with 8 a
+// token, 16 of 4096 x 2048 with 2, 128 of 1024 x 512 with 4:
+//   16 tokens an expert: on 32 102, 112, 60; on 128 106, 110, 63
+//   24 tokens an expert: on 32 119, 137, 70; on 128 108, 113, 65
+//   192, 8-bit sums:     on 128 185, 164, 139; on 256 166, 153, 128
+//   512, 8-bit sums:     on 128 421, 380, 314; on 256 391, 351, 282
+// (the last with down on 128: 410, 361, 300).
 template <int ROWS>
 struct ExpertCfg;
 template <>
@@ -260,7 +264,7 @@ struct ExpertCfg<128> {
 template <>
 struct ExpertCfg<256> {
   using GateUp = MmCfg<256, 256, 4, 2, 2, 2>;
-  using Down = MmCfg<128, 128, 2, 2, 2, 2>;
+  using Down = MmCfg<256, 256, 4, 2, 2, 2>;
 };
 
 int expert_tile(int64_t slots, int E) {
@@ -318,10 +322,10 @@ struct ExpertsPlan {
 
 // EXACT: gate and up on the 16-bit matrix instructions.  Up to 191 tokens an expert, where
 // weights are most of the time, they always do (in all, 64 experts of 2048 x 1024, 8 a
-// token, exact / 8-bit: 77 tokens 102 / 98 us, 512 127 / 113, 1024 173 / 142).  Past that
-// matrix instructions are the time (4096: 500 / 352), and it goes by the type: results in
-// binary16 and FP32 show the difference (3.0e-4 of the 2-norm off, or 1.3e-3 to 1.8e-3),
-// beside bfloat16's own rounding of 1.7e-3 it makes 2.4e-3 and the 8-bit sums stay.
+// token, exact / 8-bit: 64 tokens 100 / 97 us, 512 132 / 117, 1024 185 / 153).  Past that
+// matrix instructions are the time (4096: 525 / 358), and it goes by the type: results in
+// binary16 and FP32 show the difference (2.7e-4 and 8e-5 of the 2-norm off, or 1.5e-3),
+// beside bfloat16's own rounding of 1.7e-3 it makes 2.3e-3 and the 8-bit sums stay.
 template <int BM, bool EXACT>
 int expert_products(const MmArgs& gu, const MmArgs& down, int64_t max_tiles, hipStream_t stream) {
   using GateUp = typename ExpertCfg<EXACT && BM == 256 ? 128 : BM>::GateUp;
