@@ -120,8 +120,8 @@ using Tile5 = MmCfg<32, 64, 1, 2, 4, 2>;
 // triples (M 32 .. 8192, N 256 .. 8960, K 512 .. 9000, weights out of the cache; 438
 // with row scales): a workgroup alone on its CU takes start + kb * block, each
 // further one beside it adds `share` of the blocks' time; `per_cu` fit.  The
-// picks made with it take 1.2 % (row scales 0.1 %) longer than the best triple on
-// geometric mean, 11 % at worst.
+// picks made with it take 1.2 % (row scales 0.03 %) longer than the best triple on
+// geometric mean, 10 % at worst (profiles/fp8_tile_choices.txt has each).
 struct TileCost {
   double start, block, share;
 };
