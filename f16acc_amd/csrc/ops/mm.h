@@ -512,9 +512,9 @@ struct MmKernel {
       store_gated(p, lds, acc, m0, m_left, n0, wm, wn, t16, g);
     } else if (EXPERTS) {
       // A slot's results wait in memory for the sum over its token's experts, in FP32: they are
-      // parts of that sum.  (As binary16 over a power of two for each wave tile's columns
-      // 4096 tokens of 8 experts each, width 2048, took 355 us against 390, and lost what lay 2^14
-      // below the largest column.)
+      // parts of that sum.  (As binary16 over a power of two for each wave tile's columns they are
+      // half the bytes, and what lay 2^14 below the largest column lost its bits; 4096
+      // tokens of 8 experts each, width 2048, took 355 us, 358 now.)
       store<float>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
     } else if (p.ksplit) {
       MmArgs q = p;

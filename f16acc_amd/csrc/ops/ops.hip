@@ -508,15 +508,16 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
   const LinearPlan plan(M, N, K, w, ldw);
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   // Few tokens: one launch, from the rows as they are.  From 9 tokens on its quantising,
-  // repeated by every workgroup, costs more than a pass of its own where there are many (16 tokens:
-  // 8960 x 1536 11.5 us against 12.4 on the tiles, 8192 x 8192 32 against 25).
+  // repeated by every workgroup, costs more than a pass of its own where there are many (16 tokens,
+  // here / on the tiles, in a graph: 1536 x 1536 5.5 / 10.2 us, 4096 x 4096 10.7 / 12.6, 8960 x 1536
+  // 11.3 / 10.2, 8192 x 8192 31 / 22; 8 tokens: 4.6 / 10.0, 8.4 / 12.3, 7.8 / 10.2, 21.4 / 21.2).
   if ((M <= 8 || (M <= 16 && N * K <= (1 << 25))) && wide_loads(x, type, sr, sc)) {
     SmallArgs a{x, sr, w, ldw, sw, swn, swk, bias, y, N, 1, M, N, K};
     return by_tokens((int)M, type, [&](auto* t, auto groups) {
       using T = std::remove_pointer_t<decltype(t)>;
       constexpr int G = decltype(groups)::value;
-      // 16 waves deal K where no CU has two workgroups (one token: 4096 x 4096 7.1 us against 7.6
-      // on 8 waves, 1536 x 1536 3.8 and 4.1; 8960 x 1536 7.4 and 6.4)
+      // 16 waves deal K where no CU has two workgroups (one token: 4096 x 4096 7.3 us against 8.0
+      // on 8 waves, 1536 x 8960 8.5 and 12.1, 1536 x 1536 4.1 and 4.5; 8960 x 1536 7.5 and 6.5)
       if (cdiv(N, 16) <= kCus && cdiv(K, kBlock) >= 12)
         hipLaunchKernelGGL((linear_small_kernel<T, 16, G>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), 0, stream, a);
       else
