@@ -32,6 +32,7 @@ _SIGNATURES = {
     "f16acc_linear_fp8": [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_vp, _size, _vp],
     "f16acc_route": [_vp, _int] + [_i64] * 3 + [_int] * 3 + [_vp] + [_int] * 3 + [_f32, _vp, _vp, _vp],
     "f16acc_route_grad": [_vp, _int] + [_i64] * 3 + [_int] * 4 + [_f32, _vp, _vp, _i64, _i64, _vp, _vp],
+    "f16acc_experts_any_rows": [_vp, _int] + [_i64] * 3 + [_int],
     "f16acc_experts": [_vp, _int] + [_i64] * 3 + [_vp, _i64, _i64, _vp, _int, _int] + [_i64] * 2
                       + [_vp] + [_i64] * 3 + [_vp] + [_i64] * 4 + [_vp] + [_i64] * 2 + [_vp] + [_i64] * 3
                       + [_vp, _vp, _size, _vp],
@@ -54,8 +55,8 @@ def _bind(name):
     return f
 
 
-(quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad, experts,
- column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
+(quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad,
+ experts_any_rows, experts, column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
 
 if abi_version() != ABI_VERSION:
     raise ImportError(f"{LIB_OPS} has ABI version {abi_version()}, this package needs {ABI_VERSION}: rebuild it")

@@ -272,7 +272,7 @@ int expert_tile(int64_t slots, int E) {
   return mean >= 192 ? 256 : mean >= 24 ? 128 : 32;
 }
 
-// Whether the two kernels for a few tokens run.
+// Whether the two kernels for a few tokens run (if x's rows allow their loads).
 bool few_tokens(int64_t T, int k) { return T <= kFewTokens && T * k <= kFewSlots; }
 
 int64_t tile_count(int64_t slots, int E, int bm) { return slots / bm + (slots < E ? slots : E); }
@@ -283,14 +283,12 @@ int64_t tile_count(int64_t slots, int E, int bm) { return slots / bm + (slots < 
 struct ExpertsPlan {
   int64_t slots, chunks, max_tiles, Dp, Ip;
   int bm;
-  bool few;  // the kernels for a few tokens run (if x's rows allow their loads)
   int64_t ldy;
   size_t xq, xs, hq, hs, ys, counts, rows, pos, tiles, ntiles, total;
   ExpertsPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     slots = T * k;
     Dp = up128(D);
     Ip = up128(I);
-    few = few_tokens(T, k);
     bm = expert_tile(slots, E);
     chunks = cdiv(slots, kSortChunk);
     max_tiles = tile_count(slots, E, bm);
@@ -581,6 +579,10 @@ int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64
   return by_experts<LaunchRouteGrad>(E, type, a, (hipStream_t)stream);
 }
 
+int f16acc_experts_any_rows(const void* x, int type, int64_t T, int64_t sr, int64_t sc, int k) {
+  return T > 0 && k > 0 && few_tokens(T, k) && wide_loads(x, type, sr, sc);
+}
+
 size_t f16acc_experts_workspace(int64_t T, int k, int E, int64_t D, int64_t I) {
   if (T <= 0 || k <= 0 || E <= 0 || D <= 0 || I <= 0) return 0;
   return ExpertsPlan(T, k, E, D, I).total;
@@ -598,9 +600,10 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   if (!weights || !ids || !w1 || !s1 || !w2 || !s2 || !y) return F16ACC_OPS_E_ARG;
   if (w1e < 0 || w1u < 0 || s1e < 0 || s1u < 0 || s1n < 0 || s1k < 0 || w2e < 0 || s2e < 0 || s2n < 0 || s2k < 0)
     return F16ACC_OPS_E_ARG;
-  if (E > kMaxExperts || ld1 % 16 || ld2 % 16 || w1e % 16 || w1u % 16 || w2e % 16 || ld1 < D ||
-      ld2 < I || ld1 > kMaxRow || ld2 > kMaxRow || up128(D) > kMaxRow || up128(I) > kMaxRow || !aligned16(w1) ||
-      !aligned16(w2))
+  if (E > kMaxExperts || ld1 < 0 || ld2 < 0 || up128(D) > kMaxRow || up128(I) > kMaxRow) return F16ACC_OPS_E_UNSUPPORTED;
+  const bool few = f16acc_experts_any_rows(x, type, T, sr, sc, k);
+  if (!few && (ld1 % 16 || ld2 % 16 || w1e % 16 || w1u % 16 || w2e % 16 || ld1 < D || ld2 < I || ld1 > kMaxRow ||
+               ld2 > kMaxRow || !aligned16(w1) || !aligned16(w2)))
     return F16ACC_OPS_E_UNSUPPORTED;
   // the copies address a token's (a slot's) row by a 31-bit offset
   if (T > kOob / up128(D) || T > kOob / ((int64_t)k * up128(I))) return F16ACC_OPS_E_UNSUPPORTED;
@@ -608,7 +611,7 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_;
   char* ws = (char*)workspace;
-  if (plan.few && wide_loads(x, type, sr, sc)) {
+  if (few) {
     FewArgs f{x,   sr,  (int)T, k,   E,   (int)plan.slots, ids, weights, wt,  wk,  D,   I, w1,          w1e,     w1u,
               ld1, s1,  s1e,    s1u, s1n, s1k,             w2,  w2e,     ld2, s2,  s2e, s2n, s2k, (float*)ws, plan.Ip,
               (FewMap*)(ws + up256(plan.slots * plan.Ip * 4)), y};

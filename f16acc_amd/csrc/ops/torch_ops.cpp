@@ -549,7 +549,12 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   Tensor i32 = rows_of(ids);
   if (i32.scalar_type() == at::kLong) i32 = i32.clamp(-1, E).to(at::kInt);  // (a cast alone would wrap)
   i32 = i32.contiguous();
-  const Operand p1 = packed(w1), p2 = packed(w2);
+  // for a few tokens rows of any alignment go as they are
+  const bool any = f16acc_experts_any_rows(x2.const_data_ptr(), type_of(x), T, x2.stride(0), x2.stride(1), (int)k);
+  auto rows = [&](const Tensor& w) {
+    return any && (w.size(-1) <= 1 || w.stride(-1) == 1) ? Operand{w, w.stride(-2)} : packed(w);
+  };
+  const Operand p1 = rows(w1), p2 = rows(w2);
   // The kernels address rows of the quantised tokens and hidden values by 31 bits:
   // more tokens than that go in parts.
   const int64_t most = 0x7fff0000 / std::max(up(D, kBlock), k * up(I, kBlock));

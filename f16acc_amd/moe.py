@@ -44,7 +44,12 @@ def experts(x, weights, ids, w1, w1_scale, w2, w2_scale):
        0 .. E - 1 (-1) adds nothing, and its weight is not read
     w1: float8_e4m3fn [E, 2, I, D] (gate, up), w1_scale: float32 [E, 2, ceil(I / 128), ceil(D / 128)]
     w2: float8_e4m3fn [E, D, I], w2_scale: float32 [E, ceil(D / 128), ceil(I / 128)]
-    Returns [..., D] in x's type, the sum over the experts in FP32.  For
+    Returns [..., D] in x's type, the sum over the experts in FP32.  Weights whose rows no
+    16-byte load fits (D or I not a multiple of 16, views at odd addresses or over 4 MiB
+    apart) are copied on every call, those of all experts, except for 1 to 4 tokens with at most
+    16 ids in all and K-contiguous weights, which read the routed experts' rows as they are.
+    The products of gate and up are exact in FP32, except for bfloat16 x with 192 or more tokens
+    an expert on average; those and the products of w2 have the block sums of fp8.mm.  For
     inference: operands that require gradients are refused where gradients are
     enabled."""
     return host.experts(x, weights, ids, w1, w1_scale, w2, w2_scale)

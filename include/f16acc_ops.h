@@ -133,12 +133,14 @@ int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64
  *   y += a * (silu(x w1[e][0]^T) * (x w1[e][1]^T)) w2[e]^T
  * x [T, D] (element strides sr, sc) and the FP32 hidden values are quantised in row blocks; ids [T][k]
  * contiguous (outside 0 .. E - 1: no expert), weights element strides wt, wk; y [T][D] contiguous, of
- * x's type.  Weights are square-block e4m3, rows as in f16acc_mm_fp8:
+ * x's type.  Weights are square-block e4m3, rows as in f16acc_mm_fp8 (where
+ * f16acc_experts_any_rows says 1, at any address and with anything behind them):
  *   w1 [E][2][I][D] (gate, up), expert stride w1e bytes, up at w1u, rows ld1
  *   s1 of (e, gate or up, n / 128, k / 128): strides s1e, s1u, s1n, s1k
  *   w2 [E][D][I], strides w2e, ld2;  s2: s2e, s2n, s2k
  * Workspace of f16acc_experts_workspace bytes, 256-byte aligned; it is enough for any smaller T too.
  */
+int f16acc_experts_any_rows(const void* x, int type, int64_t T, int64_t sr, int64_t sc, int k);
 size_t f16acc_experts_workspace(int64_t T, int k, int E, int64_t D, int64_t I);
 int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const float* weights, int64_t wt,
                    int64_t wk, const int* ids, int k, int E, int64_t D, int64_t I, const uint8_t* w1, int64_t w1e,

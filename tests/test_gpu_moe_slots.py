@@ -64,3 +64,29 @@ def test_around_the_limits_of_the_kernels_for_few_tokens(T, E, k, dtype):
     check_experts(moe.experts(*args), args)
     args[2][-1, :] = torch.arange(k) % 2 - 1  # -1, 0, -1, 0 ...
     check_experts(moe.experts(*args), args)
+
+
+@pytest.mark.parametrize("T,D,I", [(1, 1000, 300), (4, 250, 130), (2, 129, 17)])
+def test_few_tokens_read_weights_of_any_alignment_in_place(T, D, I):
+    """No copy of the experts' weights: NaN bytes around the rows are not read as values, and the call needs less
+    memory than one expert."""
+    E = 40
+    x, weights, ids, w1, s1, w2, s2 = layer(T, E, 3, D, I)
+    x = torch.nn.functional.pad(x, (0, -D % 8))[:, :D]  # (rows that 16-byte loads fit)
+    aligned = [torch.zeros(*w.shape[:-1], -(-w.shape[-1] // 16) * 16, dtype=torch.uint8, device=x.device).view(F8) for w in (w1, w2)]
+    for a, w in zip(aligned, (w1, w2)):
+        a[..., :w.shape[-1]] = w
+    want = moe.experts(x, weights, ids, aligned[0][..., :D], s1, aligned[1][..., :I], s2)
+    check_experts(want, (x, weights, ids, w1, s1, w2, s2))
+    odd = []
+    for w in (w1, w2):
+        hold = torch.full((w.numel() // w.shape[-1] * (w.shape[-1] + 5) + 64,), float("nan")).to(F8).to(x.device)
+        v = hold[3:3 + w.numel() // w.shape[-1] * (w.shape[-1] + 5)].view(*w.shape[:-1], w.shape[-1] + 5)[..., :w.shape[-1]]
+        odd.append(v.copy_(w))
+    for a, b in ((w1, w2), odd):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = moe.experts(x, weights, ids, a, s1, b, s2)
+        assert torch.equal(got, want)
+        assert torch.cuda.max_memory_allocated() - before < 30 * D * I
