@@ -34,8 +34,8 @@
 // values.  Then both operands are converted to binary16, which is exact, and the
 // block is four v_mfma_f32_16x16x32_f16 in FP32: twice the matrix cycles and, on
 // 64 x 64 sums a wave, two conversions for each MFMA, which bound it (dealing them one by
-// one between the MFMAs gained 2 %).  4096 tokens, 8 of 64 experts, 2048 x 1024: 373 us
-// on 128 x 256 tiles against 193 in 8 bits on 256 x 256 (profiled; 256 x 256 spills
+// one between the MFMAs gained 2 %).  4096 tokens, 8 of 64 experts, 2048 x 1024: 419 us
+// on 128 x 256 tiles against 212 in 8 bits on 256 x 256 (profiled; 256 x 256 spills
 // with the halves).
 //
 // Measured (bfloat16 result): 8192^3 450 us, 2440 TFLOPS, where a library's product with
@@ -514,7 +514,7 @@ struct MmKernel {
       // A slot's results wait in memory for the sum over its token's experts, in FP32: they are
       // parts of that sum.  (As binary16 over a power of two for each wave tile's columns they are
       // half the bytes, and what lay 2^14 below the largest column lost its bits; 4096
-      // tokens of 8 experts each, width 2048, took 355 us, 358 now.)
+      // tokens of 8 experts each, width 2048, took 355 us, 358 to 375 now.)
       store<float>(p, lds, acc, m0, m_left, n0, wave, wm, wn, t16, g);
     } else if (p.ksplit) {
       MmArgs q = p;

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(64 * W) void linear_small_kernel(SmallArgs p) {
 // are exact (binary16 operands, FP32 sums): what the 8-bit matrix instructions drop
 // showed as 2e-3 of one token's result, and weights are what the kernels wait for.
 //
-// Measured: one token through 6 of 64 experts, 2048 x 1024, 38 MB of weights: 11.3 + 9.7
+// Measured: one token through 6 of 64 experts, 2048 x 1024, 38 MB of weights: 11.4 + 7.2
 // us against 7.6 at the copy rate.  What is left is latency: a launch, the ids, the
 // weights, one wait after another, on two launches.
 // ---------------------------------------------------------------------------

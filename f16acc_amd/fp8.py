@@ -67,7 +67,10 @@ def linear(x, w, w_scale=None, bias=None):
 
     x: [..., K] float16, bfloat16 or float32, quantised in blocks of 1 x 128
     w, w_scale: a stored float8_e4m3fn [N, K] weight with its float32
-       [ceil(N / 128), ceil(K / 128)] scales; gradients reach x and bias
+       [ceil(N / 128), ceil(K / 128)] scales; gradients reach x and bias (that of x
+       transposes the weight on every call).  Rows that no 16-byte load fits (K no multiple
+       of 16 among them) are copied on every call, except for at most 8 tokens whose own
+       rows 16-byte loads fit: those read them as they are
     w alone: a float16, bfloat16 or float32 [N, K] weight, quantised in squares
        on every call; gradients reach x, w and bias, their products in 8 bits too
     bias: [N] in x's type, or None."""

@@ -47,7 +47,8 @@ def experts(x, weights, ids, w1, w1_scale, w2, w2_scale):
     Returns [..., D] in x's type, the sum over the experts in FP32.  Weights whose rows no
     16-byte load fits (D or I not a multiple of 16, views at odd addresses or over 4 MiB
     apart) are copied on every call, those of all experts, except for 1 to 4 tokens with at most
-    16 ids in all and K-contiguous weights, which read the routed experts' rows as they are.
+    16 ids in all, rows of x that 16-byte loads fit and K-contiguous weights, which read the
+    routed experts' rows as they are.
     The products of gate and up are exact in FP32, except for bfloat16 x with 192 or more tokens
     an expert on average; those and the products of w2 have the block sums of fp8.mm.  For
     inference: operands that require gradients are refused where gradients are
