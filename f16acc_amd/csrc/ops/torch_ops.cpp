@@ -539,7 +539,9 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   REQUIRE(weights.scalar_type() == at::kFloat && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
         "experts needs float32 weights and int32 or int64 ids, got ", weights.scalar_type(), " and ",
         ids.scalar_type());
-  REQUIRE(!c10::GradMode::is_enabled() || (!x.requires_grad() && !weights.requires_grad()),
+  bool grown = false;
+  for (const Tensor* t : {&x, &weights, &w1, &s1, &w2, &s2}) grown = grown || t->requires_grad();
+  REQUIRE(!c10::GradMode::is_enabled() || !grown,
         "experts has no backward pass: call it under torch.no_grad() or torch.inference_mode()");
   const int64_t k = ids.size(-1);
   const Tensor x2 = rows_of(x), wt = rows_of(weights);

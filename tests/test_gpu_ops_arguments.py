@@ -98,3 +98,17 @@ def test_rows_wider_than_their_blocks(rows, cols, ldq):
     want = fp8.quantize(x)
     assert torch.equal(q[:, :cols], want[0].view(torch.uint8)) and bool((q[:, cols:] == 0).all())
     assert torch.equal(s[:blocks].t(), want[1]) and bool((s[blocks:] == 7.0).all())
+
+
+def test_experts_refuses_every_operand_that_requires_a_gradient():
+    x, w = normal(4, 128), torch.ones(4, 1, device=DEV)
+    ids = torch.zeros(4, 1, dtype=torch.int32, device=DEV)
+    args = [x, w, ids, *fp8.quantize_weight(normal(2, 2, 128, 128)), *fp8.quantize_weight(normal(2, 128, 128))]
+    want = moe.experts(*args)
+    for i in (0, 1, 3, 4, 5, 6):
+        grown = list(args)
+        grown[i] = args[i].detach().clone().requires_grad_()
+        with pytest.raises(ValueError, match="backward"):
+            moe.experts(*grown)
+        with torch.no_grad():
+            assert torch.equal(moe.experts(*grown), want)
