@@ -34,7 +34,7 @@ def quantize(x, transposed=False):
 
     x: [..., K] float16, bfloat16 or float32, any strides.  Returns (q, scale):
     float8_e4m3fn [..., K] (its rows lie 128-byte aligned, zero to the next
-    multiple of 128) and float32 [..., ceil(K / 128)].  transposed: for a 2-d x, the
+    multiple of 128) and float32 [..., ceil(K / 128)], without gradients.  transposed: for a 2-d x, the
     same of x.t(), in blocks of 128 rows of x: q [K, M], scale [K, ceil(M / 128)]."""
     return host.quantize(x, transposed)
 
@@ -51,8 +51,8 @@ def mm(a, a_scale, b, b_scale, out_dtype=torch.float16):
     a: float8_e4m3fn [M, K], a_scale: float32 [M, ceil(K / 128)]
     b: float8_e4m3fn [K, N], b_scale: float32 [ceil(K / 128), ceil(N / 128)] for
        square blocks, or [ceil(K / 128), N] for a scale for each column of b
-    Any strides; K-contiguous operands with 16-byte aligned rows (b = w.t() of a
-    stored [N, K] weight) are read as they are, others copied once."""
+    Any strides; K-contiguous operands with 16-byte aligned rows at most 4 MiB apart (b = w.t()
+    of a stored [N, K] weight) are read as they are, others copied on every call.  No gradients."""
     return host.mm(a, a_scale, b, b_scale, out_dtype, None, None, -1, 0)
 
 
