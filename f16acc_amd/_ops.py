@@ -55,8 +55,9 @@ def _bind(name):
     return f
 
 
-(quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad,
- experts_any_rows, experts, column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace, strerror, abi_version) = map(_bind, EXPORTS)
+(quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad, experts_any_rows,
+ experts, column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace, strerror,
+ abi_version) = map(_bind, EXPORTS)
 
 if abi_version() != ABI_VERSION:
     raise ImportError(f"{LIB_OPS} has ABI version {abi_version()}, this package needs {ABI_VERSION}: rebuild it")
