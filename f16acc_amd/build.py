@@ -3,8 +3,8 @@
     python f16acc_amd/build.py
 
 libf16acc_amd.so is the chunked GEMM: kernels, per-shape tile table and the C
-ABI declared in include/f16acc.h.  libf16acc_ops.so holds the 8-bit products and
-the mixture-of-experts operators (include/f16acc_ops.h).
+ABI declared in include/f16acc.h.  libf16acc_ops.so holds the 8- and 4-bit products
+and the mixture-of-experts operators (include/f16acc_ops.h).
 """
 
 import os
@@ -18,7 +18,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SRC = os.path.join(PKG, "csrc", "f16acc_gemm.hip")
 CHUNKRATE_SRC = os.path.join(PKG, "csrc", "chunkrate.hip")
-OPS_SRC = os.path.join(PKG, "csrc", "ops", "ops.hip")
+OPS_SRCS = [os.path.join(PKG, "csrc", "ops", f) for f in ("ops.hip", "fp4.hip")]  # (compiled side by side)
 INCLUDE = os.path.join(ROOT, "include")
 OUT_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(OUT_DIR, "libf16acc_amd.so")
@@ -32,7 +32,7 @@ LIB_SPLITREDO = os.path.join(OUT_DIR, "libf16acc_amd_splitredo.so")
 # of the persistent kernel (-DF16ACC_NO_PERSISTENT=1): only bench.py's
 # persistent A/B loads it.
 LIB_NOPERSIST = os.path.join(OUT_DIR, "libf16acc_amd_nopersist.so")
-# The 8-bit products and the mixture-of-experts operators (include/f16acc_ops.h).
+# The 8- and 4-bit products and the mixture-of-experts operators (include/f16acc_ops.h).
 LIB_OPS = os.path.join(OUT_DIR, "libf16acc_ops.so")
 # Their torch side (checks, allocation, autograd): a CPython module linked to it.
 OPS_TORCH_SRC = os.path.join(PKG, "csrc", "ops", "torch_ops.cpp")
@@ -93,11 +93,11 @@ def ops_torch_flags():
 
 
 def _start(flags, src, out, compiler=None, libs=()):
-    """Start hipcc (or `compiler`) src -> a temporary file next to out."""
+    """Start hipcc (or `compiler`) on src (one file or a list) -> a temporary file next to out."""
     os.makedirs(OUT_DIR, exist_ok=True)
     fd, tmp = tempfile.mkstemp(suffix=".tmp", dir=OUT_DIR)
     os.close(fd)
-    cmd = [compiler or hipcc(), *flags, "-I", INCLUDE, src, "-o", tmp, *libs]
+    cmd = [compiler or hipcc(), *flags, "-I", INCLUDE, *([src] if isinstance(src, str) else src), "-o", tmp, *libs]
     return cmd, tmp, out, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 
@@ -106,7 +106,8 @@ def _finish(job, verbose):
     cmd, tmp, out, proc = job
     text, _ = proc.communicate()
     if proc.returncode != 0:
-        os.unlink(tmp)
+        if os.path.exists(tmp):  # (the linker removes what it could not finish)
+            os.unlink(tmp)
         raise RuntimeError("compilation failed:\n" + " ".join(cmd) + "\n" + text)
     if verbose:
         noise = ("packed-fp32-ops", "warning generated", "warnings generated")
@@ -118,19 +119,33 @@ def _finish(job, verbose):
     return out
 
 
+def build_ops(parts, verbose):
+    """Link the operators' library from its sources' running compilations."""
+    objects, errors = [], []
+    for job in parts:
+        try:
+            objects.append(_finish(job, verbose))
+        except RuntimeError as e:
+            errors.append(str(e))
+    if errors:
+        raise RuntimeError("\n".join(errors))
+    _finish(_start([f"--offload-arch={ARCH}", "-shared"], objects, LIB_OPS), verbose)
+
+
 def build(verbose=False):
     """Compile the library, its no-redo, split-redo and no-persistent twins,
     the operators' library and its torch side, the chunkrate microbenchmark and
-    the native call path (seven compilers at once)."""
+    the native call path (eight compilers at once)."""
     flags, libs = host_flags()
-    ops = _start(HIP_FLAGS, OPS_SRC, LIB_OPS)
+    parts = [_start(COMMON_FLAGS + ["-fPIC", "-c"], src, os.path.join(OUT_DIR, os.path.basename(src) + ".o"))
+             for src in OPS_SRCS]
     jobs = [_start(HIP_FLAGS, SRC, LIB), _start(HIP_FLAGS + ["-DF16ACC_NO_REDO=1"], SRC, LIB_NOREDO),
             _start(HIP_FLAGS + ["-DF16ACC_SPLIT_REDO=1"], SRC, LIB_SPLITREDO),
             _start(HIP_FLAGS + ["-DF16ACC_NO_PERSISTENT=1"], SRC, LIB_NOPERSIST),
             _start(COMMON_FLAGS, CHUNKRATE_SRC, CHUNKRATE), _start(flags, HOST_SRC, HOST, cxx(), libs)]
     errors = []
     try:
-        _finish(ops, verbose)
+        build_ops(parts, verbose)
         flags, libs = ops_torch_flags()  # (links against the library)
         jobs.append(_start(flags, OPS_TORCH_SRC, OPS_TORCH, cxx(), libs))
     except RuntimeError as e:

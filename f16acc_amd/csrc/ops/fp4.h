@@ -1,0 +1,272 @@
+// Microscaled 4-bit operands: blocks of 32 e2m1 values with a power of two each (e8m0), two
+// values a byte, the first in its low half.  Quantisation along the rows, along the
+// columns (transposed) or both, the values back, the scales in the products' order.
+//
+//   m = max(|x|, 2^-100)   s = 2^e with 2^e <= m / 3.5 < 2^(e + 1)   q = e2m1(x / s), nearest, ties to even
+//
+// |x / s| stays below 7, the middle of 6 and the next power of two, so no value is cut off by
+// more than its rounding.  A block that holds an infinity or a NaN has the scale NaN (255).
+#pragma once
+
+#include "common.h"
+#include "quant.h"
+
+namespace f16ops {
+
+constexpr int kMx = 32;    // values of a block
+constexpr int kQuad = 128; // values of four blocks, whose scales are one dword
+
+// The e8m0 byte of a block from the bits of its largest magnitude.
+__device__ __forceinline__ uint32_t mx_exponent(uint32_t bits) { return ((umax(bits, kTinyBits) + 0x200000u) >> 23) - 2; }
+__device__ __forceinline__ uint32_t mx_byte(uint32_t bits) { return bits >= kInfBits ? 255u : mx_exponent(bits); }
+
+// Eight values over 2^(e - 127) as e2m1, the first in the lowest bits.
+__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8], uint32_t e) {
+  const float s = __uint_as_float(e << 23);  // (the conversion divides by it)
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
+}
+
+// Eight e2m1 values times 2^(e - 127); NaN where e is 255.
+__device__ __forceinline__ void unpack_e2m1(uint32_t q, uint32_t e, float (&v)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
+  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
+  const float t[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = e == 255u ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(t[i], (int)e - 127);
+}
+
+// Scale bytes: that of (row, block b) at s[row * row_stride + b / 4 * quad_stride + b % 4], both strides
+// multiples of 4.  [rows][quads] has (4 quads, 4), [quads][rows] (4, 4 rows).
+struct MxScales {
+  uint8_t* s;
+  int64_t row, quad;
+};
+
+struct MxQuantArgs {
+  const void* x;
+  int64_t rows, cols, sr, sc;  // element strides
+  uint8_t* q;                  // [rows][ldq], zero from cols on; ldq: 64 for each 128 columns
+  int64_t ldq;
+  MxScales s;
+  uint8_t* qt;  // [cols][ldqt], zero from rows on; ldqt: 64 for each 128 rows
+  int64_t ldqt;
+  MxScales st;
+  // x held in 4 bits itself: bytes [rows][..], scale of (row, block) at xs + row * xsr + block * xsc
+  const uint8_t* xs;
+  int64_t xsr, xsc;
+};
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t v) {
+  v = umax(v, dpp<0xb1>(v));  // quad_perm:[1,0,3,2], [2,3,0,1]
+  return umax(v, dpp<0x4e>(v));
+}
+
+// The four bytes of a quad of blocks, held by 16 lanes, four alike for each block, as one dword.
+__device__ __forceinline__ uint32_t quad_bytes(uint32_t byte, int lane) {
+  uint32_t v = byte << (8 * (lane >> 2 & 3));
+  v |= dpp<0x124>(v);  // row_ror:4, 8
+  return v | dpp<0x128>(v);
+}
+
+// One row of a matrix in blocks of 1 x 32.  16 lanes take 128 values, 8 each: a 16-byte load
+// a lane (16-bit types), the maximum of four lanes by two exchanges, 4 bytes a lane out.
+template <class T, bool WIDE>
+__device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t group, uint32_t groups) {
+  const int64_t quads = cdiv(p.cols, kQuad), total = p.rows * quads;
+  const int lane = threadIdx.x & 15;
+  for (int64_t b = (int64_t)group * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)groups * 16) {
+    const int64_t row = total >> 32 ? b / quads : (int64_t)((uint32_t)b / (uint32_t)quads), kq = b - row * quads;
+    const int64_t c0 = kq * kQuad + lane * 8;
+    const T* x = (const T*)p.x + row * p.sr;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (WIDE && c0 + 8 <= p.cols) {
+      load_vec(x + c0, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < p.cols) v[i] = (float)x[(c0 + i) * p.sc];
+    }
+    uint32_t m = abs_bits(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
+    m = quad_umax(m);
+    *(uint32_t*)(p.q + row * p.ldq + c0 / 2) = pack_e2m1(v, mx_exponent(m));
+    // (a block past the columns holds zeros: its byte is that of 2^-102 or 0, never NaN's)
+    const uint32_t scales = quad_bytes(mx_byte(m), lane);
+    if (lane == 0) *(uint32_t*)(p.s.s + row * p.s.row + kq * p.s.quad) = scales;
+  }
+}
+
+// Scale bytes of any strides in the products' order, [quads][rows] dwords, zero past the blocks.
+struct MxScaleArgs {
+  const uint8_t* src;
+  int64_t rows, blocks, s_r, s_b;
+  uint32_t* dst;  // [quads][ld]
+  int64_t ld;
+};
+__device__ __forceinline__ void mx_scales(const MxScaleArgs& p, uint32_t group, uint32_t groups) {
+  const int64_t quads = cdiv(p.blocks, 4), total = p.rows * quads;
+  for (int64_t i = (int64_t)group * 256 + threadIdx.x; i < total; i += (int64_t)groups * 256) {
+    const int64_t r = total >> 32 ? i / quads : (int64_t)((uint32_t)i / (uint32_t)quads), kq = i - r * quads;
+    const uint8_t* s = p.src + r * p.s_r + 4 * kq * p.s_b;
+    uint32_t v = 0;
+    if (p.s_b == 1 && 4 * kq + 4 <= p.blocks) {
+      __builtin_memcpy(&v, s, 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (4 * kq + j < p.blocks) v |= (uint32_t)s[j * p.s_b] << (8 * j);
+    }
+    p.dst[kq * p.ld + r] = v;
+  }
+}
+__global__ __launch_bounds__(256) void mx_scales_kernel(MxScaleArgs a, MxScaleArgs b, uint32_t first) {
+  if (blockIdx.x < first)
+    mx_scales(a, blockIdx.x, first);
+  else
+    mx_scales(b, blockIdx.x - first, gridDim.x - first);
+}
+
+// Tokens quantised, beside a weight's scales reordered and its rows copied to an alignment (either
+// may be none): what a product of new tokens with a stored weight needs before it.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void mx_prepare_kernel(MxQuantArgs q, MxScaleArgs s, Pack8Args w, uint32_t packs,
+                                                         uint32_t scales) {
+  if (blockIdx.x < packs)
+    pack8(w, blockIdx.x, packs);
+  else if (blockIdx.x < packs + scales)
+    mx_scales(s, blockIdx.x - packs, scales);
+  else
+    mx_quant_rows<T, WIDE>(q, blockIdx.x - packs - scales, gridDim.x - packs - scales);
+}
+
+struct Fp4Source {};  // x of MxQuantArgs held in 4 bits
+
+// Eight values of a row from column c (a multiple of 8).
+template <class T, bool WIDE>
+__device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t c, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  if (r >= p.rows || c >= p.cols) return;
+  if constexpr (std::is_same_v<T, Fp4Source>) {
+    const uint8_t* q = (const uint8_t*)p.x + r * p.sr + c / 2 * p.sc;
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + 2 * i < p.cols) u |= (uint32_t)q[i * p.sc] << (8 * i);
+    unpack_e2m1(u, p.xs[r * p.xsr + c / kMx * p.xsc], v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i >= p.cols) v[i] = 0.0f;
+  } else {
+    const T* x = (const T*)p.x + r * p.sr;
+    if (WIDE && c + 8 <= p.cols) {
+      load_vec(x + c, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < p.cols) v[i] = (float)x[(c + i) * p.sc];
+    }
+  }
+}
+
+// A 128 x 128 tile a workgroup, read once: quantised along its rows (ROWS) and its columns (the
+// result transposed).  Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's block is four
+// lanes, a column's block one wave's 32 rows, four DPP rows apart, so no maximum leaves a wave.
+template <class T, bool WIDE, bool ROWS>
+__global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs p) {
+  // The transposed tile, 64 bytes a column: 16-byte unit u (a wave's rows) of column col at u ^ (col / 8 % 4).
+  __shared__ __align__(16) uint8_t tile[kQuad * 64];
+  __shared__ uint8_t bytes[kQuad * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 4, c = tid & 15;
+  const int64_t kb = blockIdx.x, rb = blockIdx.y, r0 = rb * kQuad + r * 8, c0 = kb * kQuad + c * 8;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx_load<T, WIDE>(p, r0 + i, c0, v[i]);
+  if (ROWS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = abs_bits(v[i][0]);
+#pragma unroll
+      for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
+      m = quad_umax(m);
+      const uint32_t q = pack_e2m1(v[i], mx_exponent(m)), s = quad_bytes(mx_byte(m), lane);
+      if (r0 + i < p.rows) {
+        *(uint32_t*)(p.q + (r0 + i) * p.ldq + c0 / 2) = q;
+        if (c == 0) *(uint32_t*)(p.s.s + (r0 + i) * p.s.row + kb * p.s.quad) = s;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float col[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
+    uint32_t m = abs_bits(col[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(col[i]));
+    m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
+    *(uint32_t*)(tile + (c * 8 + j) * 64 + (wave ^ (c & 3)) * 16 + (r & 3) * 4) = pack_e2m1(col, mx_exponent(m));
+    if (lane < 16) bytes[(c * 8 + j) * 4 + wave] = (uint8_t)mx_byte(m);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int col = k * 64 + (tid >> 2), u = tid & 3;
+    if (kb * kQuad + col < p.cols)
+      *(i32x4*)(p.qt + (kb * kQuad + col) * p.ldqt + rb * 64 + u * 16) =
+          *(const i32x4*)(tile + col * 64 + (u ^ (col >> 3 & 3)) * 16);
+  }
+  if (tid < kQuad && kb * kQuad + tid < p.cols)
+    *(uint32_t*)(p.st.s + (kb * kQuad + tid) * p.st.row + rb * p.st.quad) = *(const uint32_t*)(bytes + tid * 4);
+}
+
+// The values of a 4-bit matrix, eight a thread.
+struct MxValuesArgs {
+  const uint8_t* q;
+  int64_t q_r, q_c;  // byte strides
+  const uint8_t* s;
+  int64_t s_r, s_b;
+  int64_t rows, cols;
+  void* out;  // [rows][cols]
+};
+template <class T>
+__global__ __launch_bounds__(256) void mx_values_kernel(MxValuesArgs p) {
+  const int64_t units = cdiv(p.cols, 8), total = p.rows * units;
+  struct alignas(8 * sizeof(T) < 16 ? 8 * sizeof(T) : 16) Pack {
+    T t[8];
+  };
+  const bool wide = p.cols % 8 == 0, whole = p.q_c == 1;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = total >> 32 ? i / units : (int64_t)((uint32_t)i / (uint32_t)units), c = (i - r * units) * 8;
+    const uint8_t* q = p.q + r * p.q_r + c / 2 * p.q_c;
+    uint32_t u = 0;
+    if (whole && c + 8 <= p.cols) {
+      __builtin_memcpy(&u, q, 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + 2 * j < p.cols) u |= (uint32_t)q[j * p.q_c] << (8 * j);
+    }
+    float v[8];
+    unpack_e2m1(u, p.s[r * p.s_r + c / kMx * p.s_b], v);
+    T* out = (T*)p.out + r * p.cols + c;
+    if (wide) {
+      Pack k;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k.t[j] = (T)v[j];
+      *(Pack*)out = k;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < p.cols) out[j] = (T)v[j];
+    }
+  }
+}
+
+}  // namespace f16ops

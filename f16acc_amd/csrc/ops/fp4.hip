@@ -1,0 +1,327 @@
+// C ABI of the microscaled 4-bit products (include/f16acc_ops.h): argument checks, the
+// choice of a kernel, workspaces.
+#include "fp4.h"
+
+#include "common.h"
+#include "fp4_mm.h"
+#include "fp4_small.h"
+#include "launch.h"
+
+using namespace f16ops;
+
+namespace {
+
+int64_t quads_of(int64_t v) { return cdiv(v, kQuad); }
+
+uint32_t grid_of(int64_t units, int64_t per_group) {
+  const int64_t groups = cdiv(units, per_group);
+  return (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus);
+}
+
+int scales_check(const MxScales& s) {
+  if (!s.s || s.row < 0 || s.quad < 0) return F16ACC_OPS_E_ARG;
+  return (uintptr_t)s.s % 4 || s.row % 4 || s.quad % 4 ? F16ACC_OPS_E_UNSUPPORTED : 0;
+}
+
+int out4_check(const uint8_t* q, int64_t ldq, int64_t cols, const MxScales& s) {
+  if (!q) return F16ACC_OPS_E_ARG;
+  if (ldq != 64 * quads_of(cols) || !aligned16(q)) return F16ACC_OPS_E_UNSUPPORTED;
+  return scales_check(s);
+}
+
+template <class T>
+int launch_tile(const MxQuantArgs& p, bool wide, hipStream_t stream) {
+  const int64_t gx = quads_of(p.cols), gy = quads_of(p.rows);
+  if (gx > 0x7fffffff || gy > 65535) return F16ACC_OPS_E_UNSUPPORTED;
+  const dim3 grid((uint32_t)gx, (uint32_t)gy);
+  if (p.q && wide)
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
+  else if (p.q)
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
+  else if (wide)
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
+  return hip_status();
+}
+
+// The tiles: tokens x weight rows.
+using Tile0 = Mx4Cfg<128, 128, 2, 2, 256, 2, 2>;
+using Tile1 = Mx4Cfg<64, 64, 2, 1, 256, 3, 2>;
+using Tile2 = Mx4Cfg<32, 64, 1, 2, 256, 4, 2>;
+struct TileInfo {
+  int bm, bn, bk, per_cu;
+  double start, step, share;  // us: a workgroup alone on its CU takes start + step for each stage
+};
+constexpr TileInfo kTiles[] = {
+    {128, 128, 256, 2, 2.2, 0.60, 0.61}, {64, 64, 256, 3, 1.7, 0.43, 0.33}, {32, 64, 256, 3, 1.3, 0.34, 0.32},
+};
+constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+
+struct Plan {
+  int tile, ksplit, splits;  // ksplit 0: not split
+};
+
+Plan split_of(int tile, int64_t nk, int64_t splits) {
+  if (splits > nk) splits = nk;
+  const int64_t ks = cdiv(nk, splits), n = cdiv(nk, ks);
+  return Plan{tile, n > 1 ? (int)ks : 0, (int)n};
+}
+
+double cost_of(const Plan& plan, int64_t M, int64_t N, int64_t K) {
+  const TileInfo& t = kTiles[plan.tile];
+  const int64_t nk = cdiv(K, t.bk), kb = plan.ksplit ? plan.ksplit : nk;
+  const int64_t deep = cdiv(cdiv(M, t.bm) * cdiv(N, t.bn) * plan.splits, kCus);  // workgroups on a CU
+  const int64_t full = deep / t.per_cu, rest = deep % t.per_cu;
+  double us = full * (t.start + t.step * kb * (1 + (t.per_cu - 1) * t.share));
+  if (rest) us += t.start + t.step * kb * (1 + (rest - 1) * t.share);
+  const double floor = ((double)N * K + (double)M * K) * 0.09e-6;  // the operands from HBM
+  if (us < floor) us = floor;
+  const double outputs = (double)M * N * 1e-6;
+  if (t.per_cu == 1) us += 0.3 * outputs;  // no other workgroup runs while one stores
+  if (plan.splits > 1) us += 2.1 + 0.25 * plan.splits + 1.36 * plan.splits * outputs;
+  return us;
+}
+
+Plan plan_of(int64_t M, int64_t N, int64_t K, int tile, int splits) {
+  Plan best{};
+  double least = 0;
+  for (int t = 0; t < kNumTiles; ++t) {
+    if (tile >= 0 && t != tile) continue;
+    const int64_t nk = cdiv(K, kTiles[t].bk), tiles = cdiv(M, kTiles[t].bm) * cdiv(N, kTiles[t].bn);
+    for (const int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      // (a part of at least two stages; workgroups beyond a few rounds are not split)
+      if (splits <= 0 && s > 1 && (s > nk / 2 || tiles * s > 4 * kCus)) break;
+      const Plan plan = split_of(t, nk, splits > 0 ? splits : s);
+      const double us = cost_of(plan, M, N, K);
+      if (least == 0 || us < least) {
+        best = plan;
+        least = us;
+      }
+      if (splits > 0) break;
+    }
+  }
+  return best;
+}
+
+size_t parts_bytes(const Plan& plan, int64_t M, int64_t N) {
+  return plan.splits > 1 ? up256((size_t)plan.splits * M * N * 4) : 0;
+}
+
+int product_check(const Mx4Args& p) {
+  if (p.M < 0 || p.N < 0 || p.K < 0 || p.ctype < 0 || p.ctype > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
+  if (p.M == 0 || p.N == 0) return 0;
+  if (p.K == 0 || !p.c || !p.x || !p.w || !p.sx || !p.sw) return F16ACC_OPS_E_ARG;
+  const int64_t bytes = cdiv(p.K, 2);
+  if (p.ldx % 16 || p.ldw % 16 || p.ldx < bytes || p.ldw < bytes || p.ldx > kMaxRow || p.ldw > kMaxRow ||
+      !aligned16(p.x) || !aligned16(p.w))
+    return F16ACC_OPS_E_UNSUPPORTED;
+  if (p.M > 0x7fffffff || p.N > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
+  return 0;
+}
+
+int run_product(Mx4Args p, const Plan& plan, void* parts, hipStream_t stream) {
+  p.ksplit = plan.ksplit;
+  p.parts = (float*)parts;
+  int rc = F16ACC_OPS_E_ARG;
+  switch (plan.tile) {
+    case 0: rc = launch_mm_fp4<Tile0>(p, stream, plan.splits); break;
+    case 1: rc = launch_mm_fp4<Tile1>(p, stream, plan.splits); break;
+    case 2: rc = launch_mm_fp4<Tile2>(p, stream, plan.splits); break;
+  }
+  if (rc || plan.splits == 1) return rc;
+  FinishArgs f{p.parts, p.M, p.N, p.scm, p.scn, plan.splits, p.bias, p.c};
+  return by_type(p.ctype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const int64_t groups = cdiv(p.M * p.N, p.N % 4 ? 256 : 1024);
+    hipLaunchKernelGGL((mm_finish_kernel<T>), dim3((uint32_t)(groups < 8 * kCus ? groups : 8 * kCus)), dim3(256), 0,
+                       stream, f);
+    return hip_status();
+  });
+}
+
+// Scales of the products' own order: the dword of (row, quad) at (quad * rows + row) * 4.
+size_t scale_bytes(int64_t rows, int64_t K) { return up256(quads_of(K) * rows * 4); }
+
+struct MmPlan4 {
+  Plan plan;
+  size_t sw, parts, total;
+  MmPlan4(int64_t M, int64_t N, int64_t K, int64_t sxq, int64_t swq, int tile, int splits) {
+    plan = plan_of(M, N, K, tile, splits);
+    sw = sxq ? 0 : scale_bytes(M, K);
+    parts = sw + (swq ? 0 : scale_bytes(N, K));
+    total = parts + parts_bytes(plan, M, N);
+  }
+};
+
+bool few4(int64_t M, int64_t K) { return M <= 16 && small4_lds(M, K) <= kSmall4Lds; }
+
+// The workspace of linear: the quantised tokens and their scales, the weight's scales in the
+// products' order, the weight where its rows have to be copied, the parts of a split of K.
+struct LinearPlan4 {
+  Plan plan;
+  bool packed;
+  int64_t ld;
+  size_t sx, sw, weight, parts, total;
+  LinearPlan4(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
+    plan = plan_of(M, N, K, -1, 0);
+    packed = !aligned16(w) || ldw % 16 || K % kMx || ldw > kMaxRow;
+    ld = cdiv(K, kMx) * 16;
+    sx = up256(M * 64 * quads_of(K));
+    sw = sx + scale_bytes(M, K);
+    weight = sw + scale_bytes(N, K);
+    parts = weight + (packed ? up256(N * ld) : 0);
+    total = parts + parts_bytes(plan, M, N);
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+int f16acc_fp4_quant(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
+                     int64_t ldq, uint8_t* s, int64_t s_row, int64_t s_quad, uint8_t* qt, int64_t ldqt, uint8_t* st,
+                     int64_t st_row, int64_t st_quad, void* stream) {
+  int rc = quant_check(x, type, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  if (!q && !qt) return F16ACC_OPS_E_ARG;
+  MxQuantArgs p{x, rows, cols, sr, sc, q, ldq, {s, s_row, s_quad}, qt, ldqt, {st, st_row, st_quad}, nullptr, 0, 0};
+  if (q && (rc = out4_check(q, ldq, cols, p.s))) return rc;
+  if (qt && (rc = out4_check(qt, ldqt, rows, p.st))) return rc;
+  const bool wide = wide_loads(x, type, sr, sc);
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (qt) return launch_tile<T>(p, wide, (hipStream_t)stream);
+    const Pack8Args none{};
+    const uint32_t grid = grid_of(rows * quads_of(cols), 16);
+    if (wide)
+      hipLaunchKernelGGL((mx_prepare_kernel<T, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p, MxScaleArgs{},
+                         none, 0u, 0u);
+    else
+      hipLaunchKernelGGL((mx_prepare_kernel<T, false>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p,
+                         MxScaleArgs{}, none, 0u, 0u);
+    return hip_status();
+  });
+}
+
+int f16acc_fp4_transpose(const uint8_t* x, int64_t sr, int64_t sc, const uint8_t* s, int64_t s_r, int64_t s_b,
+                         int64_t rows, int64_t cols, uint8_t* qt, int64_t ldqt, uint8_t* st, int64_t st_row,
+                         int64_t st_quad, void* stream) {
+  int rc = quant_check(x, 0, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  if (!s || !qt) return F16ACC_OPS_E_ARG;
+  MxQuantArgs p{x, rows, cols, sr, sc, nullptr, 0, {nullptr, 0, 0}, qt, ldqt, {st, st_row, st_quad}, s, s_r, s_b};
+  if ((rc = out4_check(qt, ldqt, rows, p.st))) return rc;
+  const int64_t gx = quads_of(cols), gy = quads_of(rows);
+  if (gx > 0x7fffffff || gy > 65535) return F16ACC_OPS_E_UNSUPPORTED;
+  hipLaunchKernelGGL((mx_quant_tile_kernel<Fp4Source, false, false>), dim3((uint32_t)gx, (uint32_t)gy), dim3(256), 0,
+                     (hipStream_t)stream, p);
+  return hip_status();
+}
+
+int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t* s, int64_t s_r, int64_t s_b,
+                      int64_t rows, int64_t cols, void* out, int type, void* stream) {
+  int rc = quant_check(q, type, rows, cols);
+  if (rc || rows == 0 || cols == 0) return rc;
+  if (!s || !out) return F16ACC_OPS_E_ARG;
+  if (!aligned16(out)) return F16ACC_OPS_E_UNSUPPORTED;
+  const MxValuesArgs p{q, q_r, q_c, s, s_r, s_b, rows, cols, out};
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL((mx_values_kernel<T>), dim3(grid_of(rows * cdiv(cols, 8), 256)), dim3(256), 0,
+                       (hipStream_t)stream, p);
+    return hip_status();
+  });
+}
+
+size_t f16acc_mm_fp4_workspace(int64_t M, int64_t N, int64_t K, int64_t sxq, int64_t swq, int tile, int splits) {
+  if (M <= 0 || N <= 0 || K <= 0 || tile < -1 || tile >= kNumTiles || splits < 0) return 0;
+  return MmPlan4(M, N, K, sxq, swq, tile, splits).total;
+}
+
+int f16acc_mm_fp4(const uint8_t* x, int64_t ldx, const uint8_t* sx, int64_t sxm, int64_t sxb, int64_t sxq,
+                  const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t swn, int64_t swb, int64_t swq,
+                  const void* bias, void* c, int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype,
+                  int tile, int splits, void* workspace, size_t ws_bytes, void* stream_) {
+  if (tile < -1 || tile >= kNumTiles || splits < 0) return F16ACC_OPS_E_ARG;
+  Mx4Args p{x, ldx, sx, sxm, sxq, w, ldw, sw, swn, swq, bias, c, scm, scn, M, N, K, ctype, 0, nullptr};
+  int rc = product_check(p);
+  if (rc || M == 0 || N == 0) return rc;
+  if (sxm < 0 || sxb < 0 || sxq < 0 || swn < 0 || swb < 0 || swq < 0) return F16ACC_OPS_E_ARG;
+  // scales read where they are
+  for (const auto& [s, row, quad] : {MxScales{(uint8_t*)sx, sxm, sxq}, MxScales{(uint8_t*)sw, swn, swq}})
+    if (quad && ((rc = scales_check({s, row, quad})) || row > kMaxRow)) return rc ? rc : F16ACC_OPS_E_UNSUPPORTED;
+  const MmPlan4 plan(M, N, K, sxq, swq, tile, splits);
+  if (plan.total && (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total)) return F16ACC_OPS_E_WORKSPACE;
+  char* ws = (char*)workspace;
+  hipStream_t stream = (hipStream_t)stream_;
+  const int64_t blocks = cdiv(K, kMx), quads = quads_of(K);
+  MxScaleArgs a{}, b{};
+  if (!sxq) a = {sx, M, blocks, sxm, sxb, (uint32_t*)ws, M}, p.sx = (uint8_t*)ws, p.sxm = 4, p.sxq = 4 * M;
+  if (!swq) b = {sw, N, blocks, swn, swb, (uint32_t*)(ws + plan.sw), N}, p.sw = (uint8_t*)ws + plan.sw, p.swm = 4, p.swq = 4 * N;
+  if (!sxq || !swq) {
+    const uint32_t ga = sxq ? 0 : grid_of(M * quads, 256), gb = swq ? 0 : grid_of(N * quads, 256);
+    hipLaunchKernelGGL(mx_scales_kernel, dim3(ga + gb), dim3(256), 0, stream, a, b, ga);
+    if ((rc = hip_status())) return rc;
+  }
+  return run_product(p, plan.plan, ws + plan.parts, stream);
+}
+
+size_t f16acc_linear_fp4_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return LinearPlan4(M, N, K, w, ldw).total;
+}
+
+int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw,
+                      const uint8_t* sw, int64_t swn, int64_t swb, const void* bias, void* y, int64_t M, int64_t N,
+                      int64_t K, void* workspace, size_t ws_bytes, void* stream_) {
+  int rc = quant_check(x, type, M, K);
+  if (rc) return rc;
+  if (N < 0) return F16ACC_OPS_E_ARG;
+  if (M == 0 || N == 0) return 0;
+  if (K == 0 || !w || !sw || !y || swn < 0 || swb < 0) return F16ACC_OPS_E_ARG;
+  if (ldw < cdiv(K, 2) && N > 1) return F16ACC_OPS_E_UNSUPPORTED;
+  hipStream_t stream = (hipStream_t)stream_;
+  const bool wide = wide_loads(x, type, sr, sc);
+  const LinearPlan4 plan(M, N, K, w, ldw);
+  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
+  if (few4(M, K) && wide && M <= 8) {
+    const Small4Args a{x, sr, w, ldw, sw, swn, swb, bias, y, M, N, K};
+    const size_t lds = small4_lds(M, K);
+    return by_type(type, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      if (cdiv(N, 16) <= kCus && quads_of(K) >= 12)
+        hipLaunchKernelGGL((linear_fp4_small_kernel<T, 16>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), lds, stream, a);
+      else
+        hipLaunchKernelGGL((linear_fp4_small_kernel<T, 8>), dim3((uint32_t)cdiv(N, 16)), dim3(512), lds, stream, a);
+      return hip_status();
+    });
+  }
+  char* ws = (char*)workspace;
+  Mx4Args p{};
+  p.x = (const uint8_t*)ws, p.ldx = 64 * quads_of(K);
+  p.sx = (const uint8_t*)ws + plan.sx, p.sxm = 4, p.sxq = 4 * M;
+  p.w = plan.packed ? (const uint8_t*)ws + plan.weight : w, p.ldw = plan.packed ? plan.ld : ldw;
+  p.sw = (const uint8_t*)ws + plan.sw, p.swm = 4, p.swq = 4 * N;
+  p.bias = bias, p.c = y, p.scm = N, p.scn = 1, p.M = M, p.N = N, p.K = K, p.ctype = type;
+  rc = product_check(p);
+  if (rc) return rc;
+  const MxQuantArgs q{x, M, K, sr, sc, (uint8_t*)ws, p.ldx, {(uint8_t*)p.sx, p.sxm, p.sxq}, nullptr, 0, {nullptr, 0, 0},
+                      nullptr, 0, 0};
+  const MxScaleArgs s{sw, N, cdiv(K, kMx), swn, swb, (uint32_t*)p.sw, N};
+  const Pack8Args pk{w, (uint8_t*)p.w, N, cdiv(K, 2), ldw, 1, plan.ld};
+  const uint32_t packs = plan.packed ? grid_of(N * (plan.ld / 16), 256) : 0, scales = grid_of(N * quads_of(K), 256);
+  const dim3 grid(packs + scales + grid_of(M * quads_of(K), 16));
+  rc = by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (wide)
+      hipLaunchKernelGGL((mx_prepare_kernel<T, true>), grid, dim3(256), 0, stream, q, s, pk, packs, scales);
+    else
+      hipLaunchKernelGGL((mx_prepare_kernel<T, false>), grid, dim3(256), 0, stream, q, s, pk, packs, scales);
+    return hip_status();
+  });
+  if (rc) return rc;
+  return run_product(p, plan.plan, ws + plan.parts, stream);
+}
+
+}  // extern "C"

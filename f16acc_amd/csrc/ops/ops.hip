@@ -2,6 +2,7 @@
 // operators (include/f16acc_ops.h): argument checks, the choice of a kernel,
 // workspaces.
 #include "common.h"
+#include "launch.h"
 #include "mm.h"
 #include "moe.h"
 #include "quant.h"
@@ -12,30 +13,9 @@ using namespace f16ops;
 
 namespace {
 
-// Bytes from an element of a row to the last one's end stay below the copies'
-// 31-bit offsets.
-constexpr int64_t kMaxRow = 1 << 22;  // bytes between rows of a staged operand: 256 rows stay below 2^31
-constexpr int64_t kMaxExtent = (int64_t)1 << 40;
+__global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) { pack8(p, blockIdx.x, gridDim.x); }
 
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-int64_t up128(int64_t v) { return cdiv(v, kBlock) * kBlock; }
-size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-
-bool wide_loads(const void* x, int type, int64_t sr, int64_t sc) {
-  return sc == 1 && aligned16(x) && sr * type_size(type) % 16 == 0;
-}
-
-template <class F>
-int by_type(int type, F f) {
-  switch (type) {
-    case F16ACC_TYPE_F16: return f((f16*)nullptr);
-    case F16ACC_TYPE_BF16: return f((bf16*)nullptr);
-    case F16ACC_TYPE_F32: return f((float*)nullptr);
-  }
-  return F16ACC_OPS_E_ARG;
-}
-
-// ... and by the groups of four tokens (1, 2 or 4) that hold `tokens`.
+// by_type, and by the groups of four tokens (1, 2 or 4) that hold `tokens`.
 template <class F>
 int by_tokens(int tokens, int type, F f) {
   return by_type(type, [&](auto* t) {
@@ -43,13 +23,6 @@ int by_tokens(int tokens, int type, F f) {
     if (tokens <= 8) return f(t, std::integral_constant<int, 2>());
     return f(t, std::integral_constant<int, 4>());
   });
-}
-
-int quant_check(const void* x, int type, int64_t rows, int64_t cols) {
-  if (rows < 0 || cols < 0 || type < 0 || type > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
-  if (rows > kMaxExtent || cols > kMaxExtent) return F16ACC_OPS_E_UNSUPPORTED;
-  if (rows && cols && !x) return F16ACC_OPS_E_ARG;
-  return 0;
 }
 
 int out_check(const uint8_t* q, int64_t ldq, int64_t cols, const float* s) {

@@ -186,7 +186,6 @@ __device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32
     *(i32x4*)(p.dst + r * p.ld + c) = o.v;
   }
 }
-__global__ __launch_bounds__(256) void pack8_kernel(Pack8Args p) { pack8(p, blockIdx.x, gridDim.x); }
 
 // Both at once, for a product of new tokens with a weight whose rows are not aligned: the
 // first `packs` workgroups copy.
