@@ -24,6 +24,7 @@ struct RouteArgs {
   void* dx;  // [T][E] contiguous
   bool wide;     // a lane's V logits are one load
   int lanes;     // lanes of a group where that is a power of two, else 0
+  bool nan_id;   // a token with a NaN logit and no expert gets the first one, so what follows sees its NaN weight
 };
 
 // Order-preserving map of a float to an unsigned integer, -inf lowest; 0 is
@@ -96,12 +97,10 @@ __device__ __forceinline__ void scores(const RouteArgs& a, int64_t t, int lane, 
 // selections.  Selection: k times the wave's largest key (a DPP maximum),
 // the lowest lane that holds it (ballot) and that lane's lowest expert, which
 // is the lowest index since a lane's experts are consecutive.
+// Lane j < k gets the j-th expert and its weight; `row` are 64 V floats of the wave's own.
 template <class T, int V>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
-  __shared__ float lds[4][64 * V + 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= a.T) return;
+__device__ __forceinline__ void route_token(const RouteArgs& a, int64_t t, int lane, float* row, int* expert,
+                                            float* weight) {
   float x[V], p[V];
   bool nan;
   scores<T, V>(a, t, lane, x, p, &nan);
@@ -144,13 +143,13 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   } else if (a.groups > 1) {
     // a lane per group
 #pragma unroll
-    for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = keys[i];
+    for (int i = 0; i < V; ++i) row[lane * V + i] = keys[i];
     wave_sync();
     const int size = a.E / a.groups;
     float b1 = -INFINITY, b2 = -INFINITY;
     if (lane < a.groups)
       for (int i = 0; i < size; ++i) {
-        const float f = lds[wave][lane * size + i];
+        const float f = row[lane * size + i];
         b2 = fmaxf(b2, fminf(b1, f));
         b1 = fmaxf(b1, f);
       }
@@ -194,9 +193,25 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
       if (lane == src && i == at) key[i] = 0u;
   }
   if (a.renorm) mine = mine / (wave_sum(mine) + 1e-20f);
-  if (nan) mine = __uint_as_float(0x7fc00000u);
+  if (nan) {
+    mine = __uint_as_float(0x7fc00000u);
+    if (a.nan_id && lane == 0 && id < 0) id = 0;
+  }
+  *expert = id;
+  *weight = mine * a.scale;
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  __shared__ float lds[4][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= a.T) return;
+  int id;
+  float weight;
+  route_token<T, V>(a, t, lane, lds[wave], &id, &weight);
   if (lane < a.k) {
-    a.weights[t * a.k + lane] = mine * a.scale;
+    a.weights[t * a.k + lane] = weight;
     a.ids[t * a.k + lane] = id;
   }
 }

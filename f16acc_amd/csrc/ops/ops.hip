@@ -3,6 +3,7 @@
 // workspaces.
 #include "common.h"
 #include "launch.h"
+#include "layer.h"
 #include "mm.h"
 #include "moe.h"
 #include "quant.h"
@@ -291,6 +292,38 @@ struct ExpertsPlan {
   }
 };
 
+// The experts' weights as the C entry points get them.
+struct ExpertWeights {
+  const uint8_t* w1;
+  int64_t w1e, w1u, ld1;
+  const float* s1;
+  int64_t s1e, s1u, s1n, s1k;
+  const uint8_t* w2;
+  int64_t w2e, ld2;
+  const float* s2;
+  int64_t s2e, s2n, s2k;
+};
+
+int experts_check(const void* x, int type, int64_t T, int k, int E, int64_t D, int64_t I, const ExpertWeights& w,
+                  const void* y, bool few) {
+  const int rc = quant_check(x, type, T, D);
+  if (rc) return rc;
+  if (k < 1 || E < 1 || D < 1 || I < 1) return F16ACC_OPS_E_ARG;
+  if (T == 0) return 0;
+  if (!w.w1 || !w.s1 || !w.w2 || !w.s2 || !y) return F16ACC_OPS_E_ARG;
+  if (w.w1e < 0 || w.w1u < 0 || w.s1e < 0 || w.s1u < 0 || w.s1n < 0 || w.s1k < 0 || w.w2e < 0 || w.s2e < 0 ||
+      w.s2n < 0 || w.s2k < 0)
+    return F16ACC_OPS_E_ARG;
+  if (E > kMaxExperts || w.ld1 < 0 || w.ld2 < 0 || up128(D) > kMaxRow || up128(I) > kMaxRow)
+    return F16ACC_OPS_E_UNSUPPORTED;
+  if (!few && (w.ld1 % 16 || w.ld2 % 16 || w.w1e % 16 || w.w1u % 16 || w.w2e % 16 || w.ld1 < D || w.ld2 < I ||
+               w.ld1 > kMaxRow || w.ld2 > kMaxRow || !aligned16(w.w1) || !aligned16(w.w2)))
+    return F16ACC_OPS_E_UNSUPPORTED;
+  // the copies address a token's (a slot's) row by a 31-bit offset
+  if (T > kOob / up128(D) || T > kOob / ((int64_t)k * up128(I))) return F16ACC_OPS_E_UNSUPPORTED;
+  return 0;
+}
+
 // EXACT: gate and up on the 16-bit matrix instructions.  Up to 191 tokens an expert, where
 // weights are most of the time, they always do (in all, 64 experts of 2048 x 1024, 8 a
 // token, exact / 8-bit: 64 tokens 100 / 97 us, 512 132 / 117, 1024 185 / 153).  Past that
@@ -342,11 +375,45 @@ struct LaunchRouteGrad {
   }
 };
 
+// The router's product: bytes of a row step as the loads of eight elements need them.
+template <class T, class R>
+int launch_router(RouterArgs p, hipStream_t stream) {
+  p.wide = p.sc == 1 && p.rd == 1 && aligned16(p.x) && aligned16(p.r) && p.sr * (int64_t)sizeof(T) % 16 == 0 &&
+           p.re * (int64_t)sizeof(R) % 16 == 0;
+  const dim3 grid((uint32_t)cdiv(p.T, 16), (uint32_t)cdiv(p.E, 16));
+  hipLaunchKernelGGL((router_kernel<T, R, 8>), grid, dim3(512), 0, stream, p);
+  return hip_status();
+}
+
+// Where a layer's logits, weights and ids lie in its workspace, before the experts' own.
+struct LayerPlan {
+  size_t logits, weights, ids, experts, total;
+  LayerPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += up256(bytes);
+      return here;
+    };
+    logits = take(T * E * 4);
+    weights = take(T * k * 4);
+    ids = take(T * k * 4);
+    experts = at;
+    total = at + ExpertsPlan(T, k, E, D, I).total;
+  }
+};
+
 int route_check(const RouteArgs& a, int type) {
   if (a.T < 0 || type < 0 || type > F16ACC_TYPE_F32 || a.E < 1 || a.k < 1 || a.k > a.E) return F16ACC_OPS_E_ARG;
   if (a.E > kMaxExperts || a.k > 64 || a.T > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
   if (a.T && (!a.x || !a.ids)) return F16ACC_OPS_E_ARG;
   return 0;
+}
+
+int groups_check(const RouteArgs& a) {
+  if (a.groups < 1 || a.E % a.groups || a.top < 1 || a.top > a.groups || a.k > a.E / a.groups * a.top)
+    return F16ACC_OPS_E_ARG;
+  return a.groups > 64 ? F16ACC_OPS_E_UNSUPPORTED : 0;
 }
 
 }  // namespace
@@ -530,12 +597,11 @@ int f16acc_linear_fp8(const void* x, int type, int64_t sr, int64_t sc, const uin
 int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
                  const float* bias, int groups, int top, int renorm, float scale, float* weights, int* ids,
                  void* stream) {
-  RouteArgs a{logits, T, st, se, E, k, sigmoid, bias, groups, top, renorm, scale, weights, ids, nullptr, 0, 0, nullptr, false, 0};
-  const int rc = route_check(a, type);
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, bias, groups, top, renorm, scale, weights, ids, nullptr, 0, 0, nullptr, false, 0, false};
+  int rc = route_check(a, type);
+  if (!rc) rc = groups_check(a);
   if (rc) return rc;
-  if (groups < 1 || E % groups || top < 1 || top > groups || k > E / groups * top || (T && !weights))
-    return F16ACC_OPS_E_ARG;
-  if (groups > 64) return F16ACC_OPS_E_UNSUPPORTED;
+  if (T && !weights) return F16ACC_OPS_E_ARG;
   if (T == 0) return 0;
   return by_experts<LaunchRoute>(E, type, a, (hipStream_t)stream);
 }
@@ -543,7 +609,7 @@ int f16acc_route(const void* logits, int type, int64_t T, int64_t st, int64_t se
 int f16acc_route_grad(const void* logits, int type, int64_t T, int64_t st, int64_t se, int E, int k, int sigmoid,
                       int renorm, float scale, const int* ids, const float* dw, int64_t dwt, int64_t dwk,
                       void* dlogits, void* stream) {
-  RouteArgs a{logits, T, st, se, E, k, sigmoid, nullptr, 1, 1, renorm, scale, nullptr, (int*)ids, dw, dwt, dwk, dlogits, false, 0};
+  RouteArgs a{logits, T, st, se, E, k, sigmoid, nullptr, 1, 1, renorm, scale, nullptr, (int*)ids, dw, dwt, dwk, dlogits, false, 0, false};
   const int rc = route_check(a, type);
   if (rc) return rc;
   if (T && (!dw || !dlogits)) return F16ACC_OPS_E_ARG;
@@ -566,20 +632,11 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
                    int64_t w1u, int64_t ld1, const float* s1, int64_t s1e, int64_t s1u, int64_t s1n, int64_t s1k,
                    const uint8_t* w2, int64_t w2e, int64_t ld2, const float* s2, int64_t s2e, int64_t s2n,
                    int64_t s2k, void* y, void* workspace, size_t ws_bytes, void* stream_) {
-  int rc = quant_check(x, type, T, D);
-  if (rc) return rc;
-  if (k < 1 || E < 1 || D < 1 || I < 1) return F16ACC_OPS_E_ARG;
-  if (T == 0) return 0;
-  if (!weights || !ids || !w1 || !s1 || !w2 || !s2 || !y) return F16ACC_OPS_E_ARG;
-  if (w1e < 0 || w1u < 0 || s1e < 0 || s1u < 0 || s1n < 0 || s1k < 0 || w2e < 0 || s2e < 0 || s2n < 0 || s2k < 0)
-    return F16ACC_OPS_E_ARG;
-  if (E > kMaxExperts || ld1 < 0 || ld2 < 0 || up128(D) > kMaxRow || up128(I) > kMaxRow) return F16ACC_OPS_E_UNSUPPORTED;
+  const ExpertWeights w{w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2, w2e, ld2, s2, s2e, s2n, s2k};
   const bool few = f16acc_experts_any_rows(x, type, T, sr, sc, k);
-  if (!few && (ld1 % 16 || ld2 % 16 || w1e % 16 || w1u % 16 || w2e % 16 || ld1 < D || ld2 < I || ld1 > kMaxRow ||
-               ld2 > kMaxRow || !aligned16(w1) || !aligned16(w2)))
-    return F16ACC_OPS_E_UNSUPPORTED;
-  // the copies address a token's (a slot's) row by a 31-bit offset
-  if (T > kOob / up128(D) || T > kOob / ((int64_t)k * up128(I))) return F16ACC_OPS_E_UNSUPPORTED;
+  int rc = experts_check(x, type, T, k, E, D, I, w, y, few);
+  if (rc || T == 0) return rc;
+  if (!weights || !ids) return F16ACC_OPS_E_ARG;
   const ExpertsPlan plan(T, k, E, D, I);
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_;
@@ -640,6 +697,47 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
     hipLaunchKernelGGL((combine_kernel<U>), grid, dim3(256), 0, stream, co);
     return hip_status();
   });
+}
+
+size_t f16acc_layer_workspace(int64_t T, int k, int E, int64_t D, int64_t I) {
+  if (T <= 0 || k <= 0 || E <= 0 || D <= 0 || I <= 0) return 0;
+  return LayerPlan(T, k, E, D, I).total;
+}
+
+int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const void* router, int rtype, int64_t re,
+                 int64_t rd, int E, int k, int sigmoid, const float* bias, int groups, int top, int renorm, float scale,
+                 int64_t D, int64_t I, const uint8_t* w1, int64_t w1e, int64_t w1u, int64_t ld1, const float* s1,
+                 int64_t s1e, int64_t s1u, int64_t s1n, int64_t s1k, const uint8_t* w2, int64_t w2e, int64_t ld2,
+                 const float* s2, int64_t s2e, int64_t s2n, int64_t s2k, void* y, void* workspace, size_t ws_bytes,
+                 void* stream_) {
+  const ExpertWeights w{w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2, w2e, ld2, s2, s2e, s2n, s2k};
+  const bool few = f16acc_experts_any_rows(x, type, T, sr, sc, k);
+  int rc = experts_check(x, type, T, k, E, D, I, w, y, few);
+  if (!rc) rc = quant_check(router, rtype, E, D);
+  if (rc || T == 0) return rc;
+  // (what is not there yet is not looked at)
+  RouteArgs a{router, T, E, 1, E, k, sigmoid, bias, groups, top, renorm, scale, nullptr, (int*)router, nullptr, 0, 0, nullptr,
+              false, 0, true};
+  if ((rc = route_check(a, F16ACC_TYPE_F32)) || (rc = groups_check(a))) return rc;
+  const LayerPlan plan(T, k, E, D, I);
+  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
+  char* ws = (char*)workspace;
+  float *logits = (float*)(ws + plan.logits), *weights = (float*)(ws + plan.weights);
+  int* ids = (int*)(ws + plan.ids);
+  const RouterArgs r{x, T, sr, sc, router, re, rd, E, D, false, logits};
+  rc = by_type(type, [&](auto* t) {
+    using X = std::remove_pointer_t<decltype(t)>;
+    return by_type(rtype, [&](auto* u) {
+      using R = std::remove_pointer_t<decltype(u)>;
+      return launch_router<X, R>(r, (hipStream_t)stream_);
+    });
+  });
+  if (rc) return rc;
+  a.x = logits, a.weights = weights, a.ids = ids;
+  rc = by_experts<LaunchRoute>(E, F16ACC_TYPE_F32, a, (hipStream_t)stream_);
+  if (rc) return rc;
+  return f16acc_experts(x, type, T, sr, sc, weights, k, 1, ids, k, E, D, I, w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2,
+                        w2e, ld2, s2, s2e, s2n, s2k, y, ws + plan.experts, ws_bytes - plan.experts, stream_);
 }
 
 const char* f16acc_ops_strerror(int code) {

@@ -344,26 +344,33 @@ struct Route : torch::autograd::Function<Route> {
   }
 };
 
-std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::string& scoring, const Maybe& bias,
-                                 int64_t groups, int64_t top, bool renormalize, double scale) {
-  check_call("route", {&logits, maybe(bias)});
-  check_float("route", logits);
-  REQUIRE(logits.dim() >= 1, "route needs [..., E] logits");
-  const int64_t E = logits.size(-1);
+// The options of a routing over E experts, checked.
+RouteOptions route_options(int64_t E, int64_t k, const std::string& scoring, int64_t groups, int64_t top,
+                           bool renormalize, double scale) {
   REQUIRE(scoring == "softmax" || scoring == "sigmoid", "scoring must be 'softmax' or 'sigmoid', not '", scoring, "'");
   REQUIRE(1 <= E && E <= 1024, "route needs 1 to 1024 experts, got ", E);
   REQUIRE(1 <= groups && groups <= 64 && E % groups == 0 && 1 <= top && top <= groups, E, " experts in ", groups,
         " groups of which ", top, " stay: not equal groups, or over 64");
   REQUIRE(1 <= k && k <= 64 && k <= E / groups * top,
         "k must be 1 to 64 and at most the experts of the groups that stay, got ", k);
-  Maybe b;
-  if (bias) {
-    check_device("route", logits, *bias);
-    REQUIRE(bias->scalar_type() == at::kFloat && bias->sizes() == at::IntArrayRef({E}), "bias must be float32 [", E,
-          "], got ", bias->scalar_type(), " ", bias->sizes());
-    b = bias->detach().contiguous();
-  }
-  const RouteOptions o{k, groups, top, scoring == "sigmoid", renormalize, scale};
+  return {k, groups, top, scoring == "sigmoid", renormalize, scale};
+}
+
+Maybe route_bias(const char* name, const Tensor& like, const Maybe& bias, int64_t E) {
+  if (!bias) return {};
+  check_device(name, like, *bias);
+  REQUIRE(bias->scalar_type() == at::kFloat && bias->sizes() == at::IntArrayRef({E}), "bias must be float32 [", E,
+        "], got ", bias->scalar_type(), " ", bias->sizes());
+  return bias->detach().contiguous();
+}
+
+std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::string& scoring, const Maybe& bias,
+                                 int64_t groups, int64_t top, bool renormalize, double scale) {
+  check_call("route", {&logits, maybe(bias)});
+  check_float("route", logits);
+  REQUIRE(logits.dim() >= 1, "route needs [..., E] logits");
+  const RouteOptions o = route_options(logits.size(-1), k, scoring, groups, top, renormalize, scale);
+  const Maybe b = route_bias("route", logits, bias, logits.size(-1));
   if (c10::GradMode::is_enabled() && logits.requires_grad()) {
     const variable_list r = Route::apply(logits, b, o);
     return {r[0], r[1]};
@@ -371,23 +378,54 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, const std::str
   return route_forward(logits, b, o);
 }
 
-Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const Tensor& w1, const Tensor& s1,
-               const Tensor& w2, const Tensor& s2) {
-  check_call("experts", {&x, &weights, &ids, &w1, &s1, &w2, &s2});
-  check_float("experts", x);
-  for (const Tensor* t : {&weights, &ids, &w1, &s1, &w2, &s2}) check_device("experts", x, *t);
+// The experts' weights, checked: w1 [E, 2, I, D], w2 [E, D, I] and their scales.
+void check_experts(const char* name, const Tensor& x, const Tensor& w1, const Tensor& s1, const Tensor& w2,
+                   const Tensor& s2) {
   const bool dims = x.dim() >= 1 && w1.dim() == 4 && w1.size(1) == 2 && w2.dim() == 3;
   const int64_t E = dims ? w1.size(0) : 0, I = dims ? w1.size(2) : 0, D = dims ? w1.size(3) : 0;
   REQUIRE(dims && x.size(-1) == D && w2.sizes() == at::IntArrayRef({E, D, I}) && 1 <= E && E <= 1024 && D > 0 && I > 0,
-        "experts needs x [..., D], w1 [E, 2, I, D] and w2 [E, D, I] (E 1 to 1024, D and I positive), got ", x.sizes(),
+        name, " needs x [..., D], w1 [E, 2, I, D] and w2 [E, D, I] (E 1 to 1024, D and I positive), got ", x.sizes(),
         ", ", w1.sizes(), ", ", w2.sizes());
-  REQUIRE(w1.scalar_type() == kF8 && w2.scalar_type() == kF8, "experts needs float8_e4m3fn weights");
+  REQUIRE(w1.scalar_type() == kF8 && w2.scalar_type() == kF8, name, " needs float8_e4m3fn weights");
   REQUIRE(s1.scalar_type() == at::kFloat && s1.sizes() == at::IntArrayRef({E, 2, blocks(I), blocks(D)}),
         "w1_scale must be float32 ", at::IntArrayRef({E, 2, blocks(I), blocks(D)}), ", got ", s1.scalar_type(), " ",
         s1.sizes());
   REQUIRE(s2.scalar_type() == at::kFloat && s2.sizes() == at::IntArrayRef({E, blocks(D), blocks(I)}),
         "w2_scale must be float32 ", at::IntArrayRef({E, blocks(D), blocks(I)}), ", got ", s2.scalar_type(), " ",
         s2.sizes());
+}
+
+void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensors) {
+  bool grown = false;
+  for (const Tensor* t : tensors) grown = grown || (t && t->requires_grad());
+  REQUIRE(!c10::GradMode::is_enabled() || !grown, name,
+        " has no backward pass: call it under torch.no_grad() or torch.inference_mode()");
+}
+
+// The experts' weights as the kernels read them, and how many tokens go into one call: the kernels address
+// rows of the quantised tokens and hidden values by 31 bits, more tokens go in parts.
+struct ExpertRows {
+  Operand w1, w2;
+  int64_t part;
+  ExpertRows(const Tensor& x2, int64_t k, const Tensor& q1, const Tensor& q2) {
+    const int64_t T = x2.size(0), D = q1.size(3), I = q1.size(2);
+    // for a few tokens rows of any alignment go as they are
+    const bool any = f16acc_experts_any_rows(x2.const_data_ptr(), type_of(x2), T, x2.stride(0), x2.stride(1), (int)k);
+    auto rows = [&](const Tensor& w) {
+      return any && (w.size(-1) <= 1 || w.stride(-1) == 1) ? Operand{w, w.stride(-2)} : packed(w);
+    };
+    w1 = rows(q1), w2 = rows(q2);
+    const int64_t most = 0x7fff0000 / std::max(up(D, kBlock), k * up(I, kBlock));
+    part = std::min(T, std::max<int64_t>(most, 1));
+  }
+};
+
+Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const Tensor& w1, const Tensor& s1,
+               const Tensor& w2, const Tensor& s2) {
+  check_call("experts", {&x, &weights, &ids, &w1, &s1, &w2, &s2});
+  check_float("experts", x);
+  for (const Tensor* t : {&weights, &ids, &w1, &s1, &w2, &s2}) check_device("experts", x, *t);
+  check_experts("experts", x, w1, s1, w2, s2);
   REQUIRE(ids.dim() == x.dim() && ids.sizes() == weights.sizes() && ids.size(-1) >= 1 &&
             ids.sizes().slice(0, ids.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
         "weights and ids must be [..., k] over x's tokens, got ", weights.sizes(), " and ", ids.sizes(), " for ",
@@ -395,11 +433,8 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   REQUIRE(weights.scalar_type() == at::kFloat && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong),
         "experts needs float32 weights and int32 or int64 ids, got ", weights.scalar_type(), " and ",
         ids.scalar_type());
-  bool grown = false;
-  for (const Tensor* t : {&x, &weights, &w1, &s1, &w2, &s2}) grown = grown || t->requires_grad();
-  REQUIRE(!c10::GradMode::is_enabled() || !grown,
-        "experts has no backward pass: call it under torch.no_grad() or torch.inference_mode()");
-  const int64_t k = ids.size(-1);
+  check_no_grad("experts", {&x, &weights, &w1, &s1, &w2, &s2});
+  const int64_t E = w1.size(0), I = w1.size(2), D = w1.size(3), k = ids.size(-1);
   const Tensor x2 = rows_of(x), wt = rows_of(weights);
   const int64_t T = x2.size(0);
   Tensor y = empty(x.sizes(), x, x.scalar_type());
@@ -407,28 +442,54 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   Tensor i32 = rows_of(ids);
   if (i32.scalar_type() == at::kLong) i32 = i32.clamp(-1, E).to(at::kInt);  // (a cast alone would wrap)
   i32 = i32.contiguous();
-  // for a few tokens rows of any alignment go as they are
-  const bool any = f16acc_experts_any_rows(x2.const_data_ptr(), type_of(x), T, x2.stride(0), x2.stride(1), (int)k);
-  auto rows = [&](const Tensor& w) {
-    return any && (w.size(-1) <= 1 || w.stride(-1) == 1) ? Operand{w, w.stride(-2)} : packed(w);
-  };
-  const Operand p1 = rows(w1), p2 = rows(w2);
-  // The kernels address rows of the quantised tokens and hidden values by 31 bits:
-  // more tokens than that go in parts.
-  const int64_t most = 0x7fff0000 / std::max(up(D, kBlock), k * up(I, kBlock));
-  const int64_t part = std::min(T, std::max<int64_t>(most, 1));
-  const size_t n = f16acc_experts_workspace(part, (int)k, (int)E, D, I);
+  const ExpertRows p(x2, k, w1, w2);
+  const size_t n = f16acc_experts_workspace(p.part, (int)k, (int)E, D, I);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);
-  for (int64_t t = 0; t < T; t += part) {
-    const int64_t tokens = std::min(part, T - t);
+  for (int64_t t = 0; t < T; t += p.part) {
+    const int64_t tokens = std::min(p.part, T - t);
     check_rc(f16acc_experts((const char*)x2.const_data_ptr() + t * x2.stride(0) * x2.element_size(), type_of(x),
                             tokens, x2.stride(0), x2.stride(1), floats(wt) + t * wt.stride(0), wt.stride(0),
-                            wt.stride(1), (const int*)i32.const_data_ptr() + t * k, (int)k, (int)E, D, I, bytes(p1.q),
-                            p1.q.stride(0), p1.q.stride(1), p1.ld, floats(s1), s1.stride(0), s1.stride(1),
-                            s1.stride(2), s1.stride(3), bytes(p2.q), p2.q.stride(0), p2.ld, floats(s2), s2.stride(0),
-                            s2.stride(1), s2.stride(2), (char*)y.data_ptr() + t * D * y.element_size(), bytes(ws), n,
-                            on.stream));
+                            wt.stride(1), (const int*)i32.const_data_ptr() + t * k, (int)k, (int)E, D, I,
+                            bytes(p.w1.q), p.w1.q.stride(0), p.w1.q.stride(1), p.w1.ld, floats(s1), s1.stride(0),
+                            s1.stride(1), s1.stride(2), s1.stride(3), bytes(p.w2.q), p.w2.q.stride(0), p.w2.ld,
+                            floats(s2), s2.stride(0), s2.stride(1), s2.stride(2),
+                            (char*)y.data_ptr() + t * D * y.element_size(), bytes(ws), n, on.stream));
+  }
+  return y;
+}
+
+Tensor layer(const Tensor& x, const Tensor& router, int64_t k, const Tensor& w1, const Tensor& s1, const Tensor& w2,
+             const Tensor& s2, const std::string& scoring, const Maybe& bias, int64_t groups, int64_t top,
+             bool renormalize, double scale) {
+  check_call("layer", {&x, &router, &w1, &s1, &w2, &s2, maybe(bias)});
+  check_float("layer", x);
+  for (const Tensor* t : {&router, &w1, &s1, &w2, &s2}) check_device("layer", x, *t);
+  check_experts("layer", x, w1, s1, w2, s2);
+  const int64_t E = w1.size(0), I = w1.size(2), D = w1.size(3);
+  REQUIRE(is_type(router.scalar_type()) && router.sizes() == at::IntArrayRef({E, D}),
+          "router must be torch.float16, bfloat16 or float32 ", at::IntArrayRef({E, D}), ", got ",
+          router.scalar_type(), " ", router.sizes());
+  const RouteOptions o = route_options(E, k, scoring, groups, top, renormalize, scale);
+  const Maybe b = route_bias("layer", x, bias, E);
+  check_no_grad("layer", {&x, &router, &w1, &s1, &w2, &s2, maybe(bias)});
+  const Tensor x2 = rows_of(x);
+  const int64_t T = x2.size(0);
+  Tensor y = empty(x.sizes(), x, x.scalar_type());
+  if (T == 0) return y;
+  const ExpertRows p(x2, k, w1, w2);
+  const size_t n = f16acc_layer_workspace(p.part, (int)k, (int)E, D, I);
+  const Tensor ws = empty({(int64_t)n}, x, at::kByte);
+  const On on(x);
+  for (int64_t t = 0; t < T; t += p.part) {
+    const int64_t tokens = std::min(p.part, T - t);
+    check_rc(f16acc_layer((const char*)x2.const_data_ptr() + t * x2.stride(0) * x2.element_size(), type_of(x), tokens,
+                          x2.stride(0), x2.stride(1), router.const_data_ptr(), type_of(router), router.stride(0),
+                          router.stride(1), (int)E, (int)k, o.sigmoid, (const float*)data(b), (int)o.groups, (int)o.top,
+                          o.renormalize, (float)o.scale, D, I, bytes(p.w1.q), p.w1.q.stride(0), p.w1.q.stride(1),
+                          p.w1.ld, floats(s1), s1.stride(0), s1.stride(1), s1.stride(2), s1.stride(3), bytes(p.w2.q),
+                          p.w2.q.stride(0), p.w2.ld, floats(s2), s2.stride(0), s2.stride(1), s2.stride(2),
+                          (char*)y.data_ptr() + t * D * y.element_size(), bytes(ws), n, on.stream));
   }
   return y;
 }
@@ -451,6 +512,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear", &linear, Free());
   m.def("route", &route, Free());
   m.def("experts", &experts, Free());
+  m.def("layer", &layer, Free());
   m.def("fp4_quantize", &quantize4, Free());
   m.def("fp4_dequantize", [](const Tensor& q, const Tensor& s, py::object dtype) {
     REQUIRE(THPDtype_Check(dtype.ptr()), "fp4.dequantize gives torch.float16, bfloat16 or float32");

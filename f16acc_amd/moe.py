@@ -1,7 +1,9 @@
-"""Mixture of experts: routing, and the experts' gated feed-forward in 8 bits.
+"""Mixture of experts: routing, the experts' gated feed-forward in 8 bits, and both with the
+router's product as one call.
 
     weights, ids = moe.route(logits, k=8)          # logits [T, E]
     y = moe.experts(x, weights, ids, w1, w1_scale, w2, w2_scale)
+    y = moe.layer(x, router, 8, w1, w1_scale, w2, w2_scale)
 
 Everything runs on the current torch stream of the operands' GPU, allocates
 through torch, and does not synchronise: the tokens are sorted by expert on the
@@ -11,7 +13,7 @@ make_fx, export, torch.func) or differentiates forward raises NotImplementedErro
 
 from ._ops import host
 
-__all__ = ["route", "experts"]
+__all__ = ["route", "experts", "layer"]
 
 
 def route(logits, k, *, scoring="softmax", bias=None, groups=1, top_groups=1, renormalize=True, scale=1.0):
@@ -54,3 +56,17 @@ def experts(x, weights, ids, w1, w1_scale, w2, w2_scale):
     inference: operands that require gradients are refused where gradients are
     enabled."""
     return host.experts(x, weights, ids, w1, w1_scale, w2, w2_scale)
+
+
+def layer(x, router, k, w1, w1_scale, w2, w2_scale, *, scoring="softmax", bias=None, groups=1, top_groups=1,
+          renormalize=True, scale=1.0):
+    """The whole layer: route of the logits x @ router.T, and experts of what it chooses.
+
+    x: [..., D] float16, bfloat16 or float32, any strides
+    router: [E, D] float16, bfloat16 or float32, any strides.  The logits are summed in
+       64 bits and rounded once to FP32, so a token's choice does not depend on the batch around it.
+       A token with a NaN logit gives NaN
+    k and the options are route's, the weights and their scales experts'
+    Returns [..., D] in x's type.  For inference: operands that require gradients are refused
+    where gradients are enabled."""
+    return host.layer(x, router, k, w1, w1_scale, w2, w2_scale, scoring, bias, groups, top_groups, renormalize, scale)

@@ -149,6 +149,20 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
                    int64_t s2k, void* y, void* workspace, size_t ws_bytes, void* stream);
 
 /*
+ * A whole layer: logits = x router^T (router [E, D] of rtype, element strides re, rd), summed in 64 bits and rounded
+ * once to FP32; weights and ids of f16acc_route of them; y of f16acc_experts, whose rows and
+ * alignments apply (f16acc_experts_any_rows for x and k).  A token with a NaN logit gives NaN.  D and I at least 1.
+ * Workspace of f16acc_layer_workspace bytes, 256-byte aligned; it is enough for any smaller T too.
+ */
+size_t f16acc_layer_workspace(int64_t T, int k, int E, int64_t D, int64_t I);
+int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const void* router, int rtype, int64_t re,
+                 int64_t rd, int E, int k, int sigmoid, const float* bias, int groups, int top, int renorm, float scale,
+                 int64_t D, int64_t I, const uint8_t* w1, int64_t w1e, int64_t w1u, int64_t ld1, const float* s1,
+                 int64_t s1e, int64_t s1u, int64_t s1n, int64_t s1k, const uint8_t* w2, int64_t w2e, int64_t ld2,
+                 const float* s2, int64_t s2e, int64_t s2n, int64_t s2k, void* y, void* workspace, size_t ws_bytes,
+                 void* stream);
+
+/*
  * Microscaled 4-bit operands: blocks of 32 values of a row, held as e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
  * their negatives), two a byte, the first in its low half, and a power of two s = 2^e as e8m0 (e + 127; 255: NaN):
  *     m = max(|x|, 2^-100)   2^e <= m / 3.5 < 2^(e + 1)   q = e2m1(x / s), nearest, ties to even
