@@ -45,16 +45,25 @@ int launch_tile(const MxQuantArgs& p, bool wide, hipStream_t stream) {
   return hip_status();
 }
 
-// The tiles: tokens x weight rows.
-using Tile0 = Mx4Cfg<128, 128, 2, 2, 256, 2, 2>;
-using Tile1 = Mx4Cfg<64, 64, 2, 1, 256, 3, 2>;
-using Tile2 = Mx4Cfg<32, 64, 1, 2, 256, 4, 2>;
+// The tiles: tokens x weight rows.  A stage of 256 columns everywhere: rows of whole 128-byte lines (with 128
+// columns a stage and twice the stages in the ring 8192^3 took 7 % longer).
+using Tile0 = Mx4Cfg<256, 256, 4, 2, 256, 2, 2>;
+using Tile1 = Mx4Cfg<128, 256, 2, 4, 256, 3, 2>;
+using Tile2 = Mx4Cfg<128, 128, 2, 2, 256, 2, 2>;
+using Tile3 = Mx4Cfg<64, 128, 2, 2, 256, 3, 2>;
+using Tile4 = Mx4Cfg<64, 64, 2, 1, 256, 3, 2>;
+using Tile5 = Mx4Cfg<32, 64, 1, 2, 256, 4, 2>;
+// What a tile costs, in microseconds, fitted to 2491 timed (shape, tile, split) triples (M 16 .. 8192, N 256 ..
+// 16384, K 1536 .. 12288, weights out of the cache, in a graph): a workgroup alone on its CU takes start + step for
+// each stage, each further one beside it adds `share` of the stages' time; `per_cu` fit.  The picks made
+// with it take 0.1 % longer than the best triple on geometric mean, 3 % at worst.
 struct TileInfo {
   int bm, bn, bk, per_cu;
-  double start, step, share;  // us: a workgroup alone on its CU takes start + step for each stage
+  double start, step, share;
 };
 constexpr TileInfo kTiles[] = {
-    {128, 128, 256, 2, 2.2, 0.60, 0.61}, {64, 64, 256, 3, 1.7, 0.43, 0.33}, {32, 64, 256, 3, 1.3, 0.34, 0.32},
+    {256, 256, 256, 1, 5.98, 1.134, 0.0}, {128, 256, 256, 1, 3.6, 0.82, 0.0},   {128, 128, 256, 2, 1.9, 0.638, 0.62},
+    {64, 128, 256, 2, 2.03, 0.491, 0.46}, {64, 64, 256, 3, 1.97, 0.369, 0.36}, {32, 64, 256, 3, 1.26, 0.349, 0.4},
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -75,11 +84,11 @@ double cost_of(const Plan& plan, int64_t M, int64_t N, int64_t K) {
   const int64_t full = deep / t.per_cu, rest = deep % t.per_cu;
   double us = full * (t.start + t.step * kb * (1 + (t.per_cu - 1) * t.share));
   if (rest) us += t.start + t.step * kb * (1 + (rest - 1) * t.share);
-  const double floor = ((double)N * K + (double)M * K) * 0.09e-6;  // the operands from HBM
+  const double floor = ((double)N * K + (double)M * K) * 0.107e-6;  // the operands from HBM
   if (us < floor) us = floor;
   const double outputs = (double)M * N * 1e-6;
-  if (t.per_cu == 1) us += 0.3 * outputs;  // no other workgroup runs while one stores
-  if (plan.splits > 1) us += 2.1 + 0.25 * plan.splits + 1.36 * plan.splits * outputs;
+  us += 0.33 * outputs;
+  if (plan.splits > 1) us += 2.64 + 0.28 * plan.splits + 1.33 * plan.splits * outputs;
   return us;
 }
 
@@ -128,6 +137,9 @@ int run_product(Mx4Args p, const Plan& plan, void* parts, hipStream_t stream) {
     case 0: rc = launch_mm_fp4<Tile0>(p, stream, plan.splits); break;
     case 1: rc = launch_mm_fp4<Tile1>(p, stream, plan.splits); break;
     case 2: rc = launch_mm_fp4<Tile2>(p, stream, plan.splits); break;
+    case 3: rc = launch_mm_fp4<Tile3>(p, stream, plan.splits); break;
+    case 4: rc = launch_mm_fp4<Tile4>(p, stream, plan.splits); break;
+    case 5: rc = launch_mm_fp4<Tile5>(p, stream, plan.splits); break;
   }
   if (rc || plan.splits == 1) return rc;
   FinishArgs f{p.parts, p.M, p.N, p.scm, p.scn, plan.splits, p.bias, p.c};

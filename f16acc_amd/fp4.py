@@ -54,7 +54,7 @@ def mm(a, a_scale, b, b_scale, out_dtype=torch.float16):
 
 
 def mm_tile(a, a_scale, b, b_scale, out, tile, splits, bias=None):
-    """mm into `out` ([M, N], any strides) with the tile (0 to 2) and the number of parts of K forced, and a bias
+    """mm into `out` ([M, N], any strides) with the tile (0 to 5) and the number of parts of K forced, and a bias
     [N] in out's type: for tuning and tests."""
     return host.fp4_mm(a, a_scale, b, b_scale, out.dtype, bias, out, tile, splits)
 

@@ -195,7 +195,7 @@ int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t*
  *   sx, sw: single bytes, that of (row m, block b) at m * sxm + b * sxb, where sxq is 0; else quads as above,
  *   (row, quad) at m * sxm + quad * sxq, bytes past the last block not 255 (swn, swb, swq alike)
  *   bias: [N] of ctype, or NULL;  c: element strides scm, scn
- *   tile, splits: -1 and 0 leave the choice to the library; a tile number (0 to 2) and a number of parts of K
+ *   tile, splits: -1 and 0 leave the choice to the library; a tile number (0 to 5) and a number of parts of K
  *   force them, for tuning
  *   workspace: f16acc_mm_fp4_workspace bytes for exactly these sizes (single scale bytes in quads, FP32 sums of
  *   the parts of K; may be 0), 256-byte aligned

@@ -53,11 +53,11 @@ def test_mm_checks():
     assert call(ldx=120) == call(ldw=112) == call(x=8) == call(w=264) == _ops.E_UNSUPPORTED
     assert call(K=1 << 24, ldx=1 << 23, ldw=1 << 23) == call(M=1 << 31) == _ops.E_UNSUPPORTED
     assert call(sxq=6) == call(sxq=4, sxm=6) == call(swq=4, sw=258) == call(sxq=4, sxm=1 << 23) == _ops.E_UNSUPPORTED
-    assert call(tile=3) == call(tile=-2) == call(splits=-1) == _ops.E_ARG
+    assert call(tile=6) == call(tile=-2) == call(splits=-1) == _ops.E_ARG
     assert call(ws=None) == call(ws=128) == call(n=need - 1) == _ops.E_WORKSPACE
     assert need >= 2 * 4 * 2 * 4 and _ops.mm_fp4_workspace(4, 4, 256, 4, 4, -1, 0) == 0
     assert _ops.mm_fp4_workspace(4, 4, 1024, 4, 4, 2, 2) >= 2 * 4 * 4 * 4
-    assert call(M=0) == call(N=0) == 0 == _ops.mm_fp4_workspace(0, 4, 4, 0, 0, -1, 0) == _ops.mm_fp4_workspace(4, 4, 4, 0, 0, 3, 0)
+    assert call(M=0) == call(N=0) == 0 == _ops.mm_fp4_workspace(0, 4, 4, 0, 0, -1, 0) == _ops.mm_fp4_workspace(4, 4, 4, 0, 0, 6, 0)
 
 
 def test_linear_checks():

@@ -154,7 +154,7 @@ def test_mm_scales_of_every_size():
     ref.check_product(fp4.mm(a, sa, w.t(), ws.t(), torch.float32), ref.values(a, sa), ref.values(w, ws))
 
 
-@pytest.mark.parametrize("tile,splits", [(t, s) for t in range(3) for s in (1, 3)])
+@pytest.mark.parametrize("tile,splits", [(t, s) for t in range(6) for s in (1, 3)])
 def test_mm_every_tile_and_split(tile, splits):
     """The same product in every tile, whole and in parts of K: sums of few bits, so exact; ragged edges."""
     g = torch.Generator().manual_seed(7)
@@ -226,7 +226,7 @@ def test_mm_offsets_past_32_bits():
     a, sa = stored(300, K, seed=2)
     q[-300:], s[-300:] = u8(a), u8(sa)
     w, ws = stored(N, K)
-    f32 = lambda q, s: fp4.mm_tile(q, s, w.t(), ws.t(), torch.empty(len(q), N, device=DEV), 1, 1)
+    f32 = lambda q, s: fp4.mm_tile(q, s, w.t(), ws.t(), torch.empty(len(q), N, device=DEV), 4, 1)
     c = f32(q.view(F4), s.view(E8))  # (one tile and no split for both: the same sums in the same order)
     assert torch.equal(c[-300:], f32(a, sa)) and bool((c[:-300] == 0).all())
     ref.check_product(c[-20:], ref.values(a[-20:], sa[-20:]), ref.values(w, ws))
@@ -459,13 +459,13 @@ def test_mm_tile_refuses_what_does_not_fit():
     M, N, K = 40, 72, 256
     a, sa = stored(M, K, seed=2)
     w, ws = stored(N, K)
-    f = lambda out, bias=None, tile=1, splits=1: fp4.mm_tile(a, sa, w.t(), ws.t(), out, tile, splits, bias)
+    f = lambda out, bias=None, tile=4, splits=1: fp4.mm_tile(a, sa, w.t(), ws.t(), out, tile, splits, bias)
     out = torch.empty(M, N, device=DEV)
     short, pair = torch.zeros(N - 1, device=DEV), torch.zeros(1, N, device=DEV)
     bad = [lambda: f(torch.empty(M + 1, N, device=DEV)), lambda: f(torch.empty(M, device=DEV)), lambda: f(out.int()),
            lambda: f(out.double()), lambda: f(out.cpu()), lambda: f(out[:1].expand(M, N)), lambda: f(out, short),
            lambda: f(out, pair), lambda: f(out, pair[0].half()), lambda: f(out, pair[0].cpu()),
-           lambda: f(out, tile=3), lambda: f(out, tile=-2), lambda: f(out, splits=-1)]
+           lambda: f(out, tile=6), lambda: f(out, tile=-2), lambda: f(out, splits=-1)]
     for g in bad:
         with pytest.raises(ValueError):
             g()
