@@ -40,6 +40,7 @@ _SIGNATURES = {
     "f16acc_mm_fp8_workspace": [_i64] * 3 + [_int] * 3,
     "f16acc_linear_fp8_workspace": [_i64] * 3 + [_vp, _i64],
     "f16acc_experts_workspace": [_i64, _int, _int, _i64, _i64],
+    "f16acc_layer_any_rows": [_i64, _int, _i64, _i64],
     "f16acc_layer": [_vp, _int] + [_i64] * 3 + [_vp, _int, _i64, _i64] + [_int] * 3 + [_vp] + [_int] * 3 + [_f32]
                     + [_i64] * 2 + [_vp] + [_i64] * 3 + [_vp] + [_i64] * 4 + [_vp] + [_i64] * 2 + [_vp] + [_i64] * 3
                     + [_vp, _vp, _size, _vp],
@@ -68,7 +69,7 @@ def _bind(name):
 
 (quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad, experts_any_rows,
  experts, column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace,
- layer, layer_workspace, fp4_quant, fp4_transpose, fp4_values, mm_fp4, linear_fp4, mm_fp4_workspace, linear_fp4_workspace, strerror,
+ layer_any_rows, layer, layer_workspace, fp4_quant, fp4_transpose, fp4_values, mm_fp4, linear_fp4, mm_fp4_workspace, linear_fp4_workspace, strerror,
  abi_version) = map(_bind, EXPORTS)
 
 if abi_version() != ABI_VERSION:

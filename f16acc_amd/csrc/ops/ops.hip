@@ -375,19 +375,34 @@ struct LaunchRouteGrad {
   }
 };
 
-// The router's product: bytes of a row step as the loads of eight elements need them.
+// The router's product.  wide: rows of both as the loads of eight elements need them.
 template <class T, class R>
-int launch_router(RouterArgs p, hipStream_t stream) {
+void router_wide(RouterArgs& p) {
   p.wide = p.sc == 1 && p.rd == 1 && aligned16(p.x) && aligned16(p.r) && p.sr * (int64_t)sizeof(T) % 16 == 0 &&
            p.re * (int64_t)sizeof(R) % 16 == 0;
+}
+template <class T, class R>
+int launch_router(RouterArgs p, hipStream_t stream) {
+  router_wide<T, R>(p);
   const dim3 grid((uint32_t)cdiv(p.T, 16), (uint32_t)cdiv(p.E, 16));
   hipLaunchKernelGGL((router_kernel<T, R, 8>), grid, dim3(512), 0, stream, p);
   return hip_status();
 }
 
-// Where a layer's logits, weights and ids lie in its workspace, before the experts' own.
+template <class T, int V>
+struct LaunchLayer {
+  static int go(LayerArgs a, hipStream_t s) {
+    a.route = route_args<float, V>(a.route);
+    const int64_t grid = a.e.slots * (int64_t)a.pieces + cdiv(a.e.D, 16);
+    hipLaunchKernelGGL((layer_few_kernel<V>), dim3((uint32_t)grid), dim3(64 * LayerFew::W), 0, s, a);
+    return hip_status();
+  }
+};
+
+// Where a layer's values lie in its workspace, and its size, which is enough for any smaller T as well: logits,
+// weights and ids before the experts' own; or logits, quantised tokens, hidden values and counters of a few tokens.
 struct LayerPlan {
-  size_t logits, weights, ids, experts, total;
+  size_t logits, weights, ids, experts, xq, xs, h, sync, claims, total;
   LayerPlan(int64_t T, int k, int E, int64_t D, int64_t I) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -400,6 +415,16 @@ struct LayerPlan {
     ids = take(T * k * 4);
     experts = at;
     total = at + ExpertsPlan(T, k, E, D, I).total;
+    if (few_tokens(1, k)) {
+      const int64_t most = kFewSlots / k < kFewTokens ? kFewSlots / k : kFewTokens, t = T < most ? T : most;
+      at = up256(t * E * 4);
+      xq = take(t * up128(D));
+      xs = take(t * (up128(D) / kBlock) * 4);
+      h = take(t * k * up128(I) * 4);
+      sync = take(sizeof(LayerSync));
+      claims = take(t * k * cdiv(I, 16) * sizeof(Claim));
+      if (total < at) total = at;
+    }
   }
 };
 
@@ -699,6 +724,10 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
   });
 }
 
+int f16acc_layer_any_rows(int64_t T, int k, int64_t D, int64_t I) {
+  return T > 0 && k > 0 && few_tokens(T, k) && D >= 16 && I >= 16;
+}
+
 size_t f16acc_layer_workspace(int64_t T, int k, int E, int64_t D, int64_t I) {
   if (T <= 0 || k <= 0 || E <= 0 || D <= 0 || I <= 0) return 0;
   return LayerPlan(T, k, E, D, I).total;
@@ -711,7 +740,7 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
                  const float* s2, int64_t s2e, int64_t s2n, int64_t s2k, void* y, void* workspace, size_t ws_bytes,
                  void* stream_) {
   const ExpertWeights w{w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2, w2e, ld2, s2, s2e, s2n, s2k};
-  const bool few = f16acc_experts_any_rows(x, type, T, sr, sc, k);
+  const bool few = f16acc_layer_any_rows(T, k, D, I);
   int rc = experts_check(x, type, T, k, E, D, I, w, y, few);
   if (!rc) rc = quant_check(router, rtype, E, D);
   if (rc || T == 0) return rc;
@@ -725,6 +754,28 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
   float *logits = (float*)(ws + plan.logits), *weights = (float*)(ws + plan.weights);
   int* ids = (int*)(ws + plan.ids);
   const RouterArgs r{x, T, sr, sc, router, re, rd, E, D, false, logits};
+  a.x = logits, a.weights = weights, a.ids = ids;
+  if (few) {
+    const int64_t Dp = up128(D), Ip = up128(I);
+    LayerArgs l{};
+    l.router = r, l.route = a, l.ytype = type, l.sync = (LayerSync*)(ws + plan.sync);
+    l.pieces = (int)cdiv(I, 16), l.claims = (Claim*)(ws + plan.claims);
+    l.quant = QuantArgs{x, T, D, sr, sc, (uint8_t*)(ws + plan.xq), Dp, (float*)(ws + plan.xs), T, nullptr, 0, nullptr, 0};
+    l.e = FewArgs{x,   sr,  (int)T, k,   E,   (int)(T * k), nullptr, nullptr, 0,   0,   D,   I, w1,          w1e, w1u,
+                  ld1, s1,  s1e,    s1u, s1n, s1k,          w2,      w2e,     ld2, s2,  s2e, s2n, s2k, (float*)(ws + plan.h), Ip,
+                  nullptr, y};
+    rc = by_type(type, [&](auto* t) {
+      using X = std::remove_pointer_t<decltype(t)>;
+      return by_type(rtype, [&](auto* u) {
+        using R = std::remove_pointer_t<decltype(u)>;
+        router_wide<X, R>(l.router);
+        const uint32_t grid = (uint32_t)(E + cdiv(T * (Dp / kBlock), 16));
+        hipLaunchKernelGGL((layer_router_kernel<X, R>), dim3(grid), dim3(256), 0, (hipStream_t)stream_, l);
+        return hip_status();
+      });
+    });
+    return rc ? rc : by_experts<LaunchLayer>(E, F16ACC_TYPE_F32, l, (hipStream_t)stream_);
+  }
   rc = by_type(type, [&](auto* t) {
     using X = std::remove_pointer_t<decltype(t)>;
     return by_type(rtype, [&](auto* u) {
@@ -733,7 +784,6 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
     });
   });
   if (rc) return rc;
-  a.x = logits, a.weights = weights, a.ids = ids;
   rc = by_experts<LaunchRoute>(E, F16ACC_TYPE_F32, a, (hipStream_t)stream_);
   if (rc) return rc;
   return f16acc_experts(x, type, T, sr, sc, weights, k, 1, ids, k, E, D, I, w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2,

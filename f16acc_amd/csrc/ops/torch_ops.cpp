@@ -407,10 +407,9 @@ void check_no_grad(const char* name, std::initializer_list<const Tensor*> tensor
 struct ExpertRows {
   Operand w1, w2;
   int64_t part;
-  ExpertRows(const Tensor& x2, int64_t k, const Tensor& q1, const Tensor& q2) {
-    const int64_t T = x2.size(0), D = q1.size(3), I = q1.size(2);
-    // for a few tokens rows of any alignment go as they are
-    const bool any = f16acc_experts_any_rows(x2.const_data_ptr(), type_of(x2), T, x2.stride(0), x2.stride(1), (int)k);
+  // any: rows of any alignment go as they are
+  ExpertRows(int64_t T, int64_t k, const Tensor& q1, const Tensor& q2, bool any) {
+    const int64_t D = q1.size(3), I = q1.size(2);
     auto rows = [&](const Tensor& w) {
       return any && (w.size(-1) <= 1 || w.stride(-1) == 1) ? Operand{w, w.stride(-2)} : packed(w);
     };
@@ -442,7 +441,8 @@ Tensor experts(const Tensor& x, const Tensor& weights, const Tensor& ids, const 
   Tensor i32 = rows_of(ids);
   if (i32.scalar_type() == at::kLong) i32 = i32.clamp(-1, E).to(at::kInt);  // (a cast alone would wrap)
   i32 = i32.contiguous();
-  const ExpertRows p(x2, k, w1, w2);
+  const ExpertRows p(T, k, w1, w2,
+                     f16acc_experts_any_rows(x2.const_data_ptr(), type_of(x), T, x2.stride(0), x2.stride(1), (int)k));
   const size_t n = f16acc_experts_workspace(p.part, (int)k, (int)E, D, I);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);
@@ -477,7 +477,7 @@ Tensor layer(const Tensor& x, const Tensor& router, int64_t k, const Tensor& w1,
   const int64_t T = x2.size(0);
   Tensor y = empty(x.sizes(), x, x.scalar_type());
   if (T == 0) return y;
-  const ExpertRows p(x2, k, w1, w2);
+  const ExpertRows p(T, k, w1, w2, f16acc_layer_any_rows(T, (int)k, D, I));
   const size_t n = f16acc_layer_workspace(p.part, (int)k, (int)E, D, I);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);

@@ -151,9 +151,10 @@ int f16acc_experts(const void* x, int type, int64_t T, int64_t sr, int64_t sc, c
 /*
  * A whole layer: logits = x router^T (router [E, D] of rtype, element strides re, rd), summed in 64 bits and rounded
  * once to FP32; weights and ids of f16acc_route of them; y of f16acc_experts, whose rows and
- * alignments apply (f16acc_experts_any_rows for x and k).  A token with a NaN logit gives NaN.  D and I at least 1.
+ * alignments of the weights apply (where f16acc_layer_any_rows says 1, any).  A token with a NaN logit gives NaN.  D and I at least 1.
  * Workspace of f16acc_layer_workspace bytes, 256-byte aligned; it is enough for any smaller T too.
  */
+int f16acc_layer_any_rows(int64_t T, int k, int64_t D, int64_t I);
 size_t f16acc_layer_workspace(int64_t T, int k, int E, int64_t D, int64_t I);
 int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, const void* router, int rtype, int64_t re,
                  int64_t rd, int E, int k, int sigmoid, const float* bias, int groups, int top, int renorm, float scale,
