@@ -45,16 +45,25 @@ _SIGNATURES = {
                     + [_i64] * 2 + [_vp] + [_i64] * 3 + [_vp] + [_i64] * 4 + [_vp] + [_i64] * 2 + [_vp] + [_i64] * 3
                     + [_vp, _vp, _size, _vp],
     "f16acc_layer_workspace": [_i64, _int, _int, _i64, _i64],
-    "f16acc_fp4_quant": [_vp, _int] + [_i64] * 4 + [_vp, _i64, _vp, _i64, _i64] * 2 + [_vp],
+    "f16acc_fp4_quant": [_vp, _vp, _int, _vp],
     "f16acc_fp4_transpose": [_vp, _i64, _i64] * 2 + [_i64] * 2 + [_vp, _i64, _vp, _i64, _i64, _vp],
     "f16acc_fp4_values": [_vp, _i64, _i64] * 2 + [_i64] * 2 + [_vp, _int, _vp],
-    "f16acc_mm_fp4": ([_vp, _i64, _vp] + [_i64] * 3) * 2 + [_vp, _vp] + [_i64] * 5 + [_int] * 3 + [_vp, _size, _vp],
+    "f16acc_mm_fp4": ([_vp, _i64, _i64, _vp] + [_i64] * 3) * 2 + [_vp, _vp] + [_i64] * 5 + [_int] * 3 + [_vp, _size, _vp],
     "f16acc_linear_fp4": [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_vp, _size, _vp],
-    "f16acc_mm_fp4_workspace": [_i64] * 5 + [_int] * 2,
+    "f16acc_mm_fp4_workspace": [_vp, _i64, _i64, _i64] * 2 + [_i64] * 3 + [_int] * 2,
     "f16acc_linear_fp4_workspace": [_i64] * 3 + [_vp, _i64],
     "f16acc_ops_strerror": [_int],
     "f16acc_ops_abi_version": [],
 }
+
+
+class Fp4Matrix(ctypes.Structure):
+    """f16acc_fp4_matrix."""
+    _fields_ = [("x", _vp), ("rows", _i64), ("cols", _i64), ("sr", _i64), ("sc", _i64), ("q", _vp), ("ldq", _i64), ("s", _vp),
+                ("s_row", _i64), ("s_quad", _i64), ("qt", _vp), ("ldqt", _i64), ("st", _vp), ("st_row", _i64),
+                ("st_quad", _i64)]
+
+
 EXPORTS = tuple(_SIGNATURES)  # the symbols include/f16acc_ops.h declares
 ABI_VERSION = 1
 E_ARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3

@@ -41,6 +41,15 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t q, uint32_t e, float (&v)[8
     v[i] = e == 255u ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(t[i], (int)e - 127);
 }
 
+// Eight consecutive elements from any address (a 16-byte load goes from any).
+template <class T>
+__device__ __forceinline__ void load_any(const T* p, float (&v)[8]) {
+  T t[8];
+  __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+}
+
 // Scale bytes: that of (row, block b) at s[row * row_stride + b / 4 * quad_stride + b % 4], both strides
 // multiples of 4.  [rows][quads] has (4 quads, 4), [quads][rows] (4, 4 rows).
 struct MxScales {
@@ -74,19 +83,26 @@ __device__ __forceinline__ uint32_t quad_bytes(uint32_t byte, int lane) {
   return v | dpp<0x128>(v);
 }
 
-// One row of a matrix in blocks of 1 x 32.  16 lanes take 128 values, 8 each: a 16-byte load
-// a lane (16-bit types), the maximum of four lanes by two exchanges, 4 bytes a lane out.
+// Rows of a matrix in blocks of 1 x 32.  16 lanes take 128 values of a row, 8 each: a 16-byte load a lane (16-bit
+// types), the maximum of four lanes by two exchanges, 4 bytes a lane out.  A workgroup takes 16 quads of a
+// row where a row's scales lie together, 16 rows of a quad where a quad's do: its scales are one piece
+// of 64 bytes either way.
 template <class T, bool WIDE>
 __device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t group, uint32_t groups) {
-  const int64_t quads = cdiv(p.cols, kQuad), total = p.rows * quads;
-  const int lane = threadIdx.x & 15;
-  for (int64_t b = (int64_t)group * 16 + (threadIdx.x >> 4); b < total; b += (int64_t)groups * 16) {
-    const int64_t row = total >> 32 ? b / quads : (int64_t)((uint32_t)b / (uint32_t)quads), kq = b - row * quads;
+  const bool along = p.s.quad == 4;
+  const int64_t quads = cdiv(p.cols, kQuad), total = along ? cdiv(p.rows * quads, 16) : cdiv(p.rows, 16) * quads;
+  const int lane = threadIdx.x & 15, which = threadIdx.x >> 4;
+  for (int64_t b = group; b < total; b += groups) {
+    const int64_t i = along ? b * 16 + which : b;
+    int64_t row = p.rows * quads >> 32 ? i / quads : (int64_t)((uint32_t)i / (uint32_t)quads);
+    const int64_t kq = i - row * quads;
+    if (!along) row = row * 16 + which;
+    if (row >= p.rows) continue;
     const int64_t c0 = kq * kQuad + lane * 8;
     const T* x = (const T*)p.x + row * p.sr;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (WIDE && c0 + 8 <= p.cols) {
-      load_vec(x + c0, v);
+      load_any(x + c0, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -97,7 +113,7 @@ __device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t gro
     for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
     m = quad_umax(m);
     *(uint32_t*)(p.q + row * p.ldq + c0 / 2) = pack_e2m1(v, mx_exponent(m));
-    // (a block past the columns holds zeros: its byte is that of 2^-102 or 0, never NaN's)
+    // (a block past the columns holds zeros: its byte is that of 2^-102, never NaN's)
     const uint32_t scales = quad_bytes(mx_byte(m), lane);
     if (lane == 0) *(uint32_t*)(p.s.s + row * p.s.row + kq * p.s.quad) = scales;
   }
@@ -110,10 +126,15 @@ struct MxScaleArgs {
   uint32_t* dst;  // [quads][ld]
   int64_t ld;
 };
+// 16 rows by 16 quads a workgroup: pieces of 64 bytes on both sides.
+__host__ __device__ inline int64_t mx_scales_tiles(const MxScaleArgs& p) {
+  return cdiv(p.rows, 16) * cdiv(p.blocks, 64);
+}
 __device__ __forceinline__ void mx_scales(const MxScaleArgs& p, uint32_t group, uint32_t groups) {
-  const int64_t quads = cdiv(p.blocks, 4), total = p.rows * quads;
-  for (int64_t i = (int64_t)group * 256 + threadIdx.x; i < total; i += (int64_t)groups * 256) {
-    const int64_t r = total >> 32 ? i / quads : (int64_t)((uint32_t)i / (uint32_t)quads), kq = i - r * quads;
+  const int64_t tiles_q = cdiv(p.blocks, 64), tiles = mx_scales_tiles(p);
+  for (int64_t i = group; i < tiles; i += groups) {
+    const int64_t rb = i / tiles_q, r = rb * 16 + (threadIdx.x >> 4), kq = (i - rb * tiles_q) * 16 + (threadIdx.x & 15);
+    if (r >= p.rows || 4 * kq >= p.blocks) continue;
     const uint8_t* s = p.src + r * p.s_r + 4 * kq * p.s_b;
     uint32_t v = 0;
     if (p.s_b == 1 && 4 * kq + 4 <= p.blocks) {
@@ -126,11 +147,18 @@ __device__ __forceinline__ void mx_scales(const MxScaleArgs& p, uint32_t group, 
     p.dst[kq * p.ld + r] = v;
   }
 }
-__global__ __launch_bounds__(256) void mx_scales_kernel(MxScaleArgs a, MxScaleArgs b, uint32_t first) {
-  if (blockIdx.x < first)
-    mx_scales(a, blockIdx.x, first);
-  else
-    mx_scales(b, blockIdx.x - first, gridDim.x - first);
+
+// What a product needs before it: the rows of two operands copied to an alignment, their scales in its
+// order (any of it may be none).
+__global__ __launch_bounds__(256) void mx_pack_kernel(Pack8Args x, Pack8Args w, MxScaleArgs a, MxScaleArgs b,
+                                                      uint32_t nx, uint32_t nw, uint32_t na) {
+  uint32_t group = blockIdx.x;
+  if (group < nx) return pack8(x, group, nx);
+  group -= nx;
+  if (group < nw) return pack8(w, group, nw);
+  group -= nw;
+  if (group < na) return mx_scales(a, group, na);
+  mx_scales(b, group - na, gridDim.x - nx - nw - na);
 }
 
 // Tokens quantised, beside a weight's scales reordered and its rows copied to an alignment (either
@@ -167,7 +195,7 @@ __device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t
   } else {
     const T* x = (const T*)p.x + r * p.sr;
     if (WIDE && c + 8 <= p.cols) {
-      load_vec(x + c, v);
+      load_any(x + c, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -176,20 +204,21 @@ __device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t
   }
 }
 
-// A 128 x 128 tile a workgroup, read once: quantised along its rows (ROWS) and its columns (the
-// result transposed).  Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's block is four
+// A 128 x 128 tile a workgroup, read once: quantised along its rows (q), its columns (qt, the
+// result transposed) or both.  Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's block is four
 // lanes, a column's block one wave's 32 rows, four DPP rows apart, so no maximum leaves a wave.
-template <class T, bool WIDE, bool ROWS>
-__global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs p) {
+template <class T, bool WIDE>
+__device__ __forceinline__ void mx_quant_tile(const MxQuantArgs& p, uint32_t index) {
   // The transposed tile, 64 bytes a column: 16-byte unit u (a wave's rows) of column col at u ^ (col / 8 % 4).
   __shared__ __align__(16) uint8_t tile[kQuad * 64];
-  __shared__ uint8_t bytes[kQuad * 4];
+  __shared__ __align__(4) uint8_t bytes[kQuad * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 4, c = tid & 15;
-  const int64_t kb = blockIdx.x, rb = blockIdx.y, r0 = rb * kQuad + r * 8, c0 = kb * kQuad + c * 8;
+  const uint32_t tiles_k = (uint32_t)cdiv(p.cols, kQuad);
+  const int64_t rb = index / tiles_k, kb = index - rb * tiles_k, r0 = rb * kQuad + r * 8, c0 = kb * kQuad + c * 8;
   float v[8][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) mx_load<T, WIDE>(p, r0 + i, c0, v[i]);
-  if (ROWS) {
+  if (p.q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t m = abs_bits(v[i][0]);
@@ -203,6 +232,7 @@ __global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs p) {
       }
     }
   }
+  if (!p.qt) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float col[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
@@ -224,6 +254,13 @@ __global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs p) {
   }
   if (tid < kQuad && kb * kQuad + tid < p.cols)
     *(uint32_t*)(p.st.s + (kb * kQuad + tid) * p.st.row + rb * p.st.quad) = *(const uint32_t*)(bytes + tid * 4);
+}
+
+// One matrix or two: the first `first` workgroups have a's tiles.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs a, MxQuantArgs b, uint32_t first) {
+  const bool is_a = blockIdx.x < first;
+  mx_quant_tile<T, WIDE>(is_a ? a : b, is_a ? blockIdx.x : blockIdx.x - first);
 }
 
 // The values of a 4-bit matrix, eight a thread.

@@ -7,6 +7,8 @@
 #include "fp4_small.h"
 #include "launch.h"
 
+#include <utility>
+
 using namespace f16ops;
 
 namespace {
@@ -16,6 +18,13 @@ int64_t quads_of(int64_t v) { return cdiv(v, kQuad); }
 uint32_t grid_of(int64_t units, int64_t per_group) {
   const int64_t groups = cdiv(units, per_group);
   return (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus);
+}
+
+int64_t tiles_of(const MxQuantArgs& p) { return quads_of(p.rows) * quads_of(p.cols); }
+
+uint32_t quant_grid(const MxQuantArgs& p) {
+  const int64_t quads = quads_of(p.cols);
+  return p.s.quad == 4 ? grid_of(p.rows * quads, 16) : grid_of(cdiv(p.rows, 16) * quads, 1);
 }
 
 int scales_check(const MxScales& s) {
@@ -29,19 +38,33 @@ int out4_check(const uint8_t* q, int64_t ldq, int64_t cols, const MxScales& s) {
   return scales_check(s);
 }
 
+int matrix_check(const MxQuantArgs& p, int type) {
+  int rc = quant_check(p.x, type, p.rows, p.cols);
+  if (rc || p.rows == 0 || p.cols == 0) return rc;
+  if (!p.q && !p.qt) return F16ACC_OPS_E_ARG;
+  if (p.q && (rc = out4_check(p.q, p.ldq, p.cols, p.s))) return rc;
+  if (p.qt && (rc = out4_check(p.qt, p.ldqt, p.rows, p.st))) return rc;
+  return tiles_of(p) > 0x3fffffff ? F16ACC_OPS_E_UNSUPPORTED : 0;
+}
+
+// a and b (rows 0: none), whose tiles are wanted transposed.
 template <class T>
-int launch_tile(const MxQuantArgs& p, bool wide, hipStream_t stream) {
-  const int64_t gx = quads_of(p.cols), gy = quads_of(p.rows);
-  if (gx > 0x7fffffff || gy > 65535) return F16ACC_OPS_E_UNSUPPORTED;
-  const dim3 grid((uint32_t)gx, (uint32_t)gy);
-  if (p.q && wide)
-    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true, true>), grid, dim3(256), 0, stream, p);
-  else if (p.q)
-    hipLaunchKernelGGL((mx_quant_tile_kernel<T, false, true>), grid, dim3(256), 0, stream, p);
-  else if (wide)
-    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true, false>), grid, dim3(256), 0, stream, p);
+int launch_tile(const MxQuantArgs& a, const MxQuantArgs& b, hipStream_t stream) {
+  const uint32_t first = (uint32_t)tiles_of(a), all = first + (uint32_t)tiles_of(b);
+  if (std::is_same_v<T, Fp4Source> || (a.sc == 1 && (b.sc == 1 || !b.rows)))
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true>), dim3(all), dim3(256), 0, stream, a, b, first);
   else
-    hipLaunchKernelGGL((mx_quant_tile_kernel<T, false, false>), grid, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, false>), dim3(all), dim3(256), 0, stream, a, b, first);
+  return hip_status();
+}
+
+template <class T>
+int launch_rows(const MxQuantArgs& p, hipStream_t stream) {
+  const dim3 grid(quant_grid(p));
+  if (p.sc == 1)
+    hipLaunchKernelGGL((mx_prepare_kernel<T, true>), grid, dim3(256), 0, stream, p, MxScaleArgs{}, Pack8Args{}, 0u, 0u);
+  else
+    hipLaunchKernelGGL((mx_prepare_kernel<T, false>), grid, dim3(256), 0, stream, p, MxScaleArgs{}, Pack8Args{}, 0u, 0u);
   return hip_status();
 }
 
@@ -117,18 +140,6 @@ size_t parts_bytes(const Plan& plan, int64_t M, int64_t N) {
   return plan.splits > 1 ? up256((size_t)plan.splits * M * N * 4) : 0;
 }
 
-int product_check(const Mx4Args& p) {
-  if (p.M < 0 || p.N < 0 || p.K < 0 || p.ctype < 0 || p.ctype > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
-  if (p.M == 0 || p.N == 0) return 0;
-  if (p.K == 0 || !p.c || !p.x || !p.w || !p.sx || !p.sw) return F16ACC_OPS_E_ARG;
-  const int64_t bytes = cdiv(p.K, 2);
-  if (p.ldx % 16 || p.ldw % 16 || p.ldx < bytes || p.ldw < bytes || p.ldx > kMaxRow || p.ldw > kMaxRow ||
-      !aligned16(p.x) || !aligned16(p.w))
-    return F16ACC_OPS_E_UNSUPPORTED;
-  if (p.M > 0x7fffffff || p.N > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
-  return 0;
-}
-
 int run_product(Mx4Args p, const Plan& plan, void* parts, hipStream_t stream) {
   p.ksplit = plan.ksplit;
   p.parts = (float*)parts;
@@ -155,14 +166,32 @@ int run_product(Mx4Args p, const Plan& plan, void* parts, hipStream_t stream) {
 // Scales of the products' own order: the dword of (row, quad) at (quad * rows + row) * 4.
 size_t scale_bytes(int64_t rows, int64_t K) { return up256(quads_of(K) * rows * 4); }
 
+// An operand as a caller has it: bytes of strides (r, c), scales of strides (sr, sb) or, with sq, quads.
+struct Stored4 {
+  const uint8_t* q;
+  int64_t r, c;
+  const uint8_t* s;
+  int64_t sr, sb, sq;
+  int64_t rows;
+  bool as_it_is(int64_t K) const {
+    return (c == 1 || K <= 2) && aligned16(q) && (rows == 1 || (r % 16 == 0 && r >= cdiv(K, 2) && r <= kMaxRow)) &&
+           (K % kMx == 0 || sq);
+  }
+};
+
+// The workspace of a product: rows that have to be copied, single scale bytes in quads, the parts of a split of K.
 struct MmPlan4 {
   Plan plan;
-  size_t sw, parts, total;
-  MmPlan4(int64_t M, int64_t N, int64_t K, int64_t sxq, int64_t swq, int tile, int splits) {
-    plan = plan_of(M, N, K, tile, splits);
-    sw = sxq ? 0 : scale_bytes(M, K);
-    parts = sw + (swq ? 0 : scale_bytes(N, K));
-    total = parts + parts_bytes(plan, M, N);
+  int64_t ld;
+  size_t w, sx, sw, parts, total;
+  MmPlan4(const Stored4& x, const Stored4& wt, int64_t K, int tile, int splits) {
+    plan = plan_of(x.rows, wt.rows, K, tile, splits);
+    ld = cdiv(K, kMx) * 16;
+    w = x.as_it_is(K) ? 0 : up256(x.rows * ld);
+    sx = w + (wt.as_it_is(K) ? 0 : up256(wt.rows * ld));
+    sw = sx + (x.sq ? 0 : scale_bytes(x.rows, K));
+    parts = sw + (wt.sq ? 0 : scale_bytes(wt.rows, K));
+    total = parts + parts_bytes(plan, x.rows, wt.rows);
   }
 };
 
@@ -191,44 +220,40 @@ struct LinearPlan4 {
 
 extern "C" {
 
-int f16acc_fp4_quant(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
-                     int64_t ldq, uint8_t* s, int64_t s_row, int64_t s_quad, uint8_t* qt, int64_t ldqt, uint8_t* st,
-                     int64_t st_row, int64_t st_quad, void* stream) {
-  int rc = quant_check(x, type, rows, cols);
-  if (rc || rows == 0 || cols == 0) return rc;
-  if (!q && !qt) return F16ACC_OPS_E_ARG;
-  MxQuantArgs p{x, rows, cols, sr, sc, q, ldq, {s, s_row, s_quad}, qt, ldqt, {st, st_row, st_quad}, nullptr, 0, 0};
-  if (q && (rc = out4_check(q, ldq, cols, p.s))) return rc;
-  if (qt && (rc = out4_check(qt, ldqt, rows, p.st))) return rc;
-  const bool wide = wide_loads(x, type, sr, sc);
+int f16acc_fp4_quant(const f16acc_fp4_matrix* a, const f16acc_fp4_matrix* b, int type, void* stream_) {
+  if (!a) return F16ACC_OPS_E_ARG;
+  MxQuantArgs m[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const f16acc_fp4_matrix* f = i ? b : a;
+    if (!f) continue;
+    m[i] = {f->x, f->rows, f->cols, f->sr, f->sc, f->q, f->ldq, {f->s, f->s_row, f->s_quad}, f->qt, f->ldqt,
+            {f->st, f->st_row, f->st_quad}, nullptr, 0, 0};
+    const int rc = matrix_check(m[i], type);
+    if (rc) return rc;
+    if (f->rows == 0 || f->cols == 0) m[i].rows = 0;
+  }
+  hipStream_t stream = (hipStream_t)stream_;
+  if (!m[0].rows) std::swap(m[0], m[1]);
+  if (!m[0].rows) return 0;
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (qt) return launch_tile<T>(p, wide, (hipStream_t)stream);
-    const Pack8Args none{};
-    const uint32_t grid = grid_of(rows * quads_of(cols), 16);
-    if (wide)
-      hipLaunchKernelGGL((mx_prepare_kernel<T, true>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p, MxScaleArgs{},
-                         none, 0u, 0u);
-    else
-      hipLaunchKernelGGL((mx_prepare_kernel<T, false>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p,
-                         MxScaleArgs{}, none, 0u, 0u);
-    return hip_status();
+    if (m[0].qt && (m[1].qt || !m[1].rows)) return launch_tile<T>(m[0], m[1], stream);
+    for (const MxQuantArgs& p : m) {
+      const int rc = !p.rows ? 0 : p.qt ? launch_tile<T>(p, MxQuantArgs{}, stream) : launch_rows<T>(p, stream);
+      if (rc) return rc;
+    }
+    return 0;
   });
 }
 
 int f16acc_fp4_transpose(const uint8_t* x, int64_t sr, int64_t sc, const uint8_t* s, int64_t s_r, int64_t s_b,
                          int64_t rows, int64_t cols, uint8_t* qt, int64_t ldqt, uint8_t* st, int64_t st_row,
                          int64_t st_quad, void* stream) {
-  int rc = quant_check(x, 0, rows, cols);
+  if (rows > 0 && cols > 0 && !s) return F16ACC_OPS_E_ARG;
+  const MxQuantArgs p{x, rows, cols, sr, sc, nullptr, 0, {nullptr, 0, 0}, qt, ldqt, {st, st_row, st_quad}, s, s_r, s_b};
+  const int rc = matrix_check(p, 0);
   if (rc || rows == 0 || cols == 0) return rc;
-  if (!s || !qt) return F16ACC_OPS_E_ARG;
-  MxQuantArgs p{x, rows, cols, sr, sc, nullptr, 0, {nullptr, 0, 0}, qt, ldqt, {st, st_row, st_quad}, s, s_r, s_b};
-  if ((rc = out4_check(qt, ldqt, rows, p.st))) return rc;
-  const int64_t gx = quads_of(cols), gy = quads_of(rows);
-  if (gx > 0x7fffffff || gy > 65535) return F16ACC_OPS_E_UNSUPPORTED;
-  hipLaunchKernelGGL((mx_quant_tile_kernel<Fp4Source, false, false>), dim3((uint32_t)gx, (uint32_t)gy), dim3(256), 0,
-                     (hipStream_t)stream, p);
-  return hip_status();
+  return launch_tile<Fp4Source>(p, MxQuantArgs{}, (hipStream_t)stream);
 }
 
 int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t* s, int64_t s_r, int64_t s_b,
@@ -246,34 +271,57 @@ int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t*
   });
 }
 
-size_t f16acc_mm_fp4_workspace(int64_t M, int64_t N, int64_t K, int64_t sxq, int64_t swq, int tile, int splits) {
+size_t f16acc_mm_fp4_workspace(const uint8_t* x, int64_t xr, int64_t xc, int64_t sxq, const uint8_t* w, int64_t wr,
+                               int64_t wc, int64_t swq, int64_t M, int64_t N, int64_t K, int tile, int splits) {
   if (M <= 0 || N <= 0 || K <= 0 || tile < -1 || tile >= kNumTiles || splits < 0) return 0;
-  return MmPlan4(M, N, K, sxq, swq, tile, splits).total;
+  return MmPlan4({x, xr, xc, nullptr, 0, 0, sxq, M}, {w, wr, wc, nullptr, 0, 0, swq, N}, K, tile, splits).total;
 }
 
-int f16acc_mm_fp4(const uint8_t* x, int64_t ldx, const uint8_t* sx, int64_t sxm, int64_t sxb, int64_t sxq,
-                  const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t swn, int64_t swb, int64_t swq,
+int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, int64_t sxm, int64_t sxb, int64_t sxq,
+                  const uint8_t* w, int64_t wr, int64_t wc, const uint8_t* sw, int64_t swn, int64_t swb, int64_t swq,
                   const void* bias, void* c, int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype,
                   int tile, int splits, void* workspace, size_t ws_bytes, void* stream_) {
   if (tile < -1 || tile >= kNumTiles || splits < 0) return F16ACC_OPS_E_ARG;
-  Mx4Args p{x, ldx, sx, sxm, sxq, w, ldw, sw, swn, swq, bias, c, scm, scn, M, N, K, ctype, 0, nullptr};
-  int rc = product_check(p);
-  if (rc || M == 0 || N == 0) return rc;
-  if (sxm < 0 || sxb < 0 || sxq < 0 || swn < 0 || swb < 0 || swq < 0) return F16ACC_OPS_E_ARG;
-  // scales read where they are
-  for (const auto& [s, row, quad] : {MxScales{(uint8_t*)sx, sxm, sxq}, MxScales{(uint8_t*)sw, swn, swq}})
-    if (quad && ((rc = scales_check({s, row, quad})) || row > kMaxRow)) return rc ? rc : F16ACC_OPS_E_UNSUPPORTED;
-  const MmPlan4 plan(M, N, K, sxq, swq, tile, splits);
+  if (M < 0 || N < 0 || K < 0 || ctype < 0 || ctype > F16ACC_TYPE_F32) return F16ACC_OPS_E_ARG;
+  if (M == 0 || N == 0) return 0;
+  if (K == 0 || !c) return F16ACC_OPS_E_ARG;
+  const int64_t blocks = cdiv(K, kMx), bytes = cdiv(K, 2), ld = blocks * 16;
+  if (ld > kMaxRow || M > 0x7fffffff || N > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
+  const Stored4 in[2] = {{x, xr, xc, sx, sxm, sxb, sxq, M}, {w, wr, wc, sw, swn, swb, swq, N}};
+  int rc = 0;
+  for (const Stored4& o : in) {
+    if (!o.q || !o.s || o.r < 0 || o.c < 0 || o.sr < 0 || o.sb < 0 || o.sq < 0) return F16ACC_OPS_E_ARG;
+    if (o.sq && ((rc = scales_check({(uint8_t*)o.s, o.sr, o.sq})) || o.sr > kMaxRow || !o.as_it_is(K)))
+      return rc ? rc : F16ACC_OPS_E_UNSUPPORTED;
+  }
+  const MmPlan4 plan(in[0], in[1], K, tile, splits);
   if (plan.total && (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total)) return F16ACC_OPS_E_WORKSPACE;
   char* ws = (char*)workspace;
   hipStream_t stream = (hipStream_t)stream_;
-  const int64_t blocks = cdiv(K, kMx), quads = quads_of(K);
-  MxScaleArgs a{}, b{};
-  if (!sxq) a = {sx, M, blocks, sxm, sxb, (uint32_t*)ws, M}, p.sx = (uint8_t*)ws, p.sxm = 4, p.sxq = 4 * M;
-  if (!swq) b = {sw, N, blocks, swn, swb, (uint32_t*)(ws + plan.sw), N}, p.sw = (uint8_t*)ws + plan.sw, p.swm = 4, p.swq = 4 * N;
-  if (!sxq || !swq) {
-    const uint32_t ga = sxq ? 0 : grid_of(M * quads, 256), gb = swq ? 0 : grid_of(N * quads, 256);
-    hipLaunchKernelGGL(mx_scales_kernel, dim3(ga + gb), dim3(256), 0, stream, a, b, ga);
+  Mx4Args p{x, xr, sx, sxm, sxq, w, wr, sw, swn, swq, bias, c, scm, scn, M, N, K, ctype, 0, nullptr};
+  Pack8Args pack[2] = {};
+  MxScaleArgs scales[2] = {};
+  uint32_t np[2] = {}, ns[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const Stored4& o = in[i];
+    if (!o.as_it_is(K)) {
+      uint8_t* to = (uint8_t*)ws + (i ? plan.w : 0);
+      pack[i] = {o.q, to, o.rows, bytes, o.r, o.c, ld};
+      np[i] = grid_of(o.rows * (ld / 16), 256);
+      (i ? p.w : p.x) = to, (i ? p.ldw : p.ldx) = ld;
+    } else if (o.rows == 1) {
+      (i ? p.ldw : p.ldx) = ld;  // (the stride of a single row addresses nothing)
+    }
+    if (!o.sq) {
+      uint8_t* to = (uint8_t*)ws + (i ? plan.sw : plan.sx);
+      scales[i] = {o.s, o.rows, blocks, o.sr, o.sb, (uint32_t*)to, o.rows};
+      ns[i] = grid_of(mx_scales_tiles(scales[i]), 1);
+      (i ? p.sw : p.sx) = to, (i ? p.swm : p.sxm) = 4, (i ? p.swq : p.sxq) = 4 * o.rows;
+    }
+  }
+  if (const uint32_t grid = np[0] + np[1] + ns[0] + ns[1]) {
+    hipLaunchKernelGGL(mx_pack_kernel, dim3(grid), dim3(256), 0, stream, pack[0], pack[1], scales[0], scales[1], np[0],
+                       np[1], ns[0]);
     if ((rc = hip_status())) return rc;
   }
   return run_product(p, plan.plan, ws + plan.parts, stream);
@@ -292,12 +340,13 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   if (N < 0) return F16ACC_OPS_E_ARG;
   if (M == 0 || N == 0) return 0;
   if (K == 0 || !w || !sw || !y || swn < 0 || swb < 0) return F16ACC_OPS_E_ARG;
-  if (ldw < cdiv(K, 2) && N > 1) return F16ACC_OPS_E_UNSUPPORTED;
+  if ((ldw < cdiv(K, 2) && N > 1) || 64 * quads_of(K) > kMaxRow || M > 0x7fffffff || N > 0x7fffffff)
+    return F16ACC_OPS_E_UNSUPPORTED;
   hipStream_t stream = (hipStream_t)stream_;
-  const bool wide = wide_loads(x, type, sr, sc);
+  const bool wide = sc == 1;  // (rows of any alignment)
   const LinearPlan4 plan(M, N, K, w, ldw);
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
-  if (few4(M, K) && wide && M <= 8) {
+  if (few4(M, K) && (sc == 1 || K == 1) && M <= 8) {
     const Small4Args a{x, sr, w, ldw, sw, swn, swb, bias, y, M, N, K};
     const size_t lds = small4_lds(M, K);
     return by_type(type, [&](auto* t) {
@@ -316,14 +365,12 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   p.w = plan.packed ? (const uint8_t*)ws + plan.weight : w, p.ldw = plan.packed ? plan.ld : ldw;
   p.sw = (const uint8_t*)ws + plan.sw, p.swm = 4, p.swq = 4 * N;
   p.bias = bias, p.c = y, p.scm = N, p.scn = 1, p.M = M, p.N = N, p.K = K, p.ctype = type;
-  rc = product_check(p);
-  if (rc) return rc;
   const MxQuantArgs q{x, M, K, sr, sc, (uint8_t*)ws, p.ldx, {(uint8_t*)p.sx, p.sxm, p.sxq}, nullptr, 0, {nullptr, 0, 0},
                       nullptr, 0, 0};
   const MxScaleArgs s{sw, N, cdiv(K, kMx), swn, swb, (uint32_t*)p.sw, N};
   const Pack8Args pk{w, (uint8_t*)p.w, N, cdiv(K, 2), ldw, 1, plan.ld};
-  const uint32_t packs = plan.packed ? grid_of(N * (plan.ld / 16), 256) : 0, scales = grid_of(N * quads_of(K), 256);
-  const dim3 grid(packs + scales + grid_of(M * quads_of(K), 16));
+  const uint32_t packs = plan.packed ? grid_of(N * (plan.ld / 16), 256) : 0, scales = grid_of(mx_scales_tiles(s), 1);
+  const dim3 grid(packs + scales + quant_grid(q));
   rc = by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (wide)

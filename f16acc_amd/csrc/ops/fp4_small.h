@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) 
       const T* x = (const T*)p.x + t * p.ldx;
       float v[8];
       if (k + 8 <= p.K) {
-        load_vec(x + k, v);
+        load_any(x + k, v);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? (float)x[k + j] : 0.0f;

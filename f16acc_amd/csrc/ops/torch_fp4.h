@@ -14,23 +14,34 @@ int64_t mx_blocks(int64_t v) { return (v + kMx - 1) / kMx; }
 // The bytes of a 4-bit operand or of scales (torch has few functions for their types).
 Tensor as_bytes(const Tensor& t) { return t.detach().view(at::kByte); }
 
-// An operand of a product: rows of `ld` bytes, the scales' dword of (row, quad of blocks) at row * row + quad * quad
+// An operand of a product: bytes of strides (r, c); the scales' dword of (row, quad of blocks) at row * row + quad * quad
 // bytes, or, where quad is 0, the byte of (row, block) at row * row + block * block.
 struct Operand4 {
-  Tensor q, s;
-  int64_t ld, row, block, quad;
+  const uint8_t *q, *s;
+  int64_t r, c, row, block, quad;
 };
 
-// x's row blocks, and those of x transposed, from one pass; the scales in the products' order.
-std::pair<Operand4, Operand4> quant4(const Tensor& x, bool rows, bool cols) {
-  const int64_t M = x.size(0), K = x.size(1), qm = blocks(M), qk = blocks(K);
-  Operand4 r{}, c{};
-  if (rows) r = {empty({M, 64 * qk}, x, at::kByte), empty({qk, M}, x, at::kInt), 64 * qk, 4, 1, 4 * M};
-  if (cols) c = {empty({K, 64 * qm}, x, at::kByte), empty({qm, K}, x, at::kInt), 64 * qm, 4, 1, 4 * K};
+// What quantising gives: rows of 64 bytes a quad, then the scales in the products' order, in one allocation.
+struct Quantised4 {
+  Tensor held;
+  int64_t rows, quads;
+  Quantised4() : rows(0), quads(0) {}
+  Quantised4(int64_t rows, int64_t cols, const Tensor& like)
+      : held(empty({rows * blocks(cols) * 68}, like, at::kByte)), rows(rows), quads(blocks(cols)) {}
+  Quantised4(const Tensor& held, int64_t rows, int64_t cols) : held(held), rows(rows), quads(blocks(cols)) {}
+  uint8_t* q() const { return bytes(held); }
+  uint8_t* s() const { return held.defined() ? bytes(held) + rows * quads * 64 : nullptr; }
+  Operand4 operand() const { return {q(), s(), 64 * quads, 1, 4, 1, 4 * rows}; }
+};
+
+// A matrix to quantise along its rows (q) and columns (qt), either perhaps undefined.
+f16acc_fp4_matrix matrix4(const Tensor& x, const Quantised4& q, const Quantised4& qt) {
+  return {x.const_data_ptr(), x.size(0), x.size(1), x.stride(0), x.stride(1), q.q(), 64 * q.quads, q.s(), 4, 4 * q.rows,
+          qt.q(), 64 * qt.quads, qt.s(), 4, 4 * qt.rows};
+}
+void quant4(const f16acc_fp4_matrix* a, const f16acc_fp4_matrix* b, const Tensor& x) {
   const On on(x);
-  check_rc(f16acc_fp4_quant(x.const_data_ptr(), type_of(x), M, K, x.stride(0), x.stride(1), bytes(r.q), r.ld,
-                            bytes(r.s), r.row, r.quad, bytes(c.q), c.ld, bytes(c.s), c.row, c.quad, on.stream));
-  return {r, c};
+  check_rc(f16acc_fp4_quant(a, b, type_of(x), on.stream));
 }
 
 std::tuple<Tensor, Tensor> quantize4(const Tensor& x, bool transposed) {
@@ -43,13 +54,20 @@ std::tuple<Tensor, Tensor> quantize4(const Tensor& x, bool transposed) {
   const int64_t M = x2.size(0), K = x2.size(1), R = transposed ? K : M, C = transposed ? M : K;
   const int64_t ld = 64 * blocks(C), lds = 4 * blocks(C);
   const Tensor q = empty({R, ld}, x, kF4), s = empty({R, lds}, x, kE8);
-  uint8_t *to = bytes(q), *scales = bytes(s), *none = nullptr;
-  const On on(x);
-  check_rc(f16acc_fp4_quant(x2.const_data_ptr(), type_of(x), M, K, x2.stride(0), x2.stride(1), transposed ? none : to,
-                            ld, scales, lds, 4, transposed ? to : none, ld, scales, lds, 4, on.stream));
-  const Tensor qn = q.narrow(1, 0, pairs(C)), sn = s.narrow(1, 0, mx_blocks(C));
-  if (transposed) return {qn, sn};
-  return {qn.view(with_last(x, pairs(C))), sn.view(with_last(x, mx_blocks(C)))};
+  f16acc_fp4_matrix m{x2.const_data_ptr(), M, K, x2.stride(0), x2.stride(1)};
+  if (transposed)
+    m.qt = bytes(q), m.ldqt = ld, m.st = bytes(s), m.st_row = lds, m.st_quad = 4;
+  else
+    m.q = bytes(q), m.ldq = ld, m.s = bytes(s), m.s_row = lds, m.s_quad = 4;
+  quant4(&m, nullptr, x);
+  // the rows without their padding, with x's leading dimensions
+  auto trimmed = [&](const Tensor& t, int64_t last) {
+    if (transposed) return t.narrow(1, 0, last);
+    std::vector<int64_t> strides(x.dim(), 1);
+    for (int64_t i = x.dim() - 2, step = t.size(1); i >= 0; --i) strides[i] = step, step *= std::max<int64_t>(x.size(i), 1);
+    return t.as_strided(with_last(x, last), strides);
+  };
+  return {trimmed(q, pairs(C)), trimmed(s, mx_blocks(C))};
 }
 
 Tensor dequantize4(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
@@ -71,34 +89,21 @@ Tensor dequantize4(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
   return out;
 }
 
-// Bytes [rows, pairs] as the products read them: themselves, or a copy whose rows are 16-byte aligned and zero to
-// the next multiple of 16 bytes.
-Operand packed4(const Tensor& q) {
-  const int64_t rows = q.size(0), n = q.size(1), ld = rows > 1 ? q.stride(0) : up(n, 16);
-  if (n % 16 == 0 && (q.stride(1) == 1 || n <= 1) && ld >= n && ld % 16 == 0 && ld <= kMaxRow &&
-      (uintptr_t)q.const_data_ptr() % 16 == 0)
-    return {q, ld};
-  const Tensor out = empty({rows, up(n, 16)}, q, at::kByte);
-  const On on(q);
-  check_rc(f16acc_pack8(bytes(q), bytes(out), rows, n, q.stride(0), q.stride(1), up(n, 16), on.stream));
-  return {out, up(n, 16)};
-}
 Operand4 stored4(const Tensor& q, const Tensor& s) {
-  const Operand o = packed4(q);
-  return {o.q, s, o.ld, s.stride(0), s.stride(1), 0};
+  return {bytes(q), bytes(s), q.stride(0), q.stride(1), s.stride(0), s.stride(1), 0};
 }
 
 // out [M, N] from x [M, K] and w [N, K].
 void product4(const Operand4& x, const Operand4& w, int64_t K, const Tensor& out, const Maybe& bias = {}, int tile = -1,
               int splits = 0) {
   const int64_t M = out.size(0), N = out.size(1);
-  const size_t n = f16acc_mm_fp4_workspace(M, N, K, x.quad, w.quad, tile, splits);
+  const size_t n = f16acc_mm_fp4_workspace(x.q, x.r, x.c, x.quad, w.q, w.r, w.c, w.quad, M, N, K, tile, splits);
   Tensor ws;
   if (n) ws = empty({(int64_t)n}, out, at::kByte);
   const On on(out);
-  check_rc(f16acc_mm_fp4(bytes(x.q), x.ld, bytes(x.s), x.row, x.block, x.quad, bytes(w.q), w.ld, bytes(w.s), w.row,
-                         w.block, w.quad, data(bias), out.data_ptr(), out.stride(0), out.stride(1), M, N, K,
-                         type_of(out), tile, splits, bytes(ws), n, on.stream));
+  check_rc(f16acc_mm_fp4(x.q, x.r, x.c, x.s, x.row, x.block, x.quad, w.q, w.r, w.c, w.s, w.row, w.block, w.quad,
+                         data(bias), out.data_ptr(), out.stride(0), out.stride(1), M, N, K, type_of(out), tile, splits,
+                         bytes(ws), n, on.stream));
 }
 
 Tensor mm4(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType out_dtype,
@@ -137,61 +142,78 @@ Tensor mm4(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor
 }
 
 // y = x w^T + bias; dx = dy w, dw = dy^T x, each from operands quantised along its own contraction.
-Tensor train_forward4(const Tensor& x, const Tensor& w, const Maybe& bias, bool need_x, bool need_w, Operand4* xt,
-                      Operand4* wt) {
+Tensor train_forward4(const Tensor& x, const Tensor& w, const Maybe& bias, bool need_x, bool need_w, Quantised4* xt,
+                      Quantised4* wt) {
   const Tensor x2 = rows_of(x);
-  const auto [xr, xc] = quant4(x2, true, need_w);
-  const auto [wr, wc] = quant4(w, true, need_x);
-  *xt = xc, *wt = wc;
-  const Tensor y = empty(with_last(x, w.size(0)), x, x.scalar_type());
-  product4(xr, wr, x2.size(1), y.view({x2.size(0), w.size(0)}), bias);
+  const int64_t M = x2.size(0), K = x2.size(1), N = w.size(0);
+  const Quantised4 xr(M, K, x), wr(N, K, x);
+  if (need_w) *xt = Quantised4(K, M, x);
+  if (need_x) *wt = Quantised4(K, N, x);
+  const f16acc_fp4_matrix a = matrix4(x2, xr, *xt), b = matrix4(w, wr, *wt);
+  if (x.scalar_type() == w.scalar_type()) {
+    quant4(&a, &b, x);
+  } else {
+    quant4(&a, nullptr, x);
+    quant4(&b, nullptr, w);
+  }
+  const Tensor y = empty(with_last(x, N), x, x.scalar_type());
+  product4(xr.operand(), wr.operand(), K, y.view({M, N}), bias);
   return y;
 }
 
-// An operand kept for the backward pass: rows [rows][64 quads], scales [quads][rows].
-Operand4 kept4(const Tensor& q, const Tensor& s) { return {q, s, q.size(1), 4, 1, 4 * q.size(0)}; }
-
 struct Train4 : torch::autograd::Function<Train4> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias) {
-    Operand4 xt{}, wt{};
+    Quantised4 xt, wt;
     const Tensor y = train_forward4(x, w, bias, x.requires_grad(), w.requires_grad(), &xt, &wt);
-    ctx->save_for_backward({xt.q, xt.s, wt.q, wt.s});
+    ctx->save_for_backward({xt.held, wt.held});
     ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["dtype"] = (int64_t)w.scalar_type();
-    ctx->saved_data["need"] = (int64_t)x.requires_grad() + 2 * (int64_t)w.requires_grad() +
-                              4 * (int64_t)(bias && bias->requires_grad());
+    ctx->saved_data["dtype"] = (int64_t)w.scalar_type() * 8 + (int64_t)x.requires_grad() +
+                               2 * (int64_t)w.requires_grad() + 4 * (int64_t)(bias && bias->requires_grad());
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_derivative_only();
     const auto saved = ctx->get_saved_variables();
     const auto shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t need = ctx->saved_data["need"].toInt(), K = shape.back();
+    const int64_t need = ctx->saved_data["dtype"].toInt(), K = shape.back();
     const Tensor dy = rows_of(check_grad("fp4.linear", grads[0]));
     const int64_t M = dy.size(0), N = dy.size(1);
-    Operand4 r{}, c{};
-    if (need & 3) std::tie(r, c) = quant4(dy, need & 1, need & 2);
+    Quantised4 r, c;
+    if (need & 1) r = Quantised4(M, N, dy);
+    if (need & 2) c = Quantised4(N, M, dy);
+    if (need & 3) {
+      const f16acc_fp4_matrix m = matrix4(dy, r, c);
+      quant4(&m, nullptr, dy);
+    }
     Tensor dx, dw, db;
     if (need & 1) {
-      dx = empty({M, K}, dy, dy.scalar_type());
-      product4(r, kept4(saved[2], saved[3]), N, dx);
-      dx = dx.view(shape);
+      dx = empty(shape, dy, dy.scalar_type());
+      product4(r.operand(), Quantised4(saved[1], K, N).operand(), N, dx.view({M, K}));
     }
     if (need & 2) {
-      dw = empty({N, K}, dy, (at::ScalarType)ctx->saved_data["dtype"].toInt());
-      product4(c, kept4(saved[0], saved[1]), M, dw);
+      dw = empty({N, K}, dy, (at::ScalarType)(need >> 3));
+      product4(c.operand(), Quantised4(saved[0], K, M).operand(), M, dw);
     }
     if (need & 4) db = column_sums(dy);
     return {dx, dw, db};
   }
 };
 
+// Bytes [rows, pairs] of any strides as rows.
+Operand packed4(const Tensor& q) {
+  const int64_t rows = q.size(0), n = q.size(1);
+  const Tensor out = empty({rows, up(n, 16)}, q, at::kByte);
+  const On on(q);
+  check_rc(f16acc_pack8(bytes(q), bytes(out), rows, n, q.stride(0), q.stride(1), up(n, 16), on.stream));
+  return {out, up(n, 16)};
+}
+
 Tensor stored_linear4(const Tensor& x, const Tensor& w, const Tensor& w_scale, const Maybe& bias) {
   const Tensor x2 = rows_of(x), q = as_bytes(w), s = as_bytes(w_scale);
   const int64_t M = x2.size(0), K = x2.size(1), N = w.size(0), P = pairs(K);
   // rows of any alignment go as they are (the library copies them where it has to)
   const bool rows = (P <= 1 || q.stride(1) == 1) && (N <= 1 || q.stride(0) >= P);
-  const Operand o = rows ? Operand{q, N > 1 ? q.stride(0) : up(P, 16)} : packed4(q);
+  const Operand o = rows ? Operand{q, N > 1 ? q.stride(0) : up(P, 16)} : packed4(q);  // (a row-major [K / 2, N] weight)
   Tensor y = empty(with_last(x, N), x, x.scalar_type());
   const size_t n = f16acc_linear_fp4_workspace(M, N, K, bytes(o.q), o.ld);
   const Tensor ws = empty({(int64_t)n}, x, at::kByte);
@@ -220,17 +242,16 @@ struct Stored4 : torch::autograd::Function<Stored4> {
     Tensor dx, db;
     if (need & 1) {
       const Tensor q = as_bytes(saved[0]), s = as_bytes(saved[1]);
-      const int64_t qn = blocks(N);
-      const Operand4 wt{empty({K, 64 * qn}, dy, at::kByte), empty({qn, K}, dy, at::kInt), 64 * qn, 4, 1, 4 * K};
-      const Operand4 r = quant4(dy, true, false).first;
-      dx = empty({dy.size(0), K}, dy, dy.scalar_type());
+      const Quantised4 wt(K, N, dy), r(dy.size(0), N, dy);
+      const f16acc_fp4_matrix m = matrix4(dy, r, Quantised4());
+      quant4(&m, nullptr, dy);
       {
         const On on(dy);
         check_rc(f16acc_fp4_transpose(bytes(q), q.stride(0), q.stride(1), bytes(s), s.stride(0), s.stride(1), N, K,
-                                      bytes(wt.q), wt.ld, bytes(wt.s), wt.row, wt.quad, on.stream));
+                                      wt.q(), 64 * wt.quads, wt.s(), 4, 4 * K, on.stream));
       }
-      product4(r, wt, N, dx);
-      dx = dx.view(shape);
+      dx = empty(shape, dy, dy.scalar_type());
+      product4(r.operand(), wt.operand(), N, dx.view({dy.size(0), K}));
     }
     if (need & 2) db = column_sums(dy);
     return {dx, {}, {}, db};
@@ -268,7 +289,7 @@ Tensor linear4(const Tensor& x, const Tensor& w, const Maybe& w_scale, const May
   if (bias) b = bias->contiguous();
   if (!w_scale) {
     if (grad && (x.requires_grad() || w.requires_grad() || (b && b->requires_grad()))) return Train4::apply(x, w, b);
-    Operand4 xt{}, wt{};
+    Quantised4 xt, wt;
     return train_forward4(x, w, b, false, false, &xt, &wt);
   }
   if (grad && (x.requires_grad() || (b && b->requires_grad()))) return Stored4::apply(x, w, *w_scale, b);

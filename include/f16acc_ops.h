@@ -171,7 +171,8 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
  * consecutive blocks of a row are a quad; its four scale bytes are one dword, that of an operand's (row, quad)
  * at s + row * s_row + quad * s_quad (bytes, multiples of 4, s 4-byte aligned).
  *
- * f16acc_fp4_quant: x [rows, cols] (element strides sr, sc; any) read once.
+ * f16acc_fp4_quant: one matrix or two (b NULL: none) of `type`, each x [rows, cols] (element strides sr, sc; any)
+ *   read once.
  *   q [rows][ldq], ldq = 64 ceil(cols / 128), zero from cols on (NULL: not wanted), its scales s; those of
  *   blocks that only pad a quad are 25 (2^-102)
  *   qt, st: the same of x transposed, blocks of 32 rows of each column: [cols][ldqt], ldqt = 64 ceil(rows / 128)
@@ -179,9 +180,19 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
  *   row * s_r + block * s_b) quantised again in blocks of 32 rows, as qt and st above.
  * f16acc_fp4_values: those values as `type`, each rounded once, out [rows][cols] contiguous, 16-byte aligned.
  */
-int f16acc_fp4_quant(const void* x, int type, int64_t rows, int64_t cols, int64_t sr, int64_t sc, uint8_t* q,
-                     int64_t ldq, uint8_t* s, int64_t s_row, int64_t s_quad, uint8_t* qt, int64_t ldqt, uint8_t* st,
-                     int64_t st_row, int64_t st_quad, void* stream);
+typedef struct {
+  const void* x;
+  int64_t rows, cols, sr, sc;
+  uint8_t* q;
+  int64_t ldq;
+  uint8_t* s;
+  int64_t s_row, s_quad;
+  uint8_t* qt;
+  int64_t ldqt;
+  uint8_t* st;
+  int64_t st_row, st_quad;
+} f16acc_fp4_matrix;
+int f16acc_fp4_quant(const f16acc_fp4_matrix* a, const f16acc_fp4_matrix* b, int type, void* stream);
 int f16acc_fp4_transpose(const uint8_t* x, int64_t sr, int64_t sc, const uint8_t* s, int64_t s_r, int64_t s_b,
                          int64_t rows, int64_t cols, uint8_t* qt, int64_t ldqt, uint8_t* st, int64_t st_row,
                          int64_t st_quad, void* stream);
@@ -191,19 +202,21 @@ int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t*
 /*
  * c[m][n] = sum over k of x[m][k] w[n][k] (4-bit values times their blocks' scales) + bias[n], added in FP32, rounded
  * once to ctype.
- *   x [M][ldx], w [N][ldw]: bytes, rows 16-byte aligned and zero from K to the next multiple of 32 values;
- *   K at least 1 where M and N are
+ *   x, w: the bytes of (row, pair of values) at strides (xr, xc), (wr, wc), any; rows of whole blocks that are
+ *   16-byte aligned and at most 4 MiB apart are read as they are, others copied first;  K at least 1 where M and N are
  *   sx, sw: single bytes, that of (row m, block b) at m * sxm + b * sxb, where sxq is 0; else quads as above,
- *   (row, quad) at m * sxm + quad * sxq, bytes past the last block not 255 (swn, swb, swq alike)
+ *   (row, quad) at m * sxm + quad * sxq, bytes past the last block not 255, and rows that are aligned
+ *   and zero from K to the next multiple of 32 values (swn, swb, swq alike)
  *   bias: [N] of ctype, or NULL;  c: element strides scm, scn
  *   tile, splits: -1 and 0 leave the choice to the library; a tile number (0 to 5) and a number of parts of K
  *   force them, for tuning
- *   workspace: f16acc_mm_fp4_workspace bytes for exactly these sizes (single scale bytes in quads, FP32 sums of
- *   the parts of K; may be 0), 256-byte aligned
+ *   workspace: f16acc_mm_fp4_workspace bytes for exactly these operands (copied rows, single scale bytes in
+ *   quads, FP32 sums of the parts of K; may be 0), 256-byte aligned
  */
-size_t f16acc_mm_fp4_workspace(int64_t M, int64_t N, int64_t K, int64_t sxq, int64_t swq, int tile, int splits);
-int f16acc_mm_fp4(const uint8_t* x, int64_t ldx, const uint8_t* sx, int64_t sxm, int64_t sxb, int64_t sxq,
-                  const uint8_t* w, int64_t ldw, const uint8_t* sw, int64_t swn, int64_t swb, int64_t swq,
+size_t f16acc_mm_fp4_workspace(const uint8_t* x, int64_t xr, int64_t xc, int64_t sxq, const uint8_t* w, int64_t wr,
+                               int64_t wc, int64_t swq, int64_t M, int64_t N, int64_t K, int tile, int splits);
+int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, int64_t sxm, int64_t sxb, int64_t sxq,
+                  const uint8_t* w, int64_t wr, int64_t wc, const uint8_t* sw, int64_t swn, int64_t swb, int64_t swq,
                   const void* bias, void* c, int64_t scm, int64_t scn, int64_t M, int64_t N, int64_t K, int ctype,
                   int tile, int splits, void* workspace, size_t ws_bytes, void* stream);
 

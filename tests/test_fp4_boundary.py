@@ -1,6 +1,8 @@
 """The 4-bit operators without a GPU: what the C ABI and the Python functions refuse, and that a call
 neither records into a trace nor holds the interpreter."""
 
+import ctypes
+import functools
 import sys
 import threading
 
@@ -17,15 +19,21 @@ F4, E8 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
 
 
 def test_quantisation_checks():
-    def call(x=256, t=0, rows=4, cols=200, q=256, ldq=128, s=256, sr=8, sq=4, qt=None, ldqt=0, st=None, str_=4, stq=4):
-        return _ops.fp4_quant(x, t, rows, cols, cols, 1, q, ldq, s, sr, sq, qt, ldqt, st, str_, stq, None)
+    def call(x=256, t=0, rows=4, cols=200, q=256, ldq=128, s=256, sr=8, sq=4, qt=None, ldqt=0, st=None, str_=4, stq=4, second=False):
+        m = _ops.Fp4Matrix(x, rows, cols, cols, 1, q, ldq, s, sr, sq, qt, ldqt, st, str_, stq)
+        none = _ops.Fp4Matrix(None, 0, 0, 0, 1, None, 0, None, 0, 0, None, 0, None, 0, 0)
+        a, b = (none, m) if second else (m, None)
+        return _ops.fp4_quant(ctypes.byref(a), ctypes.byref(b) if b else None, t, None)
 
-    assert call(x=None) == call(t=3) == call(t=-1) == call(rows=-1) == call(cols=-1) == call(q=None) == _ops.E_ARG
-    assert call(s=None) == call(sr=-4) == call(sq=-4) == call(qt=256, ldqt=64) == _ops.E_ARG
-    assert call(ldq=100) == call(ldq=192) == call(ldq=64) == call(q=264) == call(s=258) == call(sr=6) == _ops.E_UNSUPPORTED
-    assert call(qt=256, ldqt=128, st=256) == call(qt=260, ldqt=64, st=256) == _ops.E_UNSUPPORTED
-    assert call(rows=1 << 41) == call(qt=256, ldqt=64 << 20, st=256, rows=128 << 20, q=None) == _ops.E_UNSUPPORTED
-    assert call(rows=0) == call(cols=0) == 0
+    for second in (False, True):
+        f = functools.partial(call, second=second)
+        assert f(x=None) == f(t=3) == f(t=-1) == f(rows=-1) == f(cols=-1) == f(q=None) == _ops.E_ARG
+        assert f(s=None) == f(sr=-4) == f(sq=-4) == f(qt=256, ldqt=64) == _ops.E_ARG
+        assert f(ldq=100) == f(ldq=192) == f(ldq=64) == f(q=264) == f(s=258) == f(sr=6) == _ops.E_UNSUPPORTED
+        assert f(qt=256, ldqt=128, st=256) == f(qt=260, ldqt=64, st=256) == f(rows=1 << 41) == _ops.E_UNSUPPORTED
+        assert f(qt=256, ldqt=64 << 30, st=256, rows=128 << 30, q=None) == _ops.E_UNSUPPORTED
+        assert f(rows=0) == f(cols=0) == 0
+    assert _ops.fp4_quant(None, None, 0, None) == _ops.E_ARG
 
     def back(x=256, s=256, qt=256, ldqt=64, st=256, rows=4):
         return _ops.fp4_transpose(x, 100, 1, s, 7, 1, rows, 200, qt, ldqt, st, 4, 800, None)
@@ -41,23 +49,32 @@ def test_quantisation_checks():
 
 
 def test_mm_checks():
-    need = _ops.mm_fp4_workspace(4, 4, 256, 0, 0, -1, 0)
+    def workspace(x=256, xr=128, xc=1, sxq=0, w=256, wr=128, swq=0, M=4, N=4, K=256, tile=-1, splits=0):
+        return _ops.mm_fp4_workspace(x, xr, xc, sxq, w, wr, 1, swq, M, N, K, tile, splits)
 
-    def call(x=256, ldx=128, sx=256, sxm=8, sxb=1, sxq=0, w=256, ldw=128, sw=256, swn=8, swq=0, c=256, M=4, N=4, K=256, t=0,
+    need = workspace()
+
+    def call(x=256, xr=128, xc=1, sx=256, sxm=8, sxb=1, sxq=0, w=256, wr=128, sw=256, swn=8, swq=0, c=256, M=4, N=4, K=256, t=0,
              tile=-1, splits=0, ws=256, n=need):
-        return _ops.mm_fp4(x, ldx, sx, sxm, sxb, sxq, w, ldw, sw, swn, 1, swq, None, c, N, 1, M, N, K, t, tile, splits, ws,
+        return _ops.mm_fp4(x, xr, xc, sx, sxm, sxb, sxq, w, wr, 1, sw, swn, 1, swq, None, c, N, 1, M, N, K, t, tile, splits, ws,
                            n, None)
 
     assert call(M=-1) == call(K=-1) == call(N=-1) == call(t=3) == call(c=None) == call(x=None) == call(w=None) == _ops.E_ARG
     assert call(sx=None) == call(sw=None) == call(swn=-1) == call(sxb=-1) == call(sxq=-4) == call(K=0) == _ops.E_ARG
-    assert call(ldx=120) == call(ldw=112) == call(x=8) == call(w=264) == _ops.E_UNSUPPORTED
-    assert call(K=1 << 24, ldx=1 << 23, ldw=1 << 23) == call(M=1 << 31) == _ops.E_UNSUPPORTED
+    assert call(xr=-128) == call(wr=-1) == call(xc=-1) == _ops.E_ARG
+    assert call(K=1 << 24, xr=1 << 23, wr=1 << 23) == call(M=1 << 31) == call(N=1 << 31) == _ops.E_UNSUPPORTED
     assert call(sxq=6) == call(sxq=4, sxm=6) == call(swq=4, sw=258) == call(sxq=4, sxm=1 << 23) == _ops.E_UNSUPPORTED
+    assert call(sxq=4, x=264) == call(sxq=4, xr=120) == call(swq=4, wr=1 << 23) == call(sxq=4, xc=2) == _ops.E_UNSUPPORTED
     assert call(tile=6) == call(tile=-2) == call(splits=-1) == _ops.E_ARG
     assert call(ws=None) == call(ws=128) == call(n=need - 1) == _ops.E_WORKSPACE
-    assert need >= 2 * 4 * 2 * 4 and _ops.mm_fp4_workspace(4, 4, 256, 4, 4, -1, 0) == 0
-    assert _ops.mm_fp4_workspace(4, 4, 1024, 4, 4, 2, 2) >= 2 * 4 * 4 * 4
-    assert call(M=0) == call(N=0) == 0 == _ops.mm_fp4_workspace(0, 4, 4, 0, 0, -1, 0) == _ops.mm_fp4_workspace(4, 4, 4, 0, 0, 6, 0)
+    # single scale bytes are reordered; rows that are not aligned, or do not end with a block, are copied; parts of K
+    assert need >= 2 * 4 * 2 * 4 and workspace(sxq=4, swq=4) == 0
+    for other in (dict(x=264), dict(xr=130), dict(xc=2), dict(K=254), dict(w=257), dict(wr=1 << 23)):
+        assert workspace(**other) >= need + 4 * 128
+        assert call(**other) == _ops.E_WORKSPACE
+    assert workspace(M=1, xr=1) == workspace(M=1)  # the stride of a single row addresses nothing
+    assert workspace(sxq=4, swq=4, K=1024, xr=512, wr=512, tile=2, splits=2) >= 2 * 4 * 4 * 4
+    assert call(M=0) == call(N=0) == 0 == workspace(M=0) == workspace(tile=6) == workspace(splits=-1)
 
 
 def test_linear_checks():
