@@ -114,6 +114,16 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
   for (int i = 0; i < N; ++i) v[i] = (float)k.t[i];
 }
 
+// Up to N elements of a strided row from c on, zero past its end.  Every load reads inside the row, so all are in
+// flight together: behind a branch each, the last columns of an odd width waited for one after another.
+template <int N, class T>
+__device__ __forceinline__ void load_clamped(const T* row, int64_t c, int64_t cols, int64_t stride, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (float)row[(c + i < cols ? c + i : cols - 1) * stride];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = c + i < cols ? v[i] : 0.0f;
+}
+
 // SiLU with FP32's accuracy, behind sums of that accuracy: what is quantised from
 // it should fall on the right side of a tie.
 __device__ __forceinline__ float silu_exact(float g) { return g / (1.0f + expf(-g)); }

@@ -100,14 +100,11 @@ __device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t gro
     if (row >= p.rows) continue;
     const int64_t c0 = kq * kQuad + lane * 8;
     const T* x = (const T*)p.x + row * p.sr;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (WIDE && c0 + 8 <= p.cols) {
+    float v[8];
+    if (WIDE && c0 + 8 <= p.cols)
       load_any(x + c0, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < p.cols) v[i] = (float)x[(c0 + i) * p.sc];
-    }
+    else
+      load_clamped(x, c0, p.cols, p.sc, v);
     uint32_t m = abs_bits(v[0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
@@ -139,10 +136,12 @@ __device__ __forceinline__ void mx_scales(const MxScaleArgs& p, uint32_t group, 
     uint32_t v = 0;
     if (p.s_b == 1 && 4 * kq + 4 <= p.blocks) {
       __builtin_memcpy(&v, s, 4);
-    } else {
+    } else {  // (inside the row, all in flight together: see load_clamped)
+      uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (4 * kq + j < p.blocks) v |= (uint32_t)s[j * p.s_b] << (8 * j);
+      for (int j = 0; j < 4; ++j) b[j] = s[(4 * kq + j < p.blocks ? j : p.blocks - 1 - 4 * kq) * p.s_b];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v |= 4 * kq + j < p.blocks ? b[j] << (8 * j) : 0;
     }
     p.dst[kq * p.ld + r] = v;
   }
@@ -184,23 +183,22 @@ __device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t
   if (r >= p.rows || c >= p.cols) return;
   if constexpr (std::is_same_v<T, Fp4Source>) {
     const uint8_t* q = (const uint8_t*)p.x + r * p.sr + c / 2 * p.sc;
-    uint32_t u = 0;
+    uint32_t u = 0, b[4];
+    const int64_t last = (p.cols - 1 - c) / 2;  // (inside the row, all in flight together: see load_clamped)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + 2 * i < p.cols) u |= (uint32_t)q[i * p.sc] << (8 * i);
+    for (int i = 0; i < 4; ++i) b[i] = q[(i < last ? i : last) * p.sc];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u |= i <= last ? b[i] << (8 * i) : 0;
     unpack_e2m1(u, p.xs[r * p.xsr + c / kMx * p.xsc], v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (c + i >= p.cols) v[i] = 0.0f;
   } else {
     const T* x = (const T*)p.x + r * p.sr;
-    if (WIDE && c + 8 <= p.cols) {
+    if (WIDE && c + 8 <= p.cols)
       load_any(x + c, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < p.cols) v[i] = (float)x[(c + i) * p.sc];
-    }
+    else
+      load_clamped(x, c, p.cols, p.sc, v);
   }
 }
 
@@ -286,9 +284,12 @@ __global__ __launch_bounds__(256) void mx_values_kernel(MxValuesArgs p) {
     if (whole && c + 8 <= p.cols) {
       __builtin_memcpy(&u, q, 4);
     } else {
+      uint32_t b[4];
+      const int64_t last = (p.cols - 1 - c) / 2;  // (inside the row, all in flight together: see load_clamped)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + 2 * j < p.cols) u |= (uint32_t)q[j * p.q_c] << (8 * j);
+      for (int j = 0; j < 4; ++j) b[j] = q[(j < last ? j : last) * p.q_c];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u |= j <= last ? b[j] << (8 * j) : 0;
     }
     float v[8];
     unpack_e2m1(u, p.s[r * p.s_r + c / kMx * p.s_b], v);

@@ -87,12 +87,10 @@ __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) 
       const int64_t k = (int64_t)kq * kQuad + 8 * c;
       const T* x = (const T*)p.x + t * p.ldx;
       float v[8];
-      if (k + 8 <= p.K) {
+      if (k + 8 <= p.K)
         load_any(x + k, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? (float)x[k + j] : 0.0f;
-      }
+      else
+        load_clamped(x, k, p.K, 1, v);
       uint32_t m = abs_bits(v[0]);
 #pragma unroll
       for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[j]));

@@ -25,12 +25,10 @@ struct RouterArgs {
 // Eight elements of a row from k, zero past the end.
 template <class T>
 __device__ __forceinline__ void load8(const T* p, int64_t stride, int64_t k, int64_t D, bool wide, float (&v)[8]) {
-  if (wide && k + 8 <= D) {
+  if (wide && k + 8 <= D)
     load_vec(p + k, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < D ? (float)p[(k + i) * stride] : 0.0f;
-  }
+  else
+    load_clamped(p, k, D, stride, v);
 }
 
 // logits[t][e] = sum over d of x[t][d] r[e][d], summed in 64 bits and rounded once to FP32: products of 16-bit and
@@ -108,6 +106,7 @@ struct LayerArgs {
   RouterArgs router;
   RouteArgs route;
   QuantArgs quant;  // the tokens: [T][Dp] and the scale of (token, block) at [block][T]
+  bool wide;        // (16-byte loads of the tokens)
   FewArgs e;
   int ytype;
   int pieces;  // of an expert's hidden columns
@@ -121,7 +120,10 @@ __global__ __launch_bounds__(256) void layer_router_kernel(LayerArgs a) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)a.e.slots * a.pieces; i += (int64_t)gridDim.x * 256)
     a.claims[i].taken = 0;
   if ((int)blockIdx.x >= p.E) {
-    quant_rows<T, false>(a.quant, blockIdx.x - p.E, gridDim.x - p.E);
+    if (a.wide)
+      quant_rows<T, true>(a.quant, blockIdx.x - p.E, gridDim.x - p.E);
+    else
+      quant_rows<T, false>(a.quant, blockIdx.x - p.E, gridDim.x - p.E);
     return;
   }
   __shared__ double sums[4][kFewTokens];

@@ -758,7 +758,7 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
   if (few) {
     const int64_t Dp = up128(D), Ip = up128(I);
     LayerArgs l{};
-    l.router = r, l.route = a, l.ytype = type, l.sync = (LayerSync*)(ws + plan.sync);
+    l.router = r, l.route = a, l.ytype = type, l.wide = wide_loads(x, type, sr, sc), l.sync = (LayerSync*)(ws + plan.sync);
     l.pieces = (int)cdiv(I, 16), l.claims = (Claim*)(ws + plan.claims);
     l.quant = QuantArgs{x, T, D, sr, sc, (uint8_t*)(ws + plan.xq), Dp, (float*)(ws + plan.xs), T, nullptr, 0, nullptr, 0};
     l.e = FewArgs{x,   sr,  (int)T, k,   E,   (int)(T * k), nullptr, nullptr, 0,   0,   D,   I, w1,          w1e, w1u,

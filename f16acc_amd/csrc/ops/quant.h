@@ -35,14 +35,11 @@ __device__ __forceinline__ void quant_rows(const QuantArgs& p, uint32_t group, u
     const int64_t row = total >> 32 ? b / blocks : (int64_t)((uint32_t)b / (uint32_t)blocks), kb = b - row * blocks;
     const int64_t c0 = kb * kBlock + lane * 8;
     const T* x = (const T*)p.x + row * p.sr;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (WIDE && c0 + 8 <= p.cols) {
+    float v[8];
+    if (WIDE && c0 + 8 <= p.cols)
       load_vec(x + c0, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < p.cols) v[i] = (float)x[(c0 + i) * p.sc];
-    }
+    else
+      load_clamped(x, c0, p.cols, p.sc, v);
     uint32_t m = abs_bits(v[0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
@@ -179,9 +176,14 @@ __device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32
     } o;
     if (p.s_c == 1 && c + 16 <= p.cols) {
       __builtin_memcpy(o.b, s + c, 16);  // one 16-byte load: any alignment goes
-    } else {
+    } else if (p.cols) {  // (inside the row, all in flight together: see load_clamped)
+      uint32_t b[16];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) o.b[k] = c + k < p.cols ? s[(c + k) * p.s_c] : 0;
+      for (int k = 0; k < 16; ++k) b[k] = s[(c + k < p.cols ? c + k : p.cols - 1) * p.s_c];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o.b[k] = c + k < p.cols ? (uint8_t)b[k] : 0;
+    } else {
+      o.v = i32x4{0, 0, 0, 0};
     }
     *(i32x4*)(p.dst + r * p.ld + c) = o.v;
   }
