@@ -20,15 +20,89 @@ constexpr int kQuad = 128; // values of four blocks, whose scales are one dword
 __device__ __forceinline__ uint32_t mx_exponent(uint32_t bits) { return ((umax(bits, kTinyBits) + 0x200000u) >> 23) - 2; }
 __device__ __forceinline__ uint32_t mx_byte(uint32_t bits) { return bits >= kInfBits ? 255u : mx_exponent(bits); }
 
-// Eight values over 2^(e - 127) as e2m1, the first in the lowest bits.
-__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8], uint32_t e) {
-  const float s = __uint_as_float(e << 23);  // (the conversion divides by it)
-  uint32_t r = 0;
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
-}
+// Eight consecutive values of a row as they are held, and what quantising takes of them: the bits of the largest
+// magnitude (as FP32's, so NaN > infinity > finite) and the e2m1 values.  16-bit types stay in pairs: their
+// magnitudes compare as integers, two at a time, and the conversion takes pairs.
+template <class T>
+struct Eight {
+  static constexpr bool PAIRS = sizeof(T) == 2;
+  static constexpr int N = PAIRS ? 4 : 8;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef T Pair __attribute__((ext_vector_type(2)));
+  uint32_t d[N];
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(d, p, sizeof(d)); }  // (from any address)
+  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t cols, int64_t stride) {  // zero past cols
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = row[(c + i < cols ? c + i : cols - 1) * stride];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = c + i < cols ? t[i] : (T)0.0f;
+    __builtin_memcpy(d, t, sizeof(d));
+  }
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {  // of magnitudes, element by element
+    if constexpr (PAIRS)
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    else
+      return umax(a, b);
+  }
+  __device__ __forceinline__ static uint32_t magnitude(uint32_t v) { return v & (PAIRS ? 0x7fff7fffu : 0x7fffffffu); }
+  // FP32's bits of a magnitude: of a 16-bit one in the low half.
+  __device__ __forceinline__ static uint32_t bits(uint32_t m) {
+    if constexpr (!PAIRS)
+      return m;
+    else if constexpr (std::is_same_v<T, bf16>)
+      return m << 16;
+    else
+      return __float_as_uint((float)__builtin_bit_cast(f16, (uint16_t)m));
+  }
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = magnitude(d[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = larger(m, magnitude(d[i]));
+    if constexpr (PAIRS) m = umax(m >> 16, m & 0xffffu);
+    return bits(m);
+  }
+  __device__ __forceinline__ uint32_t packed(uint32_t e) const {
+    const float s = __uint_as_float(e << 23);  // (the conversion divides by it)
+    uint32_t r = 0;
+    if constexpr (!PAIRS) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(d[0]), __uint_as_float(d[1]), s, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(d[2]), __uint_as_float(d[3]), s, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(d[4]), __uint_as_float(d[5]), s, 2);
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(d[6]), __uint_as_float(d[7]), s, 3);
+    } else if constexpr (std::is_same_v<T, bf16>) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(Pair, d[0]), s, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(Pair, d[1]), s, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(Pair, d[2]), s, 2);
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(Pair, d[3]), s, 3);
+    } else {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(Pair, d[0]), s, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(Pair, d[1]), s, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(Pair, d[2]), s, 2);
+      return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(Pair, d[3]), s, 3);
+    }
+  }
+  // Column j of eight rows.
+  __device__ __forceinline__ static Eight column(const Eight (&v)[8], int j) {
+    Eight c;
+    if constexpr (PAIRS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = v[2 * i].d[j / 2], b = v[2 * i + 1].d[j / 2];
+        c.d[i] = j % 2 ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c.d[i] = v[i].d[j];
+    }
+    return c;
+  }
+};
 
 // Eight e2m1 values times 2^(e - 127); NaN where e is 255.
 __device__ __forceinline__ void unpack_e2m1(uint32_t q, uint32_t e, float (&v)[8]) {
@@ -39,15 +113,6 @@ __device__ __forceinline__ void unpack_e2m1(uint32_t q, uint32_t e, float (&v)[8
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     v[i] = e == 255u ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(t[i], (int)e - 127);
-}
-
-// Eight consecutive elements from any address (a 16-byte load goes from any).
-template <class T>
-__device__ __forceinline__ void load_any(const T* p, float (&v)[8]) {
-  T t[8];
-  __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
 }
 
 // Scale bytes: that of (row, block b) at s[row * row_stride + b / 4 * quad_stride + b % 4], both strides
@@ -100,16 +165,13 @@ __device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t gro
     if (row >= p.rows) continue;
     const int64_t c0 = kq * kQuad + lane * 8;
     const T* x = (const T*)p.x + row * p.sr;
-    float v[8];
+    Eight<T> v;
     if (WIDE && c0 + 8 <= p.cols)
-      load_any(x + c0, v);
+      v.load(x + c0);
     else
-      load_clamped(x, c0, p.cols, p.sc, v);
-    uint32_t m = abs_bits(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(v[i]));
-    m = quad_umax(m);
-    *(uint32_t*)(p.q + row * p.ldq + c0 / 2) = pack_e2m1(v, mx_exponent(m));
+      v.load(x, c0, p.cols, p.sc);
+    const uint32_t m = quad_umax(v.largest());
+    *(uint32_t*)(p.q + row * p.ldq + c0 / 2) = v.packed(mx_exponent(m));
     // (a block past the columns holds zeros: its byte is that of 2^-102, never NaN's)
     const uint32_t scales = quad_bytes(mx_byte(m), lane);
     if (lane == 0) *(uint32_t*)(p.s.s + row * p.s.row + kq * p.s.quad) = scales;
@@ -175,13 +237,13 @@ __global__ __launch_bounds__(256) void mx_prepare_kernel(MxQuantArgs q, MxScaleA
 
 struct Fp4Source {};  // x of MxQuantArgs held in 4 bits
 
-// Eight values of a row from column c (a multiple of 8).
-template <class T, bool WIDE>
-__device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t c, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-  if (r >= p.rows || c >= p.cols) return;
-  if constexpr (std::is_same_v<T, Fp4Source>) {
+// Eight values of a row from column c (a multiple of 8), as T.
+template <class S, class T>
+__device__ __forceinline__ Eight<T> mx_load(const MxQuantArgs& p, int64_t r, int64_t c) {
+  Eight<T> v;
+  v.zero();
+  if (r >= p.rows || c >= p.cols) return v;
+  if constexpr (std::is_same_v<S, Fp4Source>) {
     const uint8_t* q = (const uint8_t*)p.x + r * p.sr + c / 2 * p.sc;
     uint32_t u = 0, b[4];
     const int64_t last = (p.cols - 1 - c) / 2;  // (inside the row, all in flight together: see load_clamped)
@@ -189,41 +251,43 @@ __device__ __forceinline__ void mx_load(const MxQuantArgs& p, int64_t r, int64_t
     for (int i = 0; i < 4; ++i) b[i] = q[(i < last ? i : last) * p.sc];
 #pragma unroll
     for (int i = 0; i < 4; ++i) u |= i <= last ? b[i] << (8 * i) : 0;
-    unpack_e2m1(u, p.xs[r * p.xsr + c / kMx * p.xsc], v);
+    float f[8];
+    unpack_e2m1(u, p.xs[r * p.xsr + c / kMx * p.xsc], f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i >= p.cols) v[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) v.d[i] = c + i < p.cols ? __float_as_uint(f[i]) : 0;
   } else {
-    const T* x = (const T*)p.x + r * p.sr;
-    if (WIDE && c + 8 <= p.cols)
-      load_any(x + c, v);
-    else
-      load_clamped(x, c, p.cols, p.sc, v);
+    v.load((const T*)p.x + r * p.sr, c, p.cols, p.sc);
   }
+  return v;
 }
 
 // A 128 x 128 tile a workgroup, read once: quantised along its rows (q), its columns (qt, the
 // result transposed) or both.  Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's block is four
 // lanes, a column's block one wave's 32 rows, four DPP rows apart, so no maximum leaves a wave.
-template <class T, bool WIDE>
+template <class S, bool WIDE>
 __device__ __forceinline__ void mx_quant_tile(const MxQuantArgs& p, uint32_t index) {
+  typedef std::conditional_t<std::is_same_v<S, Fp4Source>, float, S> T;  // (4-bit values as FP32)
+  typedef Eight<T> E;
   // The transposed tile, 64 bytes a column: 16-byte unit u (a wave's rows) of column col at u ^ (col / 8 % 4).
   __shared__ __align__(16) uint8_t tile[kQuad * 64];
   __shared__ __align__(4) uint8_t bytes[kQuad * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = tid >> 4, c = tid & 15;
   const uint32_t tiles_k = (uint32_t)cdiv(p.cols, kQuad);
   const int64_t rb = index / tiles_k, kb = index - rb * tiles_k, r0 = rb * kQuad + r * 8, c0 = kb * kQuad + c * 8;
-  float v[8][8];
+  E v[8];
+  if (WIDE && rb * kQuad + kQuad <= p.rows && kb * kQuad + kQuad <= p.cols) {  // (the tile's, for all threads)
+    const T* x = (const T*)p.x + r0 * p.sr + c0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) mx_load<T, WIDE>(p, r0 + i, c0, v[i]);
+    for (int i = 0; i < 8; ++i) v[i].load(x + i * p.sr);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = mx_load<S, T>(p, r0 + i, c0);
+  }
   if (p.q) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t m = abs_bits(v[i][0]);
-#pragma unroll
-      for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[i][j]));
-      m = quad_umax(m);
-      const uint32_t q = pack_e2m1(v[i], mx_exponent(m)), s = quad_bytes(mx_byte(m), lane);
+      const uint32_t m = quad_umax(v[i].largest());
+      const uint32_t q = v[i].packed(mx_exponent(m)), s = quad_bytes(mx_byte(m), lane);
       if (r0 + i < p.rows) {
         *(uint32_t*)(p.q + (r0 + i) * p.ldq + c0 / 2) = q;
         if (c == 0) *(uint32_t*)(p.s.s + (r0 + i) * p.s.row + kb * p.s.quad) = s;
@@ -231,15 +295,19 @@ __device__ __forceinline__ void mx_quant_tile(const MxQuantArgs& p, uint32_t ind
     }
   }
   if (!p.qt) return;
+  uint32_t most[E::N];  // of the columns, as the values are held
+#pragma unroll
+  for (int d = 0; d < E::N; ++d) {
+    uint32_t m = E::magnitude(v[0].d[d]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = E::larger(m, E::magnitude(v[i].d[d]));
+    m = E::larger(m, (uint32_t)__shfl_xor((int)m, 16));
+    most[d] = E::larger(m, (uint32_t)__shfl_xor((int)m, 32));
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float col[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
-    uint32_t m = abs_bits(col[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = umax(m, abs_bits(col[i]));
-    m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-    *(uint32_t*)(tile + (c * 8 + j) * 64 + (wave ^ (c & 3)) * 16 + (r & 3) * 4) = pack_e2m1(col, mx_exponent(m));
+    const uint32_t m = E::bits(E::PAIRS ? most[j * E::N / 8] >> 16 * (j % 2) & 0xffffu : most[j * E::N / 8]);
+    *(uint32_t*)(tile + (c * 8 + j) * 64 + (wave ^ (c & 3)) * 16 + (r & 3) * 4) = E::column(v, j).packed(mx_exponent(m));
     if (lane < 16) bytes[(c * 8 + j) * 4 + wave] = (uint8_t)mx_byte(m);
   }
   __syncthreads();
@@ -255,10 +323,10 @@ __device__ __forceinline__ void mx_quant_tile(const MxQuantArgs& p, uint32_t ind
 }
 
 // One matrix or two: the first `first` workgroups have a's tiles.
-template <class T, bool WIDE>
+template <class S, bool WIDE>
 __global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs a, MxQuantArgs b, uint32_t first) {
   const bool is_a = blockIdx.x < first;
-  mx_quant_tile<T, WIDE>(is_a ? a : b, is_a ? blockIdx.x : blockIdx.x - first);
+  mx_quant_tile<S, WIDE>(is_a ? a : b, is_a ? blockIdx.x : blockIdx.x - first);
 }
 
 // The values of a 4-bit matrix, eight a thread.

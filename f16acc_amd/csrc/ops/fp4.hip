@@ -51,8 +51,8 @@ int matrix_check(const MxQuantArgs& p, int type) {
 template <class T>
 int launch_tile(const MxQuantArgs& a, const MxQuantArgs& b, hipStream_t stream) {
   const uint32_t first = (uint32_t)tiles_of(a), all = first + (uint32_t)tiles_of(b);
-  if (std::is_same_v<T, Fp4Source> || (a.sc == 1 && (b.sc == 1 || !b.rows)))
-    hipLaunchKernelGGL((mx_quant_tile_kernel<T, true>), dim3(all), dim3(256), 0, stream, a, b, first);
+  if (!std::is_same_v<T, Fp4Source> && a.sc == 1 && (b.sc == 1 || !b.rows))
+    hipLaunchKernelGGL((mx_quant_tile_kernel<T, !std::is_same_v<T, Fp4Source>>), dim3(all), dim3(256), 0, stream, a, b, first);
   else
     hipLaunchKernelGGL((mx_quant_tile_kernel<T, false>), dim3(all), dim3(256), 0, stream, a, b, first);
   return hip_status();

@@ -86,16 +86,13 @@ __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) 
       const int t = i / nk, kq = i - t * nk;
       const int64_t k = (int64_t)kq * kQuad + 8 * c;
       const T* x = (const T*)p.x + t * p.ldx;
-      float v[8];
+      Eight<T> v;
       if (k + 8 <= p.K)
-        load_any(x + k, v);
+        v.load(x + k);
       else
-        load_clamped(x, k, p.K, 1, v);
-      uint32_t m = abs_bits(v[0]);
-#pragma unroll
-      for (int j = 1; j < 8; ++j) m = umax(m, abs_bits(v[j]));
-      m = quad_umax(m);
-      *(uint32_t*)(tokens + t * row + kq * 64 + 4 * c) = pack_e2m1(v, mx_exponent(m));
+        v.load(x, k, p.K, 1);
+      const uint32_t m = quad_umax(v.largest());
+      *(uint32_t*)(tokens + t * row + kq * 64 + 4 * c) = v.packed(mx_exponent(m));
       const uint32_t s = quad_bytes(mx_byte(m), lane);
       if (c == 0) *(uint32_t*)(scales + (t * nk + kq) * 4) = s;
     }
