@@ -30,6 +30,18 @@ __device__ __forceinline__ void load8(const T* p, int64_t stride, int64_t k, int
   else
     load_clamped(p, k, D, stride, v);
 }
+// ... as they are.
+template <class T>
+__device__ __forceinline__ void fetch8(const T* p, int64_t stride, int64_t k, int64_t D, bool wide, T (&v)[8]) {
+  if (wide && k + 8 <= D) {
+    __builtin_memcpy(v, p + k, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[(k + i < D ? k + i : D - 1) * stride];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < D ? v[i] : (T)0.0f;
+  }
+}
 
 // logits[t][e] = sum over d of x[t][d] r[e][d], summed in 64 bits and rounded once to FP32: products of 16-bit and
 // FP32 values are exact there, so a token's logits, and with them the choice of its experts, do not depend
@@ -45,21 +57,26 @@ __global__ __launch_bounds__(64 * W) void router_kernel(RouterArgs p) {
   const int e = e0 + l16 < p.E ? e0 + l16 : p.E - 1;
   const T* x = (const T*)p.x + t * p.sr;
   const R* r = (const R*)p.r + e * p.re;
+  constexpr int AHEAD = 2;  // chunks in flight
   f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-  float a[8], b[8];
-  const int64_t step = 32 * W;
-  int64_t k = 32 * wave + 8 * g;
-  load8(x, p.sc, k, p.D, p.wide, a);
-  load8(r, p.rd, k, p.D, p.wide, b);
-  for (int64_t c = 32 * wave; c < p.D; c += step) {
-    float ca[8], cb[8];
+  T a[AHEAD][8];
+  R b[AHEAD][8];
+  auto load = [&](int i, int64_t chunk) {
+    fetch8(x, p.sc, chunk + 8 * g, p.D, p.wide, a[i]);
+    fetch8(r, p.rd, chunk + 8 * g, p.D, p.wide, b[i]);
+  };
+  constexpr int64_t step = 32 * W;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ca[i] = a[i], cb[i] = b[i];
-    k += step;
-    load8(x, p.sc, k, p.D, p.wide, a);
-    load8(r, p.rd, k, p.D, p.wide, b);
+  for (int i = 0; i < AHEAD; ++i) load(i, 32 * wave + i * step);
+#pragma unroll 1
+  for (int64_t c = 32 * wave; c < p.D; c += AHEAD * step) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)cb[i], (double)ca[i], acc, 0, 0, 0);
+    for (int i = 0; i < AHEAD; ++i) {  // (past the end zeros)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)b[i][k], (double)(float)a[i][k], acc, 0, 0, 0);
+      if (c + AHEAD * step < p.D) load(i, c + (AHEAD + i) * step);
+    }
   }
   sums[wave][lane] = acc;
   __syncthreads();

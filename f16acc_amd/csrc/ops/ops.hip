@@ -385,7 +385,7 @@ template <class T, class R>
 int launch_router(RouterArgs p, hipStream_t stream) {
   router_wide<T, R>(p);
   const dim3 grid((uint32_t)cdiv(p.T, 16), (uint32_t)cdiv(p.E, 16));
-  hipLaunchKernelGGL((router_kernel<T, R, 8>), grid, dim3(512), 0, stream, p);
+  hipLaunchKernelGGL((router_kernel<T, R, 16>), grid, dim3(1024), 0, stream, p);
   return hip_status();
 }
 
