@@ -76,6 +76,22 @@ def test_quantize_every_tie_and_the_extremes():
         q, s = fp4.quantize(y)
         same_quantised(q, s, y)
         assert bool((ref.scales(s) == scale).all())
+    for dtype, scales in ((torch.float16, (2.0 ** -12, 2.0 ** -3, 2.0 ** 12)), (torch.bfloat16, (2.0 ** -90, 1.0, 2.0 ** 100))):
+        for scale in scales:
+            y = (x * scale).to(dtype).to(DEV)
+            assert torch.equal(y.float().cpu(), x * scale)
+            same_quantised(*fp4.quantize(y), y)
+            same_quantised(*fp4.quantize(y.t(), transposed=True), y)
+    y = (torch.arange(-96, 96).view(6, 32) * 2.0 ** -24).half().to(DEV)  # binary16's subnormal values
+    same_quantised(*fp4.quantize(y), y)
+    same_quantised(*fp4.quantize(y.t(), transposed=True), y)
+    for dtype in TYPES:  # magnitudes of every size beside each other, zeros of both signs
+        g = torch.Generator().manual_seed(8)
+        big = 15 if dtype == torch.float16 else 120
+        y = torch.ldexp(torch.randn(40, 160, generator=g), torch.randint(-big, big - 4, (40, 160), generator=g)).to(dtype).to(DEV)
+        y[3, :40], y[5, 7] = -0.0, 0.0
+        same_quantised(*fp4.quantize(y), y)
+        same_quantised(*fp4.quantize(y, transposed=True), y.t())
     # the border between two scales: 7 is the next power of two's; zeros, tiny blocks, the largest finite values
     big = torch.finfo(torch.float32).max
     edge = torch.tensor([7.0, 6.9999995, 3.5, 3.4999998, 0.0, 2.0 ** -100, 2.0 ** -101, 1e-40, big, 1.0], device=DEV)
@@ -243,7 +259,8 @@ def test_mm_empty():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,bias", [(1, 1, 1, True), (1, 300, 1536, False), (3, 1537, 250, True), (8, 64, 16, True),
                                         (15, 130, 2000, False), (16, 128, 1040, True), (17, 128, 1040, True),
-                                        (77, 257, 897, True), (150, 400, 512, False), (2, 40, 4500, False), (8, 20, 12288, True)])
+                                        (77, 257, 897, True), (150, 400, 512, False), (2, 40, 4500, False), (8, 20, 12288, True),
+                                        (1, 20, 120000, False), (8, 24, 15000, True), (7, 20, 40000, False)])
 def test_linear_stored_weight(M, N, K, bias, dtype):
     x = normal(M, K, dtype=dtype)
     w, ws = stored(N, K)
@@ -300,6 +317,56 @@ def test_linear_gradients_against_the_formula(M, N, K, dtype):
     only, = torch.autograd.grad(fp4.linear(x, w.detach()), x, dy)
     assert torch.equal(only, dx)
     assert torch.equal(fp4.linear(x.detach(), w.detach()), y)
+
+
+@pytest.mark.parametrize("dtype,wtype", [(torch.bfloat16, torch.float32), (torch.float32, torch.float16), (torch.float16, torch.bfloat16)])
+def test_weights_of_another_type(dtype, wtype):
+    x, w = normal(70, 200, dtype=dtype).requires_grad_(), normal(90, 200, dtype=wtype, seed=2).requires_grad_()
+    dy = normal(70, 90, dtype=dtype, seed=3)
+    y = fp4.linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.dtype == dx.dtype == dtype and dw.dtype == wtype
+    ref.check_product(y, ref.rounded(x), ref.rounded(w))
+    ref.check_product(dx, ref.rounded(dy), ref.rounded(w.t()))
+    ref.check_product(dw, ref.rounded(dy.t()), ref.rounded(x.t()))
+
+
+def test_a_training_step_in_a_graph():
+    """Forward and backward recorded while eager steps of the same leaves come and go; every replay like eager."""
+    x, w, b = normal(64, 160).requires_grad_(), normal(96, 160, seed=2, std=0.1).requires_grad_(), normal(96).requires_grad_()
+    dy = normal(64, 96, seed=3)
+    step = lambda: torch.autograd.grad(fp4.linear(x, w, bias=b), (x, w, b), dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(normal(64, 160, seed=10 + i))
+            dy.copy_(normal(64, 96, seed=20 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(got, step()))
+
+
+def test_several_calls_at_once():
+    """Streams beside each other, every call with its own workspace."""
+    w, ws = stored(700, 1000)
+    xs = [normal(n, 1000, seed=n) for n in (3, 60, 300)]
+    want = [fp4.linear(x, w, ws) for x in xs]
+    torch.cuda.synchronize()
+    outs = []
+    for x in xs:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            outs.append([fp4.linear(x, w, ws) for _ in range(20)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, y) for y, out in zip(want, outs) for o in out)
 
 
 def test_linear_gradients_against_differences():
