@@ -151,7 +151,8 @@ __device__ __forceinline__ uint32_t quad_bytes(uint32_t byte, int lane) {
 // Rows of a matrix in blocks of 1 x 32.  16 lanes take 128 values of a row, 8 each: a 16-byte load a lane (16-bit
 // types), the maximum of four lanes by two exchanges, 4 bytes a lane out.  A workgroup takes 16 quads of a
 // row where a row's scales lie together, 16 rows of a quad where a quad's do: its scales are one piece
-// of 64 bytes either way.
+// of 64 bytes either way.  Bound by memory, 2 bytes read and 0.53 written a value: 8192 x 8192 bfloat16 in 34 us (scales by
+// rows) or 36 (by quads), 5.0 TB/s, where a copy reaches 5.2.
 template <class T, bool WIDE>
 __device__ __forceinline__ void mx_quant_rows(const MxQuantArgs& p, uint32_t group, uint32_t groups) {
   const bool along = p.s.quad == 4;
@@ -264,6 +265,7 @@ __device__ __forceinline__ Eight<T> mx_load(const MxQuantArgs& p, int64_t r, int
 // A 128 x 128 tile a workgroup, read once: quantised along its rows (q), its columns (qt, the
 // result transposed) or both.  Thread (r, c) holds rows 8 r .. 8 r + 7, columns 8 c .. 8 c + 7: a row's block is four
 // lanes, a column's block one wave's 32 rows, four DPP rows apart, so no maximum leaves a wave.
+// 8192 x 8192 bfloat16 in both directions 44 us, 4.7 TB/s (as FP32 values, each load behind its own condition, 69).
 template <class S, bool WIDE>
 __device__ __forceinline__ void mx_quant_tile(const MxQuantArgs& p, uint32_t index) {
   typedef std::conditional_t<std::is_same_v<S, Fp4Source>, float, S> T;  // (4-bit values as FP32)
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(256) void mx_quant_tile_kernel(MxQuantArgs a, MxQua
   mx_quant_tile<S, WIDE>(is_a ? a : b, is_a ? blockIdx.x : blockIdx.x - first);
 }
 
-// The values of a 4-bit matrix, eight a thread.
+// The values of a 4-bit matrix, eight a thread: 8192 x 8192 to bfloat16 in 29 us, 5.9 TB/s of which 4.7 written.
 struct MxValuesArgs {
   const uint8_t* q;
   int64_t q_r, q_c;  // byte strides

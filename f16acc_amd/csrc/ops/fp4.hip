@@ -195,7 +195,19 @@ struct MmPlan4 {
   }
 };
 
-bool few4(int64_t M, int64_t K) { return M <= 16 && small4_lds(M, K) <= kSmall4Lds; }
+// Up to 16 tokens in one kernel as long as its workgroups, 16 weight rows each, do not spend more on
+// quantising the tokens than the preparing launch costs.  In graphs, cold weights, one kernel / tiles, us: 8960 x 1536
+// one token 5.1 / 8.6, eight 7.0 / 8.7, 16 9.5 / 8.6; 4096 x 4096 eight 7.6 / 11.2, 16 10.2 / 11.6; 1536 x 8960 four
+// 8.6 / 12.3, 12 13.4 / 12.1; 14336 x 4096 two 13.1 / 14.9, four 15.5 / 14.8; 28672 x 7168 one 27.8 / 30.3, eight 46 / 30.
+bool few4(int64_t M, int64_t N, int64_t K) {
+  return M <= 16 && K < 65536 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
+}
+
+// Its workgroups have 16 waves where there are no more of them than compute units and K is long enough to give
+// each work; 8 otherwise.  (Not by the number of tokens: a token's sums stay in one order, whatever is beside it.)
+// 16 waves / 8, us: 1536 x 8960 one token 6.8 / 8.1, eight 10.8 / 13.7; 4096 x 4096 one 5.7 / 5.4, eight 7.6 / 8.1;
+// 1536 x 1536 one 3.6 / 3.4, eight 4.1 / 4.2; 8960 x 1536 one 7.8 / 5.1.
+bool few4_wide(int64_t N, int64_t K) { return cdiv(N, 16) <= kCus && quads_of(K) >= 24; }
 
 // The workspace of linear: the quantised tokens and their scales, the weight's scales in the
 // products' order, the weight where its rows have to be copied, the parts of a split of K.
@@ -346,12 +358,12 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   const bool wide = sc == 1;  // (rows of any alignment)
   const LinearPlan4 plan(M, N, K, w, ldw);
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
-  if (few4(M, K) && (sc == 1 || K == 1) && M <= 8) {
+  if (few4(M, N, K) && (sc == 1 || K == 1)) {
     const Small4Args a{x, sr, w, ldw, sw, swn, swb, bias, y, M, N, K};
     const size_t lds = small4_lds(M, K);
     return by_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      if (cdiv(N, 16) <= kCus && quads_of(K) >= 12)
+      if (few4_wide(N, K))
         hipLaunchKernelGGL((linear_fp4_small_kernel<T, 16>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), lds, stream, a);
       else
         hipLaunchKernelGGL((linear_fp4_small_kernel<T, 8>), dim3((uint32_t)cdiv(N, 16)), dim3(512), lds, stream, a);

@@ -2,6 +2,12 @@
 // whole cost.  A workgroup takes 16 weight rows; it quantises the tokens into LDS while its first weights are
 // on their way, its waves deal the quads of blocks among themselves and read the rows straight into the
 // MFMA's registers (64 contiguous bytes a row and instruction).  The waves' sums meet in LDS, in wave order.
+//
+// Measured (kernel time, weights cold): one token through 8960 x 1536 in 5.0 us, of which the weight's 7.3 MB
+// are 1.4 at the copy rate and the rest the latency of a launch, the tokens and the weights, one after another;
+// through 28672 x 7168 in 27.8 us, 3.9 TB/s.  Every workgroup quantises the tokens anew, 0.07 ns a value and
+// compute unit: one that went on to further rows with the same tokens held more registers and lost more than it saved
+// (8960 x 1536 6.7 us, 14336 x 4096 12.7 instead of 12.1).
 #pragma once
 
 #include "common.h"
@@ -21,8 +27,6 @@ struct Small4Args {
   void* y;  // [M][N]
   int64_t M, N, K;
 };
-
-constexpr int kSmall4Lds = 64 * 1024;
 
 // LDS of the quantised tokens: rows of 64 bytes a quad, 16 more to spread them over the banks, then the
 // scales, a dword a quad and row.

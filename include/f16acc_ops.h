@@ -1,6 +1,6 @@
 /*
- * f16acc for MI355X (gfx950): C ABI of the 8-bit block-scaled products and of
- * the mixture-of-experts operators (libf16acc_ops.so).
+ * f16acc for MI355X (gfx950): C ABI of the 8-bit and the 4-bit block-scaled products
+ * and of the mixture-of-experts operators (libf16acc_ops.so).
  *
  * Plain C types only.  Nothing allocates, synchronises or keeps state between
  * calls: outputs and workspaces are the caller's, work is launched on `stream`

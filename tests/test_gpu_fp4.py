@@ -260,7 +260,7 @@ def test_mm_empty():
 @pytest.mark.parametrize("M,N,K,bias", [(1, 1, 1, True), (1, 300, 1536, False), (3, 1537, 250, True), (8, 64, 16, True),
                                         (15, 130, 2000, False), (16, 128, 1040, True), (17, 128, 1040, True),
                                         (77, 257, 897, True), (150, 400, 512, False), (2, 40, 4500, False), (8, 20, 12288, True),
-                                        (1, 20, 120000, False), (8, 24, 15000, True), (7, 20, 40000, False)])
+                                        (1, 20, 65535, True), (1, 20, 120000, False), (8, 24, 15000, True), (7, 20, 40000, False)])
 def test_linear_stored_weight(M, N, K, bias, dtype):
     x = normal(M, K, dtype=dtype)
     w, ws = stored(N, K)
@@ -268,6 +268,20 @@ def test_linear_stored_weight(M, N, K, bias, dtype):
     y = fp4.linear(x, w, ws, b)
     assert y.dtype == dtype
     ref.check_product(y, ref.rounded(x), ref.values(w, ws, K), b)
+
+
+@pytest.mark.parametrize("N,K", [(40, 100), (530, 3000), (520, 3200), (4112, 2048), (4096, 4000), (4100, 4097)])
+def test_linear_where_few_tokens_become_many(N, K):
+    """Up to 16 tokens are one kernel's, of 8 or 16 waves, fewer where the weight is large; there a token's result is the same
+    whatever is beside it."""
+    x, (w, ws) = normal(17, K, dtype=torch.bfloat16), stored(N, K)
+    bias = normal(N, dtype=torch.bfloat16, seed=3)
+    values, wv = ref.values(*fp4.quantize(x), K), ref.values(w, ws, K)
+    one = fp4.linear(x[:1], w, ws, bias)
+    for M in (1, 2, 7, 8, 9, 15, 16, 17):
+        y = fp4.linear(x[:M], w, ws, bias)
+        ref.check_product(y, values[:M], wv, bias)
+        assert M > 7 or torch.equal(y[:1], one)
 
 
 @pytest.mark.parametrize("M", [1, 7, 12, 40, 200])
