@@ -95,19 +95,22 @@ __global__ __launch_bounds__(64 * W) void router_kernel(RouterArgs p) {
 // ---------------------------------------------------------------------------
 // The layer of at most 4 tokens and 16 slots in two launches.  The first sums the logits, an expert a workgroup, and
 // quantises the tokens beside it.  In the second every workgroup chooses the tokens' experts for itself (a
-// wave a token); the first ones take 16 columns of the result each, the others 16 hidden columns of one
-// expert, gate and up.  The former load their weights, which depend on the choice alone, before they wait for
+// wave a token); the first ones take 16 hidden columns of one expert, gate and up, the last ones 16 columns of
+// the result each.  The latter load their weights, which depend on the choice alone, before they wait for
 // the hidden values.
 //
 // The wait ends: a piece of hidden columns is claimed by who computes it, and who computes one waits for nobody.
 // Before it waits, a workgroup sees that every piece is claimed and computes those that are not, so it
-// takes neither a number of workgroups at once nor an order of theirs.  (And where not all of them fit at once, the
-// first ones make themselves useful: 605 workgroups, 27.7 us with them last, 25.0 so.)
+// takes neither a number of workgroups at once nor an order of theirs.  (An order of them is a matter of speed: with the
+// result's workgroups first, those that fit beside none of the others raced for their pieces, 124 us instead of
+// 48 for two tokens, 8 of 64 experts, 2048 x 1024.)
 //
-// Measured, in a graph: one token through 6 of 64 experts, 2048 x 1024, 38 MB of weights (7.6 us at the copy rate):
-// 21.6 us, against 32 for the router's product, route and experts one after another.  In it the logits take 4 us, the
-// choice 3.5, gate and up 5 to 7, at the rate of memory, and 9 pass from their last sums to the result: stores past
-// the L2, a count, a poll, hidden values from memory, each a trip of a microsecond or two.
+// Measured, in a graph, against the router's product, route and experts one after another, us: 64 experts, 2048 x 1024,
+// one token, 2 of them 17 / 26, 6 (38 MB of weights, 7.6 us at the copy rate) 22 / 31, 8 31 / 33, two tokens,
+// 6 38 / 42, 8 50 / 46; 128 experts, 4096 x 1536, one token, 1 of them 23 / 37, 8 53 / 62, four tokens, 4 90 / 86; 32
+// experts, 7168 x 2048, one token, 8 of them 88 / 105.  Of 22 us the logits take 4, the choice 3.5, gate and up 5
+// to 7, at the rate of memory, and 9 pass from their last sums to the result: stores past the L2, a count, a
+// poll, hidden values from memory, each a trip of a microsecond or two.
 // ---------------------------------------------------------------------------
 
 // The counters, in lines of their own: adds to one address follow each other at some 10 ns.
@@ -463,8 +466,8 @@ __global__ __launch_bounds__(64 * LayerFew::W, 4) void layer_few_kernel(LayerArg
   __shared__ __align__(16) char smem[L::SMEM];  // (before its uses above: the rows of the routing)
   static_assert(kFewTokens * 64 * V * 4 <= L::SMEM, "the routing's rows");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hidden = a.e.slots * a.pieces, downs = (int)gridDim.x - hidden, block = (int)blockIdx.x - downs;
-  if (tid == 0 && block >= 0)
+  const int hidden = a.e.slots * a.pieces, block = (int)blockIdx.x;
+  if (tid == 0 && block < hidden)
     c.taken = __hip_atomic_exchange(&a.claims[block].taken, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (wave < a.e.T) {
     int id;
@@ -479,11 +482,11 @@ __global__ __launch_bounds__(64 * LayerFew::W, 4) void layer_few_kernel(LayerArg
   if (wave == 0) list_choice(c, a.e.slots, a.e.k, a.e.E, lane);
   __syncthreads();
   const int items = c.count * a.pieces;
-  if (block >= 0) {
+  if (block < hidden) {
     if (block < items && !c.taken) L::gate_up(a, c, smem, block, tid);
     return;
   }
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = (int64_t)(block - hidden) * 16;
   const int nb = L::blocks_at_once(a.e);
   L::Ahead f;
   f.load_all(a.e, c, 0, nb, n0, wave, lane);
