@@ -45,27 +45,35 @@ __device__ __forceinline__ void fetch8(const T* p, int64_t stride, int64_t k, in
 
 // logits[t][e] = sum over d of x[t][d] r[e][d], summed in 64 bits and rounded once to FP32: products of 16-bit and
 // FP32 values are exact there, so a token's logits, and with them the choice of its experts, do not depend
-// on the batch it comes in.  16 tokens by 16 experts a workgroup on v_mfma_f64_16x16x4_f64; the waves deal the
+// on the batch it comes in.  16 F tokens by 16 F experts a workgroup on v_mfma_f64_16x16x4_f64; the waves deal the
 // chunks of 32 columns, a lane loads eight of a row, and their sums meet in LDS in wave order.  512 tokens of 64
 // experts, 2048 wide: 11 us in 16 waves, two chunks ahead each (15 in eight, with one), of 8 MB and 2 us of matrix
-// instructions: the launch, and two rounds of loads.
-template <class T, class R, int W>
+// instructions: the launch, and two rounds of loads.  16384 tokens of 256 experts: 340 us with F = 2, of which
+// the matrix instructions take 220 at their peak.
+template <class T, class R, int W, int F>
 __global__ __launch_bounds__(64 * W) void router_kernel(RouterArgs p) {
-  __shared__ f64x4 sums[W][64];
+  __shared__ f64x4 sums[W][F * F][64];
+  static_assert(F * F <= W, "a wave joins a fragment's sums");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
-  const int64_t t0 = (int64_t)blockIdx.x * 16;
-  const int e0 = (int)blockIdx.y * 16;
-  const int64_t t = t0 + l16 < p.T ? t0 + l16 : p.T - 1;
-  const int e = e0 + l16 < p.E ? e0 + l16 : p.E - 1;
-  const T* x = (const T*)p.x + t * p.sr;
-  const R* r = (const R*)p.r + e * p.re;
+  const int64_t t0 = (int64_t)blockIdx.x * 16 * F + l16;
+  const int e0 = (int)blockIdx.y * 16 * F;
+  const T* x[F];
+  const R* r[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    x[f] = (const T*)p.x + (t0 + 16 * f < p.T ? t0 + 16 * f : p.T - 1) * p.sr;
+    r[f] = (const R*)p.r + (e0 + 16 * f + l16 < p.E ? e0 + 16 * f + l16 : p.E - 1) * p.re;
+  }
   constexpr int AHEAD = 2;  // chunks in flight
-  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-  T a[AHEAD][8];
-  R b[AHEAD][8];
+  f64x4 acc[F][F] = {};
+  T a[AHEAD][F][8];
+  R b[AHEAD][F][8];
   auto load = [&](int i, int64_t chunk) {
-    fetch8(x, p.sc, chunk + 8 * g, p.D, p.wide, a[i]);
-    fetch8(r, p.rd, chunk + 8 * g, p.D, p.wide, b[i]);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      fetch8(x[f], p.sc, chunk + 8 * g, p.D, p.wide, a[i][f]);
+      fetch8(r[f], p.rd, chunk + 8 * g, p.D, p.wide, b[i][f]);
+    }
   };
   constexpr int64_t step = 32 * W;
 #pragma unroll
@@ -76,19 +84,27 @@ __global__ __launch_bounds__(64 * W) void router_kernel(RouterArgs p) {
     for (int i = 0; i < AHEAD; ++i) {  // (past the end zeros)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)b[i][k], (double)(float)a[i][k], acc, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < F; ++m)
+#pragma unroll
+          for (int n = 0; n < F; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)b[i][m][k], (double)(float)a[i][n][k],
+                                                             acc[m][n], 0, 0, 0);
       if (c + AHEAD * step < p.D) load(i, c + (AHEAD + i) * step);
     }
   }
-  sums[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0 || t0 + l16 >= p.T) return;
 #pragma unroll
-  for (int i = 1; i < W; ++i) acc += sums[i][lane];
+  for (int f = 0; f < F * F; ++f) sums[wave][f][lane] = acc[f / F][f % F];
+  __syncthreads();
+  const int64_t t = t0 + 16 * (wave % F);
+  if (wave >= F * F || t >= p.T) return;
+  f64x4 sum = sums[0][wave][lane];
+#pragma unroll
+  for (int i = 1; i < W; ++i) sum += sums[i][wave][lane];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = e0 + g + 4 * i;
-    if (row < p.E) p.logits[(t0 + l16) * p.E + row] = (float)acc[i];
+    const int row = e0 + 16 * (wave / F) + g + 4 * i;
+    if (row < p.E) p.logits[t * p.E + row] = (float)sum[i];
   }
 }
 

@@ -381,11 +381,17 @@ void router_wide(RouterArgs& p) {
   p.wide = p.sc == 1 && p.rd == 1 && aligned16(p.x) && aligned16(p.r) && p.sr * (int64_t)sizeof(T) % 16 == 0 &&
            p.re * (int64_t)sizeof(R) % 16 == 0;
 }
+// Four waves of 32 x 32 where there are enough workgroups of them, 16 of 16 x 16 otherwise; 32 x 32 / 16 x 16, 2048 wide, us:
+// 16384 tokens of 256 experts 342 / 528, of 64 108 / 136, 4096 of 256 (4096 wide) 201 / 245, of 64 40 / 29.
 template <class T, class R>
 int launch_router(RouterArgs p, hipStream_t stream) {
   router_wide<T, R>(p);
-  const dim3 grid((uint32_t)cdiv(p.T, 16), (uint32_t)cdiv(p.E, 16));
-  hipLaunchKernelGGL((router_kernel<T, R, 16>), grid, dim3(1024), 0, stream, p);
+  if (cdiv(p.T, 32) * cdiv(p.E, 32) >= 4 * kCus)
+    hipLaunchKernelGGL((router_kernel<T, R, 4, 2>), dim3((uint32_t)cdiv(p.T, 32), (uint32_t)cdiv(p.E, 32)), dim3(256),
+                       0, stream, p);
+  else
+    hipLaunchKernelGGL((router_kernel<T, R, 16, 1>), dim3((uint32_t)cdiv(p.T, 16), (uint32_t)cdiv(p.E, 16)), dim3(1024),
+                       0, stream, p);
   return hip_status();
 }
 

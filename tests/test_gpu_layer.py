@@ -49,6 +49,29 @@ def test_layer(T, E, k, D, I, dtype):
     check_layer(y, x, router, k, w)
 
 
+@pytest.mark.parametrize("T,E,k,D,I", [(2, 16, 8, 256, 4096), (4, 9, 4, 1100, 2000), (1, 20, 16, 300, 3000)])
+def test_more_pieces_than_workgroups_at_once(T, E, k, D, I):
+    x, router, w = layer(T, E, D, I, torch.bfloat16)
+    for _ in range(3):
+        check_layer(moe.layer(x, router, k, *w), x, router, k, w)
+
+
+@pytest.mark.parametrize("T,E,D,dtype,rtype", [(2017, 490, 100, torch.float16, torch.float16),
+                                               (1000, 1024, 130, torch.bfloat16, torch.float32),
+                                               (33000, 20, 48, torch.float32, torch.bfloat16)])
+def test_many_logits(T, E, D, dtype, rtype):
+    """Sums of whole numbers, exact in any order: tiles of 32 tokens and 32 experts, ragged at their ends."""
+    g = torch.Generator().manual_seed(T)
+    x = torch.randint(-3, 4, (T, D), generator=g).to(dtype).to(DEV)
+    router = torch.randint(-3, 4, (E, D), generator=g).to(rtype).to(DEV) / 16
+    w1, s1 = weight(1, 2, 16, D)
+    w2, s2 = weight(1, D, 16)
+    scale = s2.repeat(E, 1, 1) * torch.exp2(torch.arange(E, device=DEV) % 16).float()[:, None, None]  # the choice shows
+    w = (w1.expand(E, 2, 16, D).contiguous(), s1.repeat(E, 1, 1, 1), w2.expand(E, D, 16).contiguous(), scale)
+    weights, ids = moe.route((x.double() @ router.double().t()).float(), 2)
+    assert torch.equal(moe.layer(x, router, 2, *w), moe.experts(x, weights, ids, *w))
+
+
 @pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 33])
 @pytest.mark.parametrize("dtype,rtype", list(itertools.product(TYPES, TYPES)))
 def test_router_types(T, dtype, rtype):
