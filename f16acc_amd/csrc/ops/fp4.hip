@@ -15,6 +15,8 @@ namespace {
 
 int64_t quads_of(int64_t v) { return cdiv(v, kQuad); }
 
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;  // a launch has fewer
+
 uint32_t grid_of(int64_t units, int64_t per_group) {
   const int64_t groups = cdiv(units, per_group);
   return (uint32_t)(groups < 16 * kCus ? groups : 16 * kCus);
@@ -44,7 +46,7 @@ int matrix_check(const MxQuantArgs& p, int type) {
   if (!p.q && !p.qt) return F16ACC_OPS_E_ARG;
   if (p.q && (rc = out4_check(p.q, p.ldq, p.cols, p.s))) return rc;
   if (p.qt && (rc = out4_check(p.qt, p.ldqt, p.rows, p.st))) return rc;
-  return tiles_of(p) > 0x3fffffff ? F16ACC_OPS_E_UNSUPPORTED : 0;
+  return tiles_of(p) >= kMaxThreads / 512 ? F16ACC_OPS_E_UNSUPPORTED : 0;  // (two matrices, 256 threads a tile)
 }
 
 // a and b (rows 0: none), whose tiles are wanted transposed.
@@ -89,6 +91,8 @@ constexpr TileInfo kTiles[] = {
     {64, 128, 256, 2, 2.03, 0.491, 0.46}, {64, 64, 256, 3, 1.97, 0.369, 0.36}, {32, 64, 256, 3, 1.26, 0.349, 0.4},
 };
 constexpr int kNumTiles = sizeof(kTiles) / sizeof(kTiles[0]);
+constexpr int kThreads[kNumTiles] = {Tile0::THREADS, Tile1::THREADS, Tile2::THREADS,
+                                     Tile3::THREADS, Tile4::THREADS, Tile5::THREADS};
 
 struct Plan {
   int tile, ksplit, splits;  // ksplit 0: not split
@@ -134,6 +138,11 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int tile, int splits) {
     }
   }
   return best;
+}
+
+// Whether a launch holds the product's tiles.
+bool launches(const Plan& plan, int64_t M, int64_t N) {
+  return cdiv(M, kTiles[plan.tile].bm) * cdiv(N, kTiles[plan.tile].bn) < kMaxThreads / kThreads[plan.tile];
 }
 
 size_t parts_bytes(const Plan& plan, int64_t M, int64_t N) {
@@ -200,7 +209,7 @@ struct MmPlan4 {
 // one token 5.1 / 8.6, eight 7.0 / 8.7, 16 9.5 / 8.6; 4096 x 4096 eight 7.6 / 11.2, 16 10.2 / 11.6; 1536 x 8960 four
 // 8.6 / 12.3, 12 13.4 / 12.1; 14336 x 4096 two 13.1 / 14.9, four 15.5 / 14.8; 28672 x 7168 one 27.8 / 30.3, eight 46 / 30.
 bool few4(int64_t M, int64_t N, int64_t K) {
-  return M <= 16 && K < 65536 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
+  return M <= 16 && K < 65536 && N < kMaxThreads / 32 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
 }
 
 // Its workgroups have 16 waves where there are no more of them than compute units and K is long enough to give
@@ -307,6 +316,7 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
       return rc ? rc : F16ACC_OPS_E_UNSUPPORTED;
   }
   const MmPlan4 plan(in[0], in[1], K, tile, splits);
+  if (!launches(plan.plan, M, N)) return F16ACC_OPS_E_UNSUPPORTED;
   if (plan.total && (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total)) return F16ACC_OPS_E_WORKSPACE;
   char* ws = (char*)workspace;
   hipStream_t stream = (hipStream_t)stream_;
@@ -357,6 +367,7 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   hipStream_t stream = (hipStream_t)stream_;
   const bool wide = sc == 1;  // (rows of any alignment)
   const LinearPlan4 plan(M, N, K, w, ldw);
+  if (!launches(plan.plan, M, N)) return F16ACC_OPS_E_UNSUPPORTED;
   if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   if (few4(M, N, K) && (sc == 1 || K == 1)) {
     const Small4Args a{x, sr, w, ldw, sw, swn, swb, bias, y, M, N, K};

@@ -358,9 +358,7 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void mm_fp4_kernel(Mx4Args p) {
 
 template <class C>
 int launch_mm_fp4(Mx4Args p, hipStream_t stream, int splits) {
-  const int64_t tiles = cdiv(p.M, C::BM) * cdiv(p.N, C::BN);
-  if (tiles > 0x7fffffff) return F16ACC_OPS_E_UNSUPPORTED;
-  const dim3 grid((uint32_t)tiles, (uint32_t)splits);
+  const dim3 grid((uint32_t)(cdiv(p.M, C::BM) * cdiv(p.N, C::BN)), (uint32_t)splits);
   if (p.ksplit) p.c = p.parts, p.scm = p.N, p.scn = 1, p.bias = nullptr, p.ctype = F16ACC_TYPE_F32;
   switch (p.ctype) {
     case F16ACC_TYPE_F16: hipLaunchKernelGGL((mm_fp4_kernel<C, f16>), grid, dim3(C::THREADS), 0, stream, p); break;

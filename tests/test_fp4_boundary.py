@@ -32,6 +32,8 @@ def test_quantisation_checks():
         assert f(ldq=100) == f(ldq=192) == f(ldq=64) == f(q=264) == f(s=258) == f(sr=6) == _ops.E_UNSUPPORTED
         assert f(qt=256, ldqt=128, st=256) == f(qt=260, ldqt=64, st=256) == f(rows=1 << 41) == _ops.E_UNSUPPORTED
         assert f(qt=256, ldqt=64 << 30, st=256, rows=128 << 30, q=None) == _ops.E_UNSUPPORTED
+        big = dict(q=None, qt=256, st=256, ldqt=64 << 14, rows=1 << 21)  # more tiles than a launch holds
+        assert f(cols=1 << 17, **big) == _ops.E_UNSUPPORTED
         assert f(rows=0) == f(cols=0) == 0
     assert _ops.fp4_quant(None, None, 0, None) == _ops.E_ARG
 
@@ -65,6 +67,8 @@ def test_mm_checks():
     assert call(K=1 << 24, xr=1 << 23, wr=1 << 23) == call(M=1 << 31) == call(N=1 << 31) == _ops.E_UNSUPPORTED
     assert call(sxq=6) == call(sxq=4, sxm=6) == call(swq=4, sw=258) == call(sxq=4, sxm=1 << 23) == _ops.E_UNSUPPORTED
     assert call(sxq=4, x=264) == call(sxq=4, xr=120) == call(swq=4, wr=1 << 23) == call(sxq=4, xc=2) == _ops.E_UNSUPPORTED
+    assert call(M=1 << 20, N=1 << 16, tile=5, ws=None) == call(M=1 << 30, N=1 << 14) == _ops.E_UNSUPPORTED
+    assert call(M=1 << 20, N=(1 << 16) - 64, tile=5, ws=None) == _ops.E_WORKSPACE
     assert call(tile=6) == call(tile=-2) == call(splits=-1) == _ops.E_ARG
     assert call(ws=None) == call(ws=128) == call(n=need - 1) == _ops.E_WORKSPACE
     # single scale bytes are reordered; rows that are not aligned, or do not end with a block, are copied; parts of K
@@ -89,6 +93,7 @@ def test_linear_checks():
 
     assert call(ws=None) == call(n=need - 1) == call(ws=128) == _ops.E_WORKSPACE
     assert call(t=4) == call(M=-2) == call(N=-1) == call(K=0) == call(w=None) == call(sw=None) == call(swn=-1) == _ops.E_ARG
+    assert call(M=1 << 30, N=1 << 14) == _ops.E_UNSUPPORTED and call(M=1, N=1 << 27, K=2, ws=None) == _ops.E_WORKSPACE
     assert call(y=None) == _ops.E_ARG and call(ldw=143) == _ops.E_UNSUPPORTED and call(M=0) == call(N=0) == 0
 
 
