@@ -11,8 +11,9 @@ constexpr auto kE8 = at::ScalarType::Float8_e8m0fnu;
 int64_t pairs(int64_t v) { return (v + 1) / 2; }
 int64_t mx_blocks(int64_t v) { return (v + kMx - 1) / kMx; }
 
-// The bytes of a 4-bit operand or of scales (torch has few functions for their types).
-Tensor as_bytes(const Tensor& t) { return t.detach().view(at::kByte); }
+// A 4-bit operand, or scales, as [rows, last dimension], as bytes where torch may have to copy them (it has
+// few functions for their types).
+Tensor rows4(const Tensor& t) { return t.dim() == 2 ? t : rows_of(t.detach().view(at::kByte)); }
 
 // An operand of a product: bytes of strides (r, c); the scales' dword of (row, quad of blocks) at row * row + quad * quad
 // bytes, or, where quad is 0, the byte of (row, block) at row * row + block * block.
@@ -82,7 +83,7 @@ Tensor dequantize4(const Tensor& q, const Tensor& s, at::ScalarType dtype) {
   REQUIRE(s.sizes() == at::IntArrayRef(with_last(q, mx_blocks(C))), "scale must be ",
           at::IntArrayRef(with_last(q, mx_blocks(C))), ", got ", s.sizes());
   at::NoGradGuard no_grad;
-  const Tensor out = empty(with_last(q, C), q, dtype), q2 = rows_of(as_bytes(q)), s2 = rows_of(as_bytes(s));
+  const Tensor out = empty(with_last(q, C), q, dtype), q2 = rows4(q), s2 = rows4(s);
   const On on(q);
   check_rc(f16acc_fp4_values(bytes(q2), q2.stride(0), q2.stride(1), bytes(s2), s2.stride(0), s2.stride(1), q2.size(0),
                              C, out.data_ptr(), type_of(out), on.stream));
@@ -136,8 +137,8 @@ Tensor mm4(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor
   const Tensor out = out_ ? *out_ : empty({M, N}, a, out_dtype);
   if (M == 0 || N == 0) return out;
   if (K == 0) return b_ ? out.copy_(b_->expand({M, N})) : out.zero_();
-  product4(stored4(as_bytes(a), as_bytes(a_scale)), stored4(as_bytes(b).t(), as_bytes(b_scale).t()), K, out, b_, tile,
-           splits);
+  const Operand4 bt{bytes(b), bytes(b_scale), b.stride(1), b.stride(0), b_scale.stride(1), b_scale.stride(0), 0};
+  product4(stored4(a, a_scale), bt, K, out, b_, tile, splits);
   return out;
 }
 
@@ -208,9 +209,9 @@ Operand packed4(const Tensor& q) {
   return {out, up(n, 16)};
 }
 
-Tensor stored_linear4(const Tensor& x, const Tensor& w, const Tensor& w_scale, const Maybe& bias) {
-  const Tensor x2 = rows_of(x), q = as_bytes(w), s = as_bytes(w_scale);
-  const int64_t M = x2.size(0), K = x2.size(1), N = w.size(0), P = pairs(K);
+Tensor stored_linear4(const Tensor& x, const Tensor& q, const Tensor& s, const Maybe& bias) {
+  const Tensor x2 = rows_of(x);
+  const int64_t M = x2.size(0), K = x2.size(1), N = q.size(0), P = pairs(K);
   // rows of any alignment go as they are (the library copies them where it has to)
   const bool rows = (P <= 1 || q.stride(1) == 1) && (N <= 1 || q.stride(0) >= P);
   const Operand o = rows ? Operand{q, N > 1 ? q.stride(0) : up(P, 16)} : packed4(q);  // (a row-major [K / 2, N] weight)
@@ -241,7 +242,7 @@ struct Stored4 : torch::autograd::Function<Stored4> {
     const Tensor dy = rows_of(check_grad("fp4.linear", grads[0]));
     Tensor dx, db;
     if (need & 1) {
-      const Tensor q = as_bytes(saved[0]), s = as_bytes(saved[1]);
+      const Tensor &q = saved[0], &s = saved[1];
       const Quantised4 wt(K, N, dy), r(dy.size(0), N, dy);
       const f16acc_fp4_matrix m = matrix4(dy, r, Quantised4());
       quant4(&m, nullptr, dy);
