@@ -124,6 +124,22 @@ __device__ __forceinline__ void load_clamped(const T* row, int64_t c, int64_t co
   for (int i = 0; i < N; ++i) v[i] = c + i < cols ? v[i] : 0.0f;
 }
 
+// 16 bytes of a row of `bytes` >= 16 from k on, zero past its end: the last 16 before the end, moved down, in one load.
+// (A loop over bytes there took 70 registers amid what was in flight, and a load each a wave's time.)
+__device__ __forceinline__ i32x4 unit_of_row(const uint8_t* row, int64_t k, int64_t bytes) {
+  const int over = k + 16 <= bytes ? 0 : k >= bytes ? 16 : (int)(k + 16 - bytes), bits = 8 * over;
+  union {
+    uint64_t d[2];
+    i32x4 v;
+  } u;
+  __builtin_memcpy(&u, row + (over ? bytes - 16 : k), 16);
+  const uint64_t lo = u.d[0], hi = u.d[1];
+  u.d[0] = bits >= 64 ? hi >> (bits & 63) : bits ? lo >> bits | hi << (64 - bits) : lo;
+  u.d[1] = bits >= 64 ? 0 : hi >> bits;
+  if (over == 16) u.d[0] = 0;
+  return u.v;
+}
+
 // SiLU with FP32's accuracy, behind sums of that accuracy: what is quantised from
 // it should fall on the right side of a tie.
 __device__ __forceinline__ float silu_exact(float g) { return g / (1.0f + expf(-g)); }

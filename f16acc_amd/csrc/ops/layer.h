@@ -236,29 +236,14 @@ struct LayerFew {
   static constexpr int GATE_UP = W * 2 * 64 * 16, DOWN = W * 64 * 16 + GROUPS * (kBlock + 4);
   static constexpr int SMEM = GATE_UP > DOWN ? GATE_UP : DOWN;
 
-  // 16 bytes of a row of K >= 16 from k on, zero past its end: the last 16 before the end, moved down.  (The
-  // byte loops of load_weight, in the middle of what is in flight, took 70 registers.)
-  __device__ static __forceinline__ i32x4 last_unit(const uint8_t* w, int64_t k, int64_t K) {
-    const int over = k + 16 <= K ? 0 : k >= K ? 16 : (int)(k + 16 - K), bits = 8 * over;
-    union {
-      uint64_t d[2];
-      i32x4 v;
-    } u;
-    __builtin_memcpy(&u, w + (over ? K - 16 : k), 16);
-    const uint64_t lo = u.d[0], hi = u.d[1];
-    u.d[0] = bits >= 64 ? hi >> (bits & 63) : bits ? lo >> bits | hi << (64 - bits) : lo;
-    u.d[1] = bits >= 64 ? 0 : hi >> bits;
-    if (over == 16) u.d[0] = 0;
-    return u.v;
-  }
   __device__ static __forceinline__ i32x8 block_of(const uint8_t* w, int64_t k0, int64_t K, int g) {
     i32x4 lo, hi;
     if (k0 + kBlock <= K) {
       __builtin_memcpy(&lo, w + k0 + 16 * g, 16);
       __builtin_memcpy(&hi, w + k0 + 64 + 16 * g, 16);
     } else {
-      lo = last_unit(w, k0 + 16 * g, K);
-      hi = last_unit(w, k0 + 64 + 16 * g, K);
+      lo = unit_of_row(w, k0 + 16 * g, K);
+      hi = unit_of_row(w, k0 + 64 + 16 * g, K);
     }
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }

@@ -174,8 +174,10 @@ __device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32
       uint8_t b[16];
       i32x4 v;
     } o;
-    if (p.s_c == 1 && c + 16 <= p.cols) {
-      __builtin_memcpy(o.b, s + c, 16);  // one 16-byte load: any alignment goes
+    if (p.s_c == 1 && p.cols >= 16) {
+      // one 16-byte load, any alignment goes, the last ones of a row from its end: beside a branch for them 1537 rows of
+      // 4481 bytes took 6.1 us, without 4.3
+      o.v = unit_of_row(s, c, p.cols);
     } else if (p.cols) {  // (inside the row, all in flight together: see load_clamped)
       uint32_t b[16];
 #pragma unroll
