@@ -374,10 +374,18 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
     const size_t lds = small4_lds(M, K);
     return by_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      if (few4_wide(N, K))
-        hipLaunchKernelGGL((linear_fp4_small_kernel<T, 16>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), lds, stream, a);
+      auto go = [&](auto odd) {
+        if (few4_wide(N, K))
+          hipLaunchKernelGGL((linear_fp4_small_kernel<T, 16, odd.value>), dim3((uint32_t)cdiv(N, 16)), dim3(1024), lds,
+                             stream, a);
+        else
+          hipLaunchKernelGGL((linear_fp4_small_kernel<T, 8, odd.value>), dim3((uint32_t)cdiv(N, 16)), dim3(512), lds,
+                             stream, a);
+      };
+      if ((uintptr_t)w % 4 || ldw % 4)
+        go(std::true_type{});
       else
-        hipLaunchKernelGGL((linear_fp4_small_kernel<T, 8>), dim3((uint32_t)cdiv(N, 16)), dim3(512), lds, stream, a);
+        go(std::false_type{});
       return hip_status();
     });
   }

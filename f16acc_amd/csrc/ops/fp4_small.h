@@ -61,7 +61,10 @@ __device__ __forceinline__ f32x4 mfma_mx16(const i32x4& w, const i32x4& x, const
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, sum, 4, 4, 0, sw, 0, sx);
 }
 
-template <class T, int W>
+// ODD: rows at any address.  Their units load as the four dwords that hold their first byte and what follows, and the
+// next one, and are moved together where they are used: 16-byte loads at odd addresses took twice as long (1537 x
+// 8961, one token, 11.9 us, so 7.8; at multiples of four 6.3).  Either dword holds a byte of the unit.
+template <class T, int W, bool ODD>
 __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) {
   constexpr int AHEAD = 4;  // quads of weights in flight
   extern __shared__ __align__(16) uint8_t tokens[];
@@ -73,10 +76,18 @@ __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) 
   const int row = (int)small4_row(p.K), M = (int)p.M;
   uint8_t* scales = tokens + M * row;
 
+  const int shift = ODD ? (int)((uintptr_t)w & 3) : 0;
   i32x4 wf[AHEAD];
-  int sf[AHEAD];
+  int sf[AHEAD], next[AHEAD];
   auto load = [&](int i, int kb) {
-    wf[i] = load_mx_unit(w, (int64_t)kb * 64 + 16 * g, bytes);
+    const int64_t b0 = (int64_t)kb * 64 + 16 * g;
+    if (ODD && b0 + 16 <= bytes) {
+      const uint8_t* at = (const uint8_t*)__builtin_assume_aligned(w + b0 - shift, 4);
+      __builtin_memcpy(&wf[i], at, 16);
+      next[i] = *(const int*)(at + (shift ? 16 : 12));
+    } else {
+      wf[i] = load_mx_unit(w, b0, bytes);
+    }
     const int b = 4 * kb + g;
     sf[i] = b < blocks ? sw[b * p.swk] : 0;
   };
@@ -111,6 +122,12 @@ __global__ __launch_bounds__(64 * W) void linear_fp4_small_kernel(Small4Args p) 
     for (int i = 0; i < AHEAD; ++i) {
       const int at = kb + i * W;
       if (at < nk) {
+        if constexpr (ODD) {
+          const int s = (int64_t)at * 64 + 16 * g + 16 <= bytes ? shift : 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            wf[i][k] = __builtin_amdgcn_alignbyte(k < 3 ? wf[i][k + 1] : next[i], wf[i][k], s);
+        }
         acc = mfma_mx16(wf[i], *(const i32x4*)(xq + at * 64), acc, sf[i], xs[at * 4]);
         if (at + AHEAD * W < nk) load(i, at + AHEAD * W);
       }
