@@ -218,6 +218,10 @@ bool few4(int64_t M, int64_t N, int64_t K) {
 // 1536 x 1536 one 3.6 / 3.4, eight 4.1 / 4.2; 8960 x 1536 one 7.8 / 5.1.
 bool few4_wide(int64_t N, int64_t K) { return cdiv(N, 16) <= kCus && quads_of(K) >= 24; }
 
+// Bytes between weight rows.  That of a single row addresses nothing, and a caller may hold anything there: the row's
+// own extent, which bounds the product's reads.
+int64_t row_stride(int64_t N, int64_t K, int64_t ldw) { return N > 1 ? ldw : cdiv(K, kMx) * 16; }
+
 // The workspace of linear: the quantised tokens and their scales, the weight's scales in the
 // products' order, the weight where its rows have to be copied, the parts of a split of K.
 struct LinearPlan4 {
@@ -351,7 +355,7 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
 
 size_t f16acc_linear_fp4_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return LinearPlan4(M, N, K, w, ldw).total;
+  return LinearPlan4(M, N, K, w, row_stride(N, K, ldw)).total;
 }
 
 int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw,
@@ -362,7 +366,8 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   if (N < 0) return F16ACC_OPS_E_ARG;
   if (M == 0 || N == 0) return 0;
   if (K == 0 || !w || !sw || !y || swn < 0 || swb < 0) return F16ACC_OPS_E_ARG;
-  if ((ldw < cdiv(K, 2) && N > 1) || 64 * quads_of(K) > kMaxRow || M > 0x7fffffff || N > 0x7fffffff)
+  ldw = row_stride(N, K, ldw);
+  if (ldw < cdiv(K, 2) || 64 * quads_of(K) > kMaxRow || M > 0x7fffffff || N > 0x7fffffff)
     return F16ACC_OPS_E_UNSUPPORTED;
   hipStream_t stream = (hipStream_t)stream_;
   const bool wide = sc == 1;  // (rows of any alignment)

@@ -222,7 +222,8 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
 
 /*
  * y = x w^T + bias with x [M, K] of `type` (element strides sr, sc) quantised in 4-bit blocks on the way; w [N][ldw]
- * bytes of any alignment, ldw at least ceil(K / 2), the scale byte of (row, block) at row * swn + block * swb;
+ * bytes of any alignment, ldw at least ceil(K / 2) (that of a single row is not looked at), the scale byte of (row, block)
+ * at row * swn + block * swb;
  * y [M][N] contiguous and bias of x's type; K at least 1.  Workspace of f16acc_linear_fp4_workspace bytes for
  * exactly these sizes, 256-byte aligned.
  */

@@ -97,6 +97,13 @@ def test_linear_checks():
     assert call(y=None) == _ops.E_ARG and call(ldw=143) == _ops.E_UNSUPPORTED and call(M=0) == call(N=0) == 0
 
 
+def test_the_stride_of_a_single_weight_row_is_not_looked_at():
+    for M, K, w in ((1, 288, 256), (100, 288, 256), (100, 250, 256), (100, 288, 257)):
+        sizes = {_ops.linear_fp4_workspace(M, 1, K, w, ldw) for ldw in (0, 1, 16, 143, 144, 1 << 23, -16)}
+        assert len(sizes) == 1 and sizes.pop() > 0
+    assert _ops.linear_fp4(256, 0, 288, 1, 256, 0, 256, 9, 1, None, 256, 100, 1, 288, None, 0, None) == _ops.E_WORKSPACE
+
+
 CPU = torch.zeros(4, 64)
 Q, S = torch.zeros(4, 32, dtype=torch.uint8).view(F4), torch.zeros(4, 2, dtype=torch.uint8).view(E8)
 CALLS = {

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from f16acc_amd import fp4
+from f16acc_amd import _ops, fp4
 from tests import fp4_reference as ref
 from tests.fp4_reference import E8, F4
 
@@ -570,3 +570,19 @@ def test_rows_and_scales_more_than_4_mib_apart():
     for x in (normal(M, K), normal(3, K)):
         y = fp4.linear(x, w, ws)
         assert torch.equal(fp4.linear(x, apart(w, F4), ws), y) and torch.equal(fp4.linear(x, w, apart(ws, E8)), y)
+
+
+@pytest.mark.parametrize("ldw", [0, 16, 1 << 40])
+@pytest.mark.parametrize("K", [288, 250, 1024])
+def test_linear_of_a_single_weight_row(K, ldw):
+    """The C entry point with one weight row: the bytes between rows address nothing, whatever a caller holds there."""
+    w, ws = stored(1, K)
+    for M in (1, 7, 40, 300):
+        x = normal(M, K)
+        y = torch.full((M, 1), 7.0, dtype=torch.float16, device=DEV)
+        n = _ops.linear_fp4_workspace(M, 1, K, w.data_ptr(), ldw)
+        held = torch.full((max(n, 1),), 255, dtype=torch.uint8, device=DEV)
+        args = (x.data_ptr(), 0, K, 1, w.data_ptr(), ldw, ws.data_ptr(), 1, 1, None, y.data_ptr(), M, 1, K, held.data_ptr(), n)
+        assert _ops.linear_fp4(*args, torch.cuda.current_stream().cuda_stream) == 0
+        ref.check_product(y, ref.rounded(x), ref.values(w, ws, K))
+        assert torch.equal(y, fp4.linear(x, w, ws))
