@@ -211,13 +211,14 @@ __device__ __forceinline__ void mx_scales(const MxScaleArgs& p, uint32_t group, 
 }
 
 // What a product needs before it: the rows of two operands copied to an alignment, their scales in its
-// order (any of it may be none).
+// order (any of it may be none).  ODD: an odd number of values, whose last byte holds one.
+template <bool ODD>
 __global__ __launch_bounds__(256) void mx_pack_kernel(Pack8Args x, Pack8Args w, MxScaleArgs a, MxScaleArgs b,
                                                       uint32_t nx, uint32_t nw, uint32_t na) {
   uint32_t group = blockIdx.x;
-  if (group < nx) return pack8(x, group, nx);
+  if (group < nx) return pack8<ODD>(x, group, nx);
   group -= nx;
-  if (group < nw) return pack8(w, group, nw);
+  if (group < nw) return pack8<ODD>(w, group, nw);
   group -= nw;
   if (group < na) return mx_scales(a, group, na);
   mx_scales(b, group - na, gridDim.x - nx - nw - na);

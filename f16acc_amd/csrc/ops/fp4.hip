@@ -346,8 +346,8 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
     }
   }
   if (const uint32_t grid = np[0] + np[1] + ns[0] + ns[1]) {
-    hipLaunchKernelGGL(mx_pack_kernel, dim3(grid), dim3(256), 0, stream, pack[0], pack[1], scales[0], scales[1], np[0],
-                       np[1], ns[0]);
+    hipLaunchKernelGGL((K % 2 ? mx_pack_kernel<true> : mx_pack_kernel<false>), dim3(grid), dim3(256), 0, stream, pack[0],
+                       pack[1], scales[0], scales[1], np[0], np[1], ns[0]);
     if ((rc = hip_status())) return rc;
   }
   return run_product(p, plan.plan, ws + plan.parts, stream);

@@ -165,6 +165,8 @@ struct Pack8Args {
   uint8_t* dst;
   int64_t rows, cols, s_r, s_c, ld;
 };
+// HALF: of a row's last byte the low half alone is copied, zero above it (4-bit values, an odd number of them).
+template <bool HALF = false>
 __device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32_t groups) {
   const int64_t units = p.ld / 16, total = p.rows * units;
   for (int64_t i = (int64_t)group * 256 + threadIdx.x; i < total; i += (int64_t)groups * 256) {
@@ -186,6 +188,12 @@ __device__ __forceinline__ void pack8(const Pack8Args& p, uint32_t group, uint32
       for (int k = 0; k < 16; ++k) o.b[k] = c + k < p.cols ? (uint8_t)b[k] : 0;
     } else {
       o.v = i32x4{0, 0, 0, 0};
+    }
+    if constexpr (HALF) {
+      const int64_t last = p.cols - 1 - c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (last >> 2 == k) o.v[k] &= ~(int)(0xf0u << (8 * (last & 3)));
     }
     *(i32x4*)(p.dst + r * p.ld + c) = o.v;
   }

@@ -203,7 +203,8 @@ int f16acc_fp4_values(const uint8_t* q, int64_t q_r, int64_t q_c, const uint8_t*
  * c[m][n] = sum over k of x[m][k] w[n][k] (4-bit values times their blocks' scales) + bias[n], added in FP32, rounded
  * once to ctype.
  *   x, w: the bytes of (row, pair of values) at strides (xr, xc), (wr, wc), any; rows of whole blocks that are
- *   16-byte aligned and at most 4 MiB apart are read as they are, others copied first;  K at least 1 where M and N are
+ *   16-byte aligned and at most 4 MiB apart are read as they are, others copied first (of an odd K's last byte the low
+ *   half);  K at least 1 where M and N are
  *   sx, sw: single bytes, that of (row m, block b) at m * sxm + b * sxb, where sxq is 0; else quads as above,
  *   (row, quad) at m * sxm + quad * sxq, bytes past the last block not 255, and rows that are aligned
  *   and zero from K to the next multiple of 32 values (swn, swb, swq alike)

@@ -586,3 +586,19 @@ def test_linear_of_a_single_weight_row(K, ldw):
         assert _ops.linear_fp4(*args, torch.cuda.current_stream().cuda_stream) == 0
         ref.check_product(y, ref.rounded(x), ref.values(w, ws, K))
         assert torch.equal(y, fp4.linear(x, w, ws))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (5, 7, 31), (40, 72, 333), (300, 130, 1025), (20, 40, 8961)])
+def test_mm_of_an_odd_number_of_values(M, N, K):
+    """The C entry point: the high half of a row's last byte is no value of an odd K, whatever it holds."""
+    (a, sa), (w, ws) = stored(M, K, seed=2), stored(N, K)
+    for q, code in ((a, 0x70), (w, 0xa0)):
+        u8(q)[:, -1] += code
+    stride = lambda q, s: (q.data_ptr(), *q.stride(), s.data_ptr(), *s.stride(), 0)
+    for x, y in ((a, w), (u8(a).t().contiguous().t(), u8(w).t().contiguous().t())):
+        n = _ops.mm_fp4_workspace(x.data_ptr(), *x.stride(), 0, y.data_ptr(), *y.stride(), 0, M, N, K, -1, 0)
+        held = torch.full((max(n, 1),), 255, dtype=torch.uint8, device=DEV)
+        c = torch.full((M, N), 7.0, device=DEV)
+        assert _ops.mm_fp4(*stride(x, sa), *stride(y, ws), None, c.data_ptr(), N, 1, M, N, K, 2, -1, 0, held.data_ptr(), n,
+                           torch.cuda.current_stream().cuda_stream) == 0
+        ref.check_product(c, ref.values(a, sa, K), ref.values(w, ws, K))
