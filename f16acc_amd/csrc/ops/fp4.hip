@@ -209,7 +209,7 @@ struct MmPlan4 {
 // one token 5.1 / 8.6, eight 7.0 / 8.7, 16 9.5 / 8.6; 4096 x 4096 eight 7.6 / 11.2, 16 10.2 / 11.6; 1536 x 8960 four
 // 8.6 / 12.3, 12 13.4 / 12.1; 14336 x 4096 two 13.1 / 14.9, four 15.5 / 14.8; 28672 x 7168 one 27.8 / 30.3, eight 46 / 30.
 bool few4(int64_t M, int64_t N, int64_t K) {
-  return M <= 16 && K < 65536 && N < kMaxThreads / 32 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
+  return M <= 16 && K < 65536 && cdiv(N, 16) < kMaxThreads / 512 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
 }
 
 // Its workgroups have 16 waves where there are no more of them than compute units and K is long enough to give

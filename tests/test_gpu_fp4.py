@@ -602,3 +602,14 @@ def test_mm_of_an_odd_number_of_values(M, N, K):
         assert _ops.mm_fp4(*stride(x, sa), *stride(y, ws), None, c.data_ptr(), N, 1, M, N, K, 2, -1, 0, held.data_ptr(), n,
                            torch.cuda.current_stream().cuda_stream) == 0
         ref.check_product(c, ref.values(a, sa, K), ref.values(w, ws, K))
+
+
+@pytest.mark.parametrize("N", [(1 << 27) - 16, (1 << 27) - 1])
+def test_linear_of_more_weight_rows_than_a_launch_of_the_small_kernel_holds(N):
+    """One value times each of 2^27 weights: products of a power of two and a 4-bit value, exact."""
+    w = torch.arange(N, device=DEV).bitwise_and_(15).to(torch.uint8)[:, None]
+    s = torch.full((N, 1), 127, dtype=torch.uint8, device=DEV)
+    y = fp4.linear(torch.full((1, 1), 4.0, dtype=torch.float16, device=DEV), w.view(F4), s.view(E8))
+    table = 4 * ref.unpack(torch.arange(16, dtype=torch.uint8)[:, None], 1).half().to(DEV)[:, 0]
+    assert torch.equal(y[0, :N // 16 * 16].view(-1, 16), table.expand(N // 16, 16))
+    assert torch.equal(y[0, N // 16 * 16:], table[:N % 16])
