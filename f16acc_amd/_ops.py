@@ -50,6 +50,7 @@ _SIGNATURES = {
     "f16acc_fp4_values": [_vp, _i64, _i64] * 2 + [_i64] * 2 + [_vp, _int, _vp],
     "f16acc_mm_fp4": ([_vp, _i64, _i64, _vp] + [_i64] * 3) * 2 + [_vp, _vp] + [_i64] * 5 + [_int] * 3 + [_vp, _size, _vp],
     "f16acc_linear_fp4": [_vp, _int, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_vp, _size, _vp],
+    "f16acc_linear_fp4_few": [_i64] * 4,
     "f16acc_mm_fp4_workspace": [_vp, _i64, _i64, _i64] * 2 + [_i64] * 3 + [_int] * 2,
     "f16acc_linear_fp4_workspace": [_i64] * 3 + [_vp, _i64],
     "f16acc_ops_strerror": [_int],
@@ -78,8 +79,8 @@ def _bind(name):
 
 (quant_rows, quant_both, quant_weight, pack8, column_sums, mm_fp8, linear_fp8, route, route_grad, experts_any_rows,
  experts, column_sums_workspace, mm_fp8_workspace, linear_fp8_workspace, experts_workspace,
- layer_any_rows, layer, layer_workspace, fp4_quant, fp4_transpose, fp4_values, mm_fp4, linear_fp4, mm_fp4_workspace, linear_fp4_workspace, strerror,
- abi_version) = map(_bind, EXPORTS)
+ layer_any_rows, layer, layer_workspace, fp4_quant, fp4_transpose, fp4_values, mm_fp4, linear_fp4, linear_fp4_few,
+ mm_fp4_workspace, linear_fp4_workspace, strerror, abi_version) = map(_bind, EXPORTS)
 
 if abi_version() != ABI_VERSION:
     raise ImportError(f"{LIB_OPS} has ABI version {abi_version()}, this package needs {ABI_VERSION}: rebuild it")

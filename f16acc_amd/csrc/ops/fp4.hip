@@ -353,6 +353,10 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
   return run_product(p, plan.plan, ws + plan.parts, stream);
 }
 
+int f16acc_linear_fp4_few(int64_t M, int64_t N, int64_t K, int64_t sc) {
+  return M > 0 && N > 0 && K > 0 && few4(M, N, K) && (sc == 1 || K == 1);
+}
+
 size_t f16acc_linear_fp4_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   return LinearPlan4(M, N, K, w, row_stride(N, K, ldw)).total;
@@ -370,11 +374,7 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
   if (ldw < cdiv(K, 2) || 64 * quads_of(K) > kMaxRow || M > 0x7fffffff || N > 0x7fffffff)
     return F16ACC_OPS_E_UNSUPPORTED;
   hipStream_t stream = (hipStream_t)stream_;
-  const bool wide = sc == 1;  // (rows of any alignment)
-  const LinearPlan4 plan(M, N, K, w, ldw);
-  if (!launches(plan.plan, M, N)) return F16ACC_OPS_E_UNSUPPORTED;
-  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
-  if (few4(M, N, K) && (sc == 1 || K == 1)) {
+  if (f16acc_linear_fp4_few(M, N, K, sc)) {
     const Small4Args a{x, sr, w, ldw, sw, swn, swb, bias, y, M, N, K};
     const size_t lds = small4_lds(M, K);
     return by_type(type, [&](auto* t) {
@@ -394,6 +394,10 @@ int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uin
       return hip_status();
     });
   }
+  const bool wide = sc == 1;  // (rows of any alignment)
+  const LinearPlan4 plan(M, N, K, w, ldw);
+  if (!launches(plan.plan, M, N)) return F16ACC_OPS_E_UNSUPPORTED;
+  if (!workspace || (uintptr_t)workspace % 256 || ws_bytes < plan.total) return F16ACC_OPS_E_WORKSPACE;
   char* ws = (char*)workspace;
   Mx4Args p{};
   p.x = (const uint8_t*)ws, p.ldx = 64 * quads_of(K);

@@ -216,8 +216,10 @@ Tensor stored_linear4(const Tensor& x, const Tensor& q, const Tensor& s, const M
   const bool rows = (P <= 1 || q.stride(1) == 1) && (N <= 1 || q.stride(0) >= P);
   const Operand o = rows ? Operand{q, N > 1 ? q.stride(0) : up(P, 16)} : packed4(q);  // (a row-major [K / 2, N] weight)
   Tensor y = empty(with_last(x, N), x, x.scalar_type());
-  const size_t n = f16acc_linear_fp4_workspace(M, N, K, bytes(o.q), o.ld);
-  const Tensor ws = empty({(int64_t)n}, x, at::kByte);
+  const bool few = f16acc_linear_fp4_few(M, N, K, x2.stride(1));
+  const size_t n = few ? 0 : f16acc_linear_fp4_workspace(M, N, K, bytes(o.q), o.ld);
+  Tensor ws;
+  if (n) ws = empty({(int64_t)n}, x, at::kByte);
   const On on(x);
   check_rc(f16acc_linear_fp4(x2.const_data_ptr(), type_of(x), x2.stride(0), x2.stride(1), bytes(o.q), o.ld, bytes(s),
                              s.stride(0), s.stride(1), data(bias), y.data_ptr(), M, N, K, bytes(ws), n, on.stream));

@@ -226,8 +226,9 @@ int f16acc_mm_fp4(const uint8_t* x, int64_t xr, int64_t xc, const uint8_t* sx, i
  * bytes of any alignment, ldw at least ceil(K / 2) (that of a single row is not looked at), the scale byte of (row, block)
  * at row * swn + block * swb;
  * y [M][N] contiguous and bias of x's type; K at least 1.  Workspace of f16acc_linear_fp4_workspace bytes for
- * exactly these sizes, 256-byte aligned.
+ * exactly these sizes, 256-byte aligned; none (NULL) where f16acc_linear_fp4_few says 1: one kernel for few tokens.
  */
+int f16acc_linear_fp4_few(int64_t M, int64_t N, int64_t K, int64_t sc);
 size_t f16acc_linear_fp4_workspace(int64_t M, int64_t N, int64_t K, const uint8_t* w, int64_t ldw);
 int f16acc_linear_fp4(const void* x, int type, int64_t sr, int64_t sc, const uint8_t* w, int64_t ldw,
                       const uint8_t* sw, int64_t swn, int64_t swb, const void* bias, void* y, int64_t M, int64_t N,

@@ -104,6 +104,15 @@ def test_the_stride_of_a_single_weight_row_is_not_looked_at():
     assert _ops.linear_fp4(256, 0, 288, 1, 256, 0, 256, 9, 1, None, 256, 100, 1, 288, None, 0, None) == _ops.E_WORKSPACE
 
 
+def test_few_tokens_need_no_workspace():
+    few = _ops.linear_fp4_few
+    assert few(1, 8960, 1536, 1) == few(16, 64, 288, 1) == few(1, 28672, 7169, 1) == few(1, 64, 1, 9) == 1
+    assert few(17, 64, 288, 1) == few(1, 64, 288, 2) == few(8, 28672, 7168, 1) == few(1, 64, 1 << 16, 1) == 0
+    assert few(0, 64, 288, 1) == few(1, 0, 288, 1) == few(1, 64, 0, 1) == few(-1, 64, 288, 1) == 0
+    for M in (1, 16):  # a column stride that the kernel does not take: the tiles, and their workspace
+        assert _ops.linear_fp4(256, 0, 600, 2, 256, 144, 256, 9, 1, None, 256, M, 64, 288, None, 0, None) == _ops.E_WORKSPACE
+
+
 CPU = torch.zeros(4, 64)
 Q, S = torch.zeros(4, 32, dtype=torch.uint8).view(F4), torch.zeros(4, 2, dtype=torch.uint8).view(E8)
 CALLS = {

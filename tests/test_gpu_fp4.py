@@ -613,3 +613,22 @@ def test_linear_of_more_weight_rows_than_a_launch_of_the_small_kernel_holds(N):
     table = 4 * ref.unpack(torch.arange(16, dtype=torch.uint8)[:, None], 1).half().to(DEV)[:, 0]
     assert torch.equal(y[0, :N // 16 * 16].view(-1, 16), table.expand(N // 16, 16))
     assert torch.equal(y[0, N // 16 * 16:], table[:N % 16])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 8000, 5001), (16, 300, 1001), (3, 500, 4096)])
+def test_few_tokens_allocate_the_result_alone(M, N, K):
+    """A weight of odd rows is not copied for them, and no room for a copy is asked for."""
+    x, (w, ws) = normal(M, K), stored(N, K)
+    assert _ops.linear_fp4_few(M, N, K, 1) == 1
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = fp4.linear(x, w, ws)
+    assert torch.cuda.max_memory_allocated() - before <= -(-2 * M * N // 512) * 512
+    ref.check_product(y, ref.rounded(x), ref.values(w, ws, K))
+    z = torch.empty_like(y)
+    assert _ops.linear_fp4(x.data_ptr(), 0, K, 1, w.data_ptr(), w.stride(0), ws.data_ptr(), *ws.stride(), None, z.data_ptr(), M, N,
+                           K, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(z, y)
+    every = normal(M, 2 * K)[:, ::2]  # (columns apart: the tiles, with a workspace)
+    ref.check_product(fp4.linear(every, w, ws), ref.rounded(every), ref.values(w, ws, K))
