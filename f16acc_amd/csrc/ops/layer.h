@@ -44,8 +44,10 @@ __device__ __forceinline__ void fetch8(const T* p, int64_t stride, int64_t k, in
 }
 
 // logits[t][e] = sum over d of x[t][d] r[e][d], summed in 64 bits and rounded once to FP32: products of 16-bit and
-// FP32 values are exact there, so a token's logits, and with them the choice of its experts, do not depend
-// on the batch it comes in.  16 F tokens by 16 F experts a workgroup on v_mfma_f64_16x16x4_f64; the waves deal the
+// FP32 values are exact there.  The three kernels (16 waves, 4 waves, 256 lanes
+// of layer_router_kernel) add in different orders, so where a sum is not exact a token's logits, and with them the choice
+// of its experts, can depend on the batch it comes in: if the sum lies within its rounding, 2^-53 of the magnitudes for each
+// addition, of the middle between two FP32 values.  16 F tokens by 16 F experts a workgroup on v_mfma_f64_16x16x4_f64; the waves deal the
 // chunks of 32 columns, a lane loads eight of a row, and their sums meet in LDS in wave order.  512 tokens of 64
 // experts, 2048 wide: 11 us in 16 waves, two chunks ahead each (15 in eight, with one), of 8 MB and 2 us of matrix
 // instructions: the launch, and two rounds of loads.  16384 tokens of 256 experts: 340 us with F = 2, of which

@@ -64,8 +64,10 @@ def layer(x, router, k, w1, w1_scale, w2, w2_scale, *, scoring="softmax", bias=N
 
     x: [..., D] float16, bfloat16 or float32, any strides
     router: [E, D] float16, bfloat16 or float32, any strides.  The logits are summed in
-       64 bits and rounded once to FP32, so a token's choice does not depend on the batch around it.
-       A token with a NaN logit gives NaN
+       64 bits and rounded once to FP32.  The order of a sum goes by the number of tokens: where
+       a sum is exact in 64 bits a token's logits, and its choice, are the same in every batch; else they may
+       differ where the 64-bit sum lies within its own rounding (2^-53 of its terms' magnitudes for each
+       addition) of the middle between two FP32 values.  A token with a NaN logit gives NaN
     k and the options are route's, the weights and their scales experts'
     Returns [..., D] in x's type.  For inference: operands that require gradients are refused
     where gradients are enabled."""

@@ -249,3 +249,29 @@ def test_refusals():
             f()
     with torch.no_grad():
         moe.layer(x.clone().requires_grad_(), *args[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 40, 1100])
+def test_choice_of_exact_sums_is_the_same_in_every_batch(T, dtype):
+    """Logits of 35 bits, exact in 64 in any order, that lie two steps of FP32 apart (or one, or none) where an FP32 sum is
+    off by more: the kernels for few, some and many tokens choose alike."""
+    E, D, I = 1024, 256, 16
+    g = torch.Generator().manual_seed(3)
+    x = torch.randint(-7, 8, (1100, D), generator=g).float()
+    x[:, 0] = 1.0
+    base = torch.randint(-2 ** 23 + 2 ** 17, 2 ** 23 - 2 ** 17, (D,), generator=g).float()
+    router = base.repeat(E, 1)
+    router[:, 0] = 64.0 * torch.randperm(E, generator=g)
+    router = (router * 2.0 ** -26).to(DEV)
+    x = x.to(dtype).to(DEV)[1100 - T:]
+    w1, s1 = weight(1, 2, I, D)
+    w2, s2 = weight(1, D, I)
+    scale = s2.repeat(E, 1, 1) * torch.exp2(torch.arange(E, device=DEV) % 16).float()[:, None, None]  # the choice shows
+    w = (w1.expand(E, 2, I, D).contiguous(), s1.repeat(E, 1, 1, 1), w2.expand(E, D, I).contiguous(), scale)
+    weights, ids = moe.route(logits_of(x, router).to(DEV), 3)
+    y = moe.layer(x, router, 3, *w)
+    if T > 4:
+        assert torch.equal(y, moe.experts(x, weights, ids, *w))
+    else:
+        check_experts(y, (x, weights, ids, *w))
