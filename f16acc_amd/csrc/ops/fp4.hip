@@ -206,10 +206,11 @@ struct MmPlan4 {
 
 // Up to 16 tokens in one kernel as long as its workgroups, 16 weight rows each, do not spend more on
 // quantising the tokens than the preparing launch costs.  In graphs, cold weights, one kernel / tiles, us: 8960 x 1536
-// one token 5.1 / 8.6, eight 7.0 / 8.7, 16 9.5 / 8.6; 4096 x 4096 eight 7.6 / 11.2, 16 10.2 / 11.6; 1536 x 8960 four
-// 8.6 / 12.3, 12 13.4 / 12.1; 14336 x 4096 two 13.1 / 14.9, four 15.5 / 14.8; 28672 x 7168 one 27.8 / 30.3, eight 46 / 30.
+// one token 5.1 / 8.6, eight 7.0 / 8.7, 16 9.5 / 8.6; 4096 x 4096 eight 7.5 / 11.2, 16 10.0 / 11.5; 1024 x 4096 16
+// 9.2 / 10.4; 8192 x 4096 eight 12.0 / 12.5, 12 14.6 / 12.6; 1536 x 8960 four 8.6 / 12.3, 12 13.4 / 12.1; 14336 x 4096 two
+// 13.1 / 14.9, four 15.4 / 15.0, eight 19.1 / 14.7; 28672 x 7168 one 27.8 / 30.3, eight 46 / 30.
 bool few4(int64_t M, int64_t N, int64_t K) {
-  return M <= 16 && K < 65536 && cdiv(N, 16) < kMaxThreads / 512 && M * K * cdiv(cdiv(N, 16), kCus) < 65536;  // (small4_lds at most 36 KB)
+  return M <= 16 && K < 65536 && cdiv(N, 16) < kMaxThreads / 512 && M * K * cdiv(cdiv(N, 16), kCus) <= 65536;  // (small4_lds at most 36 KB)
 }
 
 // Its workgroups have 16 waves where there are no more of them than compute units and K is long enough to give

@@ -632,3 +632,16 @@ def test_few_tokens_allocate_the_result_alone(M, N, K):
     assert torch.equal(z, y)
     every = normal(M, 2 * K)[:, ::2]  # (columns apart: the tiles, with a workspace)
     ref.check_product(fp4.linear(every, w, ws), ref.rounded(every), ref.values(w, ws, K))
+
+
+@pytest.mark.parametrize("N,K,most", [(40, 100, 16), (530, 3000, 16), (520, 3200, 16), (4112, 2048, 16), (4096, 4000, 16),
+                                      (4096, 4096, 16), (4100, 4097, 7), (8192, 4096, 8)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_tokens_results_do_not_depend_on_those_beside_them(N, K, most, dtype):
+    """Bit for bit, for as many tokens as one kernel takes."""
+    x, (w, ws) = normal(most, K, dtype=dtype), stored(N, K)
+    assert _ops.linear_fp4_few(most, N, K, 1) == 1 and (most == 16 or _ops.linear_fp4_few(most + 1, N, K, 1) == 0)
+    rows = torch.cat([fp4.linear(x[i:i + 1], w, ws) for i in range(most)])
+    for M in range(2, most + 1):
+        assert torch.equal(fp4.linear(x[:M], w, ws), rows[:M])
+    assert torch.equal(fp4.linear(x.flip(0), w, ws).flip(0), rows)
