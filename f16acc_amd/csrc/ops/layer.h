@@ -121,12 +121,13 @@ __global__ __launch_bounds__(64 * W) void router_kernel(RouterArgs p) {
 // Before it waits, a workgroup sees that every piece is claimed and computes those that are not, so it
 // takes neither a number of workgroups at once nor an order of theirs.  (An order of them is a matter of speed: with the
 // result's workgroups first, those that fit beside none of the others raced for their pieces, 124 us instead of
-// 48 for two tokens, 8 of 64 experts, 2048 x 1024.)
+// 48 for two tokens, 8 of 64 experts, 2048 x 1024, a size that is composed now.)
 //
-// Measured, in a graph, against the router's product, route and experts one after another, us: 64 experts, 2048 x 1024,
-// one token, 2 of them 17 / 26, 6 (38 MB of weights, 7.6 us at the copy rate) 22 / 31, 8 31 / 33, two tokens,
-// 6 38 / 42, 8 50 / 46; 128 experts, 4096 x 1536, one token, 1 of them 23 / 37, 8 53 / 62, four tokens, 4 90 / 86; 32
-// experts, 7168 x 2048, one token, 8 of them 88 / 105.  Of 22 us the logits take 4, the choice 3.5, gate and up 5
+// Measured, in a graph, against the router's product, route and experts one after another, which take over where the
+// slots' hidden columns are many (layer_in_two, with the figures), us: 64 experts, 2048 x 1024, one token, 2 of them
+// 17 / 25, 6 (38 MB of weights, 7.6 us at the copy rate) 22 / 31, 8 32 / 35, two tokens, 6 40 / 43; 128 experts,
+// 4096 x 1536, one token, 1 of them 23 / 36, 8 54 / 65; 32 experts, 7168 x 2048, one token, 8 of them 95 / 107.  Of 22
+// us the logits take 4, the choice 3.5, gate and up 5
 // to 7, at the rate of memory, and 9 pass from their last sums to the result: stores past the L2, a count, a
 // poll, hidden values from memory, each a trip of a microsecond or two.
 // ---------------------------------------------------------------------------

@@ -405,6 +405,16 @@ struct LaunchLayer {
   }
 };
 
+// Whether a layer of few tokens takes two launches, or the router's product, route and experts one after another.  Each 16
+// hidden columns of a slot are a workgroup, which chooses the experts for itself and starts on cold weights: many more of
+// them than fit at once cost more than the launches they save, which the result's D / 16 workgroups hide the
+// longer, the wider it is.  Two launches / one after another, in a graph, us, at 2, 4, 8, 12 and 16 slots: 64 experts,
+// 2048 x 1024 17 / 25, 21 / 28, 32 / 35, 40 / 43, 47 to 54 / 47 to 50; 128 of 4096 x 1536 27 / 40, 37 / 45, 54 / 64, 77 / 82,
+// 91 / 84; 32 of 7168 x 2048 43 / 62, 57 / 73, 95 / 106, 113 / 110, 158 / 161; 64 of 512 x 1536 16 / 22, 19 / 25, 32 / 32, 42 / 38,
+// 60 / 47; 8 of 2048 x 5632 38 / 42, 61 / 60, 107 / 91, 128 / 89, 152 / 100; 8 of 4096 x 14336 68 to 106 / 59 to 109, 200 / 177,
+// 340 / 258, 391 / 278, 464 / 308 (one slot 63 / 67).
+bool layer_in_two(int64_t slots, int64_t D, int64_t I) { return slots * I < 9216 + 3 * D; }
+
 // Where a layer's values lie in its workspace, and its size, which is enough for any smaller T as well: logits,
 // weights and ids before the experts' own; or logits, quantised tokens, hidden values and counters of a few tokens.
 struct LayerPlan {
@@ -746,7 +756,7 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
                  const float* s2, int64_t s2e, int64_t s2n, int64_t s2k, void* y, void* workspace, size_t ws_bytes,
                  void* stream_) {
   const ExpertWeights w{w1, w1e, w1u, ld1, s1, s1e, s1u, s1n, s1k, w2, w2e, ld2, s2, s2e, s2n, s2k};
-  const bool few = f16acc_layer_any_rows(T, k, D, I);
+  bool few = f16acc_layer_any_rows(T, k, D, I);
   int rc = experts_check(x, type, T, k, E, D, I, w, y, few);
   if (!rc) rc = quant_check(router, rtype, E, D);
   if (rc || T == 0) return rc;
@@ -761,6 +771,8 @@ int f16acc_layer(const void* x, int type, int64_t T, int64_t sr, int64_t sc, con
   int* ids = (int*)(ws + plan.ids);
   const RouterArgs r{x, T, sr, sc, router, re, rd, E, D, false, logits};
   a.x = logits, a.weights = weights, a.ids = ids;
+  // (the experts take any rows of the weights where they can load x wide)
+  if (few && !layer_in_two(T * k, D, I) && f16acc_experts_any_rows(x, type, T, sr, sc, k)) few = false;
   if (few) {
     const int64_t Dp = up128(D), Ip = up128(I);
     LayerArgs l{};

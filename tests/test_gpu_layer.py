@@ -275,3 +275,26 @@ def test_choice_of_exact_sums_is_the_same_in_every_batch(T, dtype):
         assert torch.equal(y, moe.experts(x, weights, ids, *w))
     else:
         check_experts(y, (x, weights, ids, *w))
+
+
+@pytest.mark.parametrize("T,E,k,D,I", [(1, 8, 2, 256, 6000), (2, 16, 8, 256, 4096), (4, 9, 4, 1104, 2000), (3, 6, 1, 136, 9001),
+                                       (4, 5, 2, 1040, 3117), (1, 20, 16, 304, 3000)])
+def test_wide_hidden_layers_of_few_tokens(T, E, k, D, I):
+    """Far more hidden columns than workgroups at once: the composed kernels where x's rows load wide, the two launches
+    where they do not (and compute each other's pieces); weights whose rows start anywhere; tokens of NaN and without experts."""
+    x, router, w = layer(T, E, D, I, torch.bfloat16)
+    apart = torch.cat([x[:, :1], x], 1)[:, 1:]
+    odd = torch.cat([w[2].view(torch.uint8)[:, :, :1], w[2].view(torch.uint8)], 2)[:, :, 1:].view(F8)
+    for v in (x, apart):
+        y = moe.layer(v, router, k, *w)
+        check_layer(y, x, router, k, w)
+        for _ in range(3):
+            assert torch.equal(moe.layer(v, router, k, *w), y)
+        assert torch.equal(moe.layer(v, router, k, w[0], w[1], odd, w[3]), y)
+        bad = v.clone() if v is x else torch.cat([x[:, :1], x], 1)[:, 1:]
+        bad[T - 1, 17] = float("nan")
+        z = moe.layer(bad, router, k, *w)
+        assert bool(torch.isnan(z[T - 1]).all()) and torch.equal(z[:T - 1], y[:T - 1])
+        none = router.clone()
+        none[:, 5] = -float("inf")
+        assert bool((moe.layer(v.abs() + 1, none, k, *w) == 0).all())
