@@ -298,3 +298,22 @@ def test_wide_hidden_layers_of_few_tokens(T, E, k, D, I):
         none = router.clone()
         none[:, 5] = -float("inf")
         assert bool((moe.layer(v.abs() + 1, none, k, *w) == 0).all())
+
+
+def test_more_tokens_than_a_launch_addresses_go_in_parts():
+    """Rows of 4 MiB quantised: 511 tokens a part, the last part's two tokens by the kernels for few."""
+    T, D, I = 513, 1 << 22, 16
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(T, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    router = torch.randn(2, D, generator=g, device=DEV, dtype=torch.bfloat16) * D ** -0.5
+    w = []
+    for shape in ((2, 2, I, D), (2, D, I)):
+        w.append((torch.randn(*shape, generator=g, device=DEV) * 100).clamp_(-448, 448).to(F8))
+        blocks = (*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128))
+        w.append(torch.rand(*blocks, generator=g, device=DEV) * 2e-5)
+    y = moe.layer(x, router, 1, *w)
+    assert bool(torch.isfinite(y).all())
+    assert torch.equal(y[:511], moe.layer(x[:511], router, 1, *w)) and torch.equal(y[511:], moe.layer(x[511:], router, 1, *w))
+    weights, ids = moe.route((x[505:].double() @ router.double().t().contiguous()).float(), 1)
+    z = moe.experts(x[505:], weights, ids, *w).float()
+    assert len(ids.unique()) == 2 and bool(((y[505:].float() - z).norm(dim=1) <= 1e-2 * z.norm(dim=1)).all())
