@@ -11,12 +11,13 @@
 // global -> LDS copies, in a ring of NS stages; the next step's fragments and the next stage's copies go
 // out one by one between the matrix instructions.
 //
-// Measured (bfloat16 result): 8192^3 254 us on 256 x 256 tiles, 4330 TFLOPS, operands in the caches.  Alone the matrix
-// instructions would take 200 us (at the clock that they leave), the copies 207 (13 TB/s into LDS, whatever the depth
-// of the ring), the fragment reads 121; together, one after another now and then, they take 280 with
-// operands from memory.  What did not help: stages of half lines (128 columns, four of them, 300 us), four waves of
-// 128 x 128 (the accumulators leave no registers), workgroups that go on to the next tile (286),
-// touching the lines of later stages ahead (336).
+// Measured (bfloat16 result): 8192^3 on 256 x 256 tiles 257 to 270 us at best, 4.1 to 4.3 PFLOPS, and 277 to 343 in
+// the median of calls one after another, by the card and the clock that their power leaves it (operands of zeros: 191 to 221);
+// 254 with the operands in the caches.  Alone the matrix instructions would take 200 us (at the clock that they leave), the
+// copies 207 (2.28 GB, 11.0 TB/s into LDS, whatever the depth of the ring), the fragment reads 121; they do not
+// overlap all the time.  What did not help: stages of half lines (128 columns, four of them, 300 us
+// where this took 280), four waves of 128 x 128 (the accumulators leave no registers), workgroups that go on to the next tile
+// (286), touching the lines of later stages ahead (336).
 #pragma once
 
 #include "common.h"
