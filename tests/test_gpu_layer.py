@@ -317,3 +317,26 @@ def test_more_tokens_than_a_launch_addresses_go_in_parts():
     weights, ids = moe.route((x[505:].double() @ router.double().t().contiguous()).float(), 1)
     z = moe.experts(x[505:], weights, ids, *w).float()
     assert len(ids.unique()) == 2 and bool(((y[505:].float() - z).norm(dim=1) <= 1e-2 * z.norm(dim=1)).all())
+
+
+def test_wide_hidden_layers_on_a_workspace_of_garbage():
+    T, k, E, D, I = 2, 4, 10, 256, 4000
+    x, router, (w1, s1, w2, s2) = layer(T, E, D, I)
+    want = moe.layer(x, router, k, w1, s1, w2, s2)
+    n = _ops.layer_workspace(T, k, E, D, I)
+    ws = torch.full((n + 256,), 255, dtype=torch.uint8, device=DEV)
+    out = torch.full((T + 2, D), 7.0, dtype=torch.float16, device=DEV)
+    for _ in range(2):
+        assert _ops.layer(x.data_ptr(), 0, T, D, 1, router.data_ptr(), 0, D, 1, E, k, 0, None, 1, 1, 1, 1.0, D, I, w1.data_ptr(),
+                          2 * I * D, I * D, D, s1.data_ptr(), *s1.stride(), w2.data_ptr(), I * D, I, s2.data_ptr(), *s2.stride(),
+                          out[1].data_ptr(), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out[1:-1], want)
+    assert bool((out[0] == 7).all()) and bool((out[-1] == 7).all()) and bool((ws[n:] == 255).all())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = moe.layer(x, router, k, w1, s1, w2, s2)
+    for i in range(3):
+        x.copy_(normal(T, D, seed=30 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, moe.layer(x, router, k, w1, s1, w2, s2))
