@@ -67,8 +67,8 @@ def linear(x, w, w_scale=None, bias=None):
        [N, ceil(K / 32)] scales; gradients reach x and bias.  That of x is the product of dy and of w's
        values, quantised again along N (blocks of 32 rows of w) on every call.  Rows that no 16-byte load
        fits (K no multiple of 32 among them) are copied on every call, except for few
-       tokens (at most 16, fewer with large weights, their values next to each other): one kernel reads w as it is,
-       allocates nothing but the result, and a token's result there does not depend on those beside it
+       tokens (at most 16, fewer with large weights, their values next to each other): one kernel reads the rows as they
+       are, without a workspace, and a token's result there does not depend on those beside it
     w alone: a float16, bfloat16 or float32 [N, K] weight, quantised on every call; gradients reach x, w
        and bias, their products in 4 bits too, every operand quantised along its product's sum:
        dx = Q(dy) Q(w) in blocks along N, dw = Q(dy).T Q(x) in blocks along the tokens
